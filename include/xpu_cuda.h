@@ -171,6 +171,118 @@ int xpu_qwen_silu_multiply(uint16_t *gate, const uint16_t *up, uint32_t width, v
  * index of the maximum, 0xffffffff if any value is NaN or +-Inf. */
 int xpu_qwen_argmax(const uint16_t *values, uint32_t *token, uint32_t width, void *stream);
 
+/* --------------------------------------------------------- serving cache --
+ * A paged key/value cache shared by many sequences, and the operators of a
+ * serving loop over it (no counterpart in the reference, whose Engine holds
+ * one contiguous cache, qwen3/main.cpp:120-157).
+ *
+ * The pool holds `pages` pages of page_size positions. Keys and values are
+ * [layers][pages][kv_heads][page_size][head_dim], 16-bit elements of `dtype`.
+ * Sequence s uses ceil(lens[s] / page_size) pages, tables[s][0..]: one page
+ * covers the same positions of every layer. refs[p] counts the sequences that
+ * use page p; 0 = free. Only pages that are full are ever shared. The caller
+ * owns all of it in device memory and starts with lens and refs 0, tables -1,
+ * status 0. Every operator reads and writes tables, lens and refs on the
+ * device, so a serving loop needs no host synchronisation; a request that
+ * cannot be met changes nothing and sets a bit of *status. Calls on one cache
+ * must be ordered by the caller (one stream, or events).
+ */
+typedef struct {
+  void *k, *v;              /* 16-byte aligned */
+  int32_t *tables;          /* [sequences][table_width], -1 = no page */
+  int32_t *lens;            /* [sequences] */
+  int32_t *refs;            /* [pages] */
+  uint32_t *status;         /* XPU_KV_* bits, sticky */
+  int32_t *workspace;       /* xpu_kv_workspace_size bytes, 16-byte aligned */
+  int32_t dtype;            /* XPU_BF16 or XPU_FP16 */
+  uint32_t layers, pages, page_size, kv_heads, head_dim, sequences, table_width;
+} xpu_kv_cache_t;
+
+#define XPU_KV_EXHAUSTED 1u    /* not enough free pages, or a table is too narrow: the call changed nothing */
+#define XPU_KV_BAD_SEQUENCE 2u /* an id out of range or named twice, a child in use, a negative count: the same */
+#define XPU_KV_SHARED_CUT 4u   /* a trim would end inside a shared page: the same */
+#define XPU_KV_BAD_INDEX 8u    /* a row, page or length out of range: not written, read as zeros or as nothing */
+
+/* Most sequences one call may name; page_size is 16, 32, 64 or 128; head_dim
+ * 64 or 128; at most XPU_KV_MAX_SEQUENCES sequences; pages x kv_heads x
+ * page_size below 2^31. */
+#define XPU_KV_MAX_REQUESTS 1024u
+#define XPU_KV_MAX_SEQUENCES 65536u
+
+size_t xpu_kv_workspace_size(uint32_t pages);
+
+/* Gives sequences[i] room for starts[i+1] - starts[i] more positions
+ * (starts: count + 1 ascending offsets into the call's tokens) and lengthens
+ * it by them: the lowest free pages, in the order of the list. */
+int xpu_kv_extend(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *starts, uint32_t count,
+                  void *stream);
+/* Writes the positions that the last xpu_kv_extend (same list) added, in
+ * layers [layer, layer + layers): token t comes from row rows[t] (NULL: row t)
+ * of k and v, each [layers][held][kv_heads][head_dim] with the given strides
+ * in elements (multiples of 8). `tokens` is at least starts[count], of which
+ * the rest is ignored. Writes nothing if the extension was refused. */
+int xpu_kv_write(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *starts, uint32_t count,
+                 uint32_t tokens, const int32_t *rows, const void *k, const void *v, uint32_t held,
+                 uint64_t layer_stride, uint64_t row_stride, uint32_t layer, uint32_t layers, void *stream);
+/* xpu_kv_extend, then xpu_kv_write of every layer. */
+int xpu_kv_append(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *starts, uint32_t count,
+                  uint32_t tokens, const int32_t *rows, const void *k, const void *v, uint32_t held,
+                  uint64_t layer_stride, uint64_t row_stride, void *stream);
+/* Shortens sequences[i] to new_lens[i] positions (no change if it is shorter):
+ * pages wholly behind the new length lose a user and leave the table. 0 frees
+ * the sequence. A new length inside a page that others use is refused. */
+int xpu_kv_trim(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *new_lens, uint32_t count,
+                void *stream);
+/* Makes the empty sequence children[i] a copy of parents[i]: full pages are
+ * shared; the part in use of a last page that is not full is copied to the
+ * lowest free page, in the order of the list. Parents may repeat. */
+int xpu_kv_fork(const xpu_kv_cache_t *cache, const int32_t *parents, const int32_t *children, uint32_t count,
+                void *stream);
+/* With n pages in use, moves those with ids of n and more to the free pages
+ * below n, both in ascending order, and renames them in every table: the
+ * pages from n on are free afterwards. */
+int xpu_kv_compact(const xpu_kv_cache_t *cache, void *stream);
+
+/* Causal attention over packed prompts, grouped heads: q and out are
+ * [tokens][q_heads][head_dim], k and v [tokens][kv_heads][head_dim], row
+ * strides in elements (multiples of 8; k and v share theirs), prompt i the next
+ * lens[i] tokens (0 allowed). out = softmax(scale q k^T) v over the prompt's
+ * positions up to each row's own; lse (may be NULL) [tokens][q_heads] gets
+ * the natural logarithm of each row's sum of exponentials. FP32 scores,
+ * statistics and sums; the probabilities are rounded to dtype for the second
+ * product. head_dim 64 or 128, q_heads a multiple of kv_heads (at most 64 per kv head),
+ * pointers 16-byte aligned.
+ *
+ * The plan lists each thread block's tiles, longest first; it depends on the
+ * lengths and heads alone, so one plan serves every layer. xpu_prompt_plan
+ * writes it to host memory (*used ints; XPU_ERR_INVALID with *used set if
+ * `capacity` ints are too few); the caller copies it to the device. */
+int xpu_prompt_plan(const uint32_t *lens, uint32_t count, uint32_t q_heads, uint32_t kv_heads, int32_t *plan,
+                    size_t capacity, size_t *used);
+int xpu_prompt_attention(int dtype, const int32_t *plan, uint32_t plan_blocks, const void *q, const void *k, const void *v,
+                         void *out, float *lse, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                         uint32_t head_dim, uint64_t q_stride, uint64_t kv_stride, uint64_t out_stride, float scale,
+                         void *stream);
+
+/* Attention of drafted tokens over the cache: tree i (nodes starts[i] ..
+ * starts[i+1] - 1 of the packed q, k, v, at most XPU_TREE_MAX_NODES of them)
+ * continues sequences[i]. Node r attends every cached position of its
+ * sequence in `layer`, and the nodes j of its own tree whose bit j of
+ * ancestors[r] is set (its own bit included, if it is to see itself). A tree
+ * of one node is the single-token decode step. A row that attends nothing
+ * gives zeros and lse -inf. Types, strides and precision as
+ * xpu_prompt_attention. The drafts' keys and values are not in the cache:
+ * xpu_kv_append adds the accepted ones. The workspace holds
+ * xpu_tree_attention_workspace_size bytes, zeroed once before its first use
+ * (calls leave it ready for the next); calls that may overlap need their own. */
+#define XPU_TREE_MAX_NODES 64u
+size_t xpu_tree_attention_workspace_size(uint32_t count, uint32_t nodes, uint32_t q_heads, uint32_t kv_heads,
+                                         uint32_t head_dim);
+int xpu_tree_attention(const xpu_kv_cache_t *cache, uint32_t layer, const int32_t *sequences, const int32_t *starts,
+                       const uint64_t *ancestors, uint32_t count, uint32_t nodes, const void *q, const void *k,
+                       const void *v, void *out, float *lse, uint32_t q_heads, uint64_t q_stride, uint64_t kv_stride,
+                       uint64_t out_stride, float scale, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------- synthetic data --
  * Seeded, irregular inputs generated on the device (the reference generates
  * its benchmark inputs on the device too: gemv.cpp:156-167). Each element is

@@ -48,6 +48,13 @@ class Qwen3InfoC(ctypes.Structure):
     _fields_ = [("weight_bytes", u64), ("kernels_per_step", u32), ("vocab_rows", u32),
                 ("vocab_offset", u32), ("stream", vp)]
 
+
+class KvCacheC(ctypes.Structure):
+    """xpu_kv_cache_t."""
+    _fields_ = [("k", vp), ("v", vp), ("tables", vp), ("lens", vp), ("refs", vp), ("status", vp), ("workspace", vp),
+                ("dtype", i32), ("layers", u32), ("pages", u32), ("page_size", u32), ("kv_heads", u32),
+                ("head_dim", u32), ("sequences", u32), ("table_width", u32)]
+
 # name -> (restype, argtypes). Keep in step with include/xpu_cuda.h.
 SIGNATURES: dict[str, tuple] = {
     "xpu_last_error": (ctypes.c_char_p, []),
@@ -69,6 +76,17 @@ SIGNATURES: dict[str, tuple] = {
     "xpu_qwen_add": (i32, [vp, vp, u32, vp]),
     "xpu_qwen_silu_multiply": (i32, [vp, vp, u32, vp]),
     "xpu_qwen_argmax": (i32, [vp, vp, u32, vp]),
+    "xpu_kv_workspace_size": (sz, [u32]),
+    "xpu_kv_extend": (i32, [vp, vp, vp, u32, vp]),
+    "xpu_kv_write": (i32, [vp, vp, vp, u32, u32, vp, vp, vp, u32, u64, u64, u32, u32, vp]),
+    "xpu_kv_append": (i32, [vp, vp, vp, u32, u32, vp, vp, vp, u32, u64, u64, vp]),
+    "xpu_kv_trim": (i32, [vp, vp, vp, u32, vp]),
+    "xpu_kv_fork": (i32, [vp, vp, vp, u32, vp]),
+    "xpu_kv_compact": (i32, [vp, vp]),
+    "xpu_prompt_plan": (i32, [vp, u32, u32, u32, vp, sz, vp]),
+    "xpu_prompt_attention": (i32, [i32, vp, u32, vp, vp, vp, vp, vp, u32, u32, u32, u32, u64, u64, u64, f32, vp]),
+    "xpu_tree_attention_workspace_size": (sz, [u32, u32, u32, u32, u32]),
+    "xpu_tree_attention": (i32, [vp, u32, vp, vp, vp, u32, u32, vp, vp, vp, vp, vp, u32, u64, u64, u64, f32, vp, sz, vp]),
     "xpu_fill_uniform16": (i32, [i32, vp, u64, u64, u64, vp]),
     "xpu_fill_normal_bf16": (i32, [vp, u64, u64, u64, f32, vp]),
     "xpu_qwen3_create": (i32, [vp, u32, i32, u32, u32, vp]),

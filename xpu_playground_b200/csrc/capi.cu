@@ -4,6 +4,7 @@
 #include <exception>
 #include <string>
 
+#include "serving.h"
 #include "xpu_internal.h"
 
 namespace xpu {
@@ -37,14 +38,75 @@ static inline cudaStream_t as_stream(void *stream) { return static_cast<cudaStre
   } while (0)
 
 // Wraps a body so that no C++ exception crosses the C boundary.
-#define XPU_GUARD(body)                                               \
+#define XPU_GUARD(...)                                                \
   try {                                                               \
-    body                                                              \
+    __VA_ARGS__                                                       \
   } catch (const std::exception &e) {                                 \
     return fail(XPU_ERR_INVALID, std::string("exception: ") + e.what()); \
   } catch (...) {                                                     \
     return fail(XPU_ERR_INVALID, "unknown exception");                \
   }
+
+// Checks of a serving cache that every operator makes; XPU_OK if it is usable.
+static int check_cache(const xpu_kv_cache_t *c, const char *who) {
+  const std::string at = std::string(who) + ": ";
+  XPU_REQUIRE(c, at + "null cache");
+  XPU_REQUIRE(c->k && c->v && c->tables && c->lens && c->refs && c->status && c->workspace, at + "null pointer in the cache");
+  XPU_REQUIRE(aligned16(c->k) && aligned16(c->v) && aligned16(c->workspace), at + "pools and workspace must be 16-byte aligned");
+  XPU_REQUIRE(c->dtype == XPU_BF16 || c->dtype == XPU_FP16, at + "dtype must be XPU_BF16 or XPU_FP16");
+  XPU_REQUIRE(c->layers && c->pages && c->kv_heads && c->sequences && c->table_width, at + "empty cache");
+  if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+    return fail(XPU_ERR_UNSUPPORTED, at + "page_size must be 16, 32, 64 or 128");
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(XPU_ERR_UNSUPPORTED, at + "head_dim must be 64 or 128");
+  XPU_REQUIRE(c->sequences <= XPU_KV_MAX_SEQUENCES, at + "too many sequences");
+  XPU_REQUIRE(static_cast<uint64_t>(c->pages) * c->kv_heads * c->page_size < (1ull << 31) &&
+                  static_cast<uint64_t>(c->table_width) * c->page_size < (1ull << 31),
+              at + "pool too large");
+  return XPU_OK;
+}
+
+static int check_list(const void *a, const void *b, uint32_t count, const char *who) {
+  XPU_REQUIRE((a && b) || count == 0, std::string(who) + ": null pointer");
+  XPU_REQUIRE(count <= XPU_KV_MAX_REQUESTS, std::string(who) + ": more than 1024 sequences in one call");
+  return XPU_OK;
+}
+
+static int check_rows(const xpu_kv_cache_t &c, const void *k, const void *v, uint32_t held, uint64_t layer_stride,
+                      uint64_t row_stride, uint32_t layer, uint32_t layers, const char *who) {
+  const std::string at = std::string(who) + ": ";
+  XPU_REQUIRE(k && v, at + "null pointer");
+  XPU_REQUIRE(aligned16(k) && aligned16(v) && layer_stride % 8 == 0 && row_stride % 8 == 0,
+              at + "k and v must be 16-byte aligned with strides in multiples of 8 elements");
+  XPU_REQUIRE(row_stride >= static_cast<uint64_t>(c.kv_heads) * c.head_dim, at + "row stride shorter than a row");
+  XPU_REQUIRE(held < (1u << 31), at + "too many rows");
+  XPU_REQUIRE(layers > 0 && layer < c.layers && layers <= c.layers - layer, at + "layer out of range");
+  return XPU_OK;
+}
+
+static int check_attention(int dtype, const AttnTensors &t, const char *who) {
+  const std::string at = std::string(who) + ": ";
+  XPU_REQUIRE(t.q && t.k && t.v && t.out, at + "null pointer");
+  XPU_REQUIRE(aligned16(t.q) && aligned16(t.k) && aligned16(t.v) && aligned16(t.out),
+              at + "q, k, v and out must be 16-byte aligned");
+  XPU_REQUIRE(dtype == XPU_BF16 || dtype == XPU_FP16, at + "dtype must be XPU_BF16 or XPU_FP16");
+  if (t.head_dim != 64 && t.head_dim != 128) return fail(XPU_ERR_UNSUPPORTED, at + "head_dim must be 64 or 128");
+  XPU_REQUIRE(t.kv_heads > 0 && t.q_heads >= t.kv_heads && t.q_heads % t.kv_heads == 0,
+              at + "q_heads must be a positive multiple of kv_heads");
+  if (t.q_heads / t.kv_heads > 64) return fail(XPU_ERR_UNSUPPORTED, at + "more than 64 query heads per kv head");
+  XPU_REQUIRE(t.tokens < (1u << 31), at + "too many tokens");
+  XPU_REQUIRE(t.q_stride % 8 == 0 && t.kv_stride % 8 == 0 && t.out_stride % 8 == 0,
+              at + "row strides must be multiples of 8 elements");
+  const uint64_t q = static_cast<uint64_t>(t.q_heads) * t.head_dim, kv = static_cast<uint64_t>(t.kv_heads) * t.head_dim;
+  XPU_REQUIRE(t.q_stride >= q && t.out_stride >= q && t.kv_stride >= kv, at + "row stride shorter than a row");
+  XPU_REQUIRE(t.q_stride < (1ull << 38) && t.kv_stride < (1ull << 38), at + "row stride too long");
+  return XPU_OK;
+}
+
+#define XPU_CHECKED(expr)                  \
+  do {                                     \
+    const int status_ = (expr);            \
+    if (status_ != XPU_OK) return status_; \
+  } while (0)
 
 extern "C" {
 
@@ -205,6 +267,141 @@ int xpu_qwen_argmax(const uint16_t *values, uint32_t *token, uint32_t width, voi
     XPU_REQUIRE(values && token, "xpu_qwen_argmax: null pointer");
     return cuda_status(qwen_argmax_launch(values, token, width, as_stream(stream)),
                        "xpu_qwen_argmax");
+  })
+}
+
+size_t xpu_kv_workspace_size(uint32_t pages) { return kv_workspace_bytes(pages); }
+
+int xpu_kv_extend(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *starts, uint32_t count,
+                  void *stream) {
+  XPU_GUARD({
+    XPU_CHECKED(check_cache(cache, "xpu_kv_extend"));
+    XPU_CHECKED(check_list(sequences, starts, count, "xpu_kv_extend"));
+    if (count == 0) return XPU_OK;
+    return cuda_status(kv_extend_launch(*cache, sequences, starts, count, as_stream(stream)), "xpu_kv_extend");
+  })
+}
+
+int xpu_kv_write(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *starts, uint32_t count,
+                 uint32_t tokens, const int32_t *rows, const void *k, const void *v, uint32_t held,
+                 uint64_t layer_stride, uint64_t row_stride, uint32_t layer, uint32_t layers, void *stream) {
+  XPU_GUARD({
+    XPU_CHECKED(check_cache(cache, "xpu_kv_write"));
+    XPU_CHECKED(check_list(sequences, starts, count, "xpu_kv_write"));
+    if (count == 0 || tokens == 0) return XPU_OK;
+    XPU_CHECKED(check_rows(*cache, k, v, held, layer_stride, row_stride, layer, layers, "xpu_kv_write"));
+    return cuda_status(kv_write_launch(*cache, sequences, starts, count, tokens, rows, k, v, held, layer_stride, row_stride,
+                                       layer, layers, as_stream(stream)),
+                       "xpu_kv_write");
+  })
+}
+
+int xpu_kv_append(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *starts, uint32_t count,
+                  uint32_t tokens, const int32_t *rows, const void *k, const void *v, uint32_t held,
+                  uint64_t layer_stride, uint64_t row_stride, void *stream) {
+  XPU_GUARD({
+    XPU_CHECKED(check_cache(cache, "xpu_kv_append"));
+    XPU_CHECKED(check_list(sequences, starts, count, "xpu_kv_append"));
+    if (count == 0 || tokens == 0) return XPU_OK;
+    XPU_CHECKED(check_rows(*cache, k, v, held, layer_stride, row_stride, 0, cache->layers, "xpu_kv_append"));
+    XPU_CHECKED(cuda_status(kv_extend_launch(*cache, sequences, starts, count, as_stream(stream)), "xpu_kv_append"));
+    return cuda_status(kv_write_launch(*cache, sequences, starts, count, tokens, rows, k, v, held, layer_stride, row_stride,
+                                       0, cache->layers, as_stream(stream)),
+                       "xpu_kv_append");
+  })
+}
+
+int xpu_kv_trim(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *new_lens, uint32_t count,
+                void *stream) {
+  XPU_GUARD({
+    XPU_CHECKED(check_cache(cache, "xpu_kv_trim"));
+    XPU_CHECKED(check_list(sequences, new_lens, count, "xpu_kv_trim"));
+    if (count == 0) return XPU_OK;
+    return cuda_status(kv_trim_launch(*cache, sequences, new_lens, count, as_stream(stream)), "xpu_kv_trim");
+  })
+}
+
+int xpu_kv_fork(const xpu_kv_cache_t *cache, const int32_t *parents, const int32_t *children, uint32_t count,
+                void *stream) {
+  XPU_GUARD({
+    XPU_CHECKED(check_cache(cache, "xpu_kv_fork"));
+    XPU_CHECKED(check_list(parents, children, count, "xpu_kv_fork"));
+    if (count == 0) return XPU_OK;
+    return cuda_status(kv_fork_launch(*cache, parents, children, count, as_stream(stream)), "xpu_kv_fork");
+  })
+}
+
+int xpu_kv_compact(const xpu_kv_cache_t *cache, void *stream) {
+  XPU_GUARD({
+    XPU_CHECKED(check_cache(cache, "xpu_kv_compact"));
+    return cuda_status(kv_compact_launch(*cache, as_stream(stream)), "xpu_kv_compact");
+  })
+}
+
+int xpu_prompt_plan(const uint32_t *lens, uint32_t count, uint32_t q_heads, uint32_t kv_heads, int32_t *plan,
+                    size_t capacity, size_t *used) {
+  XPU_GUARD({
+    XPU_REQUIRE((lens || count == 0) && (plan || capacity == 0) && used, "xpu_prompt_plan: null pointer");
+    XPU_REQUIRE(kv_heads > 0 && q_heads >= kv_heads && q_heads % kv_heads == 0,
+                "xpu_prompt_plan: q_heads must be a positive multiple of kv_heads");
+    if (q_heads / kv_heads > 64) return fail(XPU_ERR_UNSUPPORTED, "xpu_prompt_plan: more than 64 query heads per kv head");
+    uint64_t tokens = 0;
+    for (uint32_t i = 0; i < count; ++i) tokens += lens[i];
+    XPU_REQUIRE(tokens < (1ull << 31), "xpu_prompt_plan: too many tokens");
+    int device = 0, sms = 0;  // without a device: the plan of a B200
+    if (cudaGetDevice(&device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+      cudaGetLastError();
+      sms = 148;
+    }
+    *used = prompt_plan(lens, count, q_heads, kv_heads, static_cast<uint32_t>(sms), plan, capacity);
+    if (*used > capacity)
+      return fail(XPU_ERR_INVALID, "xpu_prompt_plan: the plan needs " + std::to_string(*used) + " ints");
+    return XPU_OK;
+  })
+}
+
+int xpu_prompt_attention(int dtype, const int32_t *plan, uint32_t plan_blocks, const void *q, const void *k, const void *v,
+                         void *out, float *lse, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                         uint32_t head_dim, uint64_t q_stride, uint64_t kv_stride, uint64_t out_stride, float scale,
+                         void *stream) {
+  XPU_GUARD({
+    const AttnTensors t{q, k, v, out, lse, tokens, q_heads, kv_heads, head_dim, q_stride, kv_stride, out_stride, scale};
+    if (tokens == 0 || plan_blocks == 0) return XPU_OK;
+    XPU_REQUIRE(plan && aligned16(plan), "xpu_prompt_attention: the plan must be a 16-byte aligned device pointer");
+    XPU_CHECKED(check_attention(dtype, t, "xpu_prompt_attention"));
+    return cuda_status(prompt_attention_launch(dtype == XPU_FP16, plan, plan_blocks, t, as_stream(stream)),
+                       "xpu_prompt_attention");
+  })
+}
+
+size_t xpu_tree_attention_workspace_size(uint32_t count, uint32_t nodes, uint32_t q_heads, uint32_t kv_heads,
+                                         uint32_t head_dim) {
+  if (kv_heads == 0 || q_heads < kv_heads) return 0;
+  return tree_workspace_bytes(count, nodes, q_heads, kv_heads, head_dim);
+}
+
+int xpu_tree_attention(const xpu_kv_cache_t *cache, uint32_t layer, const int32_t *sequences, const int32_t *starts,
+                       const uint64_t *ancestors, uint32_t count, uint32_t nodes, const void *q, const void *k,
+                       const void *v, void *out, float *lse, uint32_t q_heads, uint64_t q_stride, uint64_t kv_stride,
+                       uint64_t out_stride, float scale, void *workspace, size_t workspace_bytes, void *stream) {
+  XPU_GUARD({
+    XPU_CHECKED(check_cache(cache, "xpu_tree_attention"));
+    XPU_CHECKED(check_list(sequences, starts, count, "xpu_tree_attention"));
+    XPU_REQUIRE(layer < cache->layers, "xpu_tree_attention: layer out of range");
+    if (count == 0 || nodes == 0) return XPU_OK;
+    XPU_REQUIRE(ancestors && workspace, "xpu_tree_attention: null pointer");
+    XPU_REQUIRE(aligned16(workspace), "xpu_tree_attention: workspace must be 16-byte aligned");
+    const AttnTensors t{q, k, v, out, lse, nodes, q_heads, cache->kv_heads, cache->head_dim, q_stride, kv_stride, out_stride,
+                        scale};
+    XPU_CHECKED(check_attention(cache->dtype, t, "xpu_tree_attention"));
+    const size_t need = tree_workspace_bytes(count, nodes, q_heads, cache->kv_heads, cache->head_dim);
+    if (workspace_bytes < need)
+      return fail(XPU_ERR_INVALID, "xpu_tree_attention: workspace holds " + std::to_string(workspace_bytes) +
+                                       " bytes, needs " + std::to_string(need));
+    return cuda_status(tree_attention_launch(*cache, layer, sequences, starts, ancestors, count, t, workspace,
+                                             as_stream(stream)),
+                       "xpu_tree_attention");
   })
 }
 

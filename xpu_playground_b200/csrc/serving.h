@@ -1,0 +1,54 @@
+// Launchers of the serving operators (attention over packed prompts and over
+// the paged cache, and the cache's page operators), shared between their
+// kernels and the C entry points.
+#pragma once
+
+#include "xpu_internal.h"
+
+namespace xpu {
+
+// ---- paged cache (kv_cache.cu) ----
+size_t kv_workspace_bytes(uint32_t pages);
+cudaError_t kv_extend_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *starts, uint32_t count,
+                             cudaStream_t s);
+cudaError_t kv_write_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *starts, uint32_t count,
+                            uint32_t tokens, const int32_t *rows, const void *k, const void *v, uint32_t held,
+                            uint64_t layer_stride, uint64_t row_stride, uint32_t layer, uint32_t layers,
+                            cudaStream_t s);
+cudaError_t kv_trim_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *new_lens, uint32_t count,
+                           cudaStream_t s);
+cudaError_t kv_fork_launch(const xpu_kv_cache_t &c, const int32_t *parents, const int32_t *children, uint32_t count,
+                           cudaStream_t s);
+cudaError_t kv_compact_launch(const xpu_kv_cache_t &c, cudaStream_t s);
+
+// ---- attention (serving_attention.cu) ----
+// Rows of one head group's tile: row r is position (or node) r / group, head
+// r % group of the group, so a tile of 128 rows holds 128 / group of them.
+constexpr uint32_t kTileRows = 128;
+__host__ __device__ constexpr uint32_t tile_positions(uint32_t group) { return kTileRows / group; }
+
+// Host plan of a packed batch: {blocks, tokens, items, group}, blocks + 1
+// offsets into the items, padding to 4 ints, then per item {first token of
+// the prompt, its length, first position of the item, kv head}: two tiles of
+// positions each.
+constexpr uint32_t kPlanHeader = 4;
+__host__ __device__ constexpr uint32_t plan_items_at(uint32_t blocks) { return (kPlanHeader + blocks + 1 + 3) / 4 * 4; }
+size_t prompt_plan(const uint32_t *lens, uint32_t count, uint32_t q_heads, uint32_t kv_heads, uint32_t sms, int32_t *plan,
+                   size_t capacity);
+
+struct AttnTensors {
+  const void *q, *k, *v;
+  void *out;
+  float *lse;
+  uint32_t tokens, q_heads, kv_heads, head_dim;
+  uint64_t q_stride, kv_stride, out_stride;
+  float scale;
+};
+cudaError_t prompt_attention_launch(bool fp16, const int32_t *plan, uint32_t blocks, const AttnTensors &t,
+                                    cudaStream_t s);
+size_t tree_workspace_bytes(uint32_t count, uint32_t nodes, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim);
+cudaError_t tree_attention_launch(const xpu_kv_cache_t &c, uint32_t layer, const int32_t *sequences,
+                                  const int32_t *starts, const uint64_t *ancestors, uint32_t count,
+                                  const AttnTensors &t, void *workspace, cudaStream_t s);
+
+}  // namespace xpu

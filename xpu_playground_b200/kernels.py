@@ -8,7 +8,9 @@ a contiguous CUDA tensor; 16-bit tensors are passed by their bit patterns.
 from __future__ import annotations
 
 import ctypes
+import math
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -142,3 +144,104 @@ def qwen_silu_multiply(gate, up, width: int, stream=None):
 
 def qwen_argmax(values, token, width: int, stream=None):
     call("xpu_qwen_argmax", _ptr(values), _ptr(token), width, _stream(stream))
+
+
+# ------------------------------------------------- attention for serving ----
+
+def _packed(name: str, t: torch.Tensor, heads: int, head_dim: int) -> int:
+    """Row stride of a packed [tokens, heads, head_dim] tensor whose rows may
+    stand apart (a slice of a fused projection)."""
+    if not t.is_cuda:
+        raise ValueError("libxpu_cuda entry points take CUDA tensors")
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
+        raise ValueError(f"{name} must be [tokens, {heads}, {head_dim}], not {tuple(t.shape)}")
+    row, head, element = t.stride()
+    if (element != 1 and head_dim != 1) or (head != head_dim and heads != 1):
+        raise ValueError(f"{name}: the heads of a token must be contiguous")
+    return row if t.shape[0] > 1 else max(row, heads * head_dim)
+
+
+def _attention_args(q, k, v, kv_heads, head_dim, scale, out, lse):
+    tokens, q_heads = q.shape[0], q.shape[1]
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must have one dtype")
+    q_stride, kv_stride = _packed("q", q, q_heads, head_dim), _packed("k", k, kv_heads, head_dim)
+    if _packed("v", v, kv_heads, head_dim) != kv_stride or k.shape[0] != tokens or v.shape[0] != tokens:
+        raise ValueError("k and v need q's tokens and one row stride")
+    if out is None:
+        out = torch.empty(tokens, q_heads, head_dim, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape:
+        raise ValueError("out must have q's shape and dtype")
+    if lse is None:
+        lse = torch.empty(tokens, q_heads, dtype=torch.float32, device=q.device)
+    elif lse.dtype != torch.float32 or lse.shape != q.shape[:2]:
+        raise ValueError("lse must be float32 [tokens, q_heads]")
+    return (out, lse, q_stride, kv_stride, _packed("out", out, q_heads, head_dim),
+            1.0 / math.sqrt(head_dim) if scale is None else scale)
+
+
+class PromptPlan:
+    """Which thread block computes which tiles of a batch of packed prompts
+    (xpu_prompt_plan). It depends on the lengths and heads alone: make it once
+    per batch and use it for every layer."""
+
+    def __init__(self, lens, q_heads: int, kv_heads: int, head_dim: int, device=None):
+        n = np.ascontiguousarray(lens, dtype=np.uint32)
+        used = ctypes.c_size_t()
+        lib = _lib.load()
+        room = 2048 + 4 * kv_heads * (n.size + int(n.sum()) * max(1, q_heads // max(1, kv_heads)) // 128 + 1)
+        plan = np.empty(room, np.int32)
+        status = lib.xpu_prompt_plan(n.ctypes.data, n.size, q_heads, kv_heads, plan.ctypes.data, plan.size,
+                                     ctypes.byref(used))
+        if status == _lib.XPU_ERR_INVALID and used.value > plan.size:
+            plan = np.empty(used.value, np.int32)
+            status = lib.xpu_prompt_plan(n.ctypes.data, n.size, q_heads, kv_heads, plan.ctypes.data, plan.size,
+                                         ctypes.byref(used))
+        _lib.check(status)
+        self.blocks, self.tokens = int(plan[0]), int(plan[1])
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.device_plan = torch.from_numpy(plan[:used.value]).to(device or "cuda")
+
+
+def prompt_attention(plan: PromptPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None,
+                     out: torch.Tensor | None = None, lse: torch.Tensor | None = None, stream=None):
+    """Causal attention over packed prompts (xpu_prompt_attention): q [tokens,
+    q_heads, head_dim], k and v [tokens, kv_heads, head_dim], bf16 or fp16;
+    scale defaults to 1 / sqrt(head_dim). Returns (out, lse)."""
+    if q.shape[0] != plan.tokens or q.dim() != 3 or q.shape[1] != plan.q_heads:
+        raise ValueError(f"q must be [{plan.tokens}, {plan.q_heads}, {plan.head_dim}] for this plan")
+    out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, plan.kv_heads, plan.head_dim, scale, out, lse)
+    call("xpu_prompt_attention", _dtype_code(q), plan.device_plan.data_ptr(), plan.blocks, q.data_ptr(), k.data_ptr(),
+         v.data_ptr(), out.data_ptr(), _ptr(lse), plan.tokens, plan.q_heads, plan.kv_heads, plan.head_dim, q_stride,
+         kv_stride, out_stride, scale, _stream(stream))
+    return out, lse
+
+
+def tree_attention_workspace(count: int, nodes: int, q_heads: int, kv_heads: int, head_dim: int,
+                             device=None) -> torch.Tensor:
+    """Zeroed workspace for tree_attention calls of up to `count` sequences
+    and `nodes` drafted tokens in all."""
+    size = int(_lib.load().xpu_tree_attention_workspace_size(count, nodes, q_heads, kv_heads, head_dim))
+    return torch.zeros(size, dtype=torch.uint8, device=device or "cuda")
+
+
+def tree_attention(cache, layer: int, sequences: torch.Tensor, starts: torch.Tensor, ancestors: torch.Tensor,
+                   q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, workspace: torch.Tensor,
+                   scale: float | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                   stream=None):
+    """Attention of trees of drafted tokens over a KvCache
+    (xpu_tree_attention): tree i is nodes starts[i] .. starts[i+1] - 1 of the
+    packed q, k, v and continues sequences[i]; bit j of ancestors[r] lets node
+    r attend node j of its tree. int32 sequences and starts, int64 ancestors.
+    Returns (out, lse)."""
+    if q.dtype != cache.dtype:
+        raise ValueError("q, k and v must have the cache's dtype")
+    if sequences.dtype != torch.int32 or starts.dtype != torch.int32 or ancestors.dtype != torch.int64:
+        raise ValueError("sequences and starts are int32, ancestors int64")
+    if starts.numel() != sequences.numel() + 1 or ancestors.numel() != q.shape[0]:
+        raise ValueError("starts needs one entry more than sequences, ancestors one per node")
+    out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, cache.kv_heads, cache.head_dim, scale, out, lse)
+    call("xpu_tree_attention", cache.handle, layer, _ptr(sequences), _ptr(starts), _ptr(ancestors), sequences.numel(),
+         q.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), q.shape[1], q_stride, kv_stride,
+         out_stride, scale, _ptr(workspace), workspace.numel(), _stream(stream))
+    return out, lse
