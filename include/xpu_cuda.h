@@ -68,7 +68,8 @@ int xpu_gemm_bt(int dtype, const void *a, const void *w, void *c, uint32_t m, ui
 
 /* Sticky device-side error word of this library's asynchronous kernels,
  * read and cleared (synchronises the device). Bit 0: a GEMM pipeline wait
- * timed out and its tile is incomplete; bit 1: a calibrator wait timed out. No reference counterpart (the
+ * timed out and its tile is incomplete; bit 1: a calibrator wait timed out;
+ * bit 2: a serving attention wait timed out and its outputs are incomplete. No reference counterpart (the
  * reference's kernels have no bounded waits). */
 int xpu_device_status(uint32_t *flags);
 
@@ -251,7 +252,7 @@ int xpu_kv_compact(const xpu_kv_cache_t *cache, void *stream);
  * the natural logarithm of each row's sum of exponentials. FP32 scores,
  * statistics and sums; the probabilities are rounded to dtype for the second
  * product. head_dim 64 or 128, q_heads a multiple of kv_heads (at most 64 per kv head),
- * pointers 16-byte aligned.
+ * pointers 16-byte aligned, scale positive and finite.
  *
  * The plan lists each thread block's tiles, longest first; it depends on the
  * lengths and heads alone, so one plan serves every layer. xpu_prompt_plan

@@ -60,7 +60,8 @@ PROMPT = dict(dtype=0, plan=64, blocks=1, q=64, k=64, v=64, out=64, lse=None, to
     ({"dtype": 9}, INVALID), ({"kv_heads": 0}, INVALID), ({"q_heads": 5}, INVALID), ({"q_heads": 1}, INVALID),
     ({"head_dim": 80}, UNSUPPORTED), ({"q_heads": 130, "q_stride": 8320, "out_stride": 8320}, UNSUPPORTED),
     ({"q_stride": 252}, INVALID), ({"q_stride": 248}, INVALID), ({"kv_stride": 64}, INVALID), ({"out_stride": 128}, INVALID),
-    ({"kv_stride": 1 << 38}, INVALID), ({"tokens": 1 << 31}, INVALID),
+    ({"kv_stride": 1 << 38}, INVALID), ({"tokens": 1 << 31}, INVALID), ({"scale": 0.0}, INVALID), ({"scale": -1.0}, INVALID),
+    ({"scale": float("inf")}, INVALID), ({"scale": float("nan")}, INVALID),
 ])
 def test_prompt_refusals(change, status):
     assert _lib.load().xpu_prompt_attention(*(PROMPT | change).values(), None) == status

@@ -1,6 +1,7 @@
 // extern "C" entry points of libxpu_cuda (declared in include/xpu_cuda.h).
 // Each validates its arguments on the host, launches on the caller's stream
 // and converts every failure into a status code plus a thread-local message.
+#include <cmath>
 #include <exception>
 #include <string>
 
@@ -98,6 +99,7 @@ static int check_attention(int dtype, const AttnTensors &t, const char *who) {
               at + "row strides must be multiples of 8 elements");
   const uint64_t q = static_cast<uint64_t>(t.q_heads) * t.head_dim, kv = static_cast<uint64_t>(t.kv_heads) * t.head_dim;
   XPU_REQUIRE(t.q_stride >= q && t.out_stride >= q && t.kv_stride >= kv, at + "row stride shorter than a row");
+  XPU_REQUIRE(t.scale > 0.f && t.scale < INFINITY, at + "scale must be positive and finite");
   XPU_REQUIRE(t.q_stride < (1ull << 38) && t.kv_stride < (1ull << 38), at + "row stride too long");
   return XPU_OK;
 }
@@ -161,7 +163,7 @@ int xpu_device_status(uint32_t *flags) {
     XPU_REQUIRE(flags, "xpu_device_status: null pointer");
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return cuda_status(e, "xpu_device_status");
-    *flags = take_device_error() | take_peak_error();
+    *flags = take_device_error() | take_peak_error() | take_attention_error();
     return XPU_OK;
   })
 }

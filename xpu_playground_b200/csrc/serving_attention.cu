@@ -2,126 +2,948 @@
 // token trees over the paged cache (xpu_prompt_attention and
 // xpu_tree_attention in include/xpu_cuda.h).
 //
-// One warp per (row, head): for each allowed key j, s = scale (q . k_j), and
-// the running form of the softmax
-//   m' = max(m, s), l' = l e^(m - m') + e^(s - m'), o' = o e^(m - m') + e^(s - m') v_j
-// in FP32; out = o / l rounded once, lse = m + log l. Masked keys are never
-// read, so what stands in them cannot matter.
+// Both are  out_r = sum_j p_rj v_j / sum_j p_rj,  p_rj = exp(scale q_r . k_j - m_r)
+// over the keys j that row r may attend, taken 128 keys at a time with the
+// running maximum and sum of a softmax, both products on the tensor cores
+// (tcgen05). A row is one query head of one position (node); a row tile is the
+// 128 rows of 128 / group positions, all query heads of one kv head, so one
+// read of a key serves the whole group. A thread block works on a segment: up
+// to two row tiles against a run of key tiles. Twelve warps:
+//   0-3, 4-7  softmax of row tile 0 / 1, one thread a row: scores from TMEM,
+//             mask, maximum, p = 2^(c s - c m) with c = scale log2 e, p rounded
+//             to the input type and written back to TMEM over the scores as the
+//             A operand of the second product; FP32 sum of the unrounded p.
+//             The reference maximum m moves only when the true one has passed
+//             it by 2^8 (p then stays below 2^8, exact in FP32 sums and with the
+//             same relative rounding), so the accumulator in TMEM is rarely
+//             rescaled. At the end out = O / l, rounded once;
+//   8         issues S_t = Q_t K^T (both operands in shared memory) and O_t +=
+//             P_t V (P from TMEM, V as it stands in memory, MN-major). While one
+//             tile is in its softmax the tensor cores work for the other;
+//   9         TMA loads: Q tiles, and a ring of K and V tiles;
+//   10, 11    cleaning: in key tiles with masked keys, V rows that no row may
+//             attend are zeroed (0 x NaN would reach the sums), and rows with
+//             non-finite values are zeroed and listed; the rows that do attend
+//             them get p v added at the end (fix_row).
+// A segment of at most 128 rows (drafted trees, mostly) would leave one softmax
+// group idle: there both groups work for the same rows, on even and odd key
+// tiles, and join their sums at the end.
+//
+// Waits are bounded; a timeout sets a sticky device word that
+// xpu_device_status reads, and every role leaves.
+#include <cuda.h>
+
 #include <algorithm>
-#include <numeric>
+#include <functional>
 #include <queue>
 #include <vector>
 
 #include "common.cuh"
 #include "serving.h"
+#include "stream.cuh"
+#include "tcgen05.cuh"
 
 namespace xpu {
+
+__device__ unsigned int g_attention_error = 0;
+
 namespace {
 
-template <typename T, int D>
-struct Row {
-  static constexpr int N = D / 32;
-  float q[N], o[N], m = -INFINITY, l = 0.f;
+constexpr uint32_t kKeys = 128;        // keys per tile
+constexpr uint32_t kBox = 128 * 128;   // bytes of 128 rows x 64 elements, 128-byte swizzled
+constexpr uint32_t kThreads = 384;
+constexpr uint32_t kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10;
+constexpr unsigned kErrAttentionTimeout = 4u;
+constexpr float kRescale = 8.f;        // in powers of two
+constexpr uint32_t kBadRing = 8;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-  __device__ void begin(const T *row) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      q[i] = Elem<T>::to_float(row[(threadIdx.x & 31) + 32 * i]);
-      o[i] = 0.f;
-    }
+template <int D, bool TREE>
+struct Shape {
+  static constexpr uint32_t kBoxes = D / 64, kTile = kBoxes * kBox;
+  // as many K/V tiles in flight as the shared memory holds beside Q
+  static constexpr uint32_t kStages = D == 64 ? 8 : (TREE ? 4 : 5);
+  static constexpr uint32_t kSmem = 1024 + (2 + kStages) * kTile;
+};
+
+struct BadRows {  // one cleaning warp's half (64 keys) of up to two tiles of a segment
+  uint32_t tiles;
+  uint32_t tile[2], mask[2][2];
+};
+
+struct TreeEntry {
+  uint32_t first;  // key tiles of all segments' units before this sequence's
+  uint32_t len, begin, named;  // cached positions, first node, sequence * 128 + nodes
+};
+
+struct Barriers {
+  uint64_t q_full, q_empty, drain;
+  uint64_t kv_full[8], kv_empty[8], clean[8];
+  uint64_t s_full[2], p_ready[2], o_full[2], joined;
+  uint32_t tmem;
+  int failed;
+  BadRows bad[kBadRing][2];
+};
+
+struct TreeArgs {
+  xpu_kv_cache_t cache;
+  const int32_t *sequences, *starts;
+  const uint64_t *ancestors;
+  uint32_t layer, count;
+  float *partial;  // [slot][256 rows][D], then [slot][256 rows]{m, l}
+};
+
+struct Args {
+  CUtensorMap q, k, v;              // packed
+  CUtensorMap cached_k, cached_v;   // one layer of the pool, 64 elements x page
+  AttnTensors t;
+  const int32_t *plan;
+  TreeArgs tree;
+};
+
+// A run of key tiles for one or two row tiles.
+struct Segment {
+  uint32_t q0, npos, head;   // first position's row of q, positions, kv head
+  uint32_t base, len, pos0;  // prompt: key 0's row, prompt length, first position. tree: first node, cached
+                             // positions, first node of the segment
+  uint32_t nodes;            // tree
+  int32_t sequence;
+  uint32_t first, n, n0, n1; // key tiles: first, all, row tile 0's, row tile 1's
+  bool both;                 // both softmax groups on row tile 0, even and odd key tiles
+  int32_t slot;              // partial result, -1 = whole
+};
+
+// ------------------------------------------------------------ small parts ----
+
+__device__ __forceinline__ bool failed(const Barriers &b) { return *const_cast<const volatile int *>(&b.failed) != 0; }
+// The same answers for the whole warp, so that its lanes leave together.
+__device__ __forceinline__ bool warp_failed(const Barriers &b) { return __any_sync(kFullMask, failed(b)); }
+__device__ __forceinline__ bool warp_wait(Barriers &b, uint64_t *bar, uint32_t parity) {
+  if (__all_sync(kFullMask, mbar_wait(bar, parity))) return true;
+  b.failed = 1;
+  return false;
+}
+
+__host__ __device__ constexpr uint32_t attn_idesc(bool fp16, uint32_t n, bool b_kmajor) {
+  return (1u << 4) | ((fp16 ? 0u : 1u) << 7) | ((fp16 ? 0u : 1u) << 10) | ((b_kmajor ? 0u : 1u) << 16) | ((n >> 3) << 17) |
+         ((128u >> 4) << 24);  // FP32 accumulator, A and B types, B's order, N, M = 128
+}
+
+// D (TMEM) += A (TMEM) . B (shared memory)
+__device__ __forceinline__ void mma1_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+#define XPU_R32(r)                                                                                                  \
+  "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),        \
+      "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),         \
+      "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),        \
+      "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+
+// This warp's 32 TMEM lanes x 32 columns; several may be in flight before tmem_wait_ld().
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : XPU_R32(r)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t z,
+                                            uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_addr(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// Either 16-bit half of w infinite or NaN.
+template <typename T>
+__device__ __forceinline__ bool word_not_finite(uint32_t w) {
+  constexpr uint32_t e = sizeof(T) && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+
+// --------------------------------------------------------------- segments ----
+
+// The prompt plan's items of this block, in order.
+struct PromptWalk {
+  const int4 *items;
+  int32_t i, end;
+  uint32_t positions, tokens;
+  __device__ PromptWalk(const Args &a, uint32_t group) {
+    items = reinterpret_cast<const int4 *>(a.plan + plan_items_at(static_cast<uint32_t>(a.plan[0])));
+    i = a.plan[kPlanHeader + blockIdx.x];
+    end = a.plan[kPlanHeader + blockIdx.x + 1];
+    positions = tile_positions(group);
+    tokens = a.t.tokens;
   }
-  __device__ void key(const T *k, const T *v, float scale) {
-    const int lane = threadIdx.x & 31;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(q[i], Elem<T>::to_float(k[lane + 32 * i]), s);
-    s = warp_sum(s) * scale;
-    const float top = fmaxf(m, s), keep = m == -INFINITY ? 0.f : expf(m - top), p = top == -INFINITY ? 0.f : expf(s - top);
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * keep + p * Elem<T>::to_float(v[lane + 32 * i]);
-    m = top;
-  }
-  __device__ void end(T *row, float *lse) const {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < N; ++i) row[lane + 32 * i] = Elem<T>::from_float(l == 0.f ? 0.f : o[i] / l);
-    if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : m + logf(l);
+  __device__ bool next(Segment &s) {
+    if (i >= end) return false;
+    const int4 it = items[i++];
+    s.base = it.x;
+    s.len = it.y;
+    s.pos0 = it.z;
+    s.head = it.w;
+    s.q0 = s.base + s.pos0;
+    s.npos = min(2 * positions, s.len - s.pos0);
+    s.first = 0;
+    s.n0 = (s.pos0 + min(positions, s.npos) - 1) / kKeys + 1;
+    s.n1 = s.npos > positions ? (s.pos0 + s.npos - 1) / kKeys + 1 : 0;
+    s.n = max(s.n0, s.n1);
+    s.both = false;
+    s.slot = -1;
+    s.nodes = 0;
+    s.sequence = 0;
+    return true;
   }
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) k_prompt(const int32_t *plan, const __grid_constant__ AttnTensors t) {
-  const uint32_t group = t.q_heads / t.kv_heads, warp = threadIdx.x / 32;
-  const int4 *items = reinterpret_cast<const int4 *>(plan + plan_items_at(plan[0]));
-  for (int32_t i = plan[kPlanHeader + blockIdx.x]; i < plan[kPlanHeader + blockIdx.x + 1]; ++i) {
-    const int4 it = items[i];
-    const uint32_t first = it.x, len = it.y, pos0 = it.z, head = it.w;
-    const uint32_t rows = min(2 * tile_positions(group), len - pos0) * group;
-    for (uint32_t r = warp; r < rows; r += 8) {
-      const uint32_t pos = pos0 + r / group, h = head * group + r % group;
-      const size_t token = static_cast<size_t>(first) + pos;
-      if (token >= t.tokens) continue;
-      Row<T, D> row;
-      row.begin(static_cast<const T *>(t.q) + token * t.q_stride + h * D);
-      for (uint32_t j = 0; j <= pos; ++j) {
-        const size_t at = (static_cast<size_t>(first) + j) * t.kv_stride + head * D;
-        row.key(static_cast<const T *>(t.k) + at, static_cast<const T *>(t.v) + at, t.scale);
-      }
-      row.end(static_cast<T *>(t.out) + token * t.out_stride + h * D,
-              t.lse ? t.lse + token * t.q_heads + h : nullptr);
+__device__ __forceinline__ uint32_t entry_tiles(const TreeEntry &e) { return (e.len + kKeys - 1) / kKeys + 1; }
+__device__ __forceinline__ uint32_t entry_nodes(const TreeEntry &e) { return e.named & 127u; }
+
+// Fills table[0 .. count] (count + 1 entries: the last holds the totals) from the
+// device's lists, every value brought into range; all threads of the block.
+__device__ void tree_table(const TreeArgs &a, uint32_t tokens, uint32_t kv_heads, uint32_t group, TreeEntry *table,
+                           uint32_t *scratch) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const xpu_kv_cache_t &c = a.cache;
+  uint32_t before = 0;
+  bool bad = false;
+  for (uint32_t at = 0; at < a.count; at += blockDim.x) {
+    const uint32_t i = at + threadIdx.x;
+    TreeEntry e{0, 0, 0, 0};
+    uint32_t tiles = 0;
+    if (i < a.count) {
+      const int32_t begin = a.starts[i], end = a.starts[i + 1], s = a.sequences[i];
+      const bool listed = begin >= 0 && end >= begin && static_cast<uint32_t>(end) <= tokens;
+      const bool named = s >= 0 && static_cast<uint32_t>(s) < c.sequences;
+      int32_t len = named ? c.lens[s] : 0;
+      bad |= !listed || !named || len < 0 || static_cast<uint32_t>(len) > c.table_width * c.page_size ||
+             (listed && end - begin > static_cast<int32_t>(XPU_TREE_MAX_NODES));
+      len = min(max(len, 0), static_cast<int32_t>(c.table_width * c.page_size));
+      const uint32_t nodes = listed ? min(static_cast<uint32_t>(end - begin), XPU_TREE_MAX_NODES) : 0;
+      e.len = static_cast<uint32_t>(len);
+      e.begin = listed ? static_cast<uint32_t>(begin) : 0;
+      e.named = (named ? static_cast<uint32_t>(s) : 0) * 128u + nodes;
+      const uint32_t span = 2 * tile_positions(group);
+      tiles = (nodes + span - 1) / span * kv_heads * entry_tiles(e);
     }
+    uint32_t inc = tiles;
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
+      if (lane >= o) inc += up;
+    }
+    __syncthreads();
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    uint32_t others = 0, all = 0;
+    for (uint32_t w = 0; w < warps; ++w) {
+      others += w < warp ? scratch[w] : 0;
+      all += scratch[w];
+    }
+    e.first = before + others + inc - tiles;
+    if (i < a.count) table[i] = e;
+    before += all;
   }
+  if (threadIdx.x == 0) table[a.count] = TreeEntry{before, 0, 0, 0};
+  if (bad && blockIdx.x == 0) atomicOr(c.status, XPU_KV_BAD_INDEX);
+  __syncthreads();
 }
 
+// Key tiles per block: an even share, but at least two.
+__device__ __forceinline__ uint32_t tree_share(uint32_t tiles, uint32_t blocks) {
+  return max((tiles + blocks - 1) / blocks, 2u);
+}
+
+// This block's share of all (sequence, row block, kv head, key tile), in that order.
+struct TreeWalk {
+  const TreeEntry *table;
+  uint32_t count, group, kv_heads, i, at, begin, end;
+  __device__ TreeWalk(const Args &a, const TreeEntry *t, uint32_t g) : table(t), count(a.tree.count), group(g) {
+    kv_heads = a.t.kv_heads;
+    const uint32_t total = table[count].first, share = tree_share(total, gridDim.x);
+    begin = at = min(total, blockIdx.x * share);
+    end = min(total, begin + share);
+    uint32_t lo = 0, hi = count;  // the last entry that starts at or before `at`
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (table[mid].first <= at) lo = mid;
+      else hi = mid;
+    }
+    i = lo;
+  }
+  __device__ bool next(Segment &s) {
+    if (at >= end) return false;
+    while (table[i + 1].first <= at) ++i;
+    const TreeEntry e = table[i];
+    const uint32_t tiles = entry_tiles(e), off = at - e.first, unit = off / tiles, positions = tile_positions(group);
+    s.first = off % tiles;
+    s.n = min(tiles - s.first, end - at);
+    s.head = unit % kv_heads;
+    s.pos0 = unit / kv_heads * 2 * positions;
+    s.nodes = entry_nodes(e);
+    s.npos = min(2 * positions, s.nodes - s.pos0);
+    s.base = e.begin;
+    s.q0 = e.begin + s.pos0;
+    s.len = e.len;
+    s.sequence = static_cast<int32_t>(e.named >> 7);
+    s.both = s.npos <= positions;
+    s.n0 = s.both ? (s.n + 1) / 2 : s.n;
+    s.n1 = s.both ? s.n / 2 : s.n;
+    s.slot = s.n == tiles ? -1 : static_cast<int32_t>(2 * blockIdx.x + (at == begin ? 0 : 1));
+    at += s.n;
+    return true;
+  }
+};
+
+// Key tile `tile` of a segment holds this many keys that some row may attend.
+template <bool TREE>
+__device__ __forceinline__ uint32_t valid_keys(const Segment &s, uint32_t tile) {
+  if (TREE && tile * kKeys >= s.len) return s.nodes;  // the drafts
+  return min(kKeys, s.len - tile * kKeys);
+}
+// ... and some row may not attend some key of it.
+template <bool TREE>
+__device__ __forceinline__ bool masked_tile(const Segment &s, uint32_t tile) {
+  return (TREE ? s.len : s.pos0 + 1) < (tile + 1) * kKeys;
+}
+template <bool TREE>
+__device__ __forceinline__ bool any_masked(const Segment &s) {
+  return masked_tile<TREE>(s, s.first + s.n - 1);
+}
+
+// ---------------------------------------------------------------- fix_row ----
+
+// Adds p v of the segment's listed keys (non-finite values, zeroed in the
+// product) to one row's columns [col, col + cols): dst16 (normalised by inv)
+// or dst32. Rare: plain loops over global memory.
+template <typename T, int D, bool TREE>
+__device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadRows *bad, uint32_t position, uint32_t q_head,
+                                     uint64_t set, float m, float inv, T *dst16, float *dst32, uint32_t col,
+                                     uint32_t cols) {
+  const T *q = static_cast<const T *>(a.t.q) + (s.q0 - s.pos0 + static_cast<size_t>(position)) * a.t.q_stride + q_head * D;
+  const float c = a.t.scale * kLog2e;
+  for (uint32_t w = 0; w < 2; ++w)
+    for (uint32_t i = 0; i < bad[w].tiles; ++i)
+      for (uint32_t b = 0; b < 64; ++b) {
+        if (!(bad[w].mask[i][b >> 5] >> (b & 31) & 1u)) continue;
+        const uint32_t in_tile = w * 64 + b, key = bad[w].tile[i] * kKeys + in_tile;
+        const T *k, *v;
+        if (!TREE || bad[w].tile[i] * kKeys >= s.len) {  // packed: a prompt's key, or a draft
+          if (TREE ? !(set >> in_tile & 1u) : key > position) continue;
+          const size_t at = (static_cast<size_t>(s.base) + (TREE ? in_tile : key)) * a.t.kv_stride + s.head * D;
+          k = static_cast<const T *>(a.t.k) + at;
+          v = static_cast<const T *>(a.t.v) + at;
+        } else {
+          const xpu_kv_cache_t &kc = a.tree.cache;
+          const int32_t page = kc.tables[static_cast<size_t>(s.sequence) * kc.table_width + key / kc.page_size];
+          if (page < 0 || static_cast<uint32_t>(page) >= kc.pages) continue;
+          const size_t at = (((static_cast<size_t>(a.tree.layer) * kc.pages + page) * kc.kv_heads + s.head) * kc.page_size +
+                             key % kc.page_size) * D;
+          k = static_cast<const T *>(kc.k) + at;
+          v = static_cast<const T *>(kc.v) + at;
+        }
+        float dot = 0.f;
+        for (uint32_t d = 0; d < D; ++d) dot = fmaf(Elem<T>::to_float(q[d]), Elem<T>::to_float(k[d]), dot);
+        const float p = exp2f(fmaf(dot, c, -(m == -INFINITY ? 0.f : m * c)));
+        for (uint32_t d = col; d < col + cols; ++d) {
+          if (dst32) dst32[d] = fmaf(p, Elem<T>::to_float(v[d]), dst32[d]);
+          else dst16[d] = Elem<T>::from_float(fmaf(p * inv, Elem<T>::to_float(v[d]), Elem<T>::to_float(dst16[d])));
+        }
+      }
+}
+
+// ----------------------------------------------------------------- kernel ----
+
+template <typename T, int D, bool TREE>
+__global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant__ Args a) {
+  using S = Shape<D, TREE>;
+  using Walk = typename std::conditional<TREE, TreeWalk, PromptWalk>::type;
+  constexpr bool kFp16 = std::is_same<T, __half>::value;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ Barriers b;
+  __shared__ TreeEntry table[TREE ? XPU_KV_MAX_REQUESTS + 1 : 1];
+  __shared__ float joined[TREE ? 2 : 1][TREE ? 128 : 1][2];
+  __shared__ uint32_t scratch[kThreads / 32];
+  const uint32_t a0 = smem_addr(smem_raw);
+  uint8_t *q_smem = smem_raw + ((a0 + 1023u) / 1024u * 1024u - a0), *ring = q_smem + 2 * S::kTile;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t group = a.t.q_heads / a.t.kv_heads, positions = tile_positions(group);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&b.q_full, 1);
+    mbar_init(&b.q_empty, 1);
+    mbar_init(&b.drain, 1);
+    for (uint32_t i = 0; i < S::kStages; ++i) {
+      mbar_init(&b.kv_full[i], 1);
+      mbar_init(&b.kv_empty[i], 3);  // the products and both cleaning warps
+      mbar_init(&b.clean[i], 2);
+    }
+    for (uint32_t i = 0; i < 2; ++i) {
+      mbar_init(&b.s_full[i], 1);
+      mbar_init(&b.p_ready[i], 4);
+      mbar_init(&b.o_full[i], 1);
+    }
+    mbar_init(&b.joined, 8);
+    fence_mbar_init();
+    b.failed = 0;
+  }
+  if (warp == kMmaWarp) tmem_alloc1(&b.tmem, 512);
+  if (TREE) tree_table(a.tree, a.t.tokens, a.t.kv_heads, group, table, scratch);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = b.tmem;
+  auto walk = [&] {
+    if constexpr (TREE) return Walk(a, table, group);
+    else return Walk(a, group);
+  }();
+  Segment s;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax ----
+    const uint32_t t = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = (warp & 3) * 32u << 16;
+    const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + 256;  // O_t at + 128 t
+    const float c = a.t.scale * kLog2e;
+    const uint32_t in_tile = r / group, q_head_in_group = r % group;
+    uint32_t uses = 0, done = 0, segment = 0, joins = 0;
+    // every softmax warp, bounded like every wait
+    auto meet = [&] {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b.joined);
+      const bool ok = warp_wait(b, &b.joined, joins++ & 1);
+      tc_fence_after();
+      return ok;
+    };
+    for (; walk.next(s) && !warp_failed(b); ++segment) {
+      const uint32_t index = (s.both ? 0 : t * positions) + in_tile;  // position inside the segment
+      const bool mine = r < positions * group && index < s.npos;
+      const uint32_t position = s.pos0 + min(index, s.npos - 1);
+      const uint64_t set = TREE ? a.tree.ancestors[s.base + position] : 0;
+      const uint32_t tiles = t ? s.n1 : s.n0;
+      float m = -INFINITY, l = 0.f;
+      for (uint32_t i = 0; i < tiles; ++i, ++uses) {
+        const uint32_t tile = s.first + (s.both ? 2 * i + t : i);
+        if (!warp_wait(b, &b.s_full[t], uses & 1)) break;
+        tc_fence_after();
+        uint32_t x[kKeys];
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q) tmem_ld32(s_addr + 32 * q, x + 32 * q);
+        tmem_wait_ld();
+        if (masked_tile<TREE>(s, tile)) {
+          if (TREE && tile * kKeys >= s.len) {
+            const uint32_t nodes_lo = s.nodes >= 32 ? 0xffffffffu : (1u << s.nodes) - 1u;
+            const uint32_t nodes_hi = s.nodes >= 64 ? 0xffffffffu : (s.nodes > 32 ? (1u << (s.nodes - 32)) - 1u : 0u);
+            const uint32_t lo = static_cast<uint32_t>(set) & nodes_lo, hi = static_cast<uint32_t>(set >> 32) & nodes_hi;
+#pragma unroll
+            for (uint32_t j = 0; j < kKeys; ++j)
+              if (j >= 64 || !((j < 32 ? lo >> j : hi >> (j - 32)) & 1u)) x[j] = 0xff800000u;
+          } else {
+            const uint32_t many = (TREE ? s.len : position + 1) - min(tile * kKeys, TREE ? s.len : position + 1);
+#pragma unroll
+            for (uint32_t j = 0; j < kKeys; ++j)
+              if (j >= many) x[j] = 0xff800000u;
+          }
+        }
+        float top = m;
+#pragma unroll
+        for (uint32_t j = 0; j < kKeys; j += 2) top = fmaxf(top, fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+        const bool grown = (top - m) * c > kRescale;  // m = -inf included
+        if (__any_sync(kFullMask, grown)) {
+          const float keep = grown ? exp2_approx((m - top) * c) : 1.f;
+          if (grown) m = top;
+          l *= keep;
+          if (i > 0) {
+#pragma unroll 1
+            for (uint32_t q = 0; q < D / 32; ++q) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + t * 128 + 32 * q, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+              tmem_st32(o_addr + t * 128 + 32 * q, o);
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.f : -m * c;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q) {
+          uint32_t p[16];
+#pragma unroll
+          for (uint32_t j = 0; j < 16; ++j) {
+            const float lo = exp2_approx(fmaf(__uint_as_float(x[32 * q + 2 * j]), c, mc));
+            const float hi = exp2_approx(fmaf(__uint_as_float(x[32 * q + 2 * j + 1]), c, mc));
+            sum[(2 * j) & 3] += lo;
+            sum[(2 * j + 1) & 3] += hi;
+            p[j] = pack2<T>(lo, hi);
+          }
+          tmem_st16(s_addr + 16 * q, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b.p_ready[t]);
+      }
+      if (warp_failed(b)) break;
+      if (tiles) {
+        if (!warp_wait(b, &b.o_full[t], done & 1)) break;
+        ++done;
+        tc_fence_after();
+      }
+      // ---------------------------------------------------- join and write ----
+      float weight[2] = {t == 0 ? 1.f : 0.f, t == 0 ? 0.f : 1.f};
+      uint32_t col = 0, cols = D;
+      if (TREE && s.both) {
+        joined[t][r][0] = m;
+        joined[t][r][1] = l;
+        if (!meet()) break;
+        const float m0 = joined[0][r][0], m1 = joined[1][r][0];
+        m = fmaxf(m0, m1);
+        weight[0] = m0 == -INFINITY ? 0.f : exp2_approx((m0 - m) * c);
+        weight[1] = m1 == -INFINITY ? 0.f : exp2_approx((m1 - m) * c);
+        l = weight[0] * joined[0][r][1] + weight[1] * joined[1][r][1];
+        col = t * (D / 2);
+        cols = D / 2;
+      }
+      if (tiles || s.both) {
+        const bool whole = s.slot < 0;
+        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        const size_t token = s.q0 - s.pos0 + static_cast<size_t>(position);
+        const uint32_t q_head = s.head * group + q_head_in_group;
+        T *dst16 = static_cast<T *>(a.t.out) + token * a.t.out_stride + q_head * D;
+        float *dst32 = nullptr;
+        if (TREE && !whole) {
+          const size_t row = static_cast<size_t>(s.slot) * 256 + (s.both ? 0 : t * 128) + r;
+          dst32 = a.tree.partial + row * D;
+          if (mine && col == 0) {
+            float *ml = a.tree.partial + 2ull * gridDim.x * 256 * D + row * 2;
+            ml[0] = m;
+            ml[1] = l;
+          }
+        } else if (mine && a.t.lse && col == 0 && token < a.t.tokens) {
+          a.t.lse[token * a.t.q_heads + q_head] = l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * kLn2;
+        }
+        const bool store = mine && token < a.t.tokens;
+#pragma unroll 1
+        for (uint32_t q = col; q < col + cols; q += 32) {
+          uint32_t o[32];
+          if (!TREE || !s.both) {
+            tmem_ld32(o_addr + t * 128 + q, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
+          } else {
+            tmem_ld32(o_addr + q, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * weight[0]);
+            if (s.n1) {
+              uint32_t o1[32];
+              tmem_ld32(o_addr + 128 + q, o1);
+              tmem_wait_ld();
+#pragma unroll
+              for (uint32_t j = 0; j < 32; ++j)
+                o[j] = __float_as_uint(fmaf(__uint_as_float(o1[j]), weight[1], __uint_as_float(o[j])));
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
+          }
+          if (!store) continue;
+          if (TREE && dst32) {
+#pragma unroll
+            for (uint32_t j = 0; j < 32; j += 4)
+              *reinterpret_cast<uint4 *>(dst32 + q + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 32; j += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (uint32_t e = 0; e < 4; ++e)
+                w[e] = pack2<T>(__uint_as_float(o[j + 2 * e]), __uint_as_float(o[j + 2 * e + 1]));
+              *reinterpret_cast<uint4 *>(dst16 + q + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (store && any_masked<TREE>(s)) {
+          const BadRows *bad = b.bad[segment % kBadRing];
+          if (*const_cast<const volatile uint32_t *>(&bad[0].tiles) | *const_cast<const volatile uint32_t *>(&bad[1].tiles))
+            fix_row<T, D, TREE>(a, s, bad, position, q_head, set, m, inv, dst16, dst32, col, cols);
+        }
+      }
+      // the other group may still read this one's accumulator and sums
+      if (TREE && s.both && !meet()) break;
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- MMA ----
+    if (lane == 0) {
+      constexpr uint32_t qk_desc = attn_idesc(kFp16, kKeys, true), pv_desc = attn_idesc(kFp16, D, false);
+      const uint32_t ring_addr = smem_addr(ring), q_addr = smem_addr(q_smem);
+      uint32_t loaded = 0, segment = 0, cleaned = 0;  // ring position, segments, phase of each slot's clean barrier
+      uint32_t p_uses[2] = {0, 0};
+      auto wait_kv = [&](uint32_t i) {
+        if (mbar_wait(&b.kv_full[i % S::kStages], i / S::kStages & 1)) return true;
+        b.failed = 1;
+        return false;
+      };
+      auto qk = [&](uint32_t t, uint32_t i) {
+        const uint32_t sq = q_addr + (s.both ? 0 : t) * S::kTile, sk = ring_addr + i % S::kStages * S::kTile;
+        const uint64_t dq = smem_desc(sq, 16, 1024), dk = smem_desc(sk, 16, 1024);
+#pragma unroll
+        for (uint32_t kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk / 4 * kBox + kk % 4 * 32) >> 4;
+          mma1_f16(tmem + t * 128, dq + off, dk + off, qk_desc, kk != 0);
+        }
+        mma1_commit(&b.s_full[t]);
+      };
+      for (; walk.next(s) && !failed(b); ++segment) {
+        const uint32_t k0 = loaded;  // K tile j is ring entry k0 + 2 j, V tile j the next
+        loaded += 2 * s.n;
+        if (!mbar_wait(&b.q_full, segment & 1) || !wait_kv(k0)) { b.failed = 1; break; }
+        tc_fence_after();
+        if (s.both) {
+          qk(0, k0);
+          mma1_commit(&b.kv_empty[k0 % S::kStages]);
+          if (s.n > 1) {
+            if (!wait_kv(k0 + 2)) break;
+            tc_fence_after();
+            qk(1, k0 + 2);
+            mma1_commit(&b.kv_empty[(k0 + 2) % S::kStages]);
+          }
+        } else {
+          qk(0, k0);
+          if (s.n1) qk(1, k0);
+          mma1_commit(&b.kv_empty[k0 % S::kStages]);
+        }
+        const uint32_t ahead = s.both ? 2 : 1;
+        if (s.n <= ahead) mma1_commit(&b.q_empty);
+        for (uint32_t j = 0; j < s.n; ++j) {
+          const uint32_t v = k0 + 2 * j + 1, slot = v % S::kStages;
+          if (!wait_kv(v)) break;
+          if (masked_tile<TREE>(s, s.first + j)) {
+            if (!mbar_wait(&b.clean[slot], cleaned >> slot & 1)) { b.failed = 1; break; }
+            cleaned ^= 1u << slot;
+          }
+          const uint64_t dv = smem_desc(ring_addr + slot * S::kTile, kBox, 1024);
+          bool next_loaded = false;
+#pragma unroll
+          for (uint32_t t = 0; t < 2; ++t) {
+            if (s.both && t != (j & 1)) continue;
+            const uint32_t tiles = t ? s.n1 : s.n0, i = s.both ? j / 2 : j;
+            if (i < tiles) {
+              if (!mbar_wait(&b.p_ready[t], p_uses[t]++ & 1)) { b.failed = 1; break; }
+              tc_fence_after();
+#pragma unroll
+              for (uint32_t kk = 0; kk < kKeys / 16; ++kk)
+                mma1_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, dv + (kk * 2048u >> 4), pv_desc, (i | kk) != 0);
+              if (i + 1 == tiles) mma1_commit(&b.o_full[t]);
+            }
+            if (i + 1 < tiles) {
+              if (!next_loaded && !wait_kv(k0 + 2 * (j + ahead))) break;
+              next_loaded = true;
+              tc_fence_after();
+              qk(t, k0 + 2 * (j + ahead));
+            }
+          }
+          if (failed(b)) break;
+          mma1_commit(&b.kv_empty[slot]);
+          if (j + ahead < s.n) {
+            mma1_commit(&b.kv_empty[(k0 + 2 * (j + ahead)) % S::kStages]);
+            if (j + ahead + 1 == s.n) mma1_commit(&b.q_empty);
+          }
+        }
+      }
+      if (failed(b)) {  // nothing issued may still run when TMEM is freed
+        mma1_commit(&b.drain);
+        mbar_wait(&b.drain, 0);
+      }
+    }
+  } else if (warp == kLoadWarp) {
+    // --------------------------------------------------------------- loads ----
+    uint32_t loaded = 0, segment = 0, q_loads = 0;
+    auto tile_dst = [&](uint32_t i) { return ring + i % S::kStages * S::kTile; };
+    for (; walk.next(s) && !warp_failed(b); ++segment) {
+      bool ok = true;
+      for (uint32_t j = 0; j < s.n && ok; ++j) {
+        const uint32_t tile = s.first + j, at = tile * kKeys;
+        const bool packed = !TREE || at >= s.len;
+        int32_t page = 0;
+        uint32_t pages = 0;
+        if (TREE && !packed) {  // lane p fetches the tile's page p
+          const xpu_kv_cache_t &kc = a.tree.cache;
+          pages = (min(kKeys, s.len - at) + kc.page_size - 1) / kc.page_size;
+          if (lane < pages) {
+            page = kc.tables[static_cast<size_t>(s.sequence) * kc.table_width + at / kc.page_size + lane];
+            if (page < 0 || static_cast<uint32_t>(page) >= kc.pages) {
+              atomicOr(kc.status, XPU_KV_BAD_INDEX);
+              page = static_cast<int32_t>(kc.pages);  // behind the pool: reads as zeros
+            }
+          }
+        }
+        for (uint32_t which = 0; which < 2; ++which) {
+          const uint32_t slot = loaded % S::kStages, use = loaded / S::kStages;
+          if (use > 0 && !warp_wait(b, &b.kv_empty[slot], (use - 1) & 1)) { ok = false; break; }
+          uint64_t *bar = &b.kv_full[slot];
+          uint8_t *dst = tile_dst(loaded++);
+          if (packed) {
+            if (lane == 0) {
+              // a tree's drafts: half a tile, XPU_TREE_MAX_NODES rows
+              mbar_expect_tx(bar, TREE ? S::kTile / 2 : S::kTile);
+              for (uint32_t h = 0; h < S::kBoxes; ++h)
+                tma_load_3d(dst + h * kBox, which ? &a.v : &a.k, 64 * h, s.head, s.base + (TREE ? 0 : at), bar);
+            }
+          } else {
+            const xpu_kv_cache_t &kc = a.tree.cache;
+            const uint32_t bytes = kc.page_size * 128;
+            if (lane == 0) mbar_expect_tx(bar, pages * bytes * S::kBoxes);
+            __syncwarp();
+            if (lane < pages) {
+              const int32_t row = static_cast<int32_t>((static_cast<uint32_t>(page) * kc.kv_heads + s.head) * kc.page_size);
+              for (uint32_t h = 0; h < S::kBoxes; ++h)
+                tma_load_2d_plain(dst + h * kBox + lane * bytes, which ? &a.cached_v : &a.cached_k, 64 * h, row, bar);
+            }
+          }
+          if (j == 0 && which == 0) {  // after the first keys, which need not wait for the last segment's rows
+            if (segment > 0 && !warp_wait(b, &b.q_empty, (segment - 1) & 1)) { ok = false; break; }
+            if (lane == 0) {
+              const uint32_t tiles = !s.both && s.npos > positions ? 2 : 1;
+              mbar_expect_tx(&b.q_full, tiles * positions * group * 128 * S::kBoxes);
+              for (uint32_t t = 0; t < tiles; ++t)
+                for (uint32_t h = 0; h < S::kBoxes; ++h)
+                  tma_load_3d(q_smem + t * S::kTile + h * kBox, &a.q, 64 * h, s.head * group, s.q0 + t * positions, &b.q_full);
+            }
+            ++q_loads;
+          }
+        }
+      }
+      if (!ok) break;
+    }
+    if (warp_failed(b)) {  // what was asked for lands before the block's memory is given up
+      for (uint32_t i = loaded > S::kStages ? loaded - S::kStages : 0; i < loaded; ++i)
+        mbar_wait(&b.kv_full[i % S::kStages], i / S::kStages & 1);
+      if (q_loads) mbar_wait(&b.q_full, (q_loads - 1) & 1);
+    }
+  } else {
+    // ------------------------------------------------------------ cleaning ----
+    const uint32_t half = warp - kCleanWarp;  // keys 64 half .. + 63 of a tile
+    uint32_t loaded = 0, segment = 0;
+    for (; walk.next(s) && !warp_failed(b); ++segment) {
+      BadRows *bad = &b.bad[segment % kBadRing][half];
+      uint32_t listed = 0;
+      if (lane == 0 && any_masked<TREE>(s)) bad->tiles = 0;
+      for (uint32_t e = 0; e < 2 * s.n; ++e) {  // every ring entry, so as never to be a turn ahead or behind
+        const uint32_t i = loaded + e, slot = i % S::kStages, tile = s.first + e / 2;
+        if (!warp_wait(b, &b.kv_full[slot], i / S::kStages & 1)) break;
+        if (e % 2 == 0 || !masked_tile<TREE>(s, tile)) {
+          if (lane == 0) mbar_arrive(&b.kv_empty[slot]);
+          continue;
+        }
+        const uint32_t valid = valid_keys<TREE>(s, tile);
+        uint32_t found[2];
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) {
+          const uint32_t key = half * 64 + e * 32 + lane;
+          uint8_t *row = ring + slot * S::kTile + key * 128;
+          bool spoilt = false;
+          if (key < valid) {
+#pragma unroll
+            for (uint32_t x = 0; x < 8 * S::kBoxes; ++x) {  // 16-byte pieces, each lane from another bank
+              const uint4 w = *reinterpret_cast<const uint4 *>(row + x / 8 * kBox + ((x + lane) & 7) * 16);
+              spoilt |= word_not_finite<T>(w.x) || word_not_finite<T>(w.y) || word_not_finite<T>(w.z) || word_not_finite<T>(w.w);
+            }
+          }
+          if (key >= valid || spoilt) {
+#pragma unroll
+            for (uint32_t x = 0; x < 8 * S::kBoxes; ++x)
+              *reinterpret_cast<uint4 *>(row + x / 8 * kBox + ((x + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          found[e] = __ballot_sync(kFullMask, spoilt);
+        }
+        if ((found[0] | found[1]) && lane == 0 && listed < 2) {
+          bad->tile[listed] = tile;
+          bad->mask[listed][0] = found[0];
+          bad->mask[listed][1] = found[1];
+          bad->tiles = ++listed;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&b.clean[slot]);
+          mbar_arrive(&b.kv_empty[slot]);
+        }
+      }
+      loaded += 2 * s.n;
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && b.failed) atomicOr(&g_attention_error, kErrAttentionTimeout);
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc1(tmem, 512);
+  }
+  if (TREE) grid_dep_launch();
+}
+
+// Joins the partial results of units that several blocks worked on: one warp
+// per (node, query head); the blocks' order is the order of the sum.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_tree(const __grid_constant__ xpu_kv_cache_t c, uint32_t layer,
-                                              const int32_t *sequences, const int32_t *starts,
-                                              const uint64_t *ancestors, uint32_t count,
-                                              const __grid_constant__ AttnTensors t) {
-  const uint32_t group = t.q_heads / t.kv_heads;
+__global__ void __launch_bounds__(256) k_tree_join(const __grid_constant__ Args a, uint32_t blocks) {
+  __shared__ TreeEntry table[XPU_KV_MAX_REQUESTS + 1];
+  __shared__ uint32_t scratch[8];
+  const uint32_t group = a.t.q_heads / a.t.kv_heads, positions = tile_positions(group), lane = threadIdx.x & 31;
+  grid_dep_wait();
+  tree_table(a.tree, a.t.tokens, a.t.kv_heads, group, table, scratch);
   const uint64_t w = blockIdx.x * 8ull + threadIdx.x / 32;
-  if (w >= static_cast<uint64_t>(t.tokens) * t.q_heads) return;
-  const uint32_t node = static_cast<uint32_t>(w / t.q_heads), h = static_cast<uint32_t>(w % t.q_heads), head = h / group;
-  uint32_t lo = 0, hi = count;
+  if (w >= static_cast<uint64_t>(a.t.tokens) * a.t.q_heads) return;
+  const uint32_t node = static_cast<uint32_t>(w / a.t.q_heads), q_head = static_cast<uint32_t>(w % a.t.q_heads);
+  uint32_t lo = 0, hi = a.tree.count;
   while (hi - lo > 1) {
     const uint32_t mid = (lo + hi) / 2;
-    if (starts[mid] <= static_cast<int32_t>(node)) lo = mid;
+    if (a.tree.starts[mid] <= static_cast<int32_t>(node)) lo = mid;
     else hi = mid;
   }
-  const int32_t begin = starts[lo], end = starts[lo + 1], s = sequences[lo];
-  const int32_t nodes = end - begin;
-  if (static_cast<int32_t>(node) < begin || static_cast<int32_t>(node) >= end) return;
-  uint32_t len = 0;
-  bool bad = s < 0 || static_cast<uint32_t>(s) >= c.sequences || nodes > static_cast<int32_t>(XPU_TREE_MAX_NODES);
-  if (!bad) {
-    const int32_t n = c.lens[s];
-    bad = n < 0 || static_cast<uint32_t>(n) > c.table_width * c.page_size;
-    len = bad ? 0 : n;
+  const TreeEntry e = table[lo];
+  const uint32_t index = node - e.begin;
+  if (node < e.begin || index >= entry_nodes(e)) return;
+  const uint32_t tiles = entry_tiles(e), block = index / (2 * positions), in_block = index % (2 * positions);
+  const uint32_t share = tree_share(table[a.tree.count].first, blocks);
+  const uint32_t g0 = e.first + (block * a.t.kv_heads + q_head / group) * tiles;
+  const uint32_t c0 = g0 / share, c1 = (g0 + tiles - 1) / share;
+  if (c0 == c1) return;
+  const uint32_t row = (in_block / positions) * 128 + in_block % positions * group + q_head % group;
+  const float *sums = a.tree.partial + 2ull * blocks * 256 * D, c = a.t.scale * kLog2e;
+  auto row_of = [&](uint32_t x) { return (2ull * x + (x * share >= g0 ? 0 : 1)) * 256 + row; };
+  float m = -INFINITY;
+  for (uint32_t x = c0 + lane; x <= c1; x += 32) m = fmaxf(m, sums[row_of(x) * 2]);
+  m = warp_max(m);
+  float l = 0.f, o[D / 32];
+#pragma unroll
+  for (uint32_t i = 0; i < D / 32; ++i) o[i] = 0.f;
+  for (uint32_t x = c0; x <= c1; ++x) {
+    const size_t at = row_of(x);
+    const float mx = sums[at * 2], wx = mx == -INFINITY ? 0.f : exp2f((mx - m) * c);
+    l = fmaf(wx, sums[at * 2 + 1], l);
+#pragma unroll
+    for (uint32_t i = 0; i < D / 32; ++i) o[i] = fmaf(wx, a.tree.partial[at * D + lane + 32 * i], o[i]);
   }
-  Row<T, D> row;
-  row.begin(static_cast<const T *>(t.q) + node * t.q_stride + h * D);
-  for (uint32_t j = 0; j < len; ++j) {
-    const int32_t page = c.tables[static_cast<size_t>(s) * c.table_width + j / c.page_size];
-    if (page < 0 || static_cast<uint32_t>(page) >= c.pages) {
-      bad = true;
-      continue;
-    }
-    const size_t at = (((static_cast<size_t>(layer) * c.pages + page) * c.kv_heads + head) * c.page_size + j % c.page_size) * D;
-    row.key(static_cast<const T *>(c.k) + at, static_cast<const T *>(c.v) + at, t.scale);
+  T *dst = static_cast<T *>(a.t.out) + static_cast<size_t>(node) * a.t.out_stride + q_head * D;
+#pragma unroll
+  for (uint32_t i = 0; i < D / 32; ++i) dst[lane + 32 * i] = Elem<T>::from_float(l == 0.f ? 0.f : o[i] / l);
+  if (a.t.lse && lane == 0)
+    a.t.lse[static_cast<size_t>(node) * a.t.q_heads + q_head] = l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * kLn2;
+}
+
+// ------------------------------------------------------------------- host ----
+
+cudaError_t packed_map(CUtensorMap *map, const void *base, const AttnTensors &t, uint32_t heads, uint64_t stride,
+                       uint32_t box_heads, uint32_t box_rows) {
+  return make_tmap_3d_u16_box(map, base, t.head_dim, heads, t.tokens, t.head_dim, stride, 64, box_heads, box_rows);
+}
+
+cudaError_t packed_maps(Args &a, uint32_t kv_rows) {
+  const AttnTensors &t = a.t;
+  const uint32_t group = t.q_heads / t.kv_heads;
+  cudaError_t e = packed_map(&a.q, t.q, t, t.q_heads, t.q_stride, group, tile_positions(group));
+  if (e == cudaSuccess) e = packed_map(&a.k, t.k, t, t.kv_heads, t.kv_stride, 1, kv_rows);
+  if (e == cudaSuccess) e = packed_map(&a.v, t.v, t, t.kv_heads, t.kv_stride, 1, kv_rows);
+  return e;
+}
+
+template <typename T, int D, bool TREE>
+cudaError_t launch(const Args &a, uint32_t blocks, cudaStream_t s) {
+  constexpr uint32_t smem = Shape<D, TREE>::kSmem;
+  cudaError_t e = cudaFuncSetAttribute(k_attention<T, D, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  k_attention<T, D, TREE><<<blocks, kThreads, smem, s>>>(a);
+  e = cudaGetLastError();
+  if (!TREE || e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<uint32_t>((static_cast<uint64_t>(a.t.tokens) * a.t.q_heads + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_tree_join<T, D>, a, blocks);
+}
+
+template <bool TREE>
+cudaError_t launch_any(bool fp16, const Args &a, uint32_t blocks, cudaStream_t s) {
+  if (a.t.head_dim == 128)
+    return fp16 ? launch<__half, 128, TREE>(a, blocks, s) : launch<__nv_bfloat16, 128, TREE>(a, blocks, s);
+  return fp16 ? launch<__half, 64, TREE>(a, blocks, s) : launch<__nv_bfloat16, 64, TREE>(a, blocks, s);
+}
+
+uint32_t sm_count() {
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
   }
-  const uint64_t set = ancestors[node];
-  for (int32_t j = 0; j < min(nodes, static_cast<int32_t>(XPU_TREE_MAX_NODES)); ++j) {
-    if (!(set >> j & 1u)) continue;
-    const size_t at = static_cast<size_t>(begin + j) * t.kv_stride + head * D;
-    row.key(static_cast<const T *>(t.k) + at, static_cast<const T *>(t.v) + at, t.scale);
-  }
-  row.end(static_cast<T *>(t.out) + node * t.out_stride + h * D,
-          t.lse ? t.lse + static_cast<size_t>(node) * t.q_heads + h : nullptr);
-  if (bad && (threadIdx.x & 31) == 0) atomicOr(c.status, XPU_KV_BAD_INDEX);
+  return static_cast<uint32_t>(sms);
 }
 
 }  // namespace
+
+unsigned take_attention_error() {
+  unsigned v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attention_error, sizeof(v)) != cudaSuccess) return 0;
+  if (v) cudaMemcpyToSymbol(g_attention_error, &zero, sizeof(zero));
+  return v;
+}
 
 size_t prompt_plan(const uint32_t *lens, uint32_t count, uint32_t q_heads, uint32_t kv_heads, uint32_t sms, int32_t *plan,
                    size_t capacity) {
@@ -173,22 +995,35 @@ size_t prompt_plan(const uint32_t *lens, uint32_t count, uint32_t q_heads, uint3
 
 cudaError_t prompt_attention_launch(bool fp16, const int32_t *plan, uint32_t blocks, const AttnTensors &t,
                                     cudaStream_t s) {
-  auto kernel = fp16 ? (t.head_dim == 128 ? k_prompt<__half, 128> : k_prompt<__half, 64>)
-                     : (t.head_dim == 128 ? k_prompt<__nv_bfloat16, 128> : k_prompt<__nv_bfloat16, 64>);
-  kernel<<<blocks, 256, 0, s>>>(plan, t);
-  return cudaGetLastError();
+  Args a = {};
+  a.t = t;
+  a.plan = plan;
+  const cudaError_t e = packed_maps(a, kKeys);
+  return e != cudaSuccess ? e : launch_any<false>(fp16, a, blocks, s);
 }
 
-size_t tree_workspace_bytes(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) { return 16; }
+size_t tree_workspace_bytes(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t head_dim) {
+  // two partial results a block: 256 rows of outputs, and their maxima and sums
+  return 2ull * sm_count() * 256 * (head_dim + 2) * 4;
+}
 
 cudaError_t tree_attention_launch(const xpu_kv_cache_t &c, uint32_t layer, const int32_t *sequences,
                                   const int32_t *starts, const uint64_t *ancestors, uint32_t count,
-                                  const AttnTensors &t, void *, cudaStream_t s) {
-  auto kernel = c.dtype == XPU_FP16 ? (t.head_dim == 128 ? k_tree<__half, 128> : k_tree<__half, 64>)
-                                    : (t.head_dim == 128 ? k_tree<__nv_bfloat16, 128> : k_tree<__nv_bfloat16, 64>);
-  const uint64_t warps = static_cast<uint64_t>(t.tokens) * t.q_heads;
-  kernel<<<static_cast<uint32_t>((warps + 7) / 8), 256, 0, s>>>(c, layer, sequences, starts, ancestors, count, t);
-  return cudaGetLastError();
+                                  const AttnTensors &t, void *workspace, cudaStream_t s) {
+  Args a = {};
+  a.t = t;
+  a.tree = {c, sequences, starts, ancestors, layer, count, static_cast<float *>(workspace)};
+  cudaError_t e = packed_maps(a, XPU_TREE_MAX_NODES);
+  if (e != cudaSuccess) return e;
+  const uint64_t rows = static_cast<uint64_t>(c.pages) * c.kv_heads * c.page_size;
+  const size_t offset = static_cast<size_t>(layer) * rows * c.head_dim;
+  e = make_tmap_2d_u16_swizzled(&a.cached_k, static_cast<const uint16_t *>(c.k) + offset, c.head_dim, rows, c.head_dim, 64,
+                                c.page_size);
+  if (e != cudaSuccess) return e;
+  e = make_tmap_2d_u16_swizzled(&a.cached_v, static_cast<const uint16_t *>(c.v) + offset, c.head_dim, rows, c.head_dim, 64,
+                                c.page_size);
+  if (e != cudaSuccess) return e;
+  return launch_any<true>(c.dtype == XPU_FP16, a, sm_count(), s);
 }
 
 }  // namespace xpu

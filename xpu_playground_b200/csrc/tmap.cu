@@ -71,14 +71,20 @@ cudaError_t make_tmap_2d_u16_swizzled(CUtensorMap *map, const void *base, uint64
 // reads zeros past it, not the next chunk's columns.
 cudaError_t make_tmap_3d_u16_swizzled(CUtensorMap *map, const void *base, uint64_t d0, uint64_t d1, uint64_t d2,
                                       uint64_t stride1, uint64_t stride2, uint32_t box_cols, uint32_t box_rows) {
+  return make_tmap_3d_u16_box(map, base, d0, d1, d2, stride1, stride2, box_cols, 1, box_rows);
+}
+
+// The same view with boxes of box2 x box1 x box_cols.
+cudaError_t make_tmap_3d_u16_box(CUtensorMap *map, const void *base, uint64_t d0, uint64_t d1, uint64_t d2,
+                                 uint64_t stride1, uint64_t stride2, uint32_t box_cols, uint32_t box1, uint32_t box2) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return cudaErrorNotSupported;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) || (stride1 * 2) % 16 || (stride2 * 2) % 16 || box_cols * 2 > 128 ||
-      (box_cols * 2) % 16 || box_rows > 256)
+      (box_cols * 2) % 16 || box1 > 256 || box2 > 256)
     return cudaErrorInvalidValue;
   const cuuint64_t dims[3] = {d0, d1, d2};
   const cuuint64_t strides[2] = {stride1 * 2, stride2 * 2};
-  const cuuint32_t box[3] = {box_cols, 1, box_rows};
+  const cuuint32_t box[3] = {box_cols, box1, box2};
   const cuuint32_t estride[3] = {1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(base), dims, strides, box, estride,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -34,6 +34,8 @@ cudaError_t make_tmap_2d_u16_swizzled(struct CUtensorMap_st *map, const void *ba
 cudaError_t make_tmap_3d_u16_swizzled(struct CUtensorMap_st *map, const void *base, uint64_t d0, uint64_t d1,
                                       uint64_t d2, uint64_t stride1, uint64_t stride2, uint32_t box_cols,
                                       uint32_t box_rows);
+cudaError_t make_tmap_3d_u16_box(struct CUtensorMap_st *map, const void *base, uint64_t d0, uint64_t d1, uint64_t d2,
+                                 uint64_t stride1, uint64_t stride2, uint32_t box_cols, uint32_t box1, uint32_t box2);
 
 // ---- GEMM (gemm.cu) ----
 cudaError_t gemm_launch(bool fp16, const void *A, const void *B, void *C, uint32_t m, uint32_t n, uint32_t k,
@@ -53,6 +55,8 @@ cudaError_t gemm_chunks_launch(const void *A, const void *W, float *C, uint32_t 
 unsigned take_device_error();
 // Same for the calibrator kernels (peak.cu; bit 1: a pipeline wait timed out).
 unsigned take_peak_error();
+// And for the serving attention (serving_attention.cu; bit 2).
+unsigned take_attention_error();
 
 // ---- dense prefill (prefill.cu): bf16 [M][width] row-major activations ----
 cudaError_t prefill_embed(const uint16_t *embed, const uint32_t *tokens, uint16_t *x, uint32_t M, uint32_t H,
