@@ -22,7 +22,7 @@
 //             the P_t that the product before it read. While one tile is in its
 //             softmax the tensor cores work for the other;
 //   9         TMA loads: Q tiles, and a ring of K and V tiles;
-//   10        cleaning: in key tiles with masked keys, V rows that no row may
+//   10, 11    cleaning: in key tiles with masked keys, V rows that no row may
 //             attend are zeroed (0 x NaN would reach the sums), and rows with
 //             non-finite values are zeroed and listed; the rows that do attend
 //             them get p v added at the end (fix_row).
@@ -57,8 +57,7 @@ constexpr uint32_t kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10;
 constexpr unsigned kErrAttentionTimeout = 4u;
 constexpr float kRescale = 8.f;        // in powers of two
 constexpr uint32_t kBadRing = 8;
-constexpr uint32_t kEarlyKeys = 64;    // of a tile's probabilities, handed to the tensor cores before the rest
-constexpr uint32_t kEmulated = 0;      // of every 8 pairs of exponentials, taken off the special function unit
+constexpr uint32_t kEarlyKeys = 96;    // of a tile's probabilities, handed to the tensor cores before the rest
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int D, bool TREE>
@@ -69,9 +68,9 @@ struct Shape {
   static constexpr uint32_t kSmem = 1024 + (2 + kStages) * kTile;
 };
 
-struct BadRows {  // listed keys of up to two tiles of a segment
+struct BadRows {  // one cleaning warp's half (64 keys): listed keys of up to two tiles of a segment
   uint32_t tiles;
-  uint32_t tile[2], mask[2][4];
+  uint32_t tile[2], mask[2][2];
 };
 
 struct TreeEntry {
@@ -85,15 +84,16 @@ struct Barriers {
   uint64_t s_full[2], p_early[2], p_ready[2], o_full[2], joined;
   uint32_t tmem;
   int failed;
-  BadRows bad[kBadRing];
+  BadRows bad[kBadRing][2];
 };
 
 struct TreeArgs {
   xpu_kv_cache_t cache;
   const int32_t *sequences, *starts;
   const uint64_t *ancestors;
-  uint32_t layer, count;
-  float *partial;  // [slot][256 rows][D], then [slot][256 rows]{m, l}
+  uint32_t layer, count, page_shift;  // page_size = 2^page_shift
+  uint32_t *arrived;  // per block: parts of the unit that begins there, 0 between calls
+  float *partial;     // [slot][256 rows][D], then [slot][256 rows]{m, l}
 };
 
 struct Args {
@@ -115,6 +115,7 @@ struct Segment {
   uint32_t masked_from;      // the first key tile that some row may not attend as a whole
   bool both;                 // both softmax groups on row tile 0, even and odd key tiles
   int32_t slot;              // partial result, -1 = whole
+  uint32_t unit, unit_tiles; // key tiles of the whole unit, in the order of all: first and how many
 };
 
 // ------------------------------------------------------------ small parts ----
@@ -231,27 +232,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// 2^x of two finite numbers up to 2^7 without the special function unit:
-// 2^x = 2^n 2^f with n the nearest whole number (read off the low bits of
-// x + 1.5 2^23) and f in [-1/2, 1/2]; 2^f by the polynomial of degree 4 with the
-// least maximal relative error there (found by Remez exchange: 2.7e-6), n added
-// to the exponent. Below 2^-125 it gives 2^-125, nothing beside a row's largest.
-__device__ __forceinline__ void exp2_pair(Pair x, float &lo, float &hi) {
-  x.get(lo, hi);
-  x = Pair(fmaxf(lo, -125.f), fmaxf(hi, -125.f));
-  const Pair t = add2(x, Pair(12582912.f, 12582912.f));
-  const Pair f = add2(x, fma2(add2(t, Pair(-12582912.f, -12582912.f)), Pair(-1.f, -1.f), Pair(0.f, 0.f)));
-  Pair p = fma2(f, Pair(0.009570102207362652f, 0.009570102207362652f), Pair(0.05591785907745361f, 0.05591785907745361f));
-  p = fma2(p, f, Pair(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f, Pair(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, f, Pair(0.9999992847442627f, 0.9999992847442627f));
-  float tl, th;
-  p.get(lo, hi);
-  t.get(tl, th);
-  lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(tl) << 23));
-  hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(th) << 23));
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -265,11 +245,14 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Either 16-bit half of w infinite or NaN.
+// 0 w + sum of both 16-bit halves: the sum stays 0 until a half is infinite or
+// NaN, and is NaN from then on.
 template <typename T>
-__device__ __forceinline__ bool word_not_finite(uint32_t w) {
-  constexpr uint32_t e = sizeof(T) && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || (w & (e << 16)) == (e << 16);
+__device__ __forceinline__ uint32_t add_zero_times(uint32_t w, uint32_t sum) {
+  uint32_t d;
+  if (std::is_same<T, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w), "r"(0u), "r"(sum));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w), "r"(0u), "r"(sum));
+  return d;
 }
 
 // --------------------------------------------------------------- segments ----
@@ -369,10 +352,11 @@ __device__ __forceinline__ uint32_t tree_share(uint32_t tiles, uint32_t blocks) 
 // This block's share of all (sequence, row block, kv head, key tile), in that order.
 struct TreeWalk {
   const TreeEntry *table;
-  uint32_t count, group, kv_heads, i, at, begin, end;
+  uint32_t count, group, kv_heads, i, at, begin, end, share;
   __device__ TreeWalk(const Args &a, const TreeEntry *t, uint32_t g) : table(t), count(a.tree.count), group(g) {
     kv_heads = a.t.kv_heads;
-    const uint32_t total = table[count].first, share = tree_share(total, gridDim.x);
+    const uint32_t total = table[count].first;
+    share = tree_share(total, gridDim.x);
     begin = at = min(total, blockIdx.x * share);
     end = min(total, begin + share);
     uint32_t lo = 0, hi = count;  // the last entry that starts at or before `at`
@@ -402,6 +386,8 @@ struct TreeWalk {
     s.both = s.npos <= positions;
     s.n0 = s.both ? (s.n + 1) / 2 : s.n;
     s.n1 = s.both ? s.n / 2 : s.n;
+    s.unit = e.first + unit * tiles;
+    s.unit_tiles = tiles;
     s.slot = s.n == tiles ? -1 : static_cast<int32_t>(2 * blockIdx.x + (at == begin ? 0 : 1));
     at += s.n;
     return true;
@@ -420,14 +406,15 @@ __device__ __forceinline__ uint32_t valid_keys(const Segment &s, uint32_t tile) 
 // product) to one row's columns [col, col + cols): dst16 (normalised by inv)
 // or dst32. Rare: plain loops over global memory.
 template <typename T, int D, bool TREE>
-__device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadRows *bad, uint32_t listed, uint32_t position,
-                                     uint32_t q_head, uint64_t set, float m, float inv, T *dst16, float *dst32, uint32_t col,
+__device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadRows *bad, uint32_t listed, uint32_t half,
+                                     uint32_t position, uint32_t q_head, uint64_t set, float m, float inv, T *dst16, float *dst32, uint32_t col,
                                      uint32_t cols) {
   const T *q = static_cast<const T *>(a.t.q) + (s.q0 - s.pos0 + static_cast<size_t>(position)) * a.t.q_stride + q_head * D;
   const float c = a.t.scale * kLog2e;
   for (uint32_t i = 0; i < listed; ++i)
-    for (uint32_t in_tile = 0; in_tile < kKeys; ++in_tile) {
-      if (!(bad->mask[i][in_tile >> 5] >> (in_tile & 31) & 1u)) continue;
+    for (uint32_t j = 0; j < 64; ++j) {
+      if (!(bad->mask[i][j >> 5] >> (j & 31) & 1u)) continue;
+      const uint32_t in_tile = half * 64 + j;
       const uint32_t key = bad->tile[i] * kKeys + in_tile;
       const T *k, *v;
       if (!TREE || bad->tile[i] * kKeys >= s.len) {  // packed: a prompt's key, or a draft
@@ -454,6 +441,108 @@ __device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadR
     }
 }
 
+// ------------------------------------------------------------------- join ----
+
+// Numbers 0 .. 255 of a unit's rows in use (position x group + head): quotients
+// without a division, and the row's place among the unit's two tiles of 128.
+struct JoinRows {
+  uint32_t group, positions, inverse;
+  __device__ JoinRows(uint32_t g, uint32_t p) : group(g), positions(p), inverse(65536u / g + 1) {}
+  __device__ uint32_t position(uint32_t r) const { return r * inverse >> 16; }
+  __device__ uint32_t row(uint32_t r) const { return r + (position(r) >= positions ? 128 - positions * group : 0); }
+};
+
+// Thread r of 256: row r's maximum over the parts of blocks c0 .. c1, and the
+// reciprocal of the sum, for join_rows; the row's lse.
+__device__ __forceinline__ void join_sums(const Args &a, const Segment &s, const float2 *sums, JoinRows rows, uint32_t share,
+                                          uint32_t c0, uint32_t c1, float2 *total) {
+  const uint32_t r = threadIdx.x;
+  if (r >= s.npos * rows.group) return;
+  const uint32_t row = rows.row(r);
+  const float c = a.t.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  for (uint32_t x0 = c0; x0 <= c1; x0 += 8) {  // eight loads in flight
+    float2 ml[8];
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+      const uint32_t x = min(x0 + e, c1);
+      ml[e] = __ldcg(sums + (2 * x + (x * share >= s.unit ? 0 : 1)) * 256 + row);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+      if (x0 + e > c1) continue;
+      const float top = fmaxf(m, ml[e].x);
+      if (top == -INFINITY) continue;
+      l = l * exp2_approx((m - top) * c) + ml[e].y * exp2_approx((ml[e].x - top) * c);
+      m = top;
+    }
+  }
+  total[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
+  const uint32_t index = rows.position(r);
+  if (a.t.lse)
+    a.t.lse[(static_cast<size_t>(s.q0) + index) * a.t.q_heads + s.head * rows.group + r - index * rows.group] =
+        l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * kLn2;
+}
+
+// Warp `warp` of 8: rows of the unit, the parts in order; sixteen loads in
+// flight (one row after the other took 20 us where this takes 2).
+template <typename T, int D>
+__device__ __forceinline__ void join_rows(const Args &a, const Segment &s, const float2 *sums, JoinRows rows, uint32_t share,
+                                          uint32_t c0, uint32_t c1, const float2 *total, uint32_t warp) {
+  constexpr uint32_t N = D / 32, kRows = 8, kParts = 2;  // N: this lane's columns
+  const uint32_t lane = threadIdx.x & 31, many = s.npos * rows.group;
+  const float c = a.t.scale * kLog2e;
+  for (uint32_t r0 = warp * kRows; r0 < many; r0 += 8 * kRows) {
+    float o[kRows][N] = {}, top[kRows];
+    uint32_t row[kRows];
+#pragma unroll
+    for (uint32_t i = 0; i < kRows; ++i) {
+      row[i] = rows.row(min(r0 + i, many - 1));
+      top[i] = total[min(r0 + i, many - 1)].x;
+    }
+    for (uint32_t x0 = c0; x0 <= c1; x0 += kParts) {
+      float part[kParts][kRows][N], m[kParts][kRows];
+#pragma unroll
+      for (uint32_t e = 0; e < kParts; ++e) {
+        const uint32_t x = min(x0 + e, c1), slot = 2 * x + (x * share >= s.unit ? 0 : 1);
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; ++i) {
+          const size_t at = slot * 256 + row[i];
+          m[e][i] = __ldcg(&sums[at].x);
+          const float *src = a.tree.partial + at * D + N * lane;
+          if constexpr (N == 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
+            part[e][i][0] = v.x, part[e][i][1] = v.y, part[e][i][2] = v.z, part[e][i][3] = v.w;
+          } else {
+            const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
+            part[e][i][0] = v.x, part[e][i][1] = v.y;
+          }
+        }
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < kParts; ++e)
+#pragma unroll
+        for (uint32_t i = 0; i < kRows; ++i) {
+          const float w = x0 + e > c1 || m[e][i] == -INFINITY ? 0.f : exp2_approx((m[e][i] - top[i]) * c);
+#pragma unroll
+          for (uint32_t n = 0; n < N; ++n) o[i][n] = fmaf(w, part[e][i][n], o[i][n]);
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kRows; ++i) {
+      const uint32_t r = r0 + i;
+      if (r >= many) break;
+      const float inv = total[r].y;
+      const uint32_t index = rows.position(r);
+      const size_t token = static_cast<size_t>(s.q0) + index;
+      uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(a.t.out) + token * a.t.out_stride +
+                                                   (s.head * rows.group + r - index * rows.group) * D) + N / 2 * lane;
+#pragma unroll
+      for (uint32_t n = 0; n < N / 2; ++n) dst[n] = pack2<T>(o[i][2 * n] * inv, o[i][2 * n + 1] * inv);
+    }
+  }
+}
+
 // ----------------------------------------------------------------- kernel ----
 
 template <typename T, int D, bool TREE>
@@ -466,6 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
   __shared__ TreeEntry table[TREE ? XPU_KV_MAX_REQUESTS + 1 : 1];
   __shared__ float joined[TREE ? 2 : 1][TREE ? 128 : 1][2];
   __shared__ uint32_t scratch[kThreads / 32];
+  __shared__ bool last;
   const uint32_t a0 = smem_addr(smem_raw);
   uint8_t *q_smem = smem_raw + ((a0 + 1023u) / 1024u * 1024u - a0), *ring = q_smem + 2 * S::kTile;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -477,8 +567,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     mbar_init(&b.drain, 1);
     for (uint32_t i = 0; i < S::kStages; ++i) {
       mbar_init(&b.kv_full[i], 1);
-      mbar_init(&b.kv_empty[i], 2);  // the products and the cleaning
-      mbar_init(&b.clean[i], 1);
+      mbar_init(&b.kv_empty[i], 3);  // the products and both cleaning warps
+      mbar_init(&b.clean[i], 2);
     }
     for (uint32_t i = 0; i < 2; ++i) {
       mbar_init(&b.s_full[i], 1);
@@ -548,29 +638,55 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         } else {
           many = (TREE ? s.len : position + 1) - min(tile * kKeys, TREE ? s.len : position + 1);
         }
-        // the largest of x[from ..], 64 of them, in four chains; NaN if one is NaN
-        auto largest = [&](const uint32_t *y, float first) {
-          float top4[4] = {first, first, first, first};
-#pragma unroll
-          for (uint32_t j = 0; j < 64; j += 8)
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e)
-              top4[e] = max3_nan(top4[e], __uint_as_float(y[j + 2 * e]), __uint_as_float(y[j + 2 * e + 1]));
-          return max3_nan(max3_nan(top4[0], top4[1], top4[2]), top4[3], top4[3]);
-        };
         if (masked) {
 #pragma unroll
           for (uint32_t j = 0; j < 64; ++j)
             if (drafts ? !((j < 32 ? keep_lo >> j : keep_hi >> (j - 32)) & 1u) : j >= many) x[j] = 0xff800000u;
         }
-        float top = largest(x, m);
+        // p of 32 keys from x[32 q] on, in pairs, and their sum
+        const Pair c2(c, c);
+        Pair sum0(0.f, 0.f), sum1(0.f, 0.f);
+        auto quarter = [&](uint32_t q, Pair mc2, uint32_t *p) {
+#pragma unroll
+          for (uint32_t j = 0; j < 16; ++j) {
+            const Pair y = fma2(Pair(__uint_as_float(x[32 * q + 2 * j]), __uint_as_float(x[32 * q + 2 * j + 1])), c2, mc2);
+            float lo, hi;
+            y.get(lo, hi);
+            lo = exp2_approx(lo);
+            hi = exp2_approx(hi);
+            if (j & 1) sum1 = add2(sum1, Pair(lo, hi));
+            else sum0 = add2(sum0, Pair(lo, hi));
+            p[j] = pack2<T>(lo, hi);
+          }
+        };
+        auto publish = [&](uint64_t *bar) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar);
+        };
+        // a row with an infinite or undefined score is undefined as a whole
+        auto shift = [&] {
+          const float mc = m == -INFINITY ? 0.f : (m == INFINITY ? NAN : -m * c);
+          return Pair(mc, mc);
+        };
+        float top4[4] = {m, m, m, m};  // four chains; NaN if one score is
+        auto search = [&](uint32_t from) {
+#pragma unroll
+          for (uint32_t j = from; j < from + 64; j += 8)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+              top4[e] = max3_nan(top4[e], __uint_as_float(x[j + 2 * e]), __uint_as_float(x[j + 2 * e + 1]));
+        };
+        search(0);
         tmem_wait_ld64(x + 64);
         if (masked) {
 #pragma unroll
           for (uint32_t j = 64; j < kKeys; ++j)
             if (drafts || j >= many) x[j] = 0xff800000u;
         }
-        top = largest(x + 64, top);
+        search(64);
+        const float top = max3_nan(max3_nan(top4[0], top4[1], top4[2]), top4[3], top4[3]);
         const bool grown = top != m && !((top - m) * c <= kRescale);  // m = -inf included, and NaN
         if (__any_sync(kFullMask, grown)) {
           const float keep = grown ? exp2_approx((m - top) * c) : 1.f;
@@ -588,44 +704,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
             }
           }
         }
-        // a row with an infinite or undefined score is undefined as a whole
-        const float mc = m == -INFINITY ? 0.f : (m == INFINITY ? NAN : -m * c);
-        const Pair c2(c, c), mc2(mc, mc);
-        Pair sum0(0.f, 0.f), sum1(0.f, 0.f);
-        auto quarter = [&](uint32_t q, auto emulated) {
+        const Pair mc2 = shift();
+#pragma unroll
+        for (uint32_t q = 0; q < kKeys / 32; ++q) {
           uint32_t p[16];
-#pragma unroll
-          for (uint32_t j = 0; j < 16; ++j) {
-            const Pair y = fma2(Pair(__uint_as_float(x[32 * q + 2 * j]), __uint_as_float(x[32 * q + 2 * j + 1])), c2, mc2);
-            float lo, hi;
-            if (j % 8 + 1 <= decltype(emulated)::value) {
-              exp2_pair(y, lo, hi);
-            } else {
-              y.get(lo, hi);
-              lo = exp2_approx(lo);
-              hi = exp2_approx(hi);
-            }
-            if (j & 1) sum1 = add2(sum1, Pair(lo, hi));
-            else sum0 = add2(sum0, Pair(lo, hi));
-            p[j] = pack2<T>(lo, hi);
-          }
+          quarter(q, mc2, p);
           tmem_st16(s_addr + 16 * q, p);
-        };
-        auto publish = [&](uint64_t *bar) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar);
-        };
-        auto weights = [&](auto emulated) {
-#pragma unroll
-          for (uint32_t q = 0; q < 4; ++q) {
-            quarter(q, emulated);
-            if (32 * (q + 1) == kEarlyKeys) publish(&b.p_early[t]);
-          }
-        };
-        if (masked) weights(std::integral_constant<uint32_t, 0>());
-        else weights(std::integral_constant<uint32_t, kEmulated>());
+          if (32 * (q + 1) == kEarlyKeys) publish(&b.p_early[t]);
+        }
         float sum[4];
         sum0.get(sum[0], sum[1]);
         sum1.get(sum[2], sum[3]);
@@ -713,15 +799,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           }
         }
         if (store && s.first + s.n > s.masked_from) {
-          const BadRows *bad = &b.bad[segment % kBadRing];
-          const uint32_t listed = *const_cast<const volatile uint32_t *>(&bad->tiles);
-          __threadfence_block();
-          if (listed)
-            fix_row<T, D, TREE>(a, s, bad, listed, position, q_head, set, m, inv, dst16, dst32, col, cols);
+          for (uint32_t half = 0; half < 2; ++half) {
+            const BadRows *bad = &b.bad[segment % kBadRing][half];
+            const uint32_t listed = *const_cast<const volatile uint32_t *>(&bad->tiles);
+            __threadfence_block();
+            if (listed)
+              fix_row<T, D, TREE>(a, s, bad, listed, half, position, q_head, set, m, inv, dst16, dst32, col, cols);
+          }
         }
       }
-      // the other group may still read this one's accumulator and sums
-      if (TREE && s.both && !meet()) break;
+      if constexpr (TREE) {
+        if (s.slot >= 0) {
+          // The block that completes a unit adds up its parts, in the order of the
+          // key tiles whoever comes last.
+          if (!meet()) break;
+          const uint32_t c0 = s.unit / walk.share, c1 = (s.unit + s.unit_tiles - 1) / walk.share;
+          if (threadIdx.x == 0) {
+            __threadfence();
+            last = atomicAdd(a.tree.arrived + c0, 1u) == c1 - c0;
+            if (last) a.tree.arrived[c0] = 0;
+            __threadfence();
+          }
+          if (!meet()) break;
+          if (last) {
+            const float2 *sums = reinterpret_cast<const float2 *>(a.tree.partial + 2ull * gridDim.x * 256 * D);
+            float2 *total = reinterpret_cast<float2 *>(&joined[0][0][0]);
+            join_sums(a, s, sums, JoinRows(group, positions), walk.share, c0, c1, total);
+            if (!meet()) break;
+            join_rows<T, D>(a, s, sums, JoinRows(group, positions), walk.share, c0, c1, total, warp);
+          }
+          if (!meet()) break;
+        } else if (s.both && !meet()) {  // the other group may still read this one's accumulator and sums
+          break;
+        }
+      }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -868,30 +979,46 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
   } else if (warp == kLoadWarp) {
     // --------------------------------------------------------------- loads ----
     uint32_t loaded = 0, segment = 0, q_loads = 0;
-    auto tile_dst = [&](uint32_t i) { return ring + i % S::kStages * S::kTile; };
-    for (; walk.next(s) && !warp_failed(b); ++segment) {
-      bool ok = true;
+    // lane p: the id of page p of a cached key tile (behind the pool, where reads
+    // give zeros, if it is out of range)
+    auto page_of = [&](const Segment &g, uint32_t tile) {
+      int32_t page = 0;
+      if constexpr (TREE) {
+        const xpu_kv_cache_t &kc = a.tree.cache;
+        const uint32_t at = tile * kKeys + (lane << a.tree.page_shift);
+        if (lane << a.tree.page_shift < kKeys && at < g.len) {
+          page = kc.tables[static_cast<size_t>(g.sequence) * kc.table_width + (at >> a.tree.page_shift)];
+          if (page < 0 || static_cast<uint32_t>(page) >= kc.pages) {
+            atomicOr(kc.status, XPU_KV_BAD_INDEX);
+            page = static_cast<int32_t>(kc.pages);
+          }
+        }
+      }
+      return page;
+    };
+    Segment following;
+    bool more = walk.next(following);
+    int32_t next_page = more ? page_of(following, following.first) : 0;
+    bool ok = true;
+    for (; ok && more && !warp_failed(b); ++segment) {
+      s = following;
       for (uint32_t j = 0; j < s.n && ok; ++j) {
         const uint32_t tile = s.first + j, at = tile * kKeys;
         const bool packed = !TREE || at >= s.len;
-        int32_t page = 0;
-        uint32_t pages = 0;
-        if (TREE && !packed) {  // lane p fetches the tile's page p
-          const xpu_kv_cache_t &kc = a.tree.cache;
-          pages = (min(kKeys, s.len - at) + kc.page_size - 1) / kc.page_size;
-          if (lane < pages) {
-            page = kc.tables[static_cast<size_t>(s.sequence) * kc.table_width + at / kc.page_size + lane];
-            if (page < 0 || static_cast<uint32_t>(page) >= kc.pages) {
-              atomicOr(kc.status, XPU_KV_BAD_INDEX);
-              page = static_cast<int32_t>(kc.pages);  // behind the pool: reads as zeros
-            }
-          }
+        // the next tile's pages are looked up under this tile's wait
+        const int32_t page = next_page;
+        if (j + 1 < s.n) {
+          next_page = page_of(s, tile + 1);
+        } else {
+          more = walk.next(following);
+          if (more) next_page = page_of(following, following.first);
         }
         for (uint32_t which = 0; which < 2; ++which) {
           const uint32_t slot = loaded % S::kStages, use = loaded / S::kStages;
-          if (use > 0 && !warp_wait(b, &b.kv_empty[slot], (use - 1) & 1)) { ok = false; break; }
+          if (use > 0 && !(ok = warp_wait(b, &b.kv_empty[slot], (use - 1) & 1))) break;
           uint64_t *bar = &b.kv_full[slot];
-          uint8_t *dst = tile_dst(loaded++);
+          uint8_t *dst = ring + slot * S::kTile;
+          ++loaded;
           if (packed) {
             if (lane == 0) {
               // a tree's drafts: half a tile, XPU_TREE_MAX_NODES rows
@@ -901,7 +1028,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
             }
           } else {
             const xpu_kv_cache_t &kc = a.tree.cache;
-            const uint32_t bytes = kc.page_size * 128;
+            const uint32_t bytes = kc.page_size * 128, pages = (min(kKeys, s.len - at) + kc.page_size - 1) >> a.tree.page_shift;
             if (lane == 0) mbar_expect_tx(bar, pages * bytes * S::kBoxes);
             __syncwarp();
             if (lane < pages) {
@@ -911,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
             }
           }
           if (j == 0 && which == 0) {  // after the first keys, which need not wait for the last segment's rows
-            if (segment > 0 && !warp_wait(b, &b.q_empty, (segment - 1) & 1)) { ok = false; break; }
+            if (segment > 0 && !(ok = warp_wait(b, &b.q_empty, (segment - 1) & 1))) break;
             if (lane == 0) {
               const uint32_t tiles = !s.both && s.npos > positions ? 2 : 1;
               mbar_expect_tx(&b.q_full, tiles * positions * group * 128 * S::kBoxes);
@@ -923,18 +1050,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           }
         }
       }
-      if (!ok) break;
     }
     if (warp_failed(b)) {  // what was asked for lands before the block's memory is given up
       for (uint32_t i = loaded > S::kStages ? loaded - S::kStages : 0; i < loaded; ++i)
         mbar_wait(&b.kv_full[i % S::kStages], i / S::kStages & 1);
       if (q_loads) mbar_wait(&b.q_full, (q_loads - 1) & 1);
     }
-  } else if (warp == kCleanWarp) {
+  } else {
     // ------------------------------------------------------------ cleaning ----
+    const uint32_t half = warp - kCleanWarp;  // keys 64 half .. + 63 of a tile
     uint32_t loaded = 0, segment = 0;
     for (; walk.next(s) && !warp_failed(b); ++segment) {
-      BadRows *bad = &b.bad[segment % kBadRing];
+      BadRows *bad = &b.bad[segment % kBadRing][half];
       uint32_t listed = 0;
       if (lane == 0 && s.first + s.n > s.masked_from) bad->tiles = 0;
       for (uint32_t e = 0; e < 2 * s.n; ++e) {  // every ring entry, so as never to be a turn ahead or behind
@@ -947,17 +1074,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         const uint32_t valid = valid_keys<TREE>(s, tile);
         uint32_t any = 0;
 #pragma unroll
-        for (uint32_t g = 0; g < 4; ++g) {
-          uint8_t *row = ring + slot * S::kTile + (g * 32 + lane) * 128;
-          const bool inside = g * 32 + lane < valid;
-          bool spoilt = false;
+        for (uint32_t g = 0; g < 2; ++g) {
+          const uint32_t key = half * 64 + g * 32 + lane;
+          uint8_t *row = ring + slot * S::kTile + key * 128;
+          const bool inside = key < valid;
+          uint32_t sums[4] = {0, 0, 0, 0};
           if (inside) {
 #pragma unroll
             for (uint32_t x = 0; x < 8 * S::kBoxes; ++x) {  // 16-byte pieces, each lane from another bank
               const uint4 w = *reinterpret_cast<const uint4 *>(row + x / 8 * kBox + ((x + lane) & 7) * 16);
-              spoilt |= word_not_finite<T>(w.x) || word_not_finite<T>(w.y) || word_not_finite<T>(w.z) || word_not_finite<T>(w.w);
+              sums[0] = add_zero_times<T>(w.x, sums[0]);
+              sums[1] = add_zero_times<T>(w.y, sums[1]);
+              sums[2] = add_zero_times<T>(w.z, sums[2]);
+              sums[3] = add_zero_times<T>(w.w, sums[3]);
             }
           }
+          const bool spoilt = ((sums[0] | sums[1] | sums[2] | sums[3]) & 0x7fff7fffu) != 0;
           if (!inside || spoilt) {
 #pragma unroll
             for (uint32_t x = 0; x < 8 * S::kBoxes; ++x)
@@ -993,56 +1125,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     tc_fence_after();
     tmem_dealloc1(tmem, 512);
   }
-  if (TREE) grid_dep_launch();
-}
-
-// Joins the partial results of units that several blocks worked on: one warp
-// per (node, query head); the blocks' order is the order of the sum.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) k_tree_join(const __grid_constant__ Args a, uint32_t blocks) {
-  __shared__ TreeEntry table[XPU_KV_MAX_REQUESTS + 1];
-  __shared__ uint32_t scratch[8];
-  const uint32_t group = a.t.q_heads / a.t.kv_heads, positions = tile_positions(group), lane = threadIdx.x & 31;
-  grid_dep_wait();
-  tree_table(a.tree, a.t.tokens, a.t.kv_heads, group, table, scratch);
-  const uint64_t w = blockIdx.x * 8ull + threadIdx.x / 32;
-  if (w >= static_cast<uint64_t>(a.t.tokens) * a.t.q_heads) return;
-  const uint32_t node = static_cast<uint32_t>(w / a.t.q_heads), q_head = static_cast<uint32_t>(w % a.t.q_heads);
-  uint32_t lo = 0, hi = a.tree.count;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (a.tree.starts[mid] <= static_cast<int32_t>(node)) lo = mid;
-    else hi = mid;
-  }
-  const TreeEntry e = table[lo];
-  const uint32_t index = node - e.begin;
-  if (node < e.begin || index >= entry_nodes(e)) return;
-  const uint32_t tiles = entry_tiles(e), block = index / (2 * positions), in_block = index % (2 * positions);
-  const uint32_t share = tree_share(table[a.tree.count].first, blocks);
-  const uint32_t g0 = e.first + (block * a.t.kv_heads + q_head / group) * tiles;
-  const uint32_t c0 = g0 / share, c1 = (g0 + tiles - 1) / share;
-  if (c0 == c1) return;
-  const uint32_t row = (in_block / positions) * 128 + in_block % positions * group + q_head % group;
-  const float *sums = a.tree.partial + 2ull * blocks * 256 * D, c = a.t.scale * kLog2e;
-  auto row_of = [&](uint32_t x) { return (2ull * x + (x * share >= g0 ? 0 : 1)) * 256 + row; };
-  float m = -INFINITY;
-  for (uint32_t x = c0 + lane; x <= c1; x += 32) m = fmaxf(m, sums[row_of(x) * 2]);
-  m = warp_max(m);
-  float l = 0.f, o[D / 32];
-#pragma unroll
-  for (uint32_t i = 0; i < D / 32; ++i) o[i] = 0.f;
-  for (uint32_t x = c0; x <= c1; ++x) {
-    const size_t at = row_of(x);
-    const float mx = sums[at * 2], wx = mx == -INFINITY ? 0.f : exp2f((mx - m) * c);
-    l = fmaf(wx, sums[at * 2 + 1], l);
-#pragma unroll
-    for (uint32_t i = 0; i < D / 32; ++i) o[i] = fmaf(wx, a.tree.partial[at * D + lane + 32 * i], o[i]);
-  }
-  T *dst = static_cast<T *>(a.t.out) + static_cast<size_t>(node) * a.t.out_stride + q_head * D;
-#pragma unroll
-  for (uint32_t i = 0; i < D / 32; ++i) dst[lane + 32 * i] = Elem<T>::from_float(l == 0.f ? 0.f : o[i] / l);
-  if (a.t.lse && lane == 0)
-    a.t.lse[static_cast<size_t>(node) * a.t.q_heads + q_head] = l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * kLn2;
 }
 
 // ------------------------------------------------------------------- host ----
@@ -1067,18 +1149,7 @@ cudaError_t launch(const Args &a, uint32_t blocks, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(k_attention<T, D, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   k_attention<T, D, TREE><<<blocks, kThreads, smem, s>>>(a);
-  e = cudaGetLastError();
-  if (!TREE || e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<uint32_t>((static_cast<uint64_t>(a.t.tokens) * a.t.q_heads + 7) / 8));
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_tree_join<T, D>, a, blocks);
+  return cudaGetLastError();
 }
 
 template <bool TREE>
@@ -1164,9 +1235,13 @@ cudaError_t prompt_attention_launch(bool fp16, const int32_t *plan, uint32_t blo
   return e != cudaSuccess ? e : launch_any<false>(fp16, a, blocks, s);
 }
 
+namespace {
+constexpr uint32_t kArrivedBytes = 4096;  // up to 1024 blocks
+}
+
 size_t tree_workspace_bytes(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t head_dim) {
-  // two partial results a block: 256 rows of outputs, and their maxima and sums
-  return 2ull * sm_count() * 256 * (head_dim + 2) * 4;
+  // arrivals, and two partial results a block: 256 rows of outputs, and their maxima and sums
+  return kArrivedBytes + 2ull * sm_count() * 256 * (head_dim + 2) * 4;
 }
 
 cudaError_t tree_attention_launch(const xpu_kv_cache_t &c, uint32_t layer, const int32_t *sequences,
@@ -1174,7 +1249,9 @@ cudaError_t tree_attention_launch(const xpu_kv_cache_t &c, uint32_t layer, const
                                   const AttnTensors &t, void *workspace, cudaStream_t s) {
   Args a = {};
   a.t = t;
-  a.tree = {c, sequences, starts, ancestors, layer, count, static_cast<float *>(workspace)};
+  a.tree = {c, sequences, starts, ancestors, layer, count, static_cast<uint32_t>(__builtin_ctz(c.page_size)),
+            static_cast<uint32_t *>(workspace),
+            reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kArrivedBytes)};
   cudaError_t e = packed_maps(a, XPU_TREE_MAX_NODES);
   if (e != cudaSuccess) return e;
   const uint64_t rows = static_cast<uint64_t>(c.pages) * c.kv_heads * c.page_size;
