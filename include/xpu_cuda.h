@@ -182,8 +182,8 @@ int xpu_qwen_argmax(const uint16_t *values, uint32_t *token, uint32_t width, voi
  * Sequence s uses ceil(lens[s] / page_size) pages, tables[s][0..]: one page
  * covers the same positions of every layer. refs[p] counts the sequences that
  * use page p; 0 = free. Only pages that are full are ever shared. The caller
- * owns all of it in device memory and starts with lens and refs 0, tables -1,
- * status 0. Every operator reads and writes tables, lens and refs on the
+ * owns all of it in device memory and starts with lens, refs, status and
+ * workspace 0, tables -1. Every operator reads and writes tables, lens and refs on the
  * device, so a serving loop needs no host synchronisation; a request that
  * cannot be met changes nothing and sets a bit of *status. Calls on one cache
  * must be ordered by the caller (one stream, or events).
@@ -203,6 +203,7 @@ typedef struct {
 #define XPU_KV_BAD_SEQUENCE 2u /* an id out of range or named twice, a child in use, a negative count: the same */
 #define XPU_KV_SHARED_CUT 4u   /* a trim would end inside a shared page: the same */
 #define XPU_KV_BAD_INDEX 8u    /* a row, page or length out of range: not written, read as zeros or as nothing */
+#define XPU_KV_TIMEOUT 16u     /* a bounded device-side wait gave up; zero the workspace before the next call */
 
 /* Most sequences one call may name; page_size is 16, 32, 64 or 128; head_dim
  * 64 or 128; at most XPU_KV_MAX_SEQUENCES sequences; pages x kv_heads x

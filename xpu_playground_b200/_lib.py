@@ -157,7 +157,9 @@ def check(status: int) -> None:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise XpuError on failure."""
-    check(getattr(load(), name)(*args))
+    status = getattr(_lib or load(), name)(*args)
+    if status != XPU_OK:
+        raise XpuError(status, last_error())
 
 
 def declared_functions(header: Path = HEADER) -> list[str]:

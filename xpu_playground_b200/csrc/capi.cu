@@ -293,7 +293,7 @@ int xpu_kv_write(const xpu_kv_cache_t *cache, const int32_t *sequences, const in
     if (count == 0 || tokens == 0) return XPU_OK;
     XPU_CHECKED(check_rows(*cache, k, v, held, layer_stride, row_stride, layer, layers, "xpu_kv_write"));
     return cuda_status(kv_write_launch(*cache, sequences, starts, count, tokens, rows, k, v, held, layer_stride, row_stride,
-                                       layer, layers, as_stream(stream)),
+                                       layer, layers, false, as_stream(stream)),
                        "xpu_kv_write");
   })
 }
@@ -306,9 +306,8 @@ int xpu_kv_append(const xpu_kv_cache_t *cache, const int32_t *sequences, const i
     XPU_CHECKED(check_list(sequences, starts, count, "xpu_kv_append"));
     if (count == 0 || tokens == 0) return XPU_OK;
     XPU_CHECKED(check_rows(*cache, k, v, held, layer_stride, row_stride, 0, cache->layers, "xpu_kv_append"));
-    XPU_CHECKED(cuda_status(kv_extend_launch(*cache, sequences, starts, count, as_stream(stream)), "xpu_kv_append"));
     return cuda_status(kv_write_launch(*cache, sequences, starts, count, tokens, rows, k, v, held, layer_stride, row_stride,
-                                       0, cache->layers, as_stream(stream)),
+                                       0, cache->layers, true, as_stream(stream)),
                        "xpu_kv_append");
   })
 }
@@ -350,13 +349,7 @@ int xpu_prompt_plan(const uint32_t *lens, uint32_t count, uint32_t q_heads, uint
     uint64_t tokens = 0;
     for (uint32_t i = 0; i < count; ++i) tokens += lens[i];
     XPU_REQUIRE(tokens < (1ull << 31), "xpu_prompt_plan: too many tokens");
-    int device = 0, sms = 0;  // without a device: the plan of a B200
-    if (cudaGetDevice(&device) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
-      cudaGetLastError();
-      sms = 148;
-    }
-    *used = prompt_plan(lens, count, q_heads, kv_heads, static_cast<uint32_t>(sms), plan, capacity);
+    *used = prompt_plan(lens, count, q_heads, kv_heads, sm_count(), plan, capacity);
     if (*used > capacity)
       return fail(XPU_ERR_INVALID, "xpu_prompt_plan: the plan needs " + std::to_string(*used) + " ints");
     return XPU_OK;

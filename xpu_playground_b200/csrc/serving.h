@@ -7,13 +7,17 @@
 
 namespace xpu {
 
+// SMs of the current device (a B200's where there is none).
+uint32_t sm_count();
+
 // ---- paged cache (kv_cache.cu) ----
 size_t kv_workspace_bytes(uint32_t pages);
 cudaError_t kv_extend_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *starts, uint32_t count,
                              cudaStream_t s);
+// Writes rows into the positions that the last extension added, or (extend) extends first.
 cudaError_t kv_write_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *starts, uint32_t count,
                             uint32_t tokens, const int32_t *rows, const void *k, const void *v, uint32_t held,
-                            uint64_t layer_stride, uint64_t row_stride, uint32_t layer, uint32_t layers,
+                            uint64_t layer_stride, uint64_t row_stride, uint32_t layer, uint32_t layers, bool extend,
                             cudaStream_t s);
 cudaError_t kv_trim_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *new_lens, uint32_t count,
                            cudaStream_t s);

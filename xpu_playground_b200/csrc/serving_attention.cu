@@ -35,6 +35,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <functional>
 #include <queue>
 #include <vector>
@@ -1146,8 +1147,15 @@ cudaError_t packed_maps(Args &a, uint32_t kv_rows) {
 template <typename T, int D, bool TREE>
 cudaError_t launch(const Args &a, uint32_t blocks, cudaStream_t s) {
   constexpr uint32_t smem = Shape<D, TREE>::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(k_attention<T, D, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<bool> allowed[64];  // the shared memory, once per device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
+  if (device > 63 || !allowed[device].load(std::memory_order_relaxed)) {
+    e = cudaFuncSetAttribute(k_attention<T, D, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (device < 64) allowed[device].store(true, std::memory_order_relaxed);
+  }
   k_attention<T, D, TREE><<<blocks, kThreads, smem, s>>>(a);
   return cudaGetLastError();
 }
@@ -1159,17 +1167,25 @@ cudaError_t launch_any(bool fp16, const Args &a, uint32_t blocks, cudaStream_t s
   return fp16 ? launch<__half, 64, TREE>(a, blocks, s) : launch<__nv_bfloat16, 64, TREE>(a, blocks, s);
 }
 
+}  // namespace
+
 uint32_t sm_count() {
-  int device = 0, sms = 0;
-  if (cudaGetDevice(&device) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+  static std::atomic<int> known[64];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) {
     cudaGetLastError();
     return 148;
   }
+  int sms = known[device & 63].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+      cudaGetLastError();
+      return 148;
+    }
+    known[device & 63].store(sms, std::memory_order_relaxed);
+  }
   return static_cast<uint32_t>(sms);
 }
-
-}  // namespace
 
 unsigned take_attention_error() {
   unsigned v = 0, zero = 0;

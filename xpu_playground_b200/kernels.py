@@ -8,7 +8,6 @@ a contiguous CUDA tensor; 16-bit tensors are passed by their bit patterns.
 from __future__ import annotations
 
 import ctypes
-import math
 
 import numpy as np
 import torch
@@ -26,8 +25,10 @@ def _ptr(t: torch.Tensor) -> int:
 
 
 def _stream(stream=None) -> int:
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    # torch.cuda.current_stream().cuda_stream without building a Stream object (3 us)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -151,33 +152,39 @@ def qwen_argmax(values, token, width: int, stream=None):
 def _packed(name: str, t: torch.Tensor, heads: int, head_dim: int) -> int:
     """Row stride of a packed [tokens, heads, head_dim] tensor whose rows may
     stand apart (a slice of a fused projection)."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"{name} must be [tokens, {heads}, {head_dim}], not {tuple(shape)}")
     if not t.is_cuda:
         raise ValueError("libxpu_cuda entry points take CUDA tensors")
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
-        raise ValueError(f"{name} must be [tokens, {heads}, {head_dim}], not {tuple(t.shape)}")
+    if t.is_contiguous():
+        return heads * head_dim
     row, head, element = t.stride()
-    if (element != 1 and head_dim != 1) or (head != head_dim and heads != 1):
+    if element != 1 or (head != head_dim and heads != 1):
         raise ValueError(f"{name}: the heads of a token must be contiguous")
-    return row if t.shape[0] > 1 else max(row, heads * head_dim)
+    return row if shape[0] > 1 else max(row, heads * head_dim)
 
 
 def _attention_args(q, k, v, kv_heads, head_dim, scale, out, lse):
     tokens, q_heads = q.shape[0], q.shape[1]
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         raise ValueError("q, k and v must have one dtype")
     q_stride, kv_stride = _packed("q", q, q_heads, head_dim), _packed("k", k, kv_heads, head_dim)
     if _packed("v", v, kv_heads, head_dim) != kv_stride or k.shape[0] != tokens or v.shape[0] != tokens:
         raise ValueError("k and v need q's tokens and one row stride")
+    out_stride = q_heads * head_dim
     if out is None:
-        out = torch.empty(tokens, q_heads, head_dim, dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape:
+        out = torch.empty(tokens, q_heads, head_dim, dtype=dtype, device=q.device)
+    elif out.dtype != dtype or out.shape != q.shape:
         raise ValueError("out must have q's shape and dtype")
+    else:
+        out_stride = _packed("out", out, q_heads, head_dim)
     if lse is None:
         lse = torch.empty(tokens, q_heads, dtype=torch.float32, device=q.device)
-    elif lse.dtype != torch.float32 or lse.shape != q.shape[:2]:
-        raise ValueError("lse must be float32 [tokens, q_heads]")
-    return (out, lse, q_stride, kv_stride, _packed("out", out, q_heads, head_dim),
-            1.0 / math.sqrt(head_dim) if scale is None else scale)
+    elif lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_cuda or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, q_heads]")
+    return out, lse, q_stride, kv_stride, out_stride, head_dim ** -0.5 if scale is None else scale
 
 
 class PromptPlan:
@@ -212,7 +219,7 @@ def prompt_attention(plan: PromptPlan, q: torch.Tensor, k: torch.Tensor, v: torc
         raise ValueError(f"q must be [{plan.tokens}, {plan.q_heads}, {plan.head_dim}] for this plan")
     out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, plan.kv_heads, plan.head_dim, scale, out, lse)
     call("xpu_prompt_attention", _dtype_code(q), plan.device_plan.data_ptr(), plan.blocks, q.data_ptr(), k.data_ptr(),
-         v.data_ptr(), out.data_ptr(), _ptr(lse), plan.tokens, plan.q_heads, plan.kv_heads, plan.head_dim, q_stride,
+         v.data_ptr(), out.data_ptr(), lse.data_ptr(), plan.tokens, plan.q_heads, plan.kv_heads, plan.head_dim, q_stride,
          kv_stride, out_stride, scale, _stream(stream))
     return out, lse
 
@@ -242,6 +249,6 @@ def tree_attention(cache, layer: int, sequences: torch.Tensor, starts: torch.Ten
         raise ValueError("starts needs one entry more than sequences, ancestors one per node")
     out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, cache.kv_heads, cache.head_dim, scale, out, lse)
     call("xpu_tree_attention", cache.handle, layer, _ptr(sequences), _ptr(starts), _ptr(ancestors), sequences.numel(),
-         q.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), q.shape[1], q_stride, kv_stride,
+         q.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), q.shape[1], q_stride, kv_stride,
          out_stride, scale, _ptr(workspace), workspace.numel(), _stream(stream))
     return out, lse

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib, kernels
 
-EXHAUSTED, BAD_SEQUENCE, SHARED_CUT, BAD_INDEX = 1, 2, 4, 8  # XPU_KV_*
+EXHAUSTED, BAD_SEQUENCE, SHARED_CUT, BAD_INDEX, TIMEOUT = 1, 2, 4, 8, 16  # XPU_KV_*
 
 
 class KvCache:
@@ -60,32 +60,40 @@ class KvCache:
 
     def status(self) -> int:
         """Bits that refused requests have set (EXHAUSTED, BAD_SEQUENCE,
-        SHARED_CUT, BAD_INDEX), cleared by reading; waits for the device."""
+        SHARED_CUT, BAD_INDEX, TIMEOUT), cleared by reading; waits for the device."""
         bits = int(self._status.item())
         self._status.zero_()
         return bits
 
     @staticmethod
     def _ids(t: torch.Tensor) -> int:
-        if t.dtype != torch.int32:
-            raise ValueError("ids, offsets and lengths are int32 device tensors")
-        return kernels._ptr(t)
+        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+            raise ValueError("ids, offsets and lengths are contiguous int32 CUDA tensors")
+        return t.data_ptr()
 
     def _list(self, sequences, other, more=0):
-        if other.numel() != sequences.numel() + more:
+        count = sequences.numel()
+        if other.numel() != count + more:
             raise ValueError("one entry per sequence" + (" and one more" if more else ""))
-        return self._ids(sequences), self._ids(other), sequences.numel()
+        return self._ids(sequences), self._ids(other), count
 
     def _rows(self, k, v, rows, lead):
-        if k.dtype != self.dtype or v.dtype != self.dtype or k.shape != v.shape or k.stride() != v.stride():
-            raise ValueError("k and v must have the cache's dtype, and one shape and layout")
-        if k.dim() != 4 or k.shape[0] != lead or k.shape[2:] != (self.kv_heads, self.head_dim):
+        shape = k.shape
+        if k.dtype != self.dtype or v.dtype != self.dtype or shape != v.shape:
+            raise ValueError("k and v must have the cache's dtype and one shape")
+        if len(shape) != 4 or shape[0] != lead or shape[2] != self.kv_heads or shape[3] != self.head_dim:
             raise ValueError(f"k and v must be [{lead}, rows, {self.kv_heads}, {self.head_dim}]")
-        for t in (k[0], v[0]):
-            kernels._packed("k and v", t, self.kv_heads, self.head_dim)
-        row = self.kv_heads * self.head_dim if k.shape[1] <= 1 else k.stride(1)
-        tokens = k.shape[1] if rows is None else rows.numel()
-        return tokens, (None if rows is None else self._ids(rows)), k.data_ptr(), v.data_ptr(), k.shape[1], k.stride(0), row
+        held, row = shape[1], self.kv_heads * self.head_dim
+        layer = held * row
+        if not k.is_contiguous() or not v.is_contiguous():
+            if k.stride() != v.stride():
+                raise ValueError("k and v must have one layout")
+            row = max(row, kernels._packed("k and v", k[0], self.kv_heads, self.head_dim))
+            layer = k.stride(0)
+        if not k.is_cuda or not v.is_cuda:
+            raise ValueError("libxpu_cuda entry points take CUDA tensors")
+        tokens, at = (held, None) if rows is None else (rows.numel(), self._ids(rows))
+        return tokens, at, k.data_ptr(), v.data_ptr(), held, layer, row
 
     def extend(self, sequences: torch.Tensor, starts: torch.Tensor, stream=None) -> None:
         """Lengthens sequences[i] by starts[i+1] - starts[i] positions,
