@@ -226,6 +226,12 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
   return Pair(d);
 }
+// Natural logarithm of 2^(c m) l; -inf where the sum is empty.
+__device__ __forceinline__ float log_sum(float m, float l, float c) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(l));
+  return l == 0.f ? -INFINITY : fmaf(m, c, y) * kLn2;
+}
 // Largest of three, NaN if one is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
@@ -295,30 +301,42 @@ struct PromptWalk {
 __device__ __forceinline__ uint32_t entry_tiles(const TreeEntry &e) { return (e.len + kKeys - 1) / kKeys + 1; }
 __device__ __forceinline__ uint32_t entry_nodes(const TreeEntry &e) { return e.named & 127u; }
 
-// Fills table[0 .. count] (count + 1 entries: the last holds the totals) from the
-// device's lists, every value brought into range; all threads of the block.
+// One thread's sequence of the tree call, from the device's lists, every value
+// brought into range.
+struct TreeRequest {
+  int32_t begin, end, sequence, len;
+  bool mine;
+  __device__ TreeRequest(const TreeArgs &a, uint32_t i) : begin(0), end(0), sequence(-1), len(0), mine(i < a.count) {
+    if (!mine) return;
+    begin = a.starts[i];
+    end = a.starts[i + 1];
+    sequence = a.sequences[i];
+    if (sequence >= 0 && static_cast<uint32_t>(sequence) < a.cache.sequences) len = a.cache.lens[sequence];
+  }
+};
+
+// Fills table[0 .. count] (count + 1 entries: the last holds the totals); all
+// threads of the block. `first`: this thread's first request.
 __device__ void tree_table(const TreeArgs &a, uint32_t tokens, uint32_t kv_heads, uint32_t group, TreeEntry *table,
-                           uint32_t *scratch) {
+                           uint32_t *scratch, const TreeRequest &first) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const xpu_kv_cache_t &c = a.cache;
+  const int32_t longest = static_cast<int32_t>(c.table_width * c.page_size);
   uint32_t before = 0;
   bool bad = false;
   for (uint32_t at = 0; at < a.count; at += blockDim.x) {
-    const uint32_t i = at + threadIdx.x;
+    const TreeRequest r = at ? TreeRequest(a, at + threadIdx.x) : first;
     TreeEntry e{0, 0, 0, 0};
     uint32_t tiles = 0;
-    if (i < a.count) {
-      const int32_t begin = a.starts[i], end = a.starts[i + 1], s = a.sequences[i];
-      const bool listed = begin >= 0 && end >= begin && static_cast<uint32_t>(end) <= tokens;
-      const bool named = s >= 0 && static_cast<uint32_t>(s) < c.sequences;
-      int32_t len = named ? c.lens[s] : 0;
-      bad |= !listed || !named || len < 0 || static_cast<uint32_t>(len) > c.table_width * c.page_size ||
-             (listed && end - begin > static_cast<int32_t>(XPU_TREE_MAX_NODES));
-      len = min(max(len, 0), static_cast<int32_t>(c.table_width * c.page_size));
-      const uint32_t nodes = listed ? min(static_cast<uint32_t>(end - begin), XPU_TREE_MAX_NODES) : 0;
-      e.len = static_cast<uint32_t>(len);
-      e.begin = listed ? static_cast<uint32_t>(begin) : 0;
-      e.named = (named ? static_cast<uint32_t>(s) : 0) * 128u + nodes;
+    if (r.mine) {
+      const bool listed = r.begin >= 0 && r.end >= r.begin && static_cast<uint32_t>(r.end) <= tokens;
+      const bool named = r.sequence >= 0 && static_cast<uint32_t>(r.sequence) < c.sequences;
+      bad |= !listed || !named || r.len < 0 || r.len > longest ||
+             (listed && r.end - r.begin > static_cast<int32_t>(XPU_TREE_MAX_NODES));
+      const uint32_t nodes = listed ? min(static_cast<uint32_t>(r.end - r.begin), XPU_TREE_MAX_NODES) : 0;
+      e.len = static_cast<uint32_t>(min(max(r.len, 0), longest));
+      e.begin = listed ? static_cast<uint32_t>(r.begin) : 0;
+      e.named = (named ? static_cast<uint32_t>(r.sequence) : 0) * 128u + nodes;
       const uint32_t span = 2 * tile_positions(group);
       tiles = (nodes + span - 1) / span * kv_heads * entry_tiles(e);
     }
@@ -328,7 +346,7 @@ __device__ void tree_table(const TreeArgs &a, uint32_t tokens, uint32_t kv_heads
       const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
       if (lane >= o) inc += up;
     }
-    __syncthreads();
+    if (at) __syncthreads();
     if (lane == 31) scratch[warp] = inc;
     __syncthreads();
     uint32_t others = 0, all = 0;
@@ -337,17 +355,18 @@ __device__ void tree_table(const TreeArgs &a, uint32_t tokens, uint32_t kv_heads
       all += scratch[w];
     }
     e.first = before + others + inc - tiles;
-    if (i < a.count) table[i] = e;
+    if (r.mine) table[at + threadIdx.x] = e;
     before += all;
   }
   if (threadIdx.x == 0) table[a.count] = TreeEntry{before, 0, 0, 0};
   if (bad && blockIdx.x == 0) atomicOr(c.status, XPU_KV_BAD_INDEX);
-  __syncthreads();
 }
 
-// Key tiles per block: an even share, but at least two.
+// Key tiles per block: an even share. One tile each where there are no more
+// (2048 positions, 8 kv heads: 20.7 us; two each, with blocks that finish one unit
+// and begin the next, 27.2 us).
 __device__ __forceinline__ uint32_t tree_share(uint32_t tiles, uint32_t blocks) {
-  return max((tiles + blocks - 1) / blocks, 2u);
+  return max((tiles + blocks - 1) / blocks, 1u);
 }
 
 // This block's share of all (sequence, row block, kv head, key tile), in that order.
@@ -407,18 +426,20 @@ __device__ __forceinline__ uint32_t valid_keys(const Segment &s, uint32_t tile) 
 // product) to one row's columns [col, col + cols): dst16 (normalised by inv)
 // or dst32. Rare: plain loops over global memory.
 template <typename T, int D, bool TREE>
-__device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadRows *bad, uint32_t listed, uint32_t half,
-                                     uint32_t position, uint32_t q_head, uint64_t set, float m, float inv, T *dst16, float *dst32, uint32_t col,
+__device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadRows *bad, uint32_t position, uint32_t q_head,
+                                     uint64_t set, float m, float inv, T *dst16, float *dst32, uint32_t col,
                                      uint32_t cols) {
   const T *q = static_cast<const T *>(a.t.q) + (s.q0 - s.pos0 + static_cast<size_t>(position)) * a.t.q_stride + q_head * D;
   const float c = a.t.scale * kLog2e;
-  for (uint32_t i = 0; i < listed; ++i)
-    for (uint32_t j = 0; j < 64; ++j) {
-      if (!(bad->mask[i][j >> 5] >> (j & 31) & 1u)) continue;
-      const uint32_t in_tile = half * 64 + j;
-      const uint32_t key = bad->tile[i] * kKeys + in_tile;
+  for (uint32_t at = 0; at < 4 * 64; ++at) {  // half, listed tile, key of the half
+    const uint32_t half = at >> 7, i = at >> 6 & 1, j = at & 63;
+    const uint32_t listed = *const_cast<const volatile uint32_t *>(&bad[half].tiles);
+    __threadfence_block();
+    if (i >= listed || !(bad[half].mask[i][j >> 5] >> (j & 31) & 1u)) continue;
+    {
+      const uint32_t in_tile = half * 64 + j, tile = bad[half].tile[i], key = tile * kKeys + in_tile;
       const T *k, *v;
-      if (!TREE || bad->tile[i] * kKeys >= s.len) {  // packed: a prompt's key, or a draft
+      if (!TREE || tile * kKeys >= s.len) {  // packed: a prompt's key, or a draft
         if (TREE ? !(set >> in_tile & 1u) : key > position) continue;
         const size_t at = (static_cast<size_t>(s.base) + (TREE ? in_tile : key)) * a.t.kv_stride + s.head * D;
         k = static_cast<const T *>(a.t.k) + at;
@@ -440,6 +461,7 @@ __device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadR
         else dst16[d] = Elem<T>::from_float(fmaf(p * inv, Elem<T>::to_float(v[d]), Elem<T>::to_float(dst16[d])));
       }
     }
+  }
 }
 
 // ------------------------------------------------------------------- join ----
@@ -453,96 +475,127 @@ struct JoinRows {
   __device__ uint32_t row(uint32_t r) const { return r + (position(r) >= positions ? 128 - positions * group : 0); }
 };
 
-// Thread r of 256: row r's maximum over the parts of blocks c0 .. c1, and the
-// reciprocal of the sum, for join_rows; the row's lse.
-__device__ __forceinline__ void join_sums(const Args &a, const Segment &s, const float2 *sums, JoinRows rows, uint32_t share,
-                                          uint32_t c0, uint32_t c1, float2 *total) {
-  const uint32_t r = threadIdx.x;
-  if (r >= s.npos * rows.group) return;
-  const uint32_t row = rows.row(r);
-  const float c = a.t.scale * kLog2e;
-  float m = -INFINITY, l = 0.f;
-  for (uint32_t x0 = c0; x0 <= c1; x0 += 8) {  // eight loads in flight
-    float2 ml[8];
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) {
-      const uint32_t x = min(x0 + e, c1);
-      ml[e] = __ldcg(sums + (2 * x + (x * share >= s.unit ? 0 : 1)) * 256 + row);
-    }
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) {
-      if (x0 + e > c1) continue;
-      const float top = fmaxf(m, ml[e].x);
-      if (top == -INFINITY) continue;
-      l = l * exp2_approx((m - top) * c) + ml[e].y * exp2_approx((ml[e].x - top) * c);
-      m = top;
-    }
-  }
-  total[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
-  const uint32_t index = rows.position(r);
-  if (a.t.lse)
-    a.t.lse[(static_cast<size_t>(s.q0) + index) * a.t.q_heads + s.head * rows.group + r - index * rows.group] =
-        l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * kLn2;
-}
-
-// Warp `warp` of 8: rows of the unit, the parts in order; sixteen loads in
-// flight (one row after the other took 20 us where this takes 2).
+// Rows of a unit from the partial results of blocks c0 .. c1, added in that
+// order, by the 8 softmax warps. The loops are short on purpose: a block joins once or
+// twice, and code that runs once costs about six cycles an instruction to fetch.
+// Loads take 900 cycles, so each thread has sixteen of them in flight.
 template <typename T, int D>
-__device__ __forceinline__ void join_rows(const Args &a, const Segment &s, const float2 *sums, JoinRows rows, uint32_t share,
-                                          uint32_t c0, uint32_t c1, const float2 *total, uint32_t warp) {
-  constexpr uint32_t N = D / 32, kRows = 8, kParts = 2;  // N: this lane's columns
-  const uint32_t lane = threadIdx.x & 31, many = s.npos * rows.group;
-  const float c = a.t.scale * kLog2e;
-  for (uint32_t r0 = warp * kRows; r0 < many; r0 += 8 * kRows) {
-    float o[kRows][N] = {}, top[kRows];
-    uint32_t row[kRows];
+struct Join {
+  static constexpr uint32_t N = D / 32;  // this lane's columns
+  using Columns = typename std::conditional<N == 4, float4, float2>::type;
+  const Args &a;
+  const Segment &s;
+  JoinRows rows;
+  uint32_t share, c0, c1;
+  const float2 *sums;
+  float2 *total;  // shared memory: each row's maximum and reciprocal sum
+
+  __device__ uint32_t slot(uint32_t x) const { return (2 * x + (x * share >= s.unit ? 0 : 1)) * 256u; }
+  __device__ Columns part(uint32_t x, uint32_t row) const {
+    return __ldcg(reinterpret_cast<const Columns *>(a.tree.partial + static_cast<size_t>(slot(x) + row) * D) + (threadIdx.x & 31));
+  }
+  static __device__ void add(float w, const Columns &v, float (&o)[N]) {
 #pragma unroll
-    for (uint32_t i = 0; i < kRows; ++i) {
-      row[i] = rows.row(min(r0 + i, many - 1));
-      top[i] = total[min(r0 + i, many - 1)].x;
-    }
-    for (uint32_t x0 = c0; x0 <= c1; x0 += kParts) {
-      float part[kParts][kRows][N], m[kParts][kRows];
+    for (uint32_t n = 0; n < N; ++n) o[n] = fmaf(w, (&v.x)[n], o[n]);
+  }
+  __device__ void put(uint32_t r, const float (&o)[N], float inv) const {
+    const uint32_t index = rows.position(r), head = s.head * rows.group + r - index * rows.group;
+    uint32_t w[N / 2];
 #pragma unroll
-      for (uint32_t e = 0; e < kParts; ++e) {
-        const uint32_t x = min(x0 + e, c1), slot = 2 * x + (x * share >= s.unit ? 0 : 1);
+    for (uint32_t n = 0; n < N / 2; ++n) w[n] = pack2<T>(o[2 * n] * inv, o[2 * n + 1] * inv);
+    uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(a.t.out) + (static_cast<size_t>(s.q0) + index) * a.t.out_stride +
+                                                 head * D) + N / 2 * (threadIdx.x & 31);
+    if constexpr (N == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+    else *dst = w[0];
+  }
+  __device__ void put_lse(uint32_t r, float m, float l, float c) const {
+    const uint32_t index = rows.position(r), head = s.head * rows.group + r - index * rows.group;
+    if (a.t.lse) a.t.lse[(static_cast<size_t>(s.q0) + index) * a.t.q_heads + head] = log_sum(m, l, c);
+  }
+
+  // Up to eight rows: a warp each, lane x the weight of part x.
+  __device__ void few(uint32_t warp) const {
+    const uint32_t lane = threadIdx.x & 31, r = warp;
+    if (r >= s.npos * rows.group) return;
+    const float c = a.t.scale * kLog2e;
+    const uint32_t row = rows.row(r);
+    auto get = [&](uint32_t x) { return x <= c1 ? __ldcg(sums + slot(x) + row) : make_float2(-INFINITY, 0.f); };
+    float m = -INFINITY, l = 0.f, w = 0.f, o[N] = {};
+#pragma unroll 1
+    for (uint32_t x0 = c0; x0 <= c1; x0 += 32) m = fmaxf(m, warp_max(get(x0 + lane).x));
+#pragma unroll 1
+    for (uint32_t x0 = c0; x0 <= c1; x0 += 8) {
+      Columns v[8];
 #pragma unroll
-        for (uint32_t i = 0; i < kRows; ++i) {
-          const size_t at = slot * 256 + row[i];
-          m[e][i] = __ldcg(&sums[at].x);
-          const float *src = a.tree.partial + at * D + N * lane;
-          if constexpr (N == 4) {
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
-            part[e][i][0] = v.x, part[e][i][1] = v.y, part[e][i][2] = v.z, part[e][i][3] = v.w;
-          } else {
-            const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
-            part[e][i][0] = v.x, part[e][i][1] = v.y;
-          }
-        }
+      for (uint32_t e = 0; e < 8; ++e) v[e] = part(min(x0 + e, c1), row);
+      if (((x0 - c0) & 31) == 0) {
+        const float2 ml = get(x0 + lane);
+        w = ml.x == -INFINITY ? 0.f : exp2_approx((ml.x - m) * c);
+        l += warp_sum(w * ml.y);
       }
 #pragma unroll
-      for (uint32_t e = 0; e < kParts; ++e)
-#pragma unroll
-        for (uint32_t i = 0; i < kRows; ++i) {
-          const float w = x0 + e > c1 || m[e][i] == -INFINITY ? 0.f : exp2_approx((m[e][i] - top[i]) * c);
-#pragma unroll
-          for (uint32_t n = 0; n < N; ++n) o[i][n] = fmaf(w, part[e][i][n], o[i][n]);
-        }
+      for (uint32_t e = 0; e < 8; ++e) add(__shfl_sync(kFullMask, w, (x0 + e - c0) & 31), v[e], o);  // 0 past the last
     }
+    put(r, o, l == 0.f ? 0.f : 1.f / l);
+    if (lane == 0) put_lse(r, m, l, c);
+  }
+
+  // Any number: first a thread per row ...
+  __device__ void sum_rows() const {
+    const uint32_t r = threadIdx.x;
+    if (r >= s.npos * rows.group) return;
+    const float c = a.t.scale * kLog2e;
+    const uint32_t row = rows.row(r);
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (uint32_t x0 = c0; x0 <= c1; x0 += 4) {
+      float2 ml[4];
 #pragma unroll
-    for (uint32_t i = 0; i < kRows; ++i) {
-      const uint32_t r = r0 + i;
-      if (r >= many) break;
-      const float inv = total[r].y;
-      const uint32_t index = rows.position(r);
-      const size_t token = static_cast<size_t>(s.q0) + index;
-      uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(a.t.out) + token * a.t.out_stride +
-                                                   (s.head * rows.group + r - index * rows.group) * D) + N / 2 * lane;
+      for (uint32_t e = 0; e < 4; ++e) ml[e] = __ldcg(sums + slot(min(x0 + e, c1)) + row);
 #pragma unroll
-      for (uint32_t n = 0; n < N / 2; ++n) dst[n] = pack2<T>(o[i][2 * n] * inv, o[i][2 * n + 1] * inv);
+      for (uint32_t e = 0; e < 4; ++e) {
+        const float top = fmaxf(m, ml[e].x);
+        if (x0 + e > c1 || top == -INFINITY) continue;
+        l = l * exp2_approx((m - top) * c) + ml[e].y * exp2_approx((ml[e].x - top) * c);
+        m = top;
+      }
+    }
+    total[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
+    put_lse(r, m, l, c);
+  }
+  // ... then eight rows a warp at a time, part after part.
+  __device__ void many(uint32_t warp) const {
+    const uint32_t count = s.npos * rows.group;
+    const float c = a.t.scale * kLog2e;
+#pragma unroll 1
+    for (uint32_t r0 = warp; r0 < count; r0 += 64) {
+      float o[8][N] = {};
+      uint32_t row[8];
+      float2 sum[8];
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k) {
+        const uint32_t r = min(r0 + 8 * k, count - 1);
+        row[k] = rows.row(r);
+        sum[k] = total[r];
+      }
+#pragma unroll 1
+      for (uint32_t x = c0; x <= c1; ++x) {
+        Columns v[8];
+        float mx[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+          v[k] = part(x, row[k]);
+          mx[k] = __ldcg(&sums[slot(x) + row[k]].x);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) add(mx[k] == -INFINITY ? 0.f : exp2_approx((mx[k] - sum[k].x) * c), v[k], o[k]);
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 8; ++k)
+        if (r0 + 8 * k < count) put(r0 + 8 * k, o[k], sum[k].y);
     }
   }
-}
+};
 
 // ----------------------------------------------------------------- kernel ----
 
@@ -562,6 +615,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t group = a.t.q_heads / a.t.kv_heads, positions = tile_positions(group);
 
+  // the first memory accesses of all roles, under the set-up of the block
+  [[maybe_unused]] const TreeRequest request(a.tree, TREE ? threadIdx.x : 0xffffffffu);
+  if (threadIdx.x >= 32 && threadIdx.x < (TREE ? 37 : 35)) {
+    const CUtensorMap *map = threadIdx.x == 32 ? &a.q : threadIdx.x == 33 ? &a.k : threadIdx.x == 34 ? &a.v
+                             : threadIdx.x == 35 ? &a.cached_k : &a.cached_v;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   if (threadIdx.x == 0) {
     mbar_init(&b.q_full, 1);
     mbar_init(&b.q_empty, 1);
@@ -582,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     b.failed = 0;
   }
   if (warp == kMmaWarp) tmem_alloc1(&b.tmem, 512);
-  if (TREE) tree_table(a.tree, a.t.tokens, a.t.kv_heads, group, table, scratch);
+  if (TREE) tree_table(a.tree, a.t.tokens, a.t.kv_heads, group, table, scratch, request);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -630,20 +690,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         tmem_wait_ld64(x);
         tmem_ld32(s_addr + 64, x + 64);
         tmem_ld32(s_addr + 96, x + 96);
-        uint32_t keep_lo = 0, keep_hi = 0, many = 0;  // keys that this row attends: a set of 64, or the first `many`
-        const bool drafts = TREE && tile * kKeys >= s.len;
-        if (drafts) {
-          keep_lo = static_cast<uint32_t>(set) & (s.nodes >= 32 ? 0xffffffffu : (1u << s.nodes) - 1u);
-          keep_hi = static_cast<uint32_t>(set >> 32) &
-                    (s.nodes >= 64 ? 0xffffffffu : (s.nodes > 32 ? (1u << (s.nodes - 32)) - 1u : 0u));
-        } else {
-          many = (TREE ? s.len : position + 1) - min(tile * kKeys, TREE ? s.len : position + 1);
-        }
+        uint32_t attended[4];  // this row's keys of the tile, a bit each
         if (masked) {
+          if (TREE && tile * kKeys >= s.len) {  // the drafts
+            const uint64_t own = set & (s.nodes >= 64 ? ~0ull : (1ull << s.nodes) - 1);
+            attended[0] = static_cast<uint32_t>(own), attended[1] = static_cast<uint32_t>(own >> 32);
+            attended[2] = attended[3] = 0;
+          } else {
+            const uint32_t end = TREE ? s.len : position + 1, many = end - min(tile * kKeys, end);
 #pragma unroll
-          for (uint32_t j = 0; j < 64; ++j)
-            if (drafts ? !((j < 32 ? keep_lo >> j : keep_hi >> (j - 32)) & 1u) : j >= many) x[j] = 0xff800000u;
+            for (uint32_t w = 0; w < 4; ++w)
+              attended[w] = many >= 32 * (w + 1) ? 0xffffffffu : many > 32 * w ? (1u << (many - 32 * w)) - 1u : 0u;
+          }
         }
+        auto mask = [&](uint32_t from) {
+#pragma unroll
+          for (uint32_t j = from; j < from + 64; ++j)
+            if (!(attended[j >> 5] & 1u << (j & 31))) x[j] = 0xff800000u;
+        };
+        if (masked) mask(0);
         // p of 32 keys from x[32 q] on, in pairs, and their sum
         const Pair c2(c, c);
         Pair sum0(0.f, 0.f), sum1(0.f, 0.f);
@@ -681,11 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         };
         search(0);
         tmem_wait_ld64(x + 64);
-        if (masked) {
-#pragma unroll
-          for (uint32_t j = 64; j < kKeys; ++j)
-            if (drafts || j >= many) x[j] = 0xff800000u;
-        }
+        if (masked) mask(64);
         search(64);
         const float top = max3_nan(max3_nan(top4[0], top4[1], top4[2]), top4[3], top4[3]);
         const bool grown = top != m && !((top - m) * c <= kRescale);  // m = -inf included, and NaN
@@ -756,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
             ml[1] = l;
           }
         } else if (mine && a.t.lse && col == 0 && token < a.t.tokens) {
-          a.t.lse[token * a.t.q_heads + q_head] = l == 0.f ? -INFINITY : fmaf(m, c, log2f(l)) * kLn2;
+          a.t.lse[token * a.t.q_heads + q_head] = log_sum(m, l, c);
         }
         const bool store = mine && token < a.t.tokens;
 #pragma unroll 1
@@ -800,13 +861,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           }
         }
         if (store && s.first + s.n > s.masked_from) {
-          for (uint32_t half = 0; half < 2; ++half) {
-            const BadRows *bad = &b.bad[segment % kBadRing][half];
-            const uint32_t listed = *const_cast<const volatile uint32_t *>(&bad->tiles);
-            __threadfence_block();
-            if (listed)
-              fix_row<T, D, TREE>(a, s, bad, listed, half, position, q_head, set, m, inv, dst16, dst32, col, cols);
-          }
+          const BadRows *bad = b.bad[segment % kBadRing];
+          if (*const_cast<const volatile uint32_t *>(&bad[0].tiles) | *const_cast<const volatile uint32_t *>(&bad[1].tiles))
+            fix_row<T, D, TREE>(a, s, bad, position, q_head, set, m, inv, dst16, dst32, col, cols);
         }
       }
       if constexpr (TREE) {
@@ -818,16 +875,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           if (threadIdx.x == 0) {
             __threadfence();
             last = atomicAdd(a.tree.arrived + c0, 1u) == c1 - c0;
-            if (last) a.tree.arrived[c0] = 0;
-            __threadfence();
+            if (last) {
+              a.tree.arrived[c0] = 0;
+              __threadfence();
+            }
           }
           if (!meet()) break;
           if (last) {
             const float2 *sums = reinterpret_cast<const float2 *>(a.tree.partial + 2ull * gridDim.x * 256 * D);
-            float2 *total = reinterpret_cast<float2 *>(&joined[0][0][0]);
-            join_sums(a, s, sums, JoinRows(group, positions), walk.share, c0, c1, total);
-            if (!meet()) break;
-            join_rows<T, D>(a, s, sums, JoinRows(group, positions), walk.share, c0, c1, total, warp);
+            const Join<T, D> join{a, s, JoinRows(group, positions), walk.share, c0, c1, sums,
+                                  reinterpret_cast<float2 *>(&joined[0][0][0])};
+            if (s.npos * group <= 8) {
+              join.few(warp);
+            } else {
+              join.sum_rows();
+              if (!meet()) break;
+              join.many(warp);
+            }
           }
           if (!meet()) break;
         } else if (s.both && !meet()) {  // the other group may still read this one's accumulator and sums
@@ -850,7 +914,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     const uint64_t q_desc = smem_desc(smem0, 16, 1024);
     const uint64_t k_desc = smem_desc(smem0 + 2 * S::kTile, 16, 1024), v_desc = smem_desc(smem0 + 2 * S::kTile, kBox, 1024);
     uint32_t slot = 0, phase = 0;  // the ring's next entry: K 0, V 0, K 1, V 1, ...
-    uint32_t cleaned = 0, p_uses0 = 0, p_uses1 = 0, segment = 0;
+    uint32_t cleaned = 0, p_uses = 0, segment = 0;  // phases: a bit per ring entry, per row tile
     const bool leader = elect_one();
     bool ok = true;
     auto advance = [&](uint32_t &at, uint32_t &ph) {
@@ -858,36 +922,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     };
     auto commit = [&](uint64_t *bar) {
       if (leader) mma1_commit(bar);
-    };
-    auto qk = [&](uint32_t t, uint64_t dq, uint32_t at) {
-      const uint64_t dk = k_desc + (at * S::kTile >> 4);
-      if (leader) {
-#pragma unroll
-        for (uint32_t kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4 * kBox + kk % 4 * 32) >> 4;
-          mma1_f16(tm + t * 128, dq + off, dk + off, qk_desc, kk != 0);
-        }
-        mma1_commit(&b.s_full[t]);
-      }
-    };
-    auto pv = [&](uint32_t t, uint32_t &uses, uint32_t at, uint32_t accumulate) {
-      const uint64_t dv = v_desc + (at * S::kTile >> 4);
-      if (!warp_wait(b, &b.p_early[t], uses & 1)) return false;
-      tc_fence_after();
-      if (leader) {
-#pragma unroll
-        for (uint32_t kk = 0; kk < kEarlyKeys / 16; ++kk)
-          mma1_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, dv + (kk * 2048u >> 4), pv_desc, kk ? 1 : accumulate);
-      }
-      if (!warp_wait(b, &b.p_ready[t], uses & 1)) return false;
-      tc_fence_after();
-      if (leader) {
-#pragma unroll
-        for (uint32_t kk = kEarlyKeys / 16; kk < kKeys / 16; ++kk)
-          mma1_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, dv + (kk * 2048u >> 4), pv_desc, 1);
-      }
-      ++uses;
-      return true;
     };
     auto clean = [&](uint32_t tile, uint32_t at) {
       if (tile < s.masked_from) return true;
@@ -897,79 +931,75 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     };
     for (; ok && walk.next(s); ++segment) {
       s.n = same(s.n), s.n0 = same(s.n0), s.n1 = same(s.n1), s.first = same(s.first);
-      s.masked_from = same(s.masked_from), s.both = same(s.both);
-      ok = warp_wait(b, &b.q_full, segment & 1) && warp_wait(b, &b.kv_full[slot], phase);
-      if (!ok) break;
-      tc_fence_after();
-      qk(0, q_desc, slot);
-      if (s.both) {
-        // row tile 0's even key tiles with accumulator 0, its odd ones with 1
-        commit(&b.kv_empty[slot]);
-        uint32_t v = slot, v_phase = phase;
-        advance(v, v_phase);  // V 0
-        uint32_t k = v, k_phase = v_phase;
-        advance(k, k_phase);  // K 1
-        if (s.n > 1) {
-          if (!(ok = warp_wait(b, &b.kv_full[k], k_phase))) break;
-          tc_fence_after();
-          qk(1, q_desc, k);
-          commit(&b.kv_empty[k]);
-        }
-        if (s.n <= 2) commit(&b.q_empty);
-        for (uint32_t j = 0; ok && j < s.n; ++j) {
-          advance(k, k_phase);
-          advance(k, k_phase);  // K j + 2
-          ok = warp_wait(b, &b.kv_full[v], v_phase) && clean(s.first + j, v) &&
-               (j & 1 ? pv(1, p_uses1, v, j > 1) : pv(0, p_uses0, v, j > 1));
-          if (!ok) break;
-          commit(&b.kv_empty[v]);
-          if (j + 2 >= s.n) {
-            commit(&b.o_full[j & 1]);
-          } else {
-            if (!(ok = warp_wait(b, &b.kv_full[k], k_phase))) break;
+      s.masked_from = same(s.masked_from);
+      if (TREE) s.both = same(s.both);
+      if (!(ok = warp_wait(b, &b.q_full, segment & 1))) break;
+      // Turn j: O_t += P_t V_j, then S_t of the key tile that t comes to next, for t =
+      // 0 and 1; with both groups on row tile 0, t = j & 1 alone. One place for each
+      // product keeps the code short.
+      const bool both = TREE && s.both;
+      const uint32_t ahead = both ? 2 : 1;
+      uint32_t v = slot, v_phase = phase, k = slot, k_phase = phase;  // next V and next K
+      advance(v, v_phase);
+      uint32_t seen = 0;  // K tiles known to be there
+      for (int32_t j = -static_cast<int32_t>(ahead); ok && j < static_cast<int32_t>(s.n); ++j) {
+        const uint32_t next = static_cast<uint32_t>(j) + ahead;  // key tile of this turn's S
+        if (j >= 0 && !(ok = warp_wait(b, &b.kv_full[v], v_phase) && clean(s.first + j, v))) break;
+        const uint64_t dv = v_desc + (v * S::kTile >> 4), dk = k_desc + (k * S::kTile >> 4);
+#pragma unroll(TREE ? 1 : 2)
+        for (uint32_t t = both ? j & 1 : 0; t < (both ? (j & 1) + 1u : 2u); ++t) {
+          const uint32_t tiles = both ? s.n : t ? s.n1 : s.n0, s_tmem = tm + t * 128, o_tmem = s_tmem + 256;
+          if (j >= 0 && static_cast<uint32_t>(j) < tiles) {
+            const uint32_t accumulate = j >= static_cast<int32_t>(ahead), uses = p_uses >> t & 1;
+            if (!(ok = warp_wait(b, &b.p_early[t], uses))) break;
             tc_fence_after();
-            if (j & 1) qk(1, q_desc, k);
-            else qk(0, q_desc, k);
-            commit(&b.kv_empty[k]);
-            if (j + 3 == s.n) commit(&b.q_empty);
+            if (leader) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < kEarlyKeys / 16; ++kk)
+                mma1_ts(o_tmem, s_tmem + kk * 8, dv + (kk * 2048u >> 4), pv_desc, kk ? 1 : accumulate);
+            }
+            if (!(ok = warp_wait(b, &b.p_ready[t], uses))) break;
+            tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (uint32_t kk = kEarlyKeys / 16; kk < kKeys / 16; ++kk)
+                mma1_ts(o_tmem, s_tmem + kk * 8, dv + (kk * 2048u >> 4), pv_desc, 1);
+            }
+            p_uses ^= 1u << t;
+            if (next >= tiles) commit(&b.o_full[t]);
           }
+          if (next < tiles) {
+            if (seen <= next) {
+              if (!(ok = warp_wait(b, &b.kv_full[k], k_phase))) break;
+              tc_fence_after();
+              seen = next + 1;
+            }
+            const uint64_t dq = q_desc + (both ? 0 : t * (S::kTile >> 4));
+            if (leader) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = (kk / 4 * kBox + kk % 4 * 32) >> 4;
+                mma1_f16(s_tmem, dq + off, dk + off, qk_desc, kk != 0);
+              }
+              mma1_commit(&b.s_full[t]);
+            }
+          }
+        }
+        if (!ok) break;
+        if (j >= 0) {
+          commit(&b.kv_empty[v]);
           slot = v, phase = v_phase;
           advance(v, v_phase);
           advance(v, v_phase);
         }
-        advance(slot, phase);
-        continue;
+        if (next < s.n) {
+          commit(&b.kv_empty[k]);
+          if (next + 1 == s.n) commit(&b.q_empty);
+          advance(k, k_phase);
+          advance(k, k_phase);
+        }
       }
-      if (s.n1) qk(1, q_desc + (S::kTile >> 4), slot);
-      commit(&b.kv_empty[slot]);
-      if (s.n == 1) commit(&b.q_empty);
       advance(slot, phase);
-      for (uint32_t j = 0; j < s.n; ++j) {
-        const uint32_t v = slot;
-        if (!(ok = warp_wait(b, &b.kv_full[v], phase) && clean(s.first + j, v))) break;
-        advance(slot, phase);
-        const bool more0 = j + 1 < s.n0, more1 = j + 1 < s.n1;
-        if (j < s.n0) {
-          if (!(ok = pv(0, p_uses0, v, j != 0))) break;
-          if (!more0) commit(&b.o_full[0]);
-        }
-        if (more0 || more1) {
-          if (!(ok = warp_wait(b, &b.kv_full[slot], phase))) break;
-          tc_fence_after();
-        }
-        if (more0) qk(0, q_desc, slot);
-        if (j < s.n1) {
-          if (!(ok = pv(1, p_uses1, v, j != 0))) break;
-          if (!more1) commit(&b.o_full[1]);
-        }
-        commit(&b.kv_empty[v]);
-        if (more1) qk(1, q_desc + (S::kTile >> 4), slot);
-        if (more0 || more1) {
-          commit(&b.kv_empty[slot]);
-          if (j + 2 == s.n) commit(&b.q_empty);
-          advance(slot, phase);
-        }
-      }
       ok = ok && !warp_failed(b);
     }
     if (!ok) {  // nothing issued may still run when TMEM is freed
@@ -1014,6 +1044,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           more = walk.next(following);
           if (more) next_page = page_of(following, following.first);
         }
+#pragma unroll 1
         for (uint32_t which = 0; which < 2; ++which) {
           const uint32_t slot = loaded % S::kStages, use = loaded / S::kStages;
           if (use > 0 && !(ok = warp_wait(b, &b.kv_empty[slot], (use - 1) & 1))) break;
@@ -1074,7 +1105,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         }
         const uint32_t valid = valid_keys<TREE>(s, tile);
         uint32_t any = 0;
-#pragma unroll
+#pragma unroll 1
         for (uint32_t g = 0; g < 2; ++g) {
           const uint32_t key = half * 64 + g * 32 + lane;
           uint8_t *row = ring + slot * S::kTile + key * 128;

@@ -166,23 +166,28 @@ def _packed(name: str, t: torch.Tensor, heads: int, head_dim: int) -> int:
 
 
 def _attention_args(q, k, v, kv_heads, head_dim, scale, out, lse):
-    tokens, q_heads = q.shape[0], q.shape[1]
-    dtype = q.dtype
+    dtype, shape, kv_shape = q.dtype, q.shape, k.shape
     if k.dtype != dtype or v.dtype != dtype:
         raise ValueError("q, k and v must have one dtype")
-    q_stride, kv_stride = _packed("q", q, q_heads, head_dim), _packed("k", k, kv_heads, head_dim)
-    if _packed("v", v, kv_heads, head_dim) != kv_stride or k.shape[0] != tokens or v.shape[0] != tokens:
-        raise ValueError("k and v need q's tokens and one row stride")
-    out_stride = q_heads * head_dim
+    if len(shape) != 3 or shape[2] != head_dim or kv_shape != (shape[0], kv_heads, head_dim) or v.shape != kv_shape:
+        raise ValueError(f"q must be [tokens, q_heads, {head_dim}], k and v [tokens, {kv_heads}, {head_dim}]")
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise ValueError("libxpu_cuda entry points take CUDA tensors")
+    q_stride = out_stride = shape[1] * head_dim
+    kv_stride = kv_heads * head_dim
+    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
+        q_stride, kv_stride = _packed("q", q, shape[1], head_dim), _packed("k", k, kv_heads, head_dim)
+        if _packed("v", v, kv_heads, head_dim) != kv_stride:
+            raise ValueError("k and v need one row stride")
     if out is None:
-        out = torch.empty(tokens, q_heads, head_dim, dtype=dtype, device=q.device)
-    elif out.dtype != dtype or out.shape != q.shape:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.dtype != dtype or out.shape != shape:
         raise ValueError("out must have q's shape and dtype")
     else:
-        out_stride = _packed("out", out, q_heads, head_dim)
+        out_stride = _packed("out", out, shape[1], head_dim)
     if lse is None:
-        lse = torch.empty(tokens, q_heads, dtype=torch.float32, device=q.device)
-    elif lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_cuda or not lse.is_contiguous():
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device)
+    elif lse.dtype != torch.float32 or lse.shape != shape[:2] or not lse.is_cuda or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, q_heads]")
     return out, lse, q_stride, kv_stride, out_stride, head_dim ** -0.5 if scale is None else scale
 
