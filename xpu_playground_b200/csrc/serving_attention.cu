@@ -21,8 +21,8 @@
 //             P_t V (P from TMEM, V as it stands in memory, MN-major); S_t overwrites
 //             the P_t that the product before it read. While one tile is in its
 //             softmax the tensor cores work for the other;
-//   9         TMA loads: Q tiles, and a ring of K and V tiles;
-//   10, 11    cleaning: in key tiles with masked keys, V rows that no row may
+//   9         TMA loads: Q tiles, and a ring of K and V tiles (trees: V by warp 10);
+//   10, 11    cleaning (trees: 11): in key tiles with masked keys, V rows that no row may
 //             attend are zeroed (0 x NaN would reach the sums), and rows with
 //             non-finite values are zeroed and listed; the rows that do attend
 //             them get p v added at the end (fix_row).
@@ -69,7 +69,7 @@ struct Shape {
   static constexpr uint32_t kSmem = 1024 + (2 + kStages) * kTile;
 };
 
-struct BadRows {  // one cleaning warp's half (64 keys): listed keys of up to two tiles of a segment
+struct BadRows {  // listed keys of one half (64 keys) of up to two tiles of a segment
   uint32_t tiles;
   uint32_t tile[2], mask[2][2];
 };
@@ -628,8 +628,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     mbar_init(&b.drain, 1);
     for (uint32_t i = 0; i < S::kStages; ++i) {
       mbar_init(&b.kv_full[i], 1);
-      mbar_init(&b.kv_empty[i], 3);  // the products and both cleaning warps
-      mbar_init(&b.clean[i], 2);
+      mbar_init(&b.kv_empty[i], TREE ? 2 : 3);  // the products and the cleaning warps
+      mbar_init(&b.clean[i], TREE ? 1 : 2);
     }
     for (uint32_t i = 0; i < 2; ++i) {
       mbar_init(&b.s_full[i], 1);
@@ -967,6 +967,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
             }
             p_uses ^= 1u << t;
             if (next >= tiles) commit(&b.o_full[t]);
+            // the ring entry is free before the wait for the next one
+            if (both || t == (static_cast<uint32_t>(j) < s.n1 ? 1 : 0)) commit(&b.kv_empty[v]);
           }
           if (next < tiles) {
             if (seen <= next) {
@@ -987,7 +989,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         }
         if (!ok) break;
         if (j >= 0) {
-          commit(&b.kv_empty[v]);
           slot = v, phase = v_phase;
           advance(v, v_phase);
           advance(v, v_phase);
@@ -1007,9 +1008,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
       commit(&b.drain);
       warp_wait(b, &b.drain, 0);
     }
-  } else if (warp == kLoadWarp) {
+  } else if (warp == kLoadWarp || (TREE && warp == kLoadWarp + 1)) {
     // --------------------------------------------------------------- loads ----
-    uint32_t loaded = 0, segment = 0, q_loads = 0;
+    // A tree's key tile is up to 16 copies of a page, too many for one warp to issue
+    // in the time that they take: one warp loads K, another V. The ring then has an even
+    // number of entries, so that each warp sees every turn of its own.
+    static_assert(!TREE || S::kStages % 2 == 0, "K and V keep to their entries");
+    static_assert(S::kStages >= 4, "the products hold up to three entries");
+    const uint32_t first_which = TREE ? warp - kLoadWarp : 0, last_which = TREE ? first_which : 1;
+    const bool leader = elect_one();
+    uint32_t loaded = first_which, segment = 0, q_loads = 0;
     // lane p: the id of page p of a cached key tile (behind the pool, where reads
     // give zeros, if it is out of range)
     auto page_of = [&](const Segment &g, uint32_t tile) {
@@ -1045,14 +1053,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           if (more) next_page = page_of(following, following.first);
         }
 #pragma unroll 1
-        for (uint32_t which = 0; which < 2; ++which) {
+        for (uint32_t which = first_which; which <= last_which; ++which) {
           const uint32_t slot = loaded % S::kStages, use = loaded / S::kStages;
           if (use > 0 && !(ok = warp_wait(b, &b.kv_empty[slot], (use - 1) & 1))) break;
           uint64_t *bar = &b.kv_full[slot];
           uint8_t *dst = ring + slot * S::kTile;
-          ++loaded;
+          loaded += TREE ? 2 : 1;
           if (packed) {
-            if (lane == 0) {
+            if (leader) {
               // a tree's drafts: half a tile, XPU_TREE_MAX_NODES rows
               mbar_expect_tx(bar, TREE ? S::kTile / 2 : S::kTile);
               for (uint32_t h = 0; h < S::kBoxes; ++h)
@@ -1061,17 +1069,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           } else {
             const xpu_kv_cache_t &kc = a.tree.cache;
             const uint32_t bytes = kc.page_size * 128, pages = (min(kKeys, s.len - at) + kc.page_size - 1) >> a.tree.page_shift;
-            if (lane == 0) mbar_expect_tx(bar, pages * bytes * S::kBoxes);
-            __syncwarp();
-            if (lane < pages) {
-              const int32_t row = static_cast<int32_t>((static_cast<uint32_t>(page) * kc.kv_heads + s.head) * kc.page_size);
-              for (uint32_t h = 0; h < S::kBoxes; ++h)
-                tma_load_2d_plain(dst + h * kBox + lane * bytes, which ? &a.cached_v : &a.cached_k, 64 * h, row, bar);
+            const uint32_t row = (static_cast<uint32_t>(page) * kc.kv_heads + s.head) * kc.page_size;
+            if (leader) mbar_expect_tx(bar, pages * bytes * S::kBoxes);
+#pragma unroll 1
+            for (uint32_t p = 0; p < pages; ++p) {
+              const int32_t y = static_cast<int32_t>(__shfl_sync(kFullMask, row, p));
+              if (leader) {
+#pragma unroll
+                for (uint32_t h = 0; h < S::kBoxes; ++h)
+                  tma_load_2d_plain(dst + h * kBox + p * bytes, which ? &a.cached_v : &a.cached_k, 64 * h, y, bar);
+              }
             }
           }
           if (j == 0 && which == 0) {  // after the first keys, which need not wait for the last segment's rows
             if (segment > 0 && !(ok = warp_wait(b, &b.q_empty, (segment - 1) & 1))) break;
-            if (lane == 0) {
+            if (leader) {
               const uint32_t tiles = !s.both && s.npos > positions ? 2 : 1;
               mbar_expect_tx(&b.q_full, tiles * positions * group * 128 * S::kBoxes);
               for (uint32_t t = 0; t < tiles; ++t)
@@ -1084,18 +1096,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
       }
     }
     if (warp_failed(b)) {  // what was asked for lands before the block's memory is given up
-      for (uint32_t i = loaded > S::kStages ? loaded - S::kStages : 0; i < loaded; ++i)
+      for (uint32_t i = loaded > S::kStages ? loaded - S::kStages : first_which; i < loaded; i += TREE ? 2 : 1)
         mbar_wait(&b.kv_full[i % S::kStages], i / S::kStages & 1);
       if (q_loads) mbar_wait(&b.q_full, (q_loads - 1) & 1);
     }
   } else {
     // ------------------------------------------------------------ cleaning ----
-    const uint32_t half = warp - kCleanWarp;  // keys 64 half .. + 63 of a tile
+    // keys 64 half .. of a tile: a warp each half, or (trees) one warp both
+    const uint32_t half0 = TREE ? 0 : warp - kCleanWarp;
     uint32_t loaded = 0, segment = 0;
     for (; walk.next(s) && !warp_failed(b); ++segment) {
-      BadRows *bad = &b.bad[segment % kBadRing][half];
-      uint32_t listed = 0;
-      if (lane == 0 && s.first + s.n > s.masked_from) bad->tiles = 0;
+      BadRows *bad = &b.bad[segment % kBadRing][half0];
+      uint32_t listed[2] = {0, 0};
+      if (lane < (TREE ? 2 : 1) && s.first + s.n > s.masked_from) bad[lane].tiles = 0;
+      __syncwarp();
       for (uint32_t e = 0; e < 2 * s.n; ++e) {  // every ring entry, so as never to be a turn ahead or behind
         const uint32_t i = loaded + e, slot = i % S::kStages, tile = s.first + e / 2;
         if (!warp_wait(b, &b.kv_full[slot], i / S::kStages & 1)) break;
@@ -1104,40 +1118,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           continue;
         }
         const uint32_t valid = valid_keys<TREE>(s, tile);
-        uint32_t any = 0;
+#pragma unroll
+        for (uint32_t h = 0; h < (TREE ? 2 : 1); ++h) {
+          uint32_t any = 0;
 #pragma unroll 1
-        for (uint32_t g = 0; g < 2; ++g) {
-          const uint32_t key = half * 64 + g * 32 + lane;
-          uint8_t *row = ring + slot * S::kTile + key * 128;
-          const bool inside = key < valid;
-          uint32_t sums[4] = {0, 0, 0, 0};
-          if (inside) {
+          for (uint32_t g = 0; g < 2; ++g) {
+            const uint32_t key = (half0 + h) * 64 + g * 32 + lane;
+            uint8_t *row = ring + slot * S::kTile + key * 128;
+            const bool inside = key < valid;
+            uint32_t sums[4] = {0, 0, 0, 0};
+            if (inside) {
 #pragma unroll
-            for (uint32_t x = 0; x < 8 * S::kBoxes; ++x) {  // 16-byte pieces, each lane from another bank
-              const uint4 w = *reinterpret_cast<const uint4 *>(row + x / 8 * kBox + ((x + lane) & 7) * 16);
-              sums[0] = add_zero_times<T>(w.x, sums[0]);
-              sums[1] = add_zero_times<T>(w.y, sums[1]);
-              sums[2] = add_zero_times<T>(w.z, sums[2]);
-              sums[3] = add_zero_times<T>(w.w, sums[3]);
+              for (uint32_t x = 0; x < 8 * S::kBoxes; ++x) {  // 16-byte pieces, each lane from another bank
+                const uint4 w = *reinterpret_cast<const uint4 *>(row + x / 8 * kBox + ((x + lane) & 7) * 16);
+                sums[0] = add_zero_times<T>(w.x, sums[0]);
+                sums[1] = add_zero_times<T>(w.y, sums[1]);
+                sums[2] = add_zero_times<T>(w.z, sums[2]);
+                sums[3] = add_zero_times<T>(w.w, sums[3]);
+              }
             }
-          }
-          const bool spoilt = ((sums[0] | sums[1] | sums[2] | sums[3]) & 0x7fff7fffu) != 0;
-          if (!inside || spoilt) {
+            const bool spoilt = ((sums[0] | sums[1] | sums[2] | sums[3]) & 0x7fff7fffu) != 0;
+            if (!inside || spoilt) {
 #pragma unroll
-            for (uint32_t x = 0; x < 8 * S::kBoxes; ++x)
-              *reinterpret_cast<uint4 *>(row + x / 8 * kBox + ((x + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+              for (uint32_t x = 0; x < 8 * S::kBoxes; ++x)
+                *reinterpret_cast<uint4 *>(row + x / 8 * kBox + ((x + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            const uint32_t found = __ballot_sync(kFullMask, spoilt);
+            any |= found;
+            if (lane == 0 && listed[h] < 2) bad[h].mask[listed[h]][g] = found;
           }
-          const uint32_t found = __ballot_sync(kFullMask, spoilt);
-          any |= found;
-          if (lane == 0 && listed < 2) bad->mask[listed][g] = found;
-        }
-        if (any && listed < 2) {
-          if (lane == 0) {
-            bad->tile[listed] = tile;
-            __threadfence_block();
-            *const_cast<volatile uint32_t *>(&bad->tiles) = listed + 1;
+          if (any && listed[h] < 2) {
+            if (lane == 0) {
+              bad[h].tile[listed[h]] = tile;
+              __threadfence_block();
+              *const_cast<volatile uint32_t *>(&bad[h].tiles) = listed[h] + 1;
+            }
+            ++listed[h];
           }
-          ++listed;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
