@@ -262,6 +262,48 @@ __device__ __forceinline__ uint32_t add_zero_times(uint32_t w, uint32_t sum) {
   return d;
 }
 
+// Rows of 64 bytes, one in each lane's registers, stored so that the four lanes
+// of a quad write one row at a time: 64 bytes in a row where a lane's own row
+// would make 32 lines of every store (the epilogue took 4000 cycles that way).
+struct QuadRows {
+  unsigned long long row[4];  // the quad's rows
+  uint32_t stores;            // a bit per lane whose row is stored
+  __device__ QuadRows(void *own, bool store) {
+    const uint32_t lane = threadIdx.x & 31;
+    stores = __ballot_sync(kFullMask, store);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      row[k] = __shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(own), (lane & 28) + k) + (lane & 3) * 16;
+  }
+  __device__ bool any() const { return stores != 0; }
+  // 16 words of this lane's row, for its bytes `at` ...
+  __device__ void put(const uint32_t *w, uint32_t at) const {
+    const uint32_t lane = threadIdx.x & 31;
+    uint4 v[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) v[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    // a 4 x 4 transposition: lane i of the quad ends with piece i of row k in v[k]
+    auto swap = [&](uint4 &low, uint4 &high, uint32_t bit) {
+      const bool up = lane & bit;
+      const uint4 away = up ? low : high;
+      uint4 come;
+      come.x = __shfl_xor_sync(kFullMask, away.x, bit);
+      come.y = __shfl_xor_sync(kFullMask, away.y, bit);
+      come.z = __shfl_xor_sync(kFullMask, away.z, bit);
+      come.w = __shfl_xor_sync(kFullMask, away.w, bit);
+      if (up) low = come;
+      else high = come;
+    };
+    swap(v[0], v[1], 1);
+    swap(v[2], v[3], 1);
+    swap(v[0], v[2], 2);
+    swap(v[1], v[3], 2);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      if (stores >> ((lane & 28) + k) & 1u) *reinterpret_cast<uint4 *>(row[k] + at) = v[k];
+  }
+};
+
 // --------------------------------------------------------------- segments ----
 
 // The prompt plan's items of this block, in order.
@@ -787,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         tc_fence_after();
       }
       // ---------------------------------------------------- join and write ----
-      float weight[2] = {t == 0 ? 1.f : 0.f, t == 0 ? 0.f : 1.f};
+      [[maybe_unused]] float weight[2] = {1.f, 1.f};
       uint32_t col = 0, cols = D;
       if (TREE && s.both) {
         joined[t][r][0] = m;
@@ -820,45 +862,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           a.t.lse[token * a.t.q_heads + q_head] = log_sum(m, l, c);
         }
         const bool store = mine && token < a.t.tokens;
+        const QuadRows out(TREE && dst32 ? static_cast<void *>(dst32) : dst16, store);
+        if (out.any()) {
 #pragma unroll 1
-        for (uint32_t q = col; q < col + cols; q += 32) {
-          uint32_t o[32];
-          if (!TREE || !s.both) {
-            tmem_ld32(o_addr + t * 128 + q, o);
+          for (uint32_t q = col; q < col + cols; q += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + (TREE && s.both ? 0 : t * 128) + q, o);
             tmem_wait_ld();
+            const float w0 = TREE && s.both ? weight[0] * inv : inv;
 #pragma unroll
-            for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
-          } else {
-            tmem_ld32(o_addr + q, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * weight[0]);
-            if (s.n1) {
+            for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * w0);
+            if (TREE && s.both && s.n1) {
               uint32_t o1[32];
               tmem_ld32(o_addr + 128 + q, o1);
               tmem_wait_ld();
+              const float w1 = weight[1] * inv;
 #pragma unroll
               for (uint32_t j = 0; j < 32; ++j)
-                o[j] = __float_as_uint(fmaf(__uint_as_float(o1[j]), weight[1], __uint_as_float(o[j])));
+                o[j] = __float_as_uint(fmaf(__uint_as_float(o1[j]), w1, __uint_as_float(o[j])));
             }
+            if (TREE && dst32) {
 #pragma unroll
-            for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
-          }
-          if (!store) continue;
-          if (TREE && dst32) {
+              for (uint32_t h = 0; h < 32; h += 16) out.put(&o[h], (q + h) * 4);
+            } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 32; j += 4)
-              *reinterpret_cast<uint4 *>(dst32 + q + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-          } else {
-#pragma unroll
-            for (uint32_t j = 0; j < 32; j += 8) {
-              uint32_t w[4];
-#pragma unroll
-              for (uint32_t e = 0; e < 4; ++e)
-                w[e] = pack2<T>(__uint_as_float(o[j + 2 * e]), __uint_as_float(o[j + 2 * e + 1]));
-              *reinterpret_cast<uint4 *>(dst16 + q + j) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (uint32_t j = 0; j < 16; ++j) o[j] = pack2<T>(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
+              out.put(o, q * 2);
             }
           }
+          __syncwarp();  // a row's lane sees what its quad wrote of it
         }
         if (store && s.first + s.n > s.masked_from) {
           const BadRows *bad = b.bad[segment % kBadRing];
