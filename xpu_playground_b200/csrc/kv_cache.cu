@@ -288,7 +288,7 @@ struct Writer {
     auto at = [&](uint32_t e) { return ((static_cast<size_t>(e >> shift) * c.page_size + slot) << shift) + (e & rest); };
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i)
-      if (lane + 32 * i < chunks) dst[at(lane + 32 * i)] = p.v[i];
+      if (lane + 32 * i < chunks) __stcs(dst + at(lane + 32 * i), p.v[i]);
     for (uint32_t e = lane + 128; e < chunks; e += 32) dst[at(e)] = ld_stream16(p.src + e);
   }
 
@@ -392,10 +392,10 @@ __device__ void copy_entries(const xpu_kv_cache_t &c) {
       uint4 v[8];
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i)
-        if (e0 + 32 * i < pieces) v[i] = __ldcs(src + e0 + 32 * i);
+        if (e0 + 32 * i < pieces) v[i] = src[e0 + 32 * i];
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i)
-        if (e0 + 32 * i < pieces) __stcs(dst + e0 + 32 * i, v[i]);
+        if (e0 + 32 * i < pieces) dst[e0 + 32 * i] = v[i];
     }
   }
 }

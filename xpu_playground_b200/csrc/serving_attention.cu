@@ -1067,8 +1067,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
       }
       return page;
     };
+    auto load_q = [&](const Segment &g) {
+      if (leader) {
+        const uint32_t tiles = !g.both && g.npos > positions ? 2 : 1;
+        mbar_expect_tx(&b.q_full, tiles * positions * group * 128 * S::kBoxes);
+        for (uint32_t t = 0; t < tiles; ++t)
+          for (uint32_t h = 0; h < S::kBoxes; ++h)
+            tma_load_3d(q_smem + t * S::kTile + h * kBox, &a.q, 64 * h, g.head * group, g.q0 + t * positions, &b.q_full);
+      }
+      ++q_loads;
+    };
     Segment following;
     bool more = walk.next(following);
+    if (more && first_which == 0) load_q(following);
     int32_t next_page = more ? page_of(following, following.first) : 0;
     bool ok = true;
     for (; ok && more && !warp_failed(b); ++segment) {
@@ -1113,16 +1124,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
               }
             }
           }
-          if (j == 0 && which == 0) {  // after the first keys, which need not wait for the last segment's rows
-            if (segment > 0 && !(ok = warp_wait(b, &b.q_empty, (segment - 1) & 1))) break;
-            if (leader) {
-              const uint32_t tiles = !s.both && s.npos > positions ? 2 : 1;
-              mbar_expect_tx(&b.q_full, tiles * positions * group * 128 * S::kBoxes);
-              for (uint32_t t = 0; t < tiles; ++t)
-                for (uint32_t h = 0; h < S::kBoxes; ++h)
-                  tma_load_3d(q_smem + t * S::kTile + h * kBox, &a.q, 64 * h, s.head * group, s.q0 + t * positions, &b.q_full);
-            }
-            ++q_loads;
+          // a later segment's rows after its first keys, which need not wait for the rows before them
+          if (j == 0 && which == 0 && segment > 0) {
+            if (!(ok = warp_wait(b, &b.q_empty, (segment - 1) & 1))) break;
+            load_q(s);
           }
         }
       }
