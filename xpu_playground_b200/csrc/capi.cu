@@ -390,6 +390,11 @@ int xpu_tree_attention(const xpu_kv_cache_t *cache, uint32_t layer, const int32_
     const AttnTensors t{q, k, v, out, lse, nodes, q_heads, cache->kv_heads, cache->head_dim, q_stride, kv_stride, out_stride,
                         scale};
     XPU_CHECKED(check_attention(cache->dtype, t, "xpu_tree_attention"));
+    // the work is counted in key tiles of 128, in 32 bits
+    const uint64_t tiles = (static_cast<uint64_t>(cache->table_width) * cache->page_size + 127) / 128 + 4;
+    const uint64_t blocks = (static_cast<uint64_t>(q_heads / cache->kv_heads) * XPU_TREE_MAX_NODES + 127) / 128 + 1;
+    if (tiles * blocks * cache->kv_heads * count >= (1ull << 32))
+      return fail(XPU_ERR_UNSUPPORTED, "xpu_tree_attention: too many sequences of such length in one call");
     const size_t need = tree_workspace_bytes(count, nodes, q_heads, cache->kv_heads, cache->head_dim);
     if (workspace_bytes < need)
       return fail(XPU_ERR_INVALID, "xpu_tree_attention: workspace holds " + std::to_string(workspace_bytes) +

@@ -75,7 +75,7 @@ struct BadRows {  // listed keys of one half (64 keys) of up to two tiles of a s
 };
 
 struct TreeEntry {
-  uint32_t first;  // key tiles of all segments' units before this sequence's
+  uint32_t first, units;  // key tiles and units (row block, kv head) of the sequences before this one
   uint32_t len, begin, named;  // cached positions, first node, sequence * 128 + nodes
 };
 
@@ -94,7 +94,7 @@ struct TreeArgs {
   const uint64_t *ancestors;
   uint32_t layer, count, page_shift;  // page_size = 2^page_shift
   uint32_t *arrived;  // per block: parts of the unit that begins there, 0 between calls
-  float *partial;     // [slot][256 rows][D], then [slot][256 rows]{m, l}
+  float *partial;     // two slots a block, as partial_rows() places them, then the rows' {m, l}
 };
 
 struct Args {
@@ -116,7 +116,7 @@ struct Segment {
   uint32_t masked_from;      // the first key tile that some row may not attend as a whole
   bool both;                 // both softmax groups on row tile 0, even and odd key tiles
   int32_t slot;              // partial result, -1 = whole
-  uint32_t unit, unit_tiles; // key tiles of the whole unit, in the order of all: first and how many
+  uint32_t unit, unit_size;  // the whole unit in the cut of all work
 };
 
 // ------------------------------------------------------------ small parts ----
@@ -360,16 +360,16 @@ struct TreeRequest {
 // Fills table[0 .. count] (count + 1 entries: the last holds the totals); all
 // threads of the block. `first`: this thread's first request.
 __device__ void tree_table(const TreeArgs &a, uint32_t tokens, uint32_t kv_heads, uint32_t group, TreeEntry *table,
-                           uint32_t *scratch, const TreeRequest &first) {
+                           uint2 *scratch, const TreeRequest &first) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const xpu_kv_cache_t &c = a.cache;
   const int32_t longest = static_cast<int32_t>(c.table_width * c.page_size);
-  uint32_t before = 0;
+  uint2 before = make_uint2(0, 0);
   bool bad = false;
   for (uint32_t at = 0; at < a.count; at += blockDim.x) {
     const TreeRequest r = at ? TreeRequest(a, at + threadIdx.x) : first;
-    TreeEntry e{0, 0, 0, 0};
-    uint32_t tiles = 0;
+    TreeEntry e{0, 0, 0, 0, 0};
+    uint32_t tiles = 0, units = 0;
     if (r.mine) {
       const bool listed = r.begin >= 0 && r.end >= r.begin && static_cast<uint32_t>(r.end) <= tokens;
       const bool named = r.sequence >= 0 && static_cast<uint32_t>(r.sequence) < c.sequences;
@@ -380,79 +380,92 @@ __device__ void tree_table(const TreeArgs &a, uint32_t tokens, uint32_t kv_heads
       e.begin = listed ? static_cast<uint32_t>(r.begin) : 0;
       e.named = (named ? static_cast<uint32_t>(r.sequence) : 0) * 128u + nodes;
       const uint32_t span = 2 * tile_positions(group);
-      tiles = (nodes + span - 1) / span * kv_heads * entry_tiles(e);
+      units = (nodes + span - 1) / span * kv_heads;
+      tiles = units * entry_tiles(e);
     }
-    uint32_t inc = tiles;
+    uint32_t inc = tiles, inc_units = units;
 #pragma unroll
     for (uint32_t o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
-      if (lane >= o) inc += up;
+      const uint32_t up = __shfl_up_sync(kFullMask, inc, o), up_units = __shfl_up_sync(kFullMask, inc_units, o);
+      if (lane >= o) inc += up, inc_units += up_units;
     }
     if (at) __syncthreads();
-    if (lane == 31) scratch[warp] = inc;
+    if (lane == 31) scratch[warp] = make_uint2(inc, inc_units);
     __syncthreads();
-    uint32_t others = 0, all = 0;
+    e.first = before.x + inc - tiles;
+    e.units = before.y + inc_units - units;
     for (uint32_t w = 0; w < warps; ++w) {
-      others += w < warp ? scratch[w] : 0;
-      all += scratch[w];
+      const uint2 sum = scratch[w];
+      if (w < warp) e.first += sum.x, e.units += sum.y;
+      before.x += sum.x, before.y += sum.y;
     }
-    e.first = before + others + inc - tiles;
     if (r.mine) table[at + threadIdx.x] = e;
-    before += all;
   }
-  if (threadIdx.x == 0) table[a.count] = TreeEntry{before, 0, 0, 0};
+  if (threadIdx.x == 0) table[a.count] = TreeEntry{before.x, before.y, 0, 0, 0};
   if (bad && blockIdx.x == 0) atomicOr(c.status, XPU_KV_BAD_INDEX);
 }
 
-// Key tiles per block: an even share. One tile each where there are no more
-// (2048 positions, 8 kv heads: 20.7 us; two each, with blocks that finish one unit
-// and begin the next, 27.2 us).
-__device__ __forceinline__ uint32_t tree_share(uint32_t tiles, uint32_t blocks) {
-  return max((tiles + blocks - 1) / blocks, 1u);
-}
+// How the work is cut: every unit counts as its key tiles and `lead` more, for
+// what beginning and ending one costs (about 10,000 cycles, three to four tiles), and
+// each block gets the same number. With no more tiles than blocks it is one tile each
+// (2048 positions, 8 kv heads: 20.7 us; two each, with blocks that end one unit and
+// begin the next, 27.2 us).
+struct TreeCut {
+  uint32_t lead, share, total;
+  __device__ TreeCut(const TreeEntry &sums, uint32_t blocks) {
+    lead = sums.first > blocks ? 3 : 0;
+    total = sums.first + lead * sums.units;
+    share = max((total + blocks - 1) / blocks, 1u);
+  }
+  __device__ uint32_t at(const TreeEntry &e) const { return e.first + lead * e.units; }
+};
 
 // This block's share of all (sequence, row block, kv head, key tile), in that order.
 struct TreeWalk {
   const TreeEntry *table;
-  uint32_t count, group, kv_heads, i, at, begin, end, share;
-  __device__ TreeWalk(const Args &a, const TreeEntry *t, uint32_t g) : table(t), count(a.tree.count), group(g) {
-    kv_heads = a.t.kv_heads;
-    const uint32_t total = table[count].first;
-    share = tree_share(total, gridDim.x);
-    begin = at = min(total, blockIdx.x * share);
-    end = min(total, begin + share);
-    uint32_t lo = 0, hi = count;  // the last entry that starts at or before `at`
+  TreeCut cut;
+  uint32_t group, kv_heads, i, at, begin, end;
+  __device__ TreeWalk(const Args &a, const TreeEntry *t, uint32_t g)
+      : table(t), cut(t[a.tree.count], gridDim.x), group(g), kv_heads(a.t.kv_heads) {
+    begin = at = min(cut.total, blockIdx.x * cut.share);
+    end = min(cut.total, begin + cut.share);
+    uint32_t lo = 0, hi = a.tree.count;  // the last entry that starts at or before `at`
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
-      if (table[mid].first <= at) lo = mid;
+      if (cut.at(table[mid]) <= at) lo = mid;
       else hi = mid;
     }
     i = lo;
   }
   __device__ bool next(Segment &s) {
-    if (at >= end) return false;
-    while (table[i + 1].first <= at) ++i;
-    const TreeEntry e = table[i];
-    const uint32_t tiles = entry_tiles(e), off = at - e.first, unit = off / tiles, positions = tile_positions(group);
-    s.first = off % tiles;
-    s.n = min(tiles - s.first, end - at);
-    s.head = unit % kv_heads;
-    s.pos0 = unit / kv_heads * 2 * positions;
-    s.nodes = entry_nodes(e);
-    s.npos = min(2 * positions, s.nodes - s.pos0);
-    s.base = e.begin;
-    s.q0 = e.begin + s.pos0;
-    s.len = e.len;
-    s.masked_from = e.len / kKeys;
-    s.sequence = static_cast<int32_t>(e.named >> 7);
-    s.both = s.npos <= positions;
-    s.n0 = s.both ? (s.n + 1) / 2 : s.n;
-    s.n1 = s.both ? s.n / 2 : s.n;
-    s.unit = e.first + unit * tiles;
-    s.unit_tiles = tiles;
-    s.slot = s.n == tiles ? -1 : static_cast<int32_t>(2 * blockIdx.x + (at == begin ? 0 : 1));
-    at += s.n;
-    return true;
+    for (;;) {
+      if (at >= end) return false;
+      while (cut.at(table[i + 1]) <= at) ++i;
+      const TreeEntry e = table[i];
+      const uint32_t tiles = entry_tiles(e), size = cut.lead + tiles, off = at - cut.at(e), unit = off / size;
+      const uint32_t in = off - unit * size, stop = min(size, in + end - at), positions = tile_positions(group);
+      at += stop - in;
+      if (stop <= cut.lead) continue;  // nothing of the unit but its lead
+      s.first = max(in, cut.lead) - cut.lead;
+      s.n = stop - cut.lead - s.first;
+      const uint32_t block = unit / kv_heads;
+      s.head = unit - block * kv_heads;
+      s.pos0 = block * 2 * positions;
+      s.nodes = entry_nodes(e);
+      s.npos = min(2 * positions, s.nodes - s.pos0);
+      s.base = e.begin;
+      s.q0 = e.begin + s.pos0;
+      s.len = e.len;
+      s.masked_from = e.len / kKeys;
+      s.sequence = static_cast<int32_t>(e.named >> 7);
+      s.both = s.npos <= positions;
+      s.n0 = s.both ? (s.n + 1) / 2 : s.n;
+      s.n1 = s.both ? s.n / 2 : s.n;
+      s.unit = cut.at(e) + unit * size;
+      s.unit_size = size;
+      s.slot = s.n == tiles ? -1 : static_cast<int32_t>(2 * blockIdx.x + (begin >= s.unit ? 0 : 1));
+      return true;
+    }
   }
 };
 
@@ -466,7 +479,7 @@ __device__ __forceinline__ uint32_t valid_keys(const Segment &s, uint32_t tile) 
 
 // Adds p v of the segment's listed keys (non-finite values, zeroed in the
 // product) to one row's columns [col, col + cols): dst16 (normalised by inv)
-// or dst32. Rare: plain loops over global memory.
+// or dst32 (a partial row). Rare: plain loops over global memory.
 template <typename T, int D, bool TREE>
 __device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadRows *bad, uint32_t position, uint32_t q_head,
                                      uint64_t set, float m, float inv, T *dst16, float *dst32, uint32_t col,
@@ -499,7 +512,7 @@ __device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadR
       for (uint32_t d = 0; d < D; ++d) dot = fmaf(Elem<T>::to_float(q[d]), Elem<T>::to_float(k[d]), dot);
       const float p = exp2f(fmaf(dot, c, -(m == -INFINITY ? 0.f : m * c)));
       for (uint32_t d = col; d < col + cols; ++d) {
-        if (dst32) dst32[d] = fmaf(p, Elem<T>::to_float(v[d]), dst32[d]);
+        if (dst32) dst32[(d >> 2) * 128 + (d & 3)] = fmaf(p, Elem<T>::to_float(v[d]), dst32[(d >> 2) * 128 + (d & 3)]);
         else dst16[d] = Elem<T>::from_float(fmaf(p * inv, Elem<T>::to_float(v[d]), Elem<T>::to_float(dst16[d])));
       }
     }
@@ -508,14 +521,12 @@ __device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadR
 
 // ------------------------------------------------------------------- join ----
 
-// Numbers 0 .. 255 of a unit's rows in use (position x group + head): quotients
-// without a division, and the row's place among the unit's two tiles of 128.
-struct JoinRows {
-  uint32_t group, positions, inverse;
-  __device__ JoinRows(uint32_t g, uint32_t p) : group(g), positions(p), inverse(65536u / g + 1) {}
-  __device__ uint32_t position(uint32_t r) const { return r * inverse >> 16; }
-  __device__ uint32_t row(uint32_t r) const { return r + (position(r) >= positions ? 128 - positions * group : 0); }
-};
+// Partial results lie so that a warp's 32 rows (lanes) are next to each other:
+// [slot][block of 32 rows][D / 4][32 rows][4 columns], so that both sides move
+// whole lines; and their maxima and sums [slot][256 rows]{m, l}.
+__device__ __forceinline__ float *partial_rows(const TreeArgs &a, uint32_t slot, uint32_t block, uint32_t d) {
+  return a.partial + (static_cast<size_t>(slot) * 8 + block) * 32 * d;
+}
 
 // Rows of a unit from the partial results of blocks c0 .. c1, added in that
 // order, by the 8 softmax warps. The loops are short on purpose: a block joins once or
@@ -523,119 +534,98 @@ struct JoinRows {
 // Loads take 900 cycles, so each thread has sixteen of them in flight.
 template <typename T, int D>
 struct Join {
-  static constexpr uint32_t N = D / 32;  // this lane's columns
-  using Columns = typename std::conditional<N == 4, float4, float2>::type;
   const Args &a;
   const Segment &s;
-  JoinRows rows;
-  uint32_t share, c0, c1;
+  uint32_t group, positions, share, c0, c1;
   const float2 *sums;
-  float2 *total;  // shared memory: each row's maximum and reciprocal sum
 
-  __device__ uint32_t slot(uint32_t x) const { return (2 * x + (x * share >= s.unit ? 0 : 1)) * 256u; }
-  __device__ Columns part(uint32_t x, uint32_t row) const {
-    return __ldcg(reinterpret_cast<const Columns *>(a.tree.partial + static_cast<size_t>(slot(x) + row) * D) + (threadIdx.x & 31));
-  }
-  static __device__ void add(float w, const Columns &v, float (&o)[N]) {
-#pragma unroll
-    for (uint32_t n = 0; n < N; ++n) o[n] = fmaf(w, (&v.x)[n], o[n]);
-  }
-  __device__ void put(uint32_t r, const float (&o)[N], float inv) const {
-    const uint32_t index = rows.position(r), head = s.head * rows.group + r - index * rows.group;
-    uint32_t w[N / 2];
-#pragma unroll
-    for (uint32_t n = 0; n < N / 2; ++n) w[n] = pack2<T>(o[2 * n] * inv, o[2 * n + 1] * inv);
-    uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<T *>(a.t.out) + (static_cast<size_t>(s.q0) + index) * a.t.out_stride +
-                                                 head * D) + N / 2 * (threadIdx.x & 31);
-    if constexpr (N == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
-    else *dst = w[0];
-  }
-  __device__ void put_lse(uint32_t r, float m, float l, float c) const {
-    const uint32_t index = rows.position(r), head = s.head * rows.group + r - index * rows.group;
-    if (a.t.lse) a.t.lse[(static_cast<size_t>(s.q0) + index) * a.t.q_heads + head] = log_sum(m, l, c);
-  }
+  __device__ uint32_t slot(uint32_t x) const { return 2 * x + (x * share >= s.unit ? 0 : 1); }
+  __device__ float2 part_sums(uint32_t x, uint32_t row) const { return __ldcg(sums + slot(x) * 256 + row); }
 
-  // Up to eight rows: a warp each, lane x the weight of part x.
+  // Up to eight rows, all in the first block: a warp each, lane x the weight of part x,
+  // the lanes' columns four each.
   __device__ void few(uint32_t warp) const {
     const uint32_t lane = threadIdx.x & 31, r = warp;
-    if (r >= s.npos * rows.group) return;
+    if (r >= s.npos * group) return;
     const float c = a.t.scale * kLog2e;
-    const uint32_t row = rows.row(r);
-    auto get = [&](uint32_t x) { return x <= c1 ? __ldcg(sums + slot(x) + row) : make_float2(-INFINITY, 0.f); };
-    float m = -INFINITY, l = 0.f, w = 0.f, o[N] = {};
+    auto get = [&](uint32_t x) { return x <= c1 ? part_sums(x, r) : make_float2(-INFINITY, 0.f); };
+    float m = -INFINITY, l = 0.f, w = 0.f, o[4] = {};
 #pragma unroll 1
     for (uint32_t x0 = c0; x0 <= c1; x0 += 32) m = fmaxf(m, warp_max(get(x0 + lane).x));
 #pragma unroll 1
     for (uint32_t x0 = c0; x0 <= c1; x0 += 8) {
-      Columns v[8];
+      float4 v[8];
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) v[e] = part(min(x0 + e, c1), row);
+      for (uint32_t e = 0; e < 8; ++e)
+        v[e] = __ldcg(reinterpret_cast<const float4 *>(partial_rows(a.tree, slot(min(x0 + e, c1)), 0, D)) +
+                      (lane % (D / 4)) * 32 + r);
       if (((x0 - c0) & 31) == 0) {
         const float2 ml = get(x0 + lane);
         w = ml.x == -INFINITY ? 0.f : exp2_approx((ml.x - m) * c);
         l += warp_sum(w * ml.y);
       }
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) add(__shfl_sync(kFullMask, w, (x0 + e - c0) & 31), v[e], o);  // 0 past the last
+      for (uint32_t e = 0; e < 8; ++e) {
+        const float we = __shfl_sync(kFullMask, w, (x0 + e - c0) & 31);  // 0 past the last
+        o[0] = fmaf(we, v[e].x, o[0]), o[1] = fmaf(we, v[e].y, o[1]), o[2] = fmaf(we, v[e].z, o[2]), o[3] = fmaf(we, v[e].w, o[3]);
+      }
     }
-    put(r, o, l == 0.f ? 0.f : 1.f / l);
-    if (lane == 0) put_lse(r, m, l, c);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const uint32_t index = r / group, head = s.head * group + r - index * group;
+    const size_t token = static_cast<size_t>(s.q0) + index;
+    if (lane < D / 4)
+      reinterpret_cast<uint2 *>(static_cast<T *>(a.t.out) + token * a.t.out_stride + head * D)[lane] =
+          make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+    if (a.t.lse && lane == 0) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
   }
 
-  // Any number: first a thread per row ...
-  __device__ void sum_rows() const {
-    const uint32_t r = threadIdx.x;
-    if (r >= s.npos * rows.group) return;
+  // Any number: a block of 32 rows a warp, a row a lane, 32 columns at a time.
+  __device__ void many(uint32_t warp) const {
+    const uint32_t lane = threadIdx.x & 31, in_tile = (warp & 3) * 32 + lane, row = warp * 32 + lane;
+    const uint32_t in = in_tile / group, index = (warp >> 2) * positions + in, head = s.head * group + in_tile - in * group;
+    const bool mine = in < positions && index < s.npos;
+    const size_t token = static_cast<size_t>(s.q0) + index;
+    const QuadRows out(static_cast<T *>(a.t.out) + token * a.t.out_stride + head * D, mine);
+    if (!out.any()) return;
     const float c = a.t.scale * kLog2e;
-    const uint32_t row = rows.row(r);
     float m = -INFINITY, l = 0.f;
 #pragma unroll 1
     for (uint32_t x0 = c0; x0 <= c1; x0 += 4) {
       float2 ml[4];
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) ml[e] = __ldcg(sums + slot(min(x0 + e, c1)) + row);
+      for (uint32_t e = 0; e < 4; ++e) ml[e] = part_sums(min(x0 + e, c1), row);
 #pragma unroll
       for (uint32_t e = 0; e < 4; ++e) {
+        if (x0 + e > c1 || ml[e].x == -INFINITY) continue;
         const float top = fmaxf(m, ml[e].x);
-        if (x0 + e > c1 || top == -INFINITY) continue;
         l = l * exp2_approx((m - top) * c) + ml[e].y * exp2_approx((ml[e].x - top) * c);
         m = top;
       }
     }
-    total[r] = make_float2(m, l == 0.f ? 0.f : 1.f / l);
-    put_lse(r, m, l, c);
-  }
-  // ... then eight rows a warp at a time, part after part.
-  __device__ void many(uint32_t warp) const {
-    const uint32_t count = s.npos * rows.group;
-    const float c = a.t.scale * kLog2e;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-    for (uint32_t r0 = warp; r0 < count; r0 += 64) {
-      float o[8][N] = {};
-      uint32_t row[8];
-      float2 sum[8];
-#pragma unroll
-      for (uint32_t k = 0; k < 8; ++k) {
-        const uint32_t r = min(r0 + 8 * k, count - 1);
-        row[k] = rows.row(r);
-        sum[k] = total[r];
-      }
+    for (uint32_t q = 0; q < D; q += 64) {
+      float o[64] = {};
 #pragma unroll 1
       for (uint32_t x = c0; x <= c1; ++x) {
-        Columns v[8];
-        float mx[8];
+        const float4 *src = reinterpret_cast<const float4 *>(partial_rows(a.tree, slot(x), warp, D)) + q / 4 * 32 + lane;
+        float4 v[16];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
-          v[k] = part(x, row[k]);
-          mx[k] = __ldcg(&sums[slot(x) + row[k]].x);
+        for (uint32_t k = 0; k < 16; ++k) v[k] = __ldcg(src + 32 * k);
+        const float mx = part_sums(x, row).x, w = mx == -INFINITY ? 0.f : exp2_approx((mx - m) * c) * inv;
+#pragma unroll
+        for (uint32_t k = 0; k < 16; ++k) {
+          o[4 * k] = fmaf(w, v[k].x, o[4 * k]), o[4 * k + 1] = fmaf(w, v[k].y, o[4 * k + 1]);
+          o[4 * k + 2] = fmaf(w, v[k].z, o[4 * k + 2]), o[4 * k + 3] = fmaf(w, v[k].w, o[4 * k + 3]);
         }
-#pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) add(mx[k] == -INFINITY ? 0.f : exp2_approx((mx[k] - sum[k].x) * c), v[k], o[k]);
       }
+      uint32_t p[32];
 #pragma unroll
-      for (uint32_t k = 0; k < 8; ++k)
-        if (r0 + 8 * k < count) put(r0 + 8 * k, o[k], sum[k].y);
+      for (uint32_t k = 0; k < 32; ++k) p[k] = pack2<T>(o[2 * k], o[2 * k + 1]);
+      out.put(p, q * 2);
+      out.put(p + 16, q * 2 + 64);
     }
+    if (a.t.lse && mine) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
   }
 };
 
@@ -650,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
   __shared__ Barriers b;
   __shared__ TreeEntry table[TREE ? XPU_KV_MAX_REQUESTS + 1 : 1];
   __shared__ float joined[TREE ? 2 : 1][TREE ? 128 : 1][2];
-  __shared__ uint32_t scratch[kThreads / 32];
+  __shared__ uint2 scratch[kThreads / 32];
   __shared__ bool last;
   const uint32_t a0 = smem_addr(smem_raw);
   uint8_t *q_smem = smem_raw + ((a0 + 1023u) / 1024u * 1024u - a0), *ring = q_smem + 2 * S::kTile;
@@ -851,18 +841,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         T *dst16 = static_cast<T *>(a.t.out) + token * a.t.out_stride + q_head * D;
         float *dst32 = nullptr;
         if (TREE && !whole) {
-          const size_t row = static_cast<size_t>(s.slot) * 256 + (s.both ? 0 : t * 128) + r;
-          dst32 = a.tree.partial + row * D;
-          if (mine && col == 0) {
-            float *ml = a.tree.partial + 2ull * gridDim.x * 256 * D + row * 2;
-            ml[0] = m;
-            ml[1] = l;
-          }
+          const uint32_t row = (s.both ? 0 : t * 128) + r;
+          dst32 = partial_rows(a.tree, s.slot, row >> 5, D) + (row & 31) * 4;
+          if (mine && col == 0)
+            reinterpret_cast<float2 *>(a.tree.partial + 2ull * gridDim.x * 256 * D)[s.slot * 256 + row] = make_float2(m, l);
         } else if (mine && a.t.lse && col == 0 && token < a.t.tokens) {
           a.t.lse[token * a.t.q_heads + q_head] = log_sum(m, l, c);
         }
         const bool store = mine && token < a.t.tokens;
-        const QuadRows out(TREE && dst32 ? static_cast<void *>(dst32) : dst16, store);
+        const QuadRows out(dst16, store);
         if (out.any()) {
 #pragma unroll 1
           for (uint32_t q = col; q < col + cols; q += 32) {
@@ -882,8 +869,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
                 o[j] = __float_as_uint(fmaf(__uint_as_float(o1[j]), w1, __uint_as_float(o[j])));
             }
             if (TREE && dst32) {
+              if (store) {
 #pragma unroll
-              for (uint32_t h = 0; h < 32; h += 16) out.put(&o[h], (q + h) * 4);
+                for (uint32_t j = 0; j < 32; j += 4)
+                  *reinterpret_cast<uint4 *>(dst32 + (q + j) * 32) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+              }
             } else {
 #pragma unroll
               for (uint32_t j = 0; j < 16; ++j) o[j] = pack2<T>(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
@@ -903,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           // The block that completes a unit adds up its parts, in the order of the
           // key tiles whoever comes last.
           if (!meet()) break;
-          const uint32_t c0 = s.unit / walk.share, c1 = (s.unit + s.unit_tiles - 1) / walk.share;
+          const uint32_t share = walk.cut.share, c0 = (s.unit + walk.cut.lead) / share, c1 = (s.unit + s.unit_size - 1) / share;
           if (threadIdx.x == 0) {
             __threadfence();
             last = atomicAdd(a.tree.arrived + c0, 1u) == c1 - c0;
@@ -915,15 +905,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           if (!meet()) break;
           if (last) {
             const float2 *sums = reinterpret_cast<const float2 *>(a.tree.partial + 2ull * gridDim.x * 256 * D);
-            const Join<T, D> join{a, s, JoinRows(group, positions), walk.share, c0, c1, sums,
-                                  reinterpret_cast<float2 *>(&joined[0][0][0])};
-            if (s.npos * group <= 8) {
-              join.few(warp);
-            } else {
-              join.sum_rows();
-              if (!meet()) break;
-              join.many(warp);
-            }
+            const Join<T, D> join{a, s, group, positions, share, c0, c1, sums};
+            if (s.npos * group <= 8) join.few(warp);
+            else join.many(warp);
           }
           if (!meet()) break;
         } else if (s.both && !meet()) {  // the other group may still read this one's accumulator and sums
@@ -1292,7 +1276,7 @@ size_t prompt_plan(const uint32_t *lens, uint32_t count, uint32_t q_heads, uint3
     for (uint32_t pos = 0; pos < lens[i]; pos += span)
       for (uint32_t h = 0; h < kv_heads; ++h)
         items.push_back({static_cast<int32_t>(tokens), static_cast<int32_t>(lens[i]), static_cast<int32_t>(pos),
-                         static_cast<int32_t>(h), (std::min(pos + span, lens[i]) + 127) / 128 + 1});
+                         static_cast<int32_t>(h), (std::min(pos + span, lens[i]) + 127) / 128 + 2});
     tokens += lens[i];
   }
   const uint32_t blocks = static_cast<uint32_t>(std::min<size_t>(items.size(), sms));
