@@ -173,20 +173,23 @@ def _attention_args(q, k, v, kv_heads, head_dim, scale, out, lse):
         raise ValueError(f"q must be [tokens, q_heads, {head_dim}], k and v [tokens, {kv_heads}, {head_dim}]")
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise ValueError("libxpu_cuda entry points take CUDA tensors")
-    q_stride = out_stride = shape[1] * head_dim
+    tokens, q_heads = shape[0], shape[1]
+    q_stride = out_stride = q_heads * head_dim
     kv_stride = kv_heads * head_dim
-    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
-        q_stride, kv_stride = _packed("q", q, shape[1], head_dim), _packed("k", k, kv_heads, head_dim)
+    whole = q.is_contiguous()
+    if not (whole and k.is_contiguous() and v.is_contiguous()):
+        q_stride, kv_stride = _packed("q", q, q_heads, head_dim), _packed("k", k, kv_heads, head_dim)
         if _packed("v", v, kv_heads, head_dim) != kv_stride:
             raise ValueError("k and v need one row stride")
+    # (empty_like, and sizes one by one, take half the time of a torch.Size)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = torch.empty_like(q) if whole else torch.empty(tokens, q_heads, head_dim, dtype=dtype, device=q.device)
     elif out.dtype != dtype or out.shape != shape:
         raise ValueError("out must have q's shape and dtype")
     else:
-        out_stride = _packed("out", out, shape[1], head_dim)
+        out_stride = _packed("out", out, q_heads, head_dim)
     if lse is None:
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device)
+        lse = torch.empty(tokens, q_heads, dtype=torch.float32, device=q.device)
     elif lse.dtype != torch.float32 or lse.shape != shape[:2] or not lse.is_cuda or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, q_heads]")
     return out, lse, q_stride, kv_stride, out_stride, head_dim ** -0.5 if scale is None else scale
