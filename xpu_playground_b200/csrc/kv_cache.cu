@@ -23,6 +23,7 @@
 
 #include "common.cuh"
 #include "serving.h"
+#include "stream.cuh"
 
 namespace xpu {
 namespace {
@@ -32,6 +33,13 @@ constexpr uint32_t kHeader = 8, kEntry = 3;
 constexpr uint32_t kFew = 1024;  // pages whose ids a plan keeps in shared memory
 enum { kAccepted, kEntries, kRenamedFrom, kTicket, kReady, kSeen };
 constexpr long long kPlanWaitCycles = 4000000000ll;  // ~2 s at 1.9 GHz
+
+// The next kernel may be set up from here on; this one reads nothing before the
+// one before it has ended.
+__device__ __forceinline__ void after_previous() {
+  grid_dep_launch();
+  grid_dep_wait();
+}
 
 __device__ __forceinline__ uint32_t pages_of(uint32_t positions, uint32_t size) { return (positions + size - 1) / size; }
 
@@ -309,12 +317,14 @@ struct Writer {
 __global__ void __launch_bounds__(kThreads) k_kv_extend(const __grid_constant__ xpu_kv_cache_t c, const int32_t *sequences,
                                                         const int32_t *starts, uint32_t count) {
   __shared__ uint32_t bitmap[XPU_KV_MAX_SEQUENCES / 32], few[kFew];
+  after_previous();
   plan_extend(c, Extension(c, sequences, starts, count), count, bitmap, few);
 }
 
 __global__ void __launch_bounds__(kThreads) k_kv_write(const __grid_constant__ xpu_kv_cache_t c, const int32_t *sequences,
                                                        const int32_t *starts, uint32_t count,
                                                        const __grid_constant__ Rows r) {
+  after_previous();
   if (!planned(c, kAccepted)) return;
   Writer writer(c, sequences, starts, count, r);
   Piece first;
@@ -327,6 +337,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_append(const __grid_constant__ 
                                                         const int32_t *starts, uint32_t count,
                                                         const __grid_constant__ Rows r) {
   __shared__ uint32_t bitmap[XPU_KV_MAX_SEQUENCES / 32], few[kFew];
+  after_previous();
   const Extension x(c, sequences, starts, count);
   Writer writer(c, sequences, starts, count, r);
   Piece first;
@@ -341,6 +352,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_trim(const __grid_constant__ xp
                                                       const int32_t *new_lens, uint32_t count) {
   __shared__ uint32_t bitmap[XPU_KV_MAX_SEQUENCES / 32];
   __shared__ uint32_t range[XPU_KV_MAX_REQUESTS][2];
+  after_previous();
   const uint32_t i = threadIdx.x;
   const bool mine = i < count;
   const int32_t s = mine ? sequences[i] : -1, want = mine ? new_lens[i] : 0;
@@ -431,6 +443,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_fork(const __grid_constant__ xp
                                                       const int32_t *children, uint32_t count) {
   static_assert(kFew >= XPU_KV_MAX_REQUESTS, "a page per child");
   __shared__ uint32_t bitmap[XPU_KV_MAX_SEQUENCES / 32], few[kFew];
+  after_previous();
   const int32_t from = threadIdx.x < count ? parents[threadIdx.x] : -1, to = threadIdx.x < count ? children[threadIdx.x] : -1;
   const int4 refs = refs4(c, threadIdx.x);
   if (!after_plan(c, [&] { plan_fork(c, from, to, refs, count, bitmap, few); })) return;
@@ -490,6 +503,7 @@ __device__ void plan_compact(const xpu_kv_cache_t &c, int4 first) {
 }
 
 __global__ void __launch_bounds__(kThreads) k_kv_compact(const __grid_constant__ xpu_kv_cache_t c) {
+  after_previous();
   const int4 refs = refs4(c, threadIdx.x);
   if (!after_plan(c, [&] { plan_compact(c, refs); })) return;
   const int32_t keep = planned(c, kRenamedFrom), renamed = static_cast<int32_t>(kHeader + kEntry * c.pages);
@@ -516,8 +530,7 @@ size_t kv_workspace_bytes(uint32_t pages) {
 
 cudaError_t kv_extend_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *starts, uint32_t count,
                              cudaStream_t s) {
-  k_kv_extend<<<1, kThreads, 0, s>>>(c, sequences, starts, count);
-  return cudaGetLastError();
+  return launch_after(k_kv_extend, 1, kThreads, 0, s, c, sequences, starts, count);
 }
 
 cudaError_t kv_write_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *starts, uint32_t count,
@@ -527,27 +540,23 @@ cudaError_t kv_write_launch(const xpu_kv_cache_t &c, const int32_t *sequences, c
   const Rows r{rows, static_cast<const uint16_t *>(k), static_cast<const uint16_t *>(v), tokens, held, layer_stride, row_stride,
                layer, layers};
   const uint32_t blocks = blocks_for(static_cast<uint64_t>(tokens) * layers * 2);
-  if (extend) k_kv_append<<<blocks, kThreads, 0, s>>>(c, sequences, starts, count, r);
-  else k_kv_write<<<blocks, kThreads, 0, s>>>(c, sequences, starts, count, r);
-  return cudaGetLastError();
+  return launch_after(extend ? k_kv_append : k_kv_write, blocks, kThreads, 0, s, c, sequences, starts, count, r);
 }
 
 cudaError_t kv_trim_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *new_lens, uint32_t count,
                            cudaStream_t s) {
-  k_kv_trim<<<1, kThreads, 0, s>>>(c, sequences, new_lens, count);
-  return cudaGetLastError();
+  return launch_after(k_kv_trim, 1, kThreads, 0, s, c, sequences, new_lens, count);
 }
 
 cudaError_t kv_fork_launch(const xpu_kv_cache_t &c, const int32_t *parents, const int32_t *children, uint32_t count,
                            cudaStream_t s) {
-  k_kv_fork<<<blocks_for(static_cast<uint64_t>(count) * c.layers * 2 * c.kv_heads), kThreads, 0, s>>>(c, parents, children,
-                                                                                                      count);
-  return cudaGetLastError();
+  return launch_after(k_kv_fork, blocks_for(static_cast<uint64_t>(count) * c.layers * 2 * c.kv_heads), kThreads, 0, s, c,
+                      parents, children, count);
 }
 
 cudaError_t kv_compact_launch(const xpu_kv_cache_t &c, cudaStream_t s) {
-  k_kv_compact<<<blocks_for(static_cast<uint64_t>(c.pages) / 2 * c.layers * 2 * c.kv_heads), kThreads, 0, s>>>(c);
-  return cudaGetLastError();
+  return launch_after(k_kv_compact, blocks_for(static_cast<uint64_t>(c.pages) / 2 * c.layers * 2 * c.kv_heads), kThreads, 0,
+                      s, c);
 }
 
 }  // namespace xpu

@@ -7,6 +7,26 @@
 
 namespace xpu {
 
+// Launch that may begin under the tail of the kernel before it (programmatic
+// dependent launch): every serving kernel sets itself up, then waits for that
+// kernel's end before its first access to global memory. Saves about a
+// microsecond of launch latency a kernel.
+template <typename... Params, typename... Given>
+cudaError_t launch_after(void (*kernel)(Params...), uint32_t blocks, uint32_t threads, size_t smem, cudaStream_t stream,
+                         const Given &...given) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(given)...);
+}
+
 // SMs of the current device (a B200's where there is none).
 uint32_t sm_count();
 

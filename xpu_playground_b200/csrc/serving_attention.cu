@@ -647,8 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t group = a.t.q_heads / a.t.kv_heads, positions = tile_positions(group);
 
-  // the first memory accesses of all roles, under the set-up of the block
-  [[maybe_unused]] const TreeRequest request(a.tree, TREE ? threadIdx.x : 0xffffffffu);
+  grid_dep_launch();
   if (threadIdx.x >= 32 && threadIdx.x < (TREE ? 37 : 35)) {
     const CUtensorMap *map = threadIdx.x == 32 ? &a.q : threadIdx.x == 33 ? &a.k : threadIdx.x == 34 ? &a.v
                              : threadIdx.x == 35 ? &a.cached_k : &a.cached_v;
@@ -674,7 +673,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     b.failed = 0;
   }
   if (warp == kMmaWarp) tmem_alloc1(&b.tmem, 512);
-  if (TREE) tree_table(a.tree, a.t.tokens, a.t.kv_heads, group, table, scratch, request);
+  grid_dep_wait();  // up to here nothing was read but the arguments
+  if constexpr (TREE)
+    tree_table(a.tree, a.t.tokens, a.t.kv_heads, group, table, scratch, TreeRequest(a.tree, threadIdx.x));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1225,8 +1226,7 @@ cudaError_t launch(const Args &a, uint32_t blocks, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     if (device < 64) allowed[device].store(true, std::memory_order_relaxed);
   }
-  k_attention<T, D, TREE><<<blocks, kThreads, smem, s>>>(a);
-  return cudaGetLastError();
+  return launch_after(k_attention<T, D, TREE>, blocks, kThreads, smem, s, a);
 }
 
 template <bool TREE>
