@@ -30,6 +30,16 @@
 // group idle: there both groups work for the same rows, on even and odd key
 // tiles, and join their sums at the end.
 //
+// What bounds it. Long prompts: per pair of row tiles and key tile the tensor
+// cores need 2048 cycles (32 instructions of 64) and the loop takes about 3200,
+// the chain scores -> softmax (about 2000 cycles, half of them the special
+// function unit's) -> P V -> next scores of one tile; 8192 tokens, 32/8 heads: 412
+// us (1335 TFLOP/s) for a few passes, 493 us (1110) kept up under the power limit
+// (B200's cuBLAS: 1707 and 1405). Emulating a part of the exponentials on the FMA
+// pipe, half tiles of 64 keys (64-column score products run at 55 cycles, not 32)
+// and starting the exponentials with the old maximum were all slower. Trees of up
+// to 32 nodes: reading the cache, 5.4 TB/s (16 x 12288 positions, pages of 16).
+//
 // Waits are bounded; a timeout sets a sticky device word that
 // xpu_device_status reads, and every role leaves.
 #include <cuda.h>
