@@ -657,7 +657,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t group = a.t.q_heads / a.t.kv_heads, positions = tile_positions(group);
 
-  grid_dep_launch();
   if (threadIdx.x >= 32 && threadIdx.x < (TREE ? 37 : 35)) {
     const CUtensorMap *map = threadIdx.x == 32 ? &a.q : threadIdx.x == 33 ? &a.k : threadIdx.x == 34 ? &a.v
                              : threadIdx.x == 35 ? &a.cached_k : &a.cached_v;
@@ -682,7 +681,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     fence_mbar_init();
     b.failed = 0;
   }
-  if (warp == kMmaWarp) tmem_alloc1(&b.tmem, 512);
+  if (warp == kMmaWarp) {
+    tmem_alloc1(&b.tmem, 512);
+    // The next kernel's blocks may come from here on, not earlier: one that takes TMEM before
+    // this block has its own would wait for this grid's end, and this block for that TMEM.
+    grid_dep_launch();
+  }
   grid_dep_wait();  // up to here nothing was read but the arguments
   if constexpr (TREE)
     tree_table(a.tree, a.t.tokens, a.t.kv_heads, group, table, scratch, TreeRequest(a.tree, threadIdx.x));
