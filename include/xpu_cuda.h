@@ -258,7 +258,9 @@ int xpu_kv_compact(const xpu_kv_cache_t *cache, void *stream);
  * The plan lists each thread block's tiles, longest first; it depends on the
  * lengths and heads alone, so one plan serves every layer. xpu_prompt_plan
  * writes it to host memory (*used ints; XPU_ERR_INVALID with *used set if
- * `capacity` ints are too few); the caller copies it to the device. */
+ * `capacity` ints are too few); the caller copies it to the device. A call's
+ * tokens are the sum of the plan's lengths, its heads the plan's, and
+ * plan_blocks is plan[0]. out may not overlap q, k or v. */
 int xpu_prompt_plan(const uint32_t *lens, uint32_t count, uint32_t q_heads, uint32_t kv_heads, int32_t *plan,
                     size_t capacity, size_t *used);
 int xpu_prompt_attention(int dtype, const int32_t *plan, uint32_t plan_blocks, const void *q, const void *k, const void *v,
@@ -276,7 +278,9 @@ int xpu_prompt_attention(int dtype, const int32_t *plan, uint32_t plan_blocks, c
  * xpu_prompt_attention. The drafts' keys and values are not in the cache:
  * xpu_kv_append adds the accepted ones. The workspace holds
  * xpu_tree_attention_workspace_size bytes, zeroed once before its first use
- * (calls leave it ready for the next); calls that may overlap need their own. */
+ * (calls leave it ready for the next), and again after xpu_device_status has
+ * reported a timeout; calls that may overlap need their own. out may not
+ * overlap q, k, v or the cache. */
 #define XPU_TREE_MAX_NODES 64u
 size_t xpu_tree_attention_workspace_size(uint32_t count, uint32_t nodes, uint32_t q_heads, uint32_t kv_heads,
                                          uint32_t head_dim);
