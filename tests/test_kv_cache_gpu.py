@@ -224,3 +224,15 @@ def test_python_argument_checks():
         cache.trim(ints([0]), ints([0, 1]))
     with pytest.raises(ValueError):
         cache.fork(ints([0]).cpu(), ints([1]).cpu())
+
+
+def test_status_waits_for_every_stream():
+    cache = new_cache()
+    sequences, lens = ints([cache.tables.shape[0]]), ints([0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # about 10 ms, which a status read on another stream would not wait for
+    cache.trim(sequences, lens, stream=side)
+    assert cache.status() == BAD_SEQUENCE
+    assert cache.status() == 0

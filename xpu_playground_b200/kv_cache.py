@@ -61,6 +61,7 @@ class KvCache:
     def status(self) -> int:
         """Bits that refused requests have set (EXHAUSTED, BAD_SEQUENCE,
         SHARED_CUT, BAD_INDEX, TIMEOUT), cleared by reading; waits for the device."""
+        torch.cuda.synchronize(self._status.device)  # the operators may have run on any stream
         bits = int(self._status.item())
         self._status.zero_()
         return bits
