@@ -589,10 +589,13 @@ struct Join {
     if (a.t.lse && lane == 0) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
   }
 
-  // Any number: a block of 32 rows a warp, a row a lane, 32 columns at a time.
+  // Any number: a block of 32 rows a warp, a row a lane, 64 columns at a time. With one row
+  // tile, two warps a block, half of the columns each.
   __device__ void many(uint32_t warp) const {
-    const uint32_t lane = threadIdx.x & 31, in_tile = (warp & 3) * 32 + lane, row = warp * 32 + lane;
-    const uint32_t in = in_tile / group, index = (warp >> 2) * positions + in, head = s.head * group + in_tile - in * group;
+    const bool halves = D == 128 && s.both;
+    const uint32_t block = halves ? warp & 3 : warp, first = halves ? (warp >> 2) * 64 : 0, end = halves ? first + 64 : D;
+    const uint32_t lane = threadIdx.x & 31, in_tile = (warp & 3) * 32 + lane, row = block * 32 + lane;
+    const uint32_t in = in_tile / group, index = (block >> 2) * positions + in, head = s.head * group + in_tile - in * group;
     const bool mine = in < positions && index < s.npos;
     const size_t token = static_cast<size_t>(s.q0) + index;
     const QuadRows out(static_cast<T *>(a.t.out) + token * a.t.out_stride + head * D, mine);
@@ -614,11 +617,11 @@ struct Join {
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-    for (uint32_t q = 0; q < D; q += 64) {
+    for (uint32_t q = first; q < end; q += 64) {
       float o[64] = {};
 #pragma unroll 1
       for (uint32_t x = c0; x <= c1; ++x) {
-        const float4 *src = reinterpret_cast<const float4 *>(partial_rows(a.tree, slot(x), warp, D)) + q / 4 * 32 + lane;
+        const float4 *src = reinterpret_cast<const float4 *>(partial_rows(a.tree, slot(x), block, D)) + q / 4 * 32 + lane;
         float4 v[16];
 #pragma unroll
         for (uint32_t k = 0; k < 16; ++k) v[k] = __ldcg(src + 32 * k);
@@ -635,7 +638,7 @@ struct Join {
       out.put(p, q * 2);
       out.put(p + 16, q * 2 + 64);
     }
-    if (a.t.lse && mine) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
+    if (a.t.lse && mine && first == 0) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
   }
 };
 
@@ -910,12 +913,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           if (!meet()) break;
           const uint32_t share = walk.cut.share, c0 = (s.unit + walk.cut.lead) / share, c1 = (s.unit + s.unit_size - 1) / share;
           if (threadIdx.x == 0) {
-            __threadfence();
-            last = atomicAdd(a.tree.arrived + c0, 1u) == c1 - c0;
-            if (last) {
-              a.tree.arrived[c0] = 0;
-              __threadfence();
-            }
+            uint32_t before;  // releases this block's part, acquires the others'
+            asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;"
+                         : "=r"(before)
+                         : "l"(a.tree.arrived + c0)
+                         : "memory");
+            last = before == c1 - c0;
+            if (last) a.tree.arrived[c0] = 0;
           }
           if (!meet()) break;
           if (last) {
