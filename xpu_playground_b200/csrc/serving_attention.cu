@@ -548,45 +548,54 @@ struct Join {
   const Segment &s;
   uint32_t group, positions, share, c0, c1;
   const float2 *sums;
+  static constexpr uint32_t kTogether = 8;  // parts in flight
 
   __device__ uint32_t slot(uint32_t x) const { return 2 * x + (x * share >= s.unit ? 0 : 1); }
   __device__ float2 part_sums(uint32_t x, uint32_t row) const { return __ldcg(sums + slot(x) * 256 + row); }
 
-  // Up to eight rows, all in the first block: a warp each, lane x the weight of part x,
-  // the lanes' columns four each.
+  // Up to eight rows, all in the first block: lane = row + 8 piece, each thread four columns
+  // of a row, so that the rows' pieces, which lie next to each other, are loaded together; the
+  // maximum moves along.
   __device__ void few(uint32_t warp) const {
-    const uint32_t lane = threadIdx.x & 31, r = warp;
-    if (r >= s.npos * group) return;
+    const uint32_t lane = threadIdx.x & 31, r = lane & 7, piece = warp * 4 + (lane >> 3);
+    if (piece >= D / 4) return;
     const float c = a.t.scale * kLog2e;
-    auto get = [&](uint32_t x) { return x <= c1 ? part_sums(x, r) : make_float2(-INFINITY, 0.f); };
-    float m = -INFINITY, l = 0.f, w = 0.f, o[4] = {};
+    float m = -INFINITY, l = 0.f, o[4] = {};
 #pragma unroll 1
-    for (uint32_t x0 = c0; x0 <= c1; x0 += 32) m = fmaxf(m, warp_max(get(x0 + lane).x));
-#pragma unroll 1
-    for (uint32_t x0 = c0; x0 <= c1; x0 += 8) {
-      float4 v[8];
+    for (uint32_t x0 = c0; x0 <= c1; x0 += kTogether) {
+      float2 ml[kTogether];
+      float4 v[kTogether];
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e)
-        v[e] = __ldcg(reinterpret_cast<const float4 *>(partial_rows(a.tree, slot(min(x0 + e, c1)), 0, D)) +
-                      (lane % (D / 4)) * 32 + r);
-      if (((x0 - c0) & 31) == 0) {
-        const float2 ml = get(x0 + lane);
-        w = ml.x == -INFINITY ? 0.f : exp2_approx((ml.x - m) * c);
-        l += warp_sum(w * ml.y);
+      for (uint32_t e = 0; e < kTogether; ++e) {
+        const uint32_t from = slot(min(x0 + e, c1));
+        ml[e] = __ldcg(sums + from * 256 + r);
+        v[e] = __ldcg(reinterpret_cast<const float4 *>(partial_rows(a.tree, from, 0, D)) + piece * 32 + r);
       }
+      float top = m;
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) {
-        const float we = __shfl_sync(kFullMask, w, (x0 + e - c0) & 31);  // 0 past the last
-        o[0] = fmaf(we, v[e].x, o[0]), o[1] = fmaf(we, v[e].y, o[1]), o[2] = fmaf(we, v[e].z, o[2]), o[3] = fmaf(we, v[e].w, o[3]);
+      for (uint32_t e = 0; e < kTogether; ++e) {
+        if (x0 + e > c1) ml[e].x = -INFINITY;
+        top = fmaxf(top, ml[e].x);
+      }
+      const float keep = m == -INFINITY ? 0.f : exp2_approx((m - top) * c);
+      m = top;
+      l *= keep;
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) o[k] *= keep;
+#pragma unroll
+      for (uint32_t e = 0; e < kTogether; ++e) {
+        const float w = ml[e].x == -INFINITY ? 0.f : exp2_approx((ml[e].x - top) * c);
+        l = fmaf(w, ml[e].y, l);
+        o[0] = fmaf(w, v[e].x, o[0]), o[1] = fmaf(w, v[e].y, o[1]), o[2] = fmaf(w, v[e].z, o[2]), o[3] = fmaf(w, v[e].w, o[3]);
       }
     }
+    if (r >= s.npos * group) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const uint32_t index = r / group, head = s.head * group + r - index * group;
     const size_t token = static_cast<size_t>(s.q0) + index;
-    if (lane < D / 4)
-      reinterpret_cast<uint2 *>(static_cast<T *>(a.t.out) + token * a.t.out_stride + head * D)[lane] =
-          make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
-    if (a.t.lse && lane == 0) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
+    reinterpret_cast<uint2 *>(static_cast<T *>(a.t.out) + token * a.t.out_stride + head * D)[piece] =
+        make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+    if (a.t.lse && piece == 0) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
   }
 
   // Any number: a block of 32 rows a warp, a row a lane, 64 columns at a time. With one row
