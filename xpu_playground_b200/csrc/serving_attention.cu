@@ -419,8 +419,8 @@ __device__ void tree_table(const TreeArgs &a, uint32_t tokens, uint32_t kv_heads
 // what beginning and ending one costs (about 10,000 cycles, three to four tiles), and
 // each block gets the same number (geometric mean over 16 random batches with 3, 4, 5, 6 and
 // 8 more: 31.7, 31.4, 31.6, 31.5 and 31.8 us). With no more tiles than blocks it is one tile each
-// (2048 positions, 8 kv heads: 20.7 us; two each, with blocks that end one unit and
-// begin the next, 27.2 us).
+// (2048 positions, 8 kv heads: 12.4 us in a graph; two each, with blocks that end one unit
+// and begin the next, 15.9 us).
 struct TreeCut {
   uint32_t lead, share, total;
   __device__ TreeCut(const TreeEntry &sums, uint32_t blocks) {
