@@ -95,6 +95,7 @@ struct Barriers {
   uint64_t s_full[2], p_early[2], p_ready[2], o_full[2], joined;
   uint32_t tmem;
   int failed;
+  uint32_t ended[8];  // segments that each softmax warp is done with
   BadRows bad[kBadRing][2];
 };
 
@@ -138,6 +139,24 @@ __device__ __forceinline__ bool warp_wait(Barriers &b, uint64_t *bar, uint32_t p
   if (__all_sync(kFullMask, mbar_wait(bar, parity))) return true;
   b.failed = 1;
   return false;
+}
+
+// The cleaning warps, before they list segment `segment`: every softmax warp is done with the
+// segment that had its ring entry. A count and not an mbarrier, whose two phases the softmax
+// warps could pass both while a cleaning warp is late.
+__device__ __forceinline__ bool wait_listed(Barriers &b, uint32_t segment) {
+  if (segment < kBadRing) return true;
+  const volatile uint32_t *ended = b.ended + (threadIdx.x & 7);
+  const long long start = clock64();
+  while (!__all_sync(kFullMask, *ended > segment - kBadRing)) {
+    if (warp_failed(b)) return false;
+    if (__any_sync(kFullMask, clock64() - start > kWaitCycles)) {
+      b.failed = 1;
+      return false;
+    }
+  }
+  __threadfence_block();
+  return true;
 }
 
 // A value that all lanes hold, in a form the compiler knows to be uniform.
@@ -692,6 +711,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     }
     mbar_init(&b.joined, 8);
     fence_mbar_init();
+    for (uint32_t i = 0; i < 8; ++i) b.ended[i] = 0;
     b.failed = 0;
   }
   if (warp == kMmaWarp) {
@@ -943,6 +963,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           break;
         }
       }
+      // A group without a row tile in the segments that follow runs far behind the other one if it has
+      // listed values to add.
+      __syncwarp();
+      if (lane == 0) {
+        __threadfence_block();
+        *const_cast<volatile uint32_t *>(&b.ended[warp]) = segment + 1;
+      }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -1158,6 +1185,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
     for (; walk.next(s) && !warp_failed(b); ++segment) {
       BadRows *bad = &b.bad[segment % kBadRing][half0];
       uint32_t listed[2] = {0, 0};
+      if (s.first + s.n > s.masked_from && !wait_listed(b, segment)) break;
       if (lane < (TREE ? 2 : 1) && s.first + s.n > s.masked_from) bad[lane].tiles = 0;
       __syncwarp();
       for (uint32_t e = 0; e < 2 * s.n; ++e) {  // every ring entry, so as never to be a turn ahead or behind
