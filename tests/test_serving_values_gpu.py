@@ -1,0 +1,47 @@
+"""What single values do in the serving attention: infinities and NaN that a row attends,
+finite columns beside them, and weights far below the largest."""
+
+import math
+
+import pytest
+import torch
+
+from tests._serving import UNIT, attend, check
+from tests.test_serving_attention_gpu import BF16, FP16, as_int64, make_cache, prompt_reference, randn
+from xpu_playground_b200 import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+
+def starts_of(counts):
+    return torch.tensor([0] + list(torch.tensor(counts).cumsum(0)), dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("heads", [(1, 1), (4, 2)])
+def test_prompt_columns_beside_non_finite_ones_are_rounded_once(heads):
+    """Column 0 of every value is NaN, the others are near 0.3: each weight is far below half a
+    step of the sum in 16 bits."""
+    n, d = 1000, 64
+    q, k = (randn(70 + i, n, h, d, scale=0.1) for i, h in enumerate(heads))
+    v = (randn(72, n, heads[1], d).float() * 0.05 + 0.3).bfloat16()
+    v[:, :, 0] = math.nan
+    out, lse = K.prompt_attention(K.PromptPlan([n], *heads, d), q, k, v)
+    want = prompt_reference([n], q, k, v, 1 / 8.0)
+    check(out, lse, *want, BF16)
+
+
+@pytest.mark.parametrize("length,nodes", [(0, 40), (90, 64), (700, 9)])
+def test_tree_columns_beside_non_finite_ones_are_rounded_once(length, nodes):
+    d = 128
+    cache, flat = make_cache([length], 1, d, 16, BF16, 74)
+    q, k = randn(75, nodes, 4, d, scale=0.1), randn(76, nodes, 1, d, scale=0.1)
+    v = (randn(77, nodes, 1, d).float() * 0.05 + 0.3).bfloat16()
+    v[:, 0, 3] = math.nan
+    sets = [(1 << (i + 1)) - 1 for i in range(nodes)]
+    ws = K.tree_attention_workspace(1, nodes, 4, 1, d)
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = K.tree_attention(cache, 0 + 1, ids, starts_of([nodes]), as_int64(sets), q, k, v, ws)
+    keys, values = (torch.cat([a.cpu(), b.cpu()])[:, 0] for a, b in ((flat[0][0], k), (flat[0][1], v)))
+    allowed = torch.cat([torch.ones(nodes, length, dtype=torch.bool), torch.ones(nodes, nodes, dtype=torch.bool).tril()], 1)
+    parts = [attend(q[:, h].cpu(), keys, values, allowed, 1 / math.sqrt(d)) for h in range(4)]
+    check(out, lse, *(torch.stack(p, 1) for p in zip(*parts)), BF16)

@@ -25,7 +25,7 @@
 //   10, 11    cleaning (trees: 11): in key tiles with masked keys, V rows that no row may
 //             attend are zeroed (0 x NaN would reach the sums), and rows with
 //             non-finite values are zeroed and listed; the rows that do attend
-//             them get p v added at the end (fix_row).
+//             them get p v added at the end (add_listed).
 // A segment of at most 128 rows (drafted trees, mostly) would leave one softmax
 // group idle: there both groups work for the same rows, on even and odd key
 // tiles, and join their sums at the end.
@@ -505,15 +505,14 @@ __device__ __forceinline__ uint32_t valid_keys(const Segment &s, uint32_t tile) 
   if (TREE && tile * kKeys >= s.len) return s.nodes;  // the drafts
   return min(kKeys, s.len - tile * kKeys);
 }
-// ---------------------------------------------------------------- fix_row ----
+// ------------------------------------------------------------- add_listed ----
 
 // Adds p v of the segment's listed keys (non-finite values, zeroed in the
-// product) to one row's columns [col, col + cols): dst16 (normalised by inv)
-// or dst32 (a partial row). Rare: plain loops over global memory.
+// product) to columns [col, col + 32) of one row, times inv, in FP32: the row is
+// rounded once, with everything in it. Rare: plain loops over global memory.
 template <typename T, int D, bool TREE>
-__device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadRows *bad, uint32_t position, uint32_t q_head,
-                                     uint64_t set, float m, float inv, T *dst16, float *dst32, uint32_t col,
-                                     uint32_t cols) {
+__device__ __noinline__ void add_listed(const Args &a, const Segment &s, const BadRows *bad, uint32_t position,
+                                        uint32_t q_head, uint64_t set, float m, float inv, uint32_t col, float *o) {
   const T *q = static_cast<const T *>(a.t.q) + (s.q0 - s.pos0 + static_cast<size_t>(position)) * a.t.q_stride + q_head * D;
   const float c = a.t.scale * kLog2e;
   for (uint32_t at = 0; at < 4 * 64; ++at) {  // half, listed tile, key of the half
@@ -521,31 +520,26 @@ __device__ __noinline__ void fix_row(const Args &a, const Segment &s, const BadR
     const uint32_t listed = *const_cast<const volatile uint32_t *>(&bad[half].tiles);
     __threadfence_block();
     if (i >= listed || !(bad[half].mask[i][j >> 5] >> (j & 31) & 1u)) continue;
-    {
-      const uint32_t in_tile = half * 64 + j, tile = bad[half].tile[i], key = tile * kKeys + in_tile;
-      const T *k, *v;
-      if (!TREE || tile * kKeys >= s.len) {  // packed: a prompt's key, or a draft
-        if (TREE ? !(set >> in_tile & 1u) : key > position) continue;
-        const size_t at = (static_cast<size_t>(s.base) + (TREE ? in_tile : key)) * a.t.kv_stride + s.head * D;
-        k = static_cast<const T *>(a.t.k) + at;
-        v = static_cast<const T *>(a.t.v) + at;
-      } else {
-        const xpu_kv_cache_t &kc = a.tree.cache;
-        const int32_t page = kc.tables[static_cast<size_t>(s.sequence) * kc.table_width + key / kc.page_size];
-        if (page < 0 || static_cast<uint32_t>(page) >= kc.pages) continue;
-        const size_t at = (((static_cast<size_t>(a.tree.layer) * kc.pages + page) * kc.kv_heads + s.head) * kc.page_size +
-                           key % kc.page_size) * D;
-        k = static_cast<const T *>(kc.k) + at;
-        v = static_cast<const T *>(kc.v) + at;
-      }
-      float dot = 0.f;
-      for (uint32_t d = 0; d < D; ++d) dot = fmaf(Elem<T>::to_float(q[d]), Elem<T>::to_float(k[d]), dot);
-      const float p = exp2f(fmaf(dot, c, -(m == -INFINITY ? 0.f : m * c)));
-      for (uint32_t d = col; d < col + cols; ++d) {
-        if (dst32) dst32[(d >> 2) * 128 + (d & 3)] = fmaf(p, Elem<T>::to_float(v[d]), dst32[(d >> 2) * 128 + (d & 3)]);
-        else dst16[d] = Elem<T>::from_float(fmaf(p * inv, Elem<T>::to_float(v[d]), Elem<T>::to_float(dst16[d])));
-      }
+    const uint32_t in_tile = half * 64 + j, tile = bad[half].tile[i], key = tile * kKeys + in_tile;
+    const T *k, *v;
+    if (!TREE || tile * kKeys >= s.len) {  // packed: a prompt's key, or a draft
+      if (TREE ? !(set >> in_tile & 1u) : key > position) continue;
+      const size_t at = (static_cast<size_t>(s.base) + (TREE ? in_tile : key)) * a.t.kv_stride + s.head * D;
+      k = static_cast<const T *>(a.t.k) + at;
+      v = static_cast<const T *>(a.t.v) + at;
+    } else {
+      const xpu_kv_cache_t &kc = a.tree.cache;
+      const int32_t page = kc.tables[static_cast<size_t>(s.sequence) * kc.table_width + key / kc.page_size];
+      if (page < 0 || static_cast<uint32_t>(page) >= kc.pages) continue;
+      const size_t at = (((static_cast<size_t>(a.tree.layer) * kc.pages + page) * kc.kv_heads + s.head) * kc.page_size +
+                         key % kc.page_size) * D;
+      k = static_cast<const T *>(kc.k) + at;
+      v = static_cast<const T *>(kc.v) + at;
     }
+    float dot = 0.f;
+    for (uint32_t d = 0; d < D; ++d) dot = fmaf(Elem<T>::to_float(q[d]), Elem<T>::to_float(k[d]), dot);
+    const float p = exp2f(fmaf(dot, c, -(m == -INFINITY ? 0.f : m * c))) * inv;
+    for (uint32_t d = 0; d < 32; ++d) o[d] = fmaf(p, Elem<T>::to_float(v[col + d]), o[d]);
   }
 }
 
@@ -897,6 +891,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           a.t.lse[token * a.t.q_heads + q_head] = log_sum(m, l, c);
         }
         const bool store = mine && token < a.t.tokens;
+        const BadRows *bad = b.bad[segment % kBadRing];
+        const bool listed = store && s.first + s.n > s.masked_from &&
+                            (*const_cast<const volatile uint32_t *>(&bad[0].tiles) |
+                             *const_cast<const volatile uint32_t *>(&bad[1].tiles)) != 0;
         const QuadRows out(dst16, store);
         if (out.any()) {
 #pragma unroll 1
@@ -916,6 +914,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
               for (uint32_t j = 0; j < 32; ++j)
                 o[j] = __float_as_uint(fmaf(__uint_as_float(o1[j]), w1, __uint_as_float(o[j])));
             }
+            if (listed) {
+              float f[32];
+#pragma unroll
+              for (uint32_t j = 0; j < 32; ++j) f[j] = __uint_as_float(o[j]);
+              add_listed<T, D, TREE>(a, s, bad, position, q_head, set, m, inv, q, f);
+#pragma unroll
+              for (uint32_t j = 0; j < 32; ++j) o[j] = __float_as_uint(f[j]);
+            }
+            __syncwarp();
             if (TREE && dst32) {
               if (store) {
 #pragma unroll
@@ -928,12 +935,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
               out.put(o, q * 2);
             }
           }
-          __syncwarp();  // a row's lane sees what its quad wrote of it
-        }
-        if (store && s.first + s.n > s.masked_from) {
-          const BadRows *bad = b.bad[segment % kBadRing];
-          if (*const_cast<const volatile uint32_t *>(&bad[0].tiles) | *const_cast<const volatile uint32_t *>(&bad[1].tiles))
-            fix_row<T, D, TREE>(a, s, bad, position, q_head, set, m, inv, dst16, dst32, col, cols);
         }
       }
       if constexpr (TREE) {
