@@ -218,11 +218,14 @@ size_t xpu_kv_workspace_size(uint32_t pages);
  * it by them: the lowest free pages, in the order of the list. */
 int xpu_kv_extend(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *starts, uint32_t count,
                   void *stream);
-/* Writes the positions that the last xpu_kv_extend (same list) added, in
+/* Writes the positions that the last xpu_kv_extend added (its list again), in
  * layers [layer, layer + layers): token t comes from row rows[t] (NULL: row t)
  * of k and v, each [layers][held][kv_heads][head_dim] with the given strides
  * in elements (multiples of 8). `tokens` is at least starts[count], of which
- * the rest is ignored. Writes nothing if the extension was refused. */
+ * the rest is ignored. Writes nothing if the extension was refused. Other
+ * operators may run between an extension and its writes; positions that a trim
+ * has taken off since, and sequences that are not the extension's, are not written
+ * and set XPU_KV_BAD_INDEX. */
 int xpu_kv_write(const xpu_kv_cache_t *cache, const int32_t *sequences, const int32_t *starts, uint32_t count,
                  uint32_t tokens, const int32_t *rows, const void *k, const void *v, uint32_t held,
                  uint64_t layer_stride, uint64_t row_stride, uint32_t layer, uint32_t layers, void *stream);

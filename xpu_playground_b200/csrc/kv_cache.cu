@@ -21,8 +21,10 @@
 // 13 us, 4 forks 11 us, where two launches from Python take 9 to 13.
 //
 // The workspace, zeroed once by the caller: {accepted, entries, first id that
-// compaction renames, ticket, ready, blocks that have seen it, -, -}, per entry {source page, new
-// page, rows}, and behind those compaction's new ids or a list of free pages.
+// compaction renames, ticket, ready, blocks that have seen it, sequences of the last extension, -}, per
+// entry {source page, new page, rows}, behind those compaction's new ids or a list of free pages, and
+// last the extension's sequences {id, length before it}, which no other operator touches:
+// its writes may come layer by layer with other calls between them.
 #include <algorithm>
 
 #include "common.cuh"
@@ -35,7 +37,7 @@ namespace {
 constexpr uint32_t kThreads = 1024, kWarps = kThreads / 32;
 constexpr uint32_t kHeader = 8, kEntry = 3;
 constexpr uint32_t kFew = 1024;  // pages whose ids a plan keeps in shared memory
-enum { kAccepted, kEntries, kRenamedFrom, kTicket, kReady, kSeen };
+enum { kAccepted, kEntries, kRenamedFrom, kTicket, kReady, kSeen, kExtended };
 constexpr long long kPlanWaitCycles = 4000000000ll;  // ~2 s at 1.9 GHz
 
 // The next kernel may be set up from here on; this one reads nothing before the
@@ -178,6 +180,10 @@ __device__ bool after_plan(const xpu_kv_cache_t &c, Plan plan) {
   return told == 1;
 }
 
+// Places of the workspace behind the header and the entries.
+__host__ __device__ constexpr uint32_t listed_pages(uint32_t pages) { return pages > XPU_KV_MAX_REQUESTS ? pages : XPU_KV_MAX_REQUESTS; }
+__host__ __device__ constexpr uint32_t extension_at(uint32_t pages) { return kHeader + (kEntry + 1) * listed_pages(pages); }
+
 // What the plan wrote, read past the L1.
 __device__ __forceinline__ int32_t planned(const xpu_kv_cache_t &c, uint32_t at) { return __ldcg(c.workspace + at); }
 
@@ -194,12 +200,14 @@ struct Extension {  // one thread's request
   }
 };
 
-__device__ void plan_extend(const xpu_kv_cache_t &c, const Extension &x, uint32_t count, uint32_t *bitmap, uint32_t *few) {
+// *before: this thread's sequence's length so far.
+__device__ void plan_extend(const xpu_kv_cache_t &c, const Extension &x, uint32_t count, uint32_t *bitmap, uint32_t *few,
+                            uint32_t *before) {
   const uint32_t i = threadIdx.x;
   const bool mine = i < count;
   const int32_t s = x.sequence;
   const bool in_range = mine && s >= 0 && static_cast<uint32_t>(s) < c.sequences;
-  const uint32_t old = in_range ? len_of(c, s) : 0;
+  const uint32_t old = *before = in_range ? len_of(c, s) : 0;
   if (!named_once(c, mine, s, bitmap) || __syncthreads_or(x.more < 0)) return refuse(c, XPU_KV_BAD_SEQUENCE);
   const uint32_t first = pages_of(old, c.page_size);
   const uint64_t after = static_cast<uint64_t>(old) + x.more;
@@ -220,6 +228,7 @@ __device__ void plan_extend(const xpu_kv_cache_t &c, const Extension &x, uint32_
 }
 
 struct Rows {
+  bool extended;  // the positions of the last extension, else those that this call has added
   const int32_t *rows;
   const uint16_t *k, *v;
   uint32_t tokens, held;
@@ -232,7 +241,8 @@ struct Rows {
 struct Piece {
   const uint4 *src;
   uint4 v[4];
-  uint32_t which, after, t;  // layer * 2 + K or V; tokens of the sequence from this one on
+  uint32_t which, after, t;  // layer * 2 + K or V; tokens of the sequence from this one on, and before it
+  uint32_t request;
   int32_t sequence;
 };
 
@@ -261,7 +271,6 @@ struct Writer {
   __device__ void fetch(Piece &p) {
     const uint32_t lane = threadIdx.x & 31, t = static_cast<uint32_t>(w % tokens);
     p.which = static_cast<uint32_t>(w / tokens);
-    p.t = t;
     w += warps;
     uint32_t lo = 0, hi = count;  // the last i with starts[i] <= t
     while (hi - lo > 1) {
@@ -275,6 +284,8 @@ struct Writer {
                     static_cast<int32_t>(t) >= begin && static_cast<int32_t>(t) < end;
     p.sequence = ok ? s : -1;
     p.after = static_cast<uint32_t>(end) - t;
+    p.t = t - static_cast<uint32_t>(begin);
+    p.request = lo;
     p.src = nullptr;
     if (!ok) return;
     p.src = reinterpret_cast<const uint4 *>((p.which & 1 ? r.v : r.k) + (p.which >> 1) * r.layer_stride + row * r.row_stride);
@@ -286,7 +297,17 @@ struct Writer {
   __device__ void put(const Piece &p) const {
     const uint32_t lane = threadIdx.x & 31;
     int64_t position = -1;
-    if (p.sequence >= 0) position = static_cast<int64_t>(__ldcg(c.lens + p.sequence)) - p.after;
+    if (p.sequence >= 0) {
+      const int32_t len = __ldcg(c.lens + p.sequence);
+      position = static_cast<int64_t>(len) - p.after;
+      if (r.extended) {
+        const int32_t *record = c.workspace + extension_at(c.pages) + 2 * p.request;
+        position = p.request < static_cast<uint32_t>(planned(c, kExtended)) && __ldcg(record) == p.sequence
+                       ? static_cast<int64_t>(__ldcg(record + 1)) + p.t
+                       : -1;
+        if (position >= len) position = -1;  // trimmed off since
+      }
+    }
     int32_t page = -1;
     if (position >= 0 && position < static_cast<int64_t>(c.table_width) * c.page_size)
       page = __ldcg(c.tables + static_cast<size_t>(p.sequence) * c.table_width + (position >> page_shift));
@@ -322,14 +343,24 @@ __global__ void __launch_bounds__(kThreads) k_kv_extend(const __grid_constant__ 
                                                         const int32_t *starts, uint32_t count) {
   __shared__ uint32_t bitmap[XPU_KV_MAX_SEQUENCES / 32], few[kFew];
   after_previous();
-  plan_extend(c, Extension(c, sequences, starts, count), count, bitmap, few);
+  const Extension x(c, sequences, starts, count);
+  uint32_t before;
+  plan_extend(c, x, count, bitmap, few, &before);
+  __syncthreads();
+  const bool accepted = c.workspace[kAccepted];
+  if (accepted && threadIdx.x < count) {
+    int32_t *record = c.workspace + extension_at(c.pages) + 2 * threadIdx.x;
+    record[0] = x.sequence;
+    record[1] = static_cast<int32_t>(before);
+  }
+  if (threadIdx.x == 0) c.workspace[kExtended] = accepted ? static_cast<int32_t>(count) : 0;
 }
 
 __global__ void __launch_bounds__(kThreads) k_kv_write(const __grid_constant__ xpu_kv_cache_t c, const int32_t *sequences,
                                                        const int32_t *starts, uint32_t count,
                                                        const __grid_constant__ Rows r) {
   after_previous();
-  if (!planned(c, kAccepted)) return;
+  if (!planned(c, kExtended)) return;  // refused
   Writer writer(c, sequences, starts, count, r);
   Piece first;
   const bool have = writer.more();
@@ -347,7 +378,8 @@ __global__ void __launch_bounds__(kThreads) k_kv_append(const __grid_constant__ 
   Piece first;
   const bool have = writer.more();
   if (have) writer.fetch(first);
-  if (after_plan(c, [&] { plan_extend(c, x, count, bitmap, few); })) writer.run(first, have);
+  uint32_t before;
+  if (after_plan(c, [&] { plan_extend(c, x, count, bitmap, few, &before); })) writer.run(first, have);
 }
 
 // -------------------------------------------------------------------- trim ----
@@ -527,9 +559,8 @@ uint32_t blocks_for(uint64_t warps) {
 }  // namespace
 
 size_t kv_workspace_bytes(uint32_t pages) {
-  // header, an entry per page (or request), and a page list or the new ids
-  return 4 * (kHeader + kEntry * static_cast<size_t>(std::max(pages, XPU_KV_MAX_REQUESTS)) +
-              std::max(pages, XPU_KV_MAX_REQUESTS));
+  // header, an entry per page (or request), a page list or the new ids, and the last extension
+  return 4 * (kHeader + (kEntry + 1) * static_cast<size_t>(listed_pages(pages)) + 2 * XPU_KV_MAX_REQUESTS);
 }
 
 cudaError_t kv_extend_launch(const xpu_kv_cache_t &c, const int32_t *sequences, const int32_t *starts, uint32_t count,
@@ -541,7 +572,7 @@ cudaError_t kv_write_launch(const xpu_kv_cache_t &c, const int32_t *sequences, c
                             uint32_t tokens, const int32_t *rows, const void *k, const void *v, uint32_t held,
                             uint64_t layer_stride, uint64_t row_stride, uint32_t layer, uint32_t layers, bool extend,
                             cudaStream_t s) {
-  const Rows r{rows, static_cast<const uint16_t *>(k), static_cast<const uint16_t *>(v), tokens, held, layer_stride, row_stride,
+  const Rows r{!extend, rows, static_cast<const uint16_t *>(k), static_cast<const uint16_t *>(v), tokens, held, layer_stride, row_stride,
                layer, layers};
   const uint32_t blocks = blocks_for(static_cast<uint64_t>(tokens) * layers * 2);
   return launch_after(extend ? k_kv_append : k_kv_write, blocks, kThreads, 0, s, c, sequences, starts, count, r);
