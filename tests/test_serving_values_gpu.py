@@ -45,3 +45,21 @@ def test_tree_columns_beside_non_finite_ones_are_rounded_once(length, nodes):
     allowed = torch.cat([torch.ones(nodes, length, dtype=torch.bool), torch.ones(nodes, nodes, dtype=torch.bool).tril()], 1)
     parts = [attend(q[:, h].cpu(), keys, values, allowed, 1 / math.sqrt(d)) for h in range(4)]
     check(out, lse, *(torch.stack(p, 1) for p in zip(*parts)), BF16)
+
+
+@pytest.mark.parametrize("length", [200, 1000, 2040, 5000])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+def test_attended_infinity_of_a_single_token_stays_one(length, value):
+    """A draft's infinite value comes out in its column, whatever number of parts the sequence was cut into."""
+    d = 128
+    cache, flat = make_cache([length], 1, d, 16, BF16, 80)
+    q, k, v = randn(81, 1, 4, d), randn(82, 1, 1, d), randn(83, 1, 1, d)
+    v[0, 0, 5] = value
+    ws = K.tree_attention_workspace(1, 1, 4, 1, d)
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = K.tree_attention(cache, 1, ids, starts_of([1]), as_int64([1]), q, k, v, ws)
+    keys, values = (torch.cat([a.cpu(), b.cpu()])[:, 0] for a, b in ((flat[0][0], k), (flat[0][1], v)))
+    parts = [attend(q[:, h].cpu(), keys, values, torch.ones(1, length + 1, dtype=torch.bool), 1 / math.sqrt(d)) for h in range(4)]
+    want, want_lse, size = (torch.stack(p, 1) for p in zip(*parts))
+    assert bool((out[0, :, 5] == value).all())
+    check(out, lse, want, want_lse, size, BF16)

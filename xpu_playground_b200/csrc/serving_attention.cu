@@ -588,7 +588,10 @@ struct Join {
       float top = m;
 #pragma unroll
       for (uint32_t e = 0; e < kTogether; ++e) {
-        if (x0 + e > c1) ml[e].x = -INFINITY;
+        if (x0 + e > c1) {  // behind the last part: nothing, also where its copy holds an infinity
+          ml[e].x = -INFINITY;
+          v[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
         top = fmaxf(top, ml[e].x);
       }
       const float keep = m == -INFINITY ? 0.f : exp2_approx((m - top) * c);
