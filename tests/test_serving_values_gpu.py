@@ -9,6 +9,7 @@ import torch
 from tests._serving import UNIT, attend, check
 from tests.test_serving_attention_gpu import BF16, FP16, as_int64, make_cache, prompt_reference, randn
 from xpu_playground_b200 import kernels as K
+from xpu_playground_b200.kv_cache import KvCache
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +64,48 @@ def test_attended_infinity_of_a_single_token_stays_one(length, value):
     want, want_lse, size = (torch.stack(p, 1) for p in zip(*parts))
     assert bool((out[0, :, 5] == value).all())
     check(out, lse, want, want_lse, size, BF16)
+
+
+def sink(keys, gap, at):
+    """Keys and values of which number `at` is `gap` nats above the others and has value 0, the others 1:
+    q = 8 e0, scale 1/8. The exact result is n w / (1 + n w) with w = exp(-gap)."""
+    k, v = torch.zeros(keys, 1, 64, dtype=FP16, device="cuda"), torch.ones(keys, 1, 64, dtype=FP16, device="cuda")
+    k[at, 0, 0], v[at] = gap, 0
+    return k, v
+
+
+def check_sink(out, lse, keys, gap):
+    """Each weight is rounded to 2^-11 of itself or 2^-36 of the largest (fp16's smallest step is 2^-24, half of it
+    2^-25, and the largest weight is held as 2^11 or more); 1e-4 for the FP32 arithmetic; then the output's own rounding."""
+    others = (keys - 1) * math.exp(-gap)
+    want = others / (1 + others)
+    tol = (2 * UNIT[FP16] + 1e-4) * want + keys * 2.0 ** -36 + 2.0 ** -25
+    assert float((out.double() - want).abs().max()) <= tol
+    assert float((lse.double() - gap - math.log1p(others)).abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("gap", [8.0, 14.0, 17.5, 20.0])
+@pytest.mark.parametrize("length,at", [(4095, 0), (4095, 4000), (16383, 7000), (65535, 0)])
+def test_many_small_weights_beside_a_large_one_tree(gap, length, at):
+    k, v = sink(length + 1, gap, at)
+    cache = KvCache(1, 512, 128, 1, 64, 1, 65536, dtype=FP16)
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache.append(ids, starts_of([length]), k[None, :length], v[None, :length])
+    q = torch.zeros(1, 2, 64, dtype=FP16, device="cuda")
+    q[:, :, 0] = 8
+    ws = K.tree_attention_workspace(1, 1, 2, 1, 64)
+    out, lse = K.tree_attention(cache, 0, ids, starts_of([1]), as_int64([1]), q, k[length:], v[length:], ws)
+    check_sink(out, lse, length + 1, gap)
+    assert cache.status() == 0
+
+
+@pytest.mark.parametrize("gap", [8.0, 17.5])
+@pytest.mark.parametrize("at", [0, 4000])
+def test_many_small_weights_beside_a_large_one_prompt(gap, at):
+    n = 8200
+    k, v = sink(n, gap, at)
+    q = torch.zeros(n, 2, 64, dtype=FP16, device="cuda")
+    q[:, :, 0] = 8
+    out, lse = K.prompt_attention(K.PromptPlan([n], 2, 1, 64), q, k, v)
+    for row in (at, at + 1, at + 100, 6000, n - 1):
+        check_sink(out[row], lse[row], row + 1, gap)

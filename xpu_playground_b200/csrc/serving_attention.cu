@@ -14,9 +14,9 @@
 //             to the input type and written back to TMEM over the scores as the
 //             A operand of the second product; FP32 sum of the unrounded p.
 //             The reference maximum m moves only when the true one has passed
-//             it by 2^8 (p then stays below 2^8, exact in FP32 sums and with the
-//             same relative rounding), so the accumulator in TMEM is rarely
-//             rescaled. At the end out = O / l, rounded once;
+//             it by 2^8 (fp16: 2^4), so the accumulator in TMEM is rarely
+//             rescaled; in fp16 p is 2^11 times as large, for its range (Weights).
+//             At the end out = O / l, rounded once;
 //   8         issues S_t = Q_t K^T (both operands in shared memory) and O_t +=
 //             P_t V (P from TMEM, V as it stands in memory, MN-major); S_t overwrites
 //             the P_t that the product before it read. While one tile is in its
@@ -66,10 +66,25 @@ constexpr uint32_t kBox = 128 * 128;   // bytes of 128 rows x 64 elements, 128-b
 constexpr uint32_t kThreads = 384;
 constexpr uint32_t kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10;
 constexpr unsigned kErrAttentionTimeout = 4u;
-constexpr float kRescale = 8.f;        // in powers of two
 constexpr uint32_t kBadRing = 8;
 constexpr uint32_t kEarlyKeys = 96;    // of a tile's probabilities, handed to the tensor cores before the rest
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Powers of two: how far a maximum may pass the reference before the accumulator is rescaled, and
+// the weight of the reference itself, so that no weight passes 2^15. bf16 holds FP32's exponents.
+// fp16's smallest step is 2^-24: lifted by 2^kLift, weights keep their relative rounding down to
+// 2^-(14 + kLift) of the reference's and are lost below 2^-(25 + kLift), not below 2^-25, where many
+// of them can still make up the result (16384 keys 17.5 nats below one). The sum of weights is lifted
+// with them; its logarithm takes the lift out. Rescaling from 2^4 on costs 16 packed prompts of 1 to 2047
+// tokens, 16/8 heads, 149 -> 154 us (2^6 with a lift of 9: 149, with a quarter of the range lost).
+template <typename T>
+struct Weights {
+  static constexpr float kRescale = 8.f, kLift = 0.f;
+};
+template <>
+struct Weights<__half> {
+  static constexpr float kRescale = 4.f, kLift = 15.f - kRescale;
+};
 
 template <int D, bool TREE>
 struct Shape {
@@ -255,11 +270,12 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
   return Pair(d);
 }
-// Natural logarithm of 2^(c m) l; -inf where the sum is empty.
+// Natural logarithm of 2^(c m - lift) l; -inf where the sum is empty.
+template <typename T>
 __device__ __forceinline__ float log_sum(float m, float l, float c) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(l));
-  return l == 0.f ? -INFINITY : fmaf(m, c, y) * kLn2;
+  return l == 0.f ? -INFINITY : fmaf(m, c, y - Weights<T>::kLift) * kLn2;
 }
 // Largest of three, NaN if one is.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
@@ -538,7 +554,7 @@ __device__ __noinline__ void add_listed(const Args &a, const Segment &s, const B
     }
     float dot = 0.f;
     for (uint32_t d = 0; d < D; ++d) dot = fmaf(Elem<T>::to_float(q[d]), Elem<T>::to_float(k[d]), dot);
-    const float p = exp2f(fmaf(dot, c, -(m == -INFINITY ? 0.f : m * c))) * inv;
+    const float p = exp2f(fmaf(dot, c, m == -INFINITY ? 0.f : fmaf(-m, c, Weights<T>::kLift))) * inv;
     for (uint32_t d = 0; d < 32; ++d) o[d] = fmaf(p, Elem<T>::to_float(v[col + d]), o[d]);
   }
 }
@@ -612,7 +628,7 @@ struct Join {
     const size_t token = static_cast<size_t>(s.q0) + index;
     reinterpret_cast<uint2 *>(static_cast<T *>(a.t.out) + token * a.t.out_stride + head * D)[piece] =
         make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
-    if (a.t.lse && piece == 0) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
+    if (a.t.lse && piece == 0) a.t.lse[token * a.t.q_heads + head] = log_sum<T>(m, l, c);
   }
 
   // Any number: a block of 32 rows a warp, a row a lane, 64 columns at a time. With one row
@@ -664,7 +680,7 @@ struct Join {
       out.put(p, q * 2);
       out.put(p + 16, q * 2 + 64);
     }
-    if (a.t.lse && mine && first == 0) a.t.lse[token * a.t.q_heads + head] = log_sum(m, l, c);
+    if (a.t.lse && mine && first == 0) a.t.lse[token * a.t.q_heads + head] = log_sum<T>(m, l, c);
   }
 };
 
@@ -810,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         };
         // a row with an infinite or undefined score is undefined as a whole
         auto shift = [&] {
-          const float mc = m == -INFINITY ? 0.f : (m == INFINITY ? NAN : -m * c);
+          const float mc = m == -INFINITY ? 0.f : (m == INFINITY ? NAN : fmaf(-m, c, Weights<T>::kLift));
           return Pair(mc, mc);
         };
         float top4[4] = {m, m, m, m};  // four chains; NaN if one score is
@@ -826,10 +842,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         if (masked) mask(64);
         search(64);
         const float top = max3_nan(max3_nan(top4[0], top4[1], top4[2]), top4[3], top4[3]);
-        const bool grown = top != m && !((top - m) * c <= kRescale);  // m = -inf included, and NaN
+        const bool grown = top != m && !((top - m) * c <= Weights<T>::kRescale);  // m = -inf included, and NaN
         if (__any_sync(kFullMask, grown)) {
-          const float keep = grown ? exp2_approx((m - top) * c) : 1.f;
-          if (grown) m = top;
+          // the others of the warp go along, so that they need none of their own soon
+          const float keep = top != m ? exp2_approx((m - top) * c) : 1.f;
+          m = top;
           l *= keep;
           if (i > 0) {
 #pragma unroll 1
@@ -891,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
           if (mine && col == 0)
             reinterpret_cast<float2 *>(a.tree.partial + 2ull * gridDim.x * 256 * D)[s.slot * 256 + row] = make_float2(m, l);
         } else if (mine && a.t.lse && col == 0 && token < a.t.tokens) {
-          a.t.lse[token * a.t.q_heads + q_head] = log_sum(m, l, c);
+          a.t.lse[token * a.t.q_heads + q_head] = log_sum<T>(m, l, c);
         }
         const bool store = mine && token < a.t.tokens;
         const BadRows *bad = b.bad[segment % kBadRing];
