@@ -842,7 +842,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attention(const __grid_constant
         if (masked) mask(64);
         search(64);
         const float top = max3_nan(max3_nan(top4[0], top4[1], top4[2]), top4[3], top4[3]);
-        const bool grown = top != m && !((top - m) * c <= Weights<T>::kRescale);  // m = -inf included, and NaN
+        // m = -inf included, and NaN; not the rows behind the last whole position (126 and 127 of a group of 7),
+        // whose queries no load writes: stale NaN would rescale for every key tile
+        const bool grown = mine && top != m && !((top - m) * c <= Weights<T>::kRescale);
         if (__any_sync(kFullMask, grown)) {
           // the others of the warp go along, so that they need none of their own soon
           const float keep = top != m ? exp2_approx((m - top) * c) : 1.f;
