@@ -3,6 +3,10 @@
 These pass device pointers and sizes straight through to libxpu_cuda; torch
 only provides device memory and the current CUDA stream. Every tensor must be
 a contiguous CUDA tensor; 16-bit tensors are passed by their bit patterns.
+
+With ``stream`` a call is queued on that stream; outputs that are not given are
+then allocated for it. As with any torch operation on another stream, inputs
+have to be ready there and other streams have to wait for the results.
 """
 
 from __future__ import annotations
@@ -31,6 +35,18 @@ def _stream(stream=None) -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def _allocate(make, stream, *args, **kwargs) -> torch.Tensor:
+    """make(*args, **kwargs) for a kernel on `stream`: memory of that stream, so that nothing
+    still queued elsewhere uses it, and kept from reuse until the current stream's work is done too."""
+    if stream is None or stream == torch.cuda.current_stream(stream.device):
+        return make(*args, **kwargs)
+    current = torch.cuda.current_stream(stream.device)
+    with torch.cuda.stream(stream):
+        t = make(*args, **kwargs)
+    t.record_stream(current)
+    return t
+
+
 def _dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.bfloat16:
         return XPU_BF16
@@ -43,7 +59,7 @@ def gemv(matrix: torch.Tensor, vector: torch.Tensor, out: torch.Tensor | None = 
          stream=None) -> torch.Tensor:
     m, k = matrix.shape
     if out is None:
-        out = torch.empty(m, dtype=matrix.dtype, device=matrix.device)
+        out = _allocate(torch.empty, stream, m, dtype=matrix.dtype, device=matrix.device)
     call("xpu_gemv", _dtype_code(matrix), _ptr(matrix), _ptr(vector), _ptr(out), m, k,
          _stream(stream))
     return out
@@ -56,7 +72,7 @@ def gemm_bt(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None, s
     if k2 != k or a.dtype != w.dtype:
         raise ValueError("gemm_bt: A is [m,k] and W is [n,k] of the same dtype")
     if out is None:
-        out = torch.empty(m, n, dtype=a.dtype, device=a.device)
+        out = _allocate(torch.empty, stream, m, n, dtype=a.dtype, device=a.device)
     call("xpu_gemm_bt", _dtype_code(a), _ptr(a), _ptr(w), _ptr(out), m, n, k, _stream(stream))
     return out
 
@@ -69,7 +85,7 @@ def gemm(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None = None,
     if k2 != k or a.dtype != b.dtype:
         raise ValueError("gemm: A is [m,k] and B is [k,n] of the same dtype")
     if out is None:
-        out = torch.empty(m, n, dtype=a.dtype, device=a.device)
+        out = _allocate(torch.empty, stream, m, n, dtype=a.dtype, device=a.device)
     call("xpu_gemm", _dtype_code(a), _ptr(a), _ptr(b), _ptr(out), m, n, k, _stream(stream))
     return out
 
@@ -91,7 +107,7 @@ def peak_mem_read(surface: torch.Tensor, sink: torch.Tensor | None = None, strea
     checksums (one per 2 KiB unit: height * 2 of them)."""
     height = surface.numel() // 1024
     if sink is None:
-        sink = torch.zeros(height * 2, dtype=torch.float32, device=surface.device)
+        sink = _allocate(torch.zeros, stream, height * 2, dtype=torch.float32, device=surface.device)
     call("xpu_peak_mem_read", _ptr(surface), _ptr(sink), height, _stream(stream))
     return sink
 
@@ -99,7 +115,7 @@ def peak_mem_read(surface: torch.Tensor, sink: torch.Tensor | None = None, strea
 def peak_compute(ctas: int, rounds: int, sink: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """ctas x rounds x 8 tensor-core MMAs; returns sink (1 + 32 rounds each)."""
     if sink is None:
-        sink = torch.zeros(ctas, dtype=torch.float32, device="cuda")
+        sink = _allocate(torch.zeros, stream, ctas, dtype=torch.float32, device="cuda")
     call("xpu_peak_compute", _ptr(sink), ctas, rounds, _stream(stream))
     return sink
 
@@ -165,7 +181,7 @@ def _packed(name: str, t: torch.Tensor, heads: int, head_dim: int) -> int:
     return row if shape[0] > 1 else max(row, heads * head_dim)
 
 
-def _attention_args(q, k, v, kv_heads, head_dim, scale, out, lse):
+def _attention_args(q, k, v, kv_heads, head_dim, scale, out, lse, stream):
     dtype, shape, kv_shape = q.dtype, q.shape, k.shape
     if k.dtype != dtype or v.dtype != dtype:
         raise ValueError("q, k and v must have one dtype")
@@ -183,13 +199,14 @@ def _attention_args(q, k, v, kv_heads, head_dim, scale, out, lse):
             raise ValueError("k and v need one row stride")
     # (empty_like, and sizes one by one, take half the time of a torch.Size)
     if out is None:
-        out = torch.empty_like(q) if whole else torch.empty(tokens, q_heads, head_dim, dtype=dtype, device=q.device)
+        out = (_allocate(torch.empty_like, stream, q) if whole else
+               _allocate(torch.empty, stream, tokens, q_heads, head_dim, dtype=dtype, device=q.device))
     elif out.dtype != dtype or out.shape != shape:
         raise ValueError("out must have q's shape and dtype")
     else:
         out_stride = _packed("out", out, q_heads, head_dim)
     if lse is None:
-        lse = torch.empty(tokens, q_heads, dtype=torch.float32, device=q.device)
+        lse = _allocate(torch.empty, stream, tokens, q_heads, dtype=torch.float32, device=q.device)
     elif lse.dtype != torch.float32 or lse.shape != shape[:2] or not lse.is_cuda or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous float32 CUDA tensor [tokens, q_heads]")
     return out, lse, q_stride, kv_stride, out_stride, head_dim ** -0.5 if scale is None else scale
@@ -225,7 +242,8 @@ def prompt_attention(plan: PromptPlan, q: torch.Tensor, k: torch.Tensor, v: torc
     scale defaults to 1 / sqrt(head_dim). Returns (out, lse)."""
     if q.shape[0] != plan.tokens or q.dim() != 3 or q.shape[1] != plan.q_heads:
         raise ValueError(f"q must be [{plan.tokens}, {plan.q_heads}, {plan.head_dim}] for this plan")
-    out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, plan.kv_heads, plan.head_dim, scale, out, lse)
+    out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, plan.kv_heads, plan.head_dim, scale, out, lse,
+                                                                    stream)
     call("xpu_prompt_attention", _dtype_code(q), plan.device_plan.data_ptr(), plan.blocks, q.data_ptr(), k.data_ptr(),
          v.data_ptr(), out.data_ptr(), lse.data_ptr(), plan.tokens, plan.q_heads, plan.kv_heads, plan.head_dim, q_stride,
          kv_stride, out_stride, scale, _stream(stream))
@@ -255,7 +273,8 @@ def tree_attention(cache, layer: int, sequences: torch.Tensor, starts: torch.Ten
         raise ValueError("sequences and starts are int32, ancestors int64")
     if starts.numel() != sequences.numel() + 1 or ancestors.numel() != q.shape[0]:
         raise ValueError("starts needs one entry more than sequences, ancestors one per node")
-    out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, cache.kv_heads, cache.head_dim, scale, out, lse)
+    out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, cache.kv_heads, cache.head_dim, scale, out, lse,
+                                                                    stream)
     call("xpu_tree_attention", cache.handle, layer, _ptr(sequences), _ptr(starts), _ptr(ancestors), sequences.numel(),
          q.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), q.shape[1], q_stride, kv_stride,
          out_stride, scale, _ptr(workspace), workspace.numel(), _stream(stream))
