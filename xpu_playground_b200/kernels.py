@@ -212,10 +212,14 @@ def _attention_args(q, k, v, kv_heads, head_dim, scale, out, lse, stream):
     return out, lse, q_stride, kv_stride, out_stride, head_dim ** -0.5 if scale is None else scale
 
 
+_copy_streams: dict[int, torch.cuda.Stream] = {}
+
+
 class PromptPlan:
     """Which thread block computes which tiles of a batch of packed prompts
     (xpu_prompt_plan). It depends on the lengths and heads alone: make it once
-    per batch and use it for every layer."""
+    per batch and use it for every layer. Making it waits for its own copy to
+    the device and for nothing that is queued there; any stream may use it."""
 
     def __init__(self, lens, q_heads: int, kv_heads: int, head_dim: int, device=None):
         n = np.ascontiguousarray(lens, dtype=np.uint32)
@@ -232,7 +236,18 @@ class PromptPlan:
         _lib.check(status)
         self.blocks, self.tokens = int(plan[0]), int(plan[1])
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
-        self.device_plan = torch.from_numpy(plan[:used.value]).to(device or "cuda")
+        device = torch.device(device or "cuda")
+        index = torch.cuda.current_device() if device.index is None else device.index
+        stream = _copy_streams.get(index)
+        if stream is None:
+            stream = _copy_streams[index] = torch.cuda.Stream(index)
+        with torch.cuda.stream(stream):
+            self.device_plan = torch.from_numpy(plan[:used.value]).to(f"cuda:{index}")
+        self._readers: set[int] = set()  # streams that the memory is kept for when the plan goes
+
+    def _read_on(self, stream, raw: int) -> None:
+        self._readers.add(raw)
+        self.device_plan.record_stream(stream if stream is not None else torch.cuda.current_stream())
 
 
 def prompt_attention(plan: PromptPlan, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None,
@@ -244,9 +259,12 @@ def prompt_attention(plan: PromptPlan, q: torch.Tensor, k: torch.Tensor, v: torc
         raise ValueError(f"q must be [{plan.tokens}, {plan.q_heads}, {plan.head_dim}] for this plan")
     out, lse, q_stride, kv_stride, out_stride, scale = _attention_args(q, k, v, plan.kv_heads, plan.head_dim, scale, out, lse,
                                                                     stream)
+    raw = _stream(stream)
+    if raw not in plan._readers:
+        plan._read_on(stream, raw)
     call("xpu_prompt_attention", _dtype_code(q), plan.device_plan.data_ptr(), plan.blocks, q.data_ptr(), k.data_ptr(),
          v.data_ptr(), out.data_ptr(), lse.data_ptr(), plan.tokens, plan.q_heads, plan.kv_heads, plan.head_dim, q_stride,
-         kv_stride, out_stride, scale, _stream(stream))
+         kv_stride, out_stride, scale, raw)
     return out, lse
 
 
