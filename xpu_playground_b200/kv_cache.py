@@ -87,10 +87,10 @@ class KvCache:
         held, row = shape[1], self.kv_heads * self.head_dim
         layer = held * row
         if not k.is_contiguous() or not v.is_contiguous():
-            if k.stride() != v.stride():
+            row = kernels._packed("k and v", k[0], self.kv_heads, self.head_dim)  # too short a stride is refused below
+            layer = k.stride(0) if lead > 1 else 0
+            if kernels._packed("k and v", v[0], self.kv_heads, self.head_dim) != row or lead > 1 and v.stride(0) != layer:
                 raise ValueError("k and v must have one layout")
-            row = max(row, kernels._packed("k and v", k[0], self.kv_heads, self.head_dim))
-            layer = k.stride(0)
         if not k.is_cuda or not v.is_cuda:
             raise ValueError("libxpu_cuda entry points take CUDA tensors")
         tokens, at = (held, None) if rows is None else (rows.numel(), self._ids(rows))
