@@ -60,10 +60,15 @@ class KvCache:
 
     def status(self) -> int:
         """Bits that refused requests have set (EXHAUSTED, BAD_SEQUENCE,
-        SHARED_CUT, BAD_INDEX, TIMEOUT), cleared by reading; waits for the device."""
+        SHARED_CUT, BAD_INDEX, TIMEOUT), cleared by reading; waits for the device.
+        After a TIMEOUT the workspace is made ready again."""
         torch.cuda.synchronize(self._status.device)  # the operators may have run on any stream
         bits = int(self._status.item())
-        self._status.zero_()
+        if bits:
+            self._status.zero_()
+            if bits & TIMEOUT:
+                self._workspace.zero_()
+            torch.cuda.synchronize(self._status.device)  # before a call on any stream can set a bit again
         return bits
 
     @staticmethod
