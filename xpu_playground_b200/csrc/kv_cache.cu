@@ -47,6 +47,17 @@ __device__ __forceinline__ void after_previous() {
   grid_dep_wait();
 }
 
+// 16 bytes of a row that is read once. The rows may come from the kernel before, which can still run
+// when this one has begun: coherent loads, kept behind the wait for its end.
+__device__ __forceinline__ uint4 ld_row16(const uint4 *p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 __device__ __forceinline__ uint32_t pages_of(uint32_t positions, uint32_t size) { return (positions + size - 1) / size; }
 
 // Exclusive prefix sum over the CTA in thread order; *total gets the sum.
@@ -291,7 +302,7 @@ struct Writer {
     p.src = reinterpret_cast<const uint4 *>((p.which & 1 ? r.v : r.k) + (p.which >> 1) * r.layer_stride + row * r.row_stride);
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i)
-      if (lane + 32 * i < chunks) p.v[i] = ld_stream16(p.src + lane + 32 * i);
+      if (lane + 32 * i < chunks) p.v[i] = ld_row16(p.src + lane + 32 * i);
   }
 
   __device__ void put(const Piece &p) const {
@@ -322,7 +333,7 @@ struct Writer {
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i)
       if (lane + 32 * i < chunks) __stcs(dst + at(lane + 32 * i), p.v[i]);
-    for (uint32_t e = lane + 128; e < chunks; e += 32) dst[at(e)] = ld_stream16(p.src + e);
+    for (uint32_t e = lane + 128; e < chunks; e += 32) dst[at(e)] = ld_row16(p.src + e);
   }
 
   // `have`: the first piece is fetched already
