@@ -362,7 +362,8 @@ int xpu_prompt_attention(int dtype, const int32_t *plan, uint32_t plan_blocks, c
                          void *stream) {
   XPU_GUARD({
     const AttnTensors t{q, k, v, out, lse, tokens, q_heads, kv_heads, head_dim, q_stride, kv_stride, out_stride, scale};
-    if (tokens == 0 || plan_blocks == 0) return XPU_OK;
+    if (tokens == 0) return XPU_OK;
+    XPU_REQUIRE(plan_blocks > 0, "xpu_prompt_attention: the plan has no tiles for these tokens");
     XPU_REQUIRE(plan && aligned16(plan), "xpu_prompt_attention: the plan must be a 16-byte aligned device pointer");
     XPU_CHECKED(check_attention(dtype, t, "xpu_prompt_attention"));
     return cuda_status(prompt_attention_launch(dtype == XPU_FP16, plan, plan_blocks, t, as_stream(stream)),
