@@ -207,6 +207,8 @@ class Server:
                  depth: int = 6) -> list[list[list[int]]]:
         """`samples` continuations of each prompt, of new_tokens tokens: sample i begins with the
         prompt's i-th most likely next token and goes on greedily."""
+        if not all(prompts):
+            raise ValueError("a prompt needs at least one token")
         s, cache, many = self.model.shape, self.cache, len(prompts)
         first = self.prefill(prompts, list(range(many))).topk(samples, -1).indices.tolist()
         owners = [p for p in range(many) for _ in range(samples)]
