@@ -255,7 +255,7 @@ int xpu_kv_compact(const xpu_kv_cache_t *cache, void *stream);
  * positions up to each row's own; lse (may be NULL) [tokens][q_heads] gets
  * the natural logarithm of each row's sum of exponentials. FP32 scores,
  * statistics and sums; the probabilities are rounded to dtype for the second
- * product. head_dim 64 or 128, q_heads a multiple of kv_heads (at most 64 per kv head),
+ * product (fp16: weights below 2^-36 of a row's largest are lost). head_dim 64 or 128, q_heads a multiple of kv_heads (at most 64 per kv head),
  * pointers 16-byte aligned, scale positive and finite.
  *
  * The plan lists each thread block's tiles, longest first; it depends on the
@@ -277,7 +277,8 @@ int xpu_prompt_attention(int dtype, const int32_t *plan, uint32_t plan_blocks, c
  * sequence in `layer`, and the nodes j of its own tree whose bit j of
  * ancestors[r] is set (its own bit included, if it is to see itself). A tree
  * of one node is the single-token decode step. A row that attends nothing
- * gives zeros and lse -inf. Types, strides and precision as
+ * gives zeros and lse -inf. Rows of nodes that no tree names, or behind a tree's 64th
+ * (which sets XPU_KV_BAD_INDEX), are not written. Types, strides and precision as
  * xpu_prompt_attention. The drafts' keys and values are not in the cache:
  * xpu_kv_append adds the accepted ones. The workspace holds
  * xpu_tree_attention_workspace_size bytes, zeroed once before its first use

@@ -10,8 +10,8 @@ a tree of drafted tokens per sequence in one forward pass
 frees sequences that are done (``KvCache.trim``, ``KvCache.compact``). Drafts come
 from the sequence's own text: what followed the last occurrences of its newest
 token. With ``width`` 0 a tree is one node and the loop is plain greedy decoding;
-drafts change how many steps it takes, not the tokens (up to exact ties of the
-rounded logits).
+drafts change how many steps it takes, not the tokens (up to logits that differ
+by no more than their rounding).
 
     python -m xpu_playground_b200.speculative --preset tiny --prompts 3 --new-tokens 48
 """
