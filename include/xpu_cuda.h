@@ -293,6 +293,58 @@ int xpu_tree_attention(const xpu_kv_cache_t *cache, uint32_t layer, const int32_
                        const void *v, void *out, float *lse, uint32_t q_heads, uint64_t q_stride, uint64_t kv_stride,
                        uint64_t out_stride, float scale, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------ 8-bit rows --
+ * Products of activations and weights that are held in 8 bits (e4m3), and the
+ * operators that bring a decoder layer's activations to that form (no
+ * counterpart in the reference, whose weights are bf16). Each XPU_FP8_BLOCK columns of
+ * a row y have the scale s = max(max |y| / 448, 2^-126) and are e4m3(y / s), rounded
+ * to nearest: q [rows][width] and scales [ceil(width / 128)][rows], FP32, a group's
+ * scales side by side. A group with a NaN or an infinity stands for NaN there
+ * or throughout. Arithmetic in FP32. width is a multiple of 16, pointers are 16-byte
+ * aligned (scales: 4), strides in elements of `dtype` and multiples of 8. rows
+ * 0: nothing is done. q and scales may not overlap the inputs.
+ *
+ * xpu_fp8_quantize: y = x.
+ * xpu_fp8_silu_multiply: y = gate / (1 + exp(-gate)) * up, of one row stride.
+ * xpu_fp8_rms_norm: t = x + residual (NULL: x) rounded to dtype and stored in
+ *   total (may be NULL, and may be x or residual itself, with its stride); y = t * rsqrt(mean(t^2)
+ *   + epsilon) * weight. width up to 32768. */
+#define XPU_FP8_BLOCK 128u
+int xpu_fp8_quantize(int dtype, const void *x, uint64_t stride, void *q, float *scales, uint32_t rows, uint32_t width,
+                     void *stream);
+int xpu_fp8_silu_multiply(int dtype, const void *gate, const void *up, uint64_t stride, void *q, float *scales, uint32_t rows,
+                          uint32_t width, void *stream);
+int xpu_fp8_rms_norm(int dtype, const void *x, uint64_t x_stride, const void *residual, uint64_t residual_stride,
+                     const void *weight, float epsilon, void *total, uint64_t total_stride, void *q, float *scales,
+                     uint32_t rows, uint32_t width, void *stream);
+/* c[m][n] = sum over groups g of 128 columns of a_scales[g][m] * w_scales[n / 128][g] *
+ * sum_{k in g} a[m][k] w[n][k]: rows in the form above against weights w [n][k] (e4m3) with
+ * a scale for each block of 128 x 128, w_scales [ceil(n / 128)][ceil(k / 128)]. FP32 sums,
+ * c [m][n] rounded once to dtype. k is a multiple of 16; a, w and c are contiguous,
+ * 16-byte aligned. Stands beside xpu_gemm_bt. */
+int xpu_fp8_gemm(int dtype, const void *a, const float *a_scales, const void *w, const float *w_scales, void *c, uint32_t m,
+                 uint32_t n, uint32_t k, void *stream);
+
+/* -------------------------------------------------------------- sampling --
+ * A token for each row of logits [rows][vocabulary] (16 bits, row stride in elements), from
+ * given random numbers u in [0, 1) (no counterpart in the reference, whose
+ * QwenArgmax is greedy). Order a row's tokens by falling logit, of equal ones the
+ * lowest id first, and give each the weight exp((l - l_max) / temperature).
+ * Kept are the first top_k (0: all); of those the shortest beginning with at
+ * least top_p of their weight; of those the tokens whose weight is at least min_p; and the first in any case.
+ * The token is the first whose sum of weights exceeds u times that of all kept,
+ * logprob (may be NULL) the natural logarithm of its share. temperature 0: the first
+ * token, logprob 0. Settings are one a row on the device; NULL: temperature 1,
+ * no top-k, top-p 1, min-p 0. A token of -inf is never chosen. A row with a NaN or
+ * +inf, with nothing but -inf, or with settings that are NaN or
+ * negative (temperature, top_k) or a u outside [0, 1) gives token -1 and logprob -inf.
+ * Weights and sums in FP64, in a fixed order. vocabulary is 1 to
+ * XPU_SAMPLE_MAX_VOCABULARY. */
+#define XPU_SAMPLE_MAX_VOCABULARY 1048576u
+int xpu_sample(int dtype, const void *logits, uint64_t stride, const float *temperature, const int32_t *top_k,
+               const float *top_p, const float *min_p, const float *u, int32_t *tokens, float *logprobs, uint32_t rows,
+               uint32_t vocabulary, void *stream);
+
 /* ------------------------------------------------------- synthetic data --
  * Seeded, irregular inputs generated on the device (the reference generates
  * its benchmark inputs on the device too: gemv.cpp:156-167). Each element is

@@ -87,6 +87,11 @@ SIGNATURES: dict[str, tuple] = {
     "xpu_prompt_attention": (i32, [i32, vp, u32, vp, vp, vp, vp, vp, u32, u32, u32, u32, u64, u64, u64, f32, vp]),
     "xpu_tree_attention_workspace_size": (sz, [u32, u32, u32, u32, u32]),
     "xpu_tree_attention": (i32, [vp, u32, vp, vp, vp, u32, u32, vp, vp, vp, vp, vp, u32, u64, u64, u64, f32, vp, sz, vp]),
+    "xpu_fp8_quantize": (i32, [i32, vp, u64, vp, vp, u32, u32, vp]),
+    "xpu_fp8_silu_multiply": (i32, [i32, vp, vp, u64, vp, vp, u32, u32, vp]),
+    "xpu_fp8_rms_norm": (i32, [i32, vp, u64, vp, u64, vp, f32, vp, u64, vp, vp, u32, u32, vp]),
+    "xpu_fp8_gemm": (i32, [i32, vp, vp, vp, vp, vp, u32, u32, u32, vp]),
+    "xpu_sample": (i32, [i32, vp, u64, vp, vp, vp, vp, vp, vp, vp, u32, u32, vp]),
     "xpu_fill_uniform16": (i32, [i32, vp, u64, u64, u64, vp]),
     "xpu_fill_normal_bf16": (i32, [vp, u64, u64, u64, f32, vp]),
     "xpu_qwen3_create": (i32, [vp, u32, i32, u32, u32, vp]),

@@ -104,6 +104,22 @@ static int check_attention(int dtype, const AttnTensors &t, const char *who) {
   return XPU_OK;
 }
 
+static bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+// Checks of the operators that write 8-bit rows; `other` is their second input.
+static int check_fp8_rows(int dtype, const void *x, const void *other, uint64_t stride, const void *q, const float *scales,
+                          uint32_t rows, uint32_t width, const char *who) {
+  const std::string at = std::string(who) + ": ";
+  XPU_REQUIRE(x && other && q && scales, at + "null pointer");
+  XPU_REQUIRE(aligned16(x) && aligned16(other) && aligned16(q), at + "inputs and q must be 16-byte aligned");
+  XPU_REQUIRE(aligned4(scales), at + "scales must be 4-byte aligned");
+  XPU_REQUIRE(dtype == XPU_BF16 || dtype == XPU_FP16, at + "dtype must be XPU_BF16 or XPU_FP16");
+  XPU_REQUIRE(width > 0 && width % 16 == 0, at + "width must be a positive multiple of 16");
+  XPU_REQUIRE(rows < (1u << 31) && width < (1u << 31), at + "too many rows or columns");
+  XPU_REQUIRE(stride % 8 == 0 && stride >= width && stride < (1ull << 32), at + "row strides must be multiples of 8 elements and hold a row");
+  return XPU_OK;
+}
+
 #define XPU_CHECKED(expr)                  \
   do {                                     \
     const int status_ = (expr);            \
@@ -336,6 +352,81 @@ int xpu_kv_compact(const xpu_kv_cache_t *cache, void *stream) {
   XPU_GUARD({
     XPU_CHECKED(check_cache(cache, "xpu_kv_compact"));
     return cuda_status(kv_compact_launch(*cache, as_stream(stream)), "xpu_kv_compact");
+  })
+}
+
+int xpu_fp8_quantize(int dtype, const void *x, uint64_t stride, void *q, float *scales, uint32_t rows, uint32_t width,
+                     void *stream) {
+  XPU_GUARD({
+    if (rows == 0) return XPU_OK;
+    XPU_CHECKED(check_fp8_rows(dtype, x, x, stride, q, scales, rows, width, "xpu_fp8_quantize"));
+    return cuda_status(fp8_rows_launch(dtype == XPU_FP16, static_cast<const uint16_t *>(x), nullptr, stride,
+                                       static_cast<uint8_t *>(q), scales, rows, width, as_stream(stream)),
+                       "xpu_fp8_quantize");
+  })
+}
+
+int xpu_fp8_silu_multiply(int dtype, const void *gate, const void *up, uint64_t stride, void *q, float *scales, uint32_t rows,
+                          uint32_t width, void *stream) {
+  XPU_GUARD({
+    if (rows == 0) return XPU_OK;
+    XPU_CHECKED(check_fp8_rows(dtype, gate, up, stride, q, scales, rows, width, "xpu_fp8_silu_multiply"));
+    return cuda_status(fp8_rows_launch(dtype == XPU_FP16, static_cast<const uint16_t *>(gate), static_cast<const uint16_t *>(up),
+                                       stride, static_cast<uint8_t *>(q), scales, rows, width, as_stream(stream)),
+                       "xpu_fp8_silu_multiply");
+  })
+}
+
+int xpu_fp8_rms_norm(int dtype, const void *x, uint64_t x_stride, const void *residual, uint64_t residual_stride,
+                     const void *weight, float epsilon, void *total, uint64_t total_stride, void *q, float *scales,
+                     uint32_t rows, uint32_t width, void *stream) {
+  XPU_GUARD({
+    if (rows == 0) return XPU_OK;
+    XPU_CHECKED(check_fp8_rows(dtype, x, weight, x_stride, q, scales, rows, width, "xpu_fp8_rms_norm"));
+    XPU_REQUIRE(aligned16(residual) && aligned16(total), "xpu_fp8_rms_norm: residual and total must be 16-byte aligned");
+    XPU_REQUIRE((!residual || (residual_stride % 8 == 0 && residual_stride >= width && residual_stride < (1ull << 32))) &&
+                    (!total || (total_stride % 8 == 0 && total_stride >= width && total_stride < (1ull << 32))),
+                "xpu_fp8_rms_norm: row strides must be multiples of 8 elements and hold a row");
+    XPU_REQUIRE(epsilon >= 0.f && epsilon < INFINITY, "xpu_fp8_rms_norm: epsilon must be finite and not negative");
+    if (width > 32768) return fail(XPU_ERR_UNSUPPORTED, "xpu_fp8_rms_norm: width above 32768");
+    const Fp8Norm n{static_cast<const uint16_t *>(x), static_cast<const uint16_t *>(residual),
+                    static_cast<const uint16_t *>(weight), static_cast<uint16_t *>(total), x_stride, residual_stride,
+                    total_stride, static_cast<uint8_t *>(q), scales, rows, width, epsilon};
+    return cuda_status(fp8_rms_norm_launch(dtype == XPU_FP16, n, as_stream(stream)), "xpu_fp8_rms_norm");
+  })
+}
+
+int xpu_fp8_gemm(int dtype, const void *a, const float *a_scales, const void *w, const float *w_scales, void *c, uint32_t m,
+                 uint32_t n, uint32_t k, void *stream) {
+  XPU_GUARD({
+    XPU_REQUIRE(dtype == XPU_BF16 || dtype == XPU_FP16, "xpu_fp8_gemm: dtype must be XPU_BF16 or XPU_FP16");
+    XPU_REQUIRE(n > 0 && k > 0 && k % 16 == 0, "xpu_fp8_gemm: n and k must be positive, k a multiple of 16");
+    XPU_REQUIRE(m < (1u << 31) && n < (1u << 31) && k < (1u << 31), "xpu_fp8_gemm: too large");
+    if (m == 0) return XPU_OK;
+    XPU_REQUIRE(a && a_scales && w && w_scales && c, "xpu_fp8_gemm: null pointer");
+    XPU_REQUIRE(aligned16(a) && aligned16(w) && aligned16(c), "xpu_fp8_gemm: operands must be 16-byte aligned");
+    XPU_REQUIRE(aligned4(a_scales) && aligned4(w_scales), "xpu_fp8_gemm: scales must be 4-byte aligned");
+    const Fp8Product p{static_cast<const uint8_t *>(a), static_cast<const uint8_t *>(w), a_scales, w_scales, c, m, n, k};
+    return cuda_status(fp8_gemm_launch(dtype == XPU_FP16, p, as_stream(stream)), "xpu_fp8_gemm");
+  })
+}
+
+int xpu_sample(int dtype, const void *logits, uint64_t stride, const float *temperature, const int32_t *top_k,
+               const float *top_p, const float *min_p, const float *u, int32_t *tokens, float *logprobs, uint32_t rows,
+               uint32_t vocabulary, void *stream) {
+  XPU_GUARD({
+    XPU_REQUIRE(dtype == XPU_BF16 || dtype == XPU_FP16, "xpu_sample: dtype must be XPU_BF16 or XPU_FP16");
+    XPU_REQUIRE(vocabulary > 0 && vocabulary <= XPU_SAMPLE_MAX_VOCABULARY, "xpu_sample: vocabulary must be 1 to 1048576");
+    XPU_REQUIRE(stride >= vocabulary && stride < (1ull << 32), "xpu_sample: row stride shorter than a row, or too long");
+    XPU_REQUIRE(rows < (1u << 27), "xpu_sample: too many rows");
+    if (rows == 0) return XPU_OK;
+    XPU_REQUIRE(logits && u && tokens, "xpu_sample: null pointer");
+    XPU_REQUIRE((reinterpret_cast<uintptr_t>(logits) & 1u) == 0 && aligned4(temperature) && aligned4(top_k) && aligned4(top_p) &&
+                    aligned4(min_p) && aligned4(u) && aligned4(tokens) && aligned4(logprobs),
+                "xpu_sample: misaligned pointer");
+    const SampleArgs a{static_cast<const uint16_t *>(logits), stride, temperature, top_p, min_p, u, top_k, tokens, logprobs, rows,
+                       vocabulary};
+    return cuda_status(sample_launch(dtype == XPU_FP16, a, as_stream(stream)), "xpu_sample");
   })
 }
 

@@ -1,0 +1,544 @@
+// Choosing a token from a row of 16-bit logits (xpu_sample in include/xpu_cuda.h).
+//
+// The order is that of falling logits, of equal ones the lowest id first; what top-k,
+// top-p and min-p keep is a beginning of it, and the token is the first whose sum of
+// weights exceeds u times that of the beginning. Nothing is sorted: a row has at most
+// 65536 different values, so a histogram of them, in shared memory with 16-bit counters,
+// says all about it. A weight exp((l - l_max) / T) is computed once a value, in 64 bits, as
+// are the sums: where u falls between 151936 sums must not hang on rounding. Prefix
+// sums over groups of 32 values, then over the values of one group, answer each
+// question ("the last value whose prefix is below x"); the answer is a value
+// and which of its occurrences it is, and a second look at the row finds its place.
+// Sums are in a fixed order: results repeat bit for bit.
+//
+// SIZE blocks of a cluster share a row, a run of it each: eight where there are few
+// rows. Rows with a small top-k (a temperature of 0 is top-k 1) count only what can be among
+// the k: each thread's largest logit first, and no logit below the k-th of those.
+#include <algorithm>
+
+#include "common.cuh"
+#include "serving.h"
+#include "stream.cuh"
+#include "tcgen05.cuh"
+
+namespace xpu {
+namespace {
+
+constexpr uint32_t kThreads = 1024, kWarps = kThreads / 32;
+constexpr uint32_t kKeys = 65536, kGroups = kKeys / 32;
+constexpr uint32_t kSmem = kKeys * 2;
+constexpr uint32_t kMostPruned = 256;  // top-k up to which the largest logits are looked for first
+constexpr uint32_t kHeavy = 2 * XPU_SAMPLE_MAX_VOCABULARY / 32768 + 1;
+constexpr uint32_t kRound = 32768;  // logits after which counters near overflow are emptied (slow way)
+
+// 16-bit floats as whole numbers of the same order; -0 is 0.
+__device__ __forceinline__ uint32_t key_of(uint32_t bits) {
+  const uint32_t key = bits & 0x8000u ? bits ^ 0xffffu : bits | 0x8000u;
+  return key == 0x7fffu ? 0x8000u : key;
+}
+
+template <typename T>
+struct Keys;
+template <>
+struct Keys<__nv_bfloat16> {
+  static constexpr uint32_t kMinusInf = 0x007f, kPlusInf = 0xff80, kMask = 0xff80ff80u;  // two bits patterns of -inf
+};
+template <>
+struct Keys<__half> {
+  static constexpr uint32_t kMinusInf = 0x03ff, kPlusInf = 0xfc00, kMask = 0xfc00fc00u;
+};
+
+template <typename T>
+__device__ __forceinline__ double value_of(uint32_t key) {
+  const uint32_t bits = key & 0x8000u ? key & 0x7fffu : key ^ 0xffffu;
+  return static_cast<double>(Elem<T>::lo(bits));
+}
+
+// A row of logits at any 2-byte aligned address, in pieces of 8 from a 16-byte boundary on; places outside are -inf.
+template <typename T>
+struct Row {
+  const uint16_t *base;  // 16-byte aligned, at or before the first logit
+  uint32_t skipped, count, pieces;
+  __device__ Row(const uint16_t *row, uint32_t vocabulary) : count(vocabulary) {
+    skipped = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15u) / 2;
+    base = row - skipped;
+    pieces = (skipped + count + 7) / 8;
+  }
+  __device__ __forceinline__ uint4 piece(uint32_t p) const {
+    const uint32_t first = 8 * p;  // counted from base
+    if (first >= skipped && first + 8 <= skipped + count) {
+      uint4 v;
+      asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(base + first) : "memory");
+      return v;
+    }
+    uint32_t u[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      u[i] = Keys<T>::kMask;
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t at = first + 2 * i + h;
+        if (at >= skipped && at < skipped + count)
+          u[i] = (u[i] & (h ? 0xffffu : 0xffff0000u)) | static_cast<uint32_t>(*reinterpret_cast<const volatile uint16_t *>(base + at)) << (16 * h);
+      }
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+
+__device__ __forceinline__ uint32_t element(const uint4 &v, int i) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  return u[i / 2] >> (16 * (i % 2)) & 0xffffu;
+}
+
+struct Shared {
+  uint32_t counts[kGroups];  // of each group of 32 values; then of the groups above it
+  double masses[kGroups];    // likewise their weights
+  double warp_mass[kWarps];
+  uint32_t warp_count[kWarps];
+  uint32_t heavy_key[kHeavy], heavy_count[kHeavy], heavies;
+  uint32_t top[8], bad[8];  // of each block of the cluster
+  uint32_t found[5];        // group that answers a question, in falling order of groups, plus 1
+  uint32_t answer_key, answer_at;  // the token: its value, and which occurrence; kKeys: none
+  uint32_t counted, bound;
+};
+
+template <int SIZE>
+__device__ __forceinline__ void row_sync() {
+  if (SIZE == 1) __syncthreads();
+  else cluster_sync();
+}
+
+// Occurrences of a value in block r's run.
+template <int SIZE>
+__device__ __forceinline__ uint32_t occurrences(const uint16_t *histogram, const Shared *sh, uint32_t key, uint32_t r, bool any_heavy) {
+  uint32_t n;
+  if (SIZE == 1) n = histogram[key];
+  else asm volatile("{\n .reg .u16 t;\n ld.shared::cluster.u16 t, [%1];\n cvt.u32.u16 %0, t;\n}" : "=r"(n) : "r"(cluster_addr(histogram + key, r)) : "memory");
+  if (any_heavy) {
+    for (uint32_t i = 0; i < kHeavy; ++i) {
+      uint32_t k, c, many;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(many) : "r"(cluster_addr(&sh->heavies, r)) : "memory");
+      if (i >= many) break;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(k) : "r"(cluster_addr(&sh->heavy_key[i], r)) : "memory");
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(cluster_addr(&sh->heavy_count[i], r)) : "memory");
+      if (k == key) n += c;
+    }
+  }
+  return n;
+}
+
+struct Bin {  // one value of a group, a lane each, the largest in lane 0
+  uint32_t key, count, before;  // occurrences, and tokens before them in the order
+  double weight, mass;          // of one, and of all before
+};
+
+__device__ __forceinline__ uint32_t last_lane(bool yes) {
+  const uint32_t votes = __ballot_sync(kFullMask, yes);
+  return votes ? 31 - __clz(votes) : 0;
+}
+
+template <typename T, int SIZE>
+__global__ void __launch_bounds__(kThreads, 1)
+k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, const int32_t *top_ks, const float *top_ps,
+         const float *min_ps, const float *us, int32_t *tokens, float *logprobs, uint32_t vocabulary) {
+  extern __shared__ __align__(16) uint16_t histogram[];
+  __shared__ Shared sh;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rank = SIZE == 1 ? 0 : cluster_rank(), row = blockIdx.x / SIZE;
+  uint4 *const words = reinterpret_cast<uint4 *>(histogram);
+  for (uint32_t i = threadIdx.x; i < kSmem / 16; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
+  for (uint32_t i = threadIdx.x; i < kGroups; i += kThreads) {
+    sh.counts[i] = 0;
+    sh.masses[i] = 0.0;
+  }
+  if (threadIdx.x == 0) {
+    sh.heavies = sh.counted = sh.bound = 0;
+    sh.top[rank] = sh.bad[rank] = 0;
+    for (int i = 0; i < 5; ++i) sh.found[i] = 0;
+  }
+  grid_dep_launch();
+  grid_dep_wait();
+  __syncthreads();
+
+  const volatile float *const vt = temperatures, *const vp = top_ps, *const vm = min_ps, *const vu = us;
+  const volatile int32_t *const vk = top_ks;
+  const float temperature = temperatures ? vt[row] : 1.f, top_p = top_ps ? vp[row] : 1.f, min_p = min_ps ? vm[row] : 0.f;
+  const int32_t top_k = top_ks ? vk[row] : 0;
+  const float u = vu[row];
+  const bool asked = temperature >= 0.f && top_p == top_p && min_p == min_p && u >= 0.f && u < 1.f && top_k >= 0;
+  const bool greedy = temperature == 0.f;
+  const uint32_t most = greedy ? 1 : (top_k == 0 ? UINT32_MAX : static_cast<uint32_t>(top_k));
+
+  const Row<T> r(logits + row * stride, vocabulary);
+  const uint32_t share = (r.pieces + SIZE - 1) / SIZE;
+  const uint32_t begin = min(rank * share, r.pieces), end = min(begin + share, r.pieces);
+
+  // No logit below the `most`-th largest of the threads' largest ones can be among the first `most`.
+  if (most <= kMostPruned) {
+    uint32_t top = 0;
+    for (uint32_t p = begin + threadIdx.x; p < end; p += kThreads) {
+      const uint4 v = r.piece(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, key_of(element(v, i)));
+    }
+    if (top > Keys<T>::kMinusInf) atomicAdd(&sh.counts[top / 32], 1u);
+    __syncthreads();
+    // thread i: groups 2047 - 2 i and 2046 - 2 i
+    const uint32_t hi = kGroups - 1 - 2 * threadIdx.x;
+    const uint32_t a = sh.counts[hi], b = sh.counts[hi - 1];
+    uint32_t inc = a + b;
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) sh.warp_count[warp] = inc;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t w = 0; w < warp; ++w) before += sh.warp_count[w];
+    before += inc - a - b;
+    if (before < most && before + a >= most) sh.bound = 32 * hi;
+    else if (before + a < most && before + a + b >= most) sh.bound = 32 * (hi - 1);
+    sh.counts[hi] = sh.counts[hi - 1] = 0;
+    __syncthreads();
+  }
+  const uint32_t bound = max(sh.bound, Keys<T>::kMinusInf + 1);
+  constexpr uint32_t kLowest = Keys<T>::kMinusInf + 1;  // the lowest finite value masks too: counted without the histogram
+
+  uint32_t top = 0, counted = 0, lowest = 0, bad = 0;
+  const auto count = [&](uint32_t from, uint32_t to) {
+    for (uint32_t p = from + threadIdx.x; p < to; p += kThreads) {
+      const uint4 v = r.piece(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t key = key_of(element(v, i));
+        bad |= key >= Keys<T>::kPlusInf || key < Keys<T>::kMinusInf;
+        top = max(top, key);
+        if (key < bound) continue;
+        ++counted;
+        if (key == kLowest) ++lowest;
+        else atomicAdd(reinterpret_cast<uint32_t *>(histogram) + key / 2, 1u << (16 * (key & 1)));
+      }
+    }
+  };
+  count(begin, end);
+  const auto add_lowest = [&] {
+    const uint32_t n = __reduce_add_sync(kFullMask, lowest);
+    if (lane == 0 && n) atomicAdd(&sh.heavy_count[0], n);
+  };
+  if (threadIdx.x == 0) {
+    sh.heavy_key[0] = kLowest;
+    sh.heavy_count[0] = 0;
+  }
+  __syncthreads();
+  add_lowest();
+  if (8 * (end - begin) > 65535) {
+    // A counter may have passed 65535: then the sum of all is too small by a multiple of 65535 or 65536.
+    uint32_t sum = 0;
+    for (uint32_t i = threadIdx.x; i < kSmem / 16; i += kThreads) {
+      const uint4 v = words[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += element(v, e);
+    }
+    if (__syncthreads_or(bad) == 0) {
+      const uint32_t missing = __reduce_add_sync(kFullMask, counted - lowest - sum);
+      if (lane == 0) atomicAdd(&sh.counted, missing);
+    }
+    __syncthreads();
+    if (sh.counted) {  // once more, emptying counters of 32768 and more after every 32768 logits
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < kSmem / 16; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
+      if (threadIdx.x == 0) sh.heavies = 1;
+      __syncthreads();
+      for (uint32_t from = begin; from < end; from += kRound / 8) {
+        count(from, min(end, from + kRound / 8));
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < kKeys; i += kThreads) {
+          if (histogram[i] < kRound) continue;
+          const uint32_t at = atomicAdd(&sh.heavies, 1u);
+          sh.heavy_key[at] = i;
+          sh.heavy_count[at] = histogram[i];
+          histogram[i] = 0;
+        }
+        __syncthreads();
+      }
+    }
+  }
+  top = __reduce_max_sync(kFullMask, top);
+  bad = __any_sync(kFullMask, bad);
+  if (lane == 0) {
+    atomicMax(&sh.top[rank], top);
+    atomicOr(&sh.bad[rank], bad);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && sh.heavies == 0 && sh.heavy_count[0]) sh.heavies = 1;
+  if (SIZE > 1 && threadIdx.x < SIZE && threadIdx.x != rank) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.top[rank], threadIdx.x)), "r"(sh.top[rank]) : "memory");
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bad[rank], threadIdx.x)), "r"(sh.bad[rank]) : "memory");
+  }
+  row_sync<SIZE>();
+
+  uint32_t any_heavy = 0;
+  top = bad = 0;
+  for (int i = 0; i < SIZE; ++i) {
+    top = max(top, sh.top[i]);
+    bad |= sh.bad[i];
+    if (SIZE == 1) {
+      any_heavy = sh.heavies;
+    } else {
+      uint32_t h;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(h) : "r"(cluster_addr(&sh.heavies, i)) : "memory");
+      any_heavy |= h;
+    }
+  }
+  const bool none = bad || !asked || top <= Keys<T>::kMinusInf;
+  const double largest = none ? 0.0 : value_of<T>(top), divisor = greedy ? 1.0 : static_cast<double>(temperature);
+  const auto log_weight = [&](uint32_t key) { return (value_of<T>(key) - largest) / divisor; };
+
+  if (none || greedy) {  // the same for every block of the row
+    if (threadIdx.x == 0) {
+      sh.answer_key = none ? kKeys : top;
+      sh.answer_at = 0;
+      if (rank == 0 && logprobs) logprobs[row] = none ? -INFINITY : 0.f;
+      if (rank == 0 && none) tokens[row] = -1;
+    }
+    __syncthreads();
+  } else {
+    // Each block's share of the groups, their sums to block 0.
+    for (uint32_t i = warp; i < kGroups / SIZE; i += kWarps) {
+      const uint32_t g = i * SIZE + rank, key = 32 * g + lane;
+      if (g > top / 32) break;
+      uint32_t n = 0;
+      for (int b = 0; b < SIZE; ++b) n += occurrences<SIZE>(histogram, &sh, key, b, any_heavy);
+      if (!__any_sync(kFullMask, n)) continue;
+      double mass = n ? n * exp(log_weight(key)) : 0.0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
+      n = __reduce_add_sync(kFullMask, n);
+      if (lane == 0) {
+        if (SIZE == 1) {
+          sh.counts[g] = n;
+          sh.masses[g] = mass;
+        } else {
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.counts[g], 0)), "r"(n) : "memory");
+          asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&sh.masses[g], 0)), "d"(mass) : "memory");
+        }
+      }
+    }
+    row_sync<SIZE>();
+    if (rank == 0) {
+      // Sums over the groups above each; thread i has groups 2047 - 2 i and 2046 - 2 i.
+      const uint32_t hi = kGroups - 1 - 2 * threadIdx.x, own[2] = {sh.counts[hi], sh.counts[hi - 1]};
+      uint32_t before[2];
+      double mass[2];
+      const double m0 = sh.masses[hi], m1 = sh.masses[hi - 1];
+      uint32_t inc = own[0] + own[1];
+      double minc = m0 + m1;
+#pragma unroll
+      for (uint32_t o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
+        const double mup = __shfl_up_sync(kFullMask, minc, o);
+        if (lane >= o) {
+          inc += up;
+          minc += mup;
+        }
+      }
+      if (lane == 31) {
+        sh.warp_count[warp] = inc;
+        sh.warp_mass[warp] = minc;
+      }
+      __syncthreads();
+      uint32_t all = 0, lower = 0;
+      double all_mass = 0.0, lower_mass = 0.0;
+      for (uint32_t w = 0; w < kWarps; ++w) {
+        if (w == warp) {
+          lower = all;
+          lower_mass = all_mass;
+        }
+        all += sh.warp_count[w];
+        all_mass += sh.warp_mass[w];
+      }
+      const uint32_t up1 = __shfl_up_sync(kFullMask, inc, 1);
+      const double mup1 = __shfl_up_sync(kFullMask, minc, 1);
+      before[0] = lower + (lane ? up1 : 0);
+      mass[0] = lower_mass + (lane ? mup1 : 0.0);
+      before[1] = before[0] + own[0];
+      mass[1] = mass[0] + m0;
+      sh.counts[hi] = before[0];
+      sh.counts[hi - 1] = before[1];
+      sh.masses[hi] = mass[0];
+      sh.masses[hi - 1] = mass[1];
+
+      // The values of the last group that is not empty and of which yes(tokens before it, their weight, the group).
+      const auto ask = [&](int question, auto yes) {
+        uint32_t last = 0;  // place in falling order, plus 1
+        if (own[0] && yes(before[0], mass[0], hi)) last = 2 * threadIdx.x + 1;
+        if (own[1] && yes(before[1], mass[1], hi - 1)) last = 2 * threadIdx.x + 2;
+        last = __reduce_max_sync(kFullMask, last);
+        if (lane == 0 && last) atomicMax(&sh.found[question], last);
+        __syncthreads();
+        const uint32_t g = kGroups - max(sh.found[question], 1u);
+        Bin bin;
+        bin.key = 32 * g + 31 - lane;
+        bin.count = 0;
+        for (int b = 0; b < SIZE; ++b) bin.count += occurrences<SIZE>(histogram, &sh, bin.key, b, any_heavy);
+        bin.weight = bin.count ? exp(log_weight(bin.key)) : 0.0;
+        uint32_t n = bin.count;
+        double m = bin.count * bin.weight;
+#pragma unroll
+        for (uint32_t o = 1; o < 32; o <<= 1) {
+          const uint32_t up = __shfl_up_sync(kFullMask, n, o);
+          const double mup = __shfl_up_sync(kFullMask, m, o);
+          if (lane >= o) {
+            n += up;
+            m += mup;
+          }
+        }
+        const double mup = __shfl_up_sync(kFullMask, m, 1);
+        bin.before = sh.counts[g] + n - bin.count;
+        bin.mass = sh.masses[g] + (lane ? mup : 0.0);
+        return bin;
+      };
+      // Weight of the first n tokens.
+      const auto weight_of_first = [&](int question, uint32_t n) {
+        const Bin b = ask(question, [&](uint32_t c, double, uint32_t) { return c < n; });
+        const uint32_t at = last_lane(b.count && b.before < n);
+        return __shfl_sync(kFullMask, b.mass + min(n - b.before, b.count) * b.weight, at);
+      };
+      uint32_t kept = min(most, all);
+      double total = kept == all ? all_mass : weight_of_first(0, kept);
+      uint32_t fewer = kept;
+      if (top_p < 1.f) {
+        const double wanted = static_cast<double>(top_p) * total;
+        const Bin b = ask(1, [&](uint32_t, double m, uint32_t) { return m < wanted; });
+        const uint32_t at = last_lane(b.count && b.mass < wanted);
+        const double need = fmin(fmax(ceil((wanted - b.mass) / b.weight), 1.0), static_cast<double>(b.count));
+        fewer = min(fewer, __shfl_sync(kFullMask, b.before + (b.count ? static_cast<uint32_t>(need) : 0), at));
+      }
+      if (min_p > 0.f) {
+        // of the last group with values that would be heavy enough, those that are; all above it are
+        const double least = static_cast<double>(min_p);
+        const Bin b = ask(2, [&](uint32_t, double, uint32_t g) { return exp(log_weight(min(32 * g + 31, top))) >= least; });
+        const uint32_t at = last_lane(b.count && b.weight >= least);
+        const uint32_t heavy = __shfl_sync(kFullMask, b.count && b.weight >= least ? b.before + b.count : b.before, at);
+        fewer = min(fewer, heavy);
+      }
+      fewer = max(fewer, 1u);
+      if (fewer < kept) total = weight_of_first(3, kept = fewer);
+      const double wanted = static_cast<double>(u) * total;
+      const Bin b = ask(4, [&](uint32_t c, double m, uint32_t) { return c < kept && m <= wanted; });
+      const uint32_t at = last_lane(b.count && b.weight > 0.0 && b.before < kept && b.mass <= wanted);
+      if (warp == 0 && lane == at) {
+        const uint32_t in = min(b.count, kept - b.before);  // of its occurrences are kept
+        const double which = floor((wanted - b.mass) / b.weight);
+        const uint32_t j = which < in ? static_cast<uint32_t>(which) : in - 1;
+        if (logprobs) logprobs[row] = static_cast<float>(log_weight(b.key) - log(total));
+        for (int i = 0; i < SIZE; ++i) {
+          if (SIZE == 1) {
+            sh.answer_key = b.key;
+            sh.answer_at = j;
+          } else {
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_key, i)), "r"(b.key) : "memory");
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_at, i)), "r"(j) : "memory");
+          }
+        }
+      }
+    }
+    row_sync<SIZE>();
+  }
+
+  // The answer's place in the row: which block's run has that occurrence, then which warp's.
+  const uint32_t key = sh.answer_key;
+  uint32_t j = sh.answer_at, here = 0;
+  bool mine = key < kKeys;
+  for (uint32_t b = 0; mine && b <= rank; ++b) {
+    const uint32_t n = occurrences<SIZE>(histogram, &sh, key, b, any_heavy);
+    if (b == rank) {
+      here = n;
+      mine = j < n;
+    } else if (j < n) {
+      mine = false;
+    } else {
+      j -= n;
+    }
+  }
+  if (mine) {
+    const uint32_t run = (end - begin + kWarps - 1) / kWarps, from = begin + warp * run, to = min(from + run, end);
+    const auto matches = [&](uint32_t p) {
+      uint32_t mask = 0;
+      if (p < to) {
+        const uint4 v = r.piece(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mask |= static_cast<uint32_t>(key_of(element(v, i)) == key) << i;
+      }
+      return mask;
+    };
+    uint32_t n = 0;
+    for (uint32_t p = from + lane; p < to; p += 32) {
+      const uint32_t mask = matches(p);
+      if (mask && here == 1) tokens[row] = static_cast<int32_t>(8 * p + __ffs(mask) - 1 - r.skipped);
+      n += __popc(mask);
+    }
+    if (here > 1) {
+      n = __reduce_add_sync(kFullMask, n);
+      if (lane == 0) sh.warp_count[warp] = n;
+      __syncthreads();
+      uint32_t earlier = 0;
+      for (uint32_t w = 0; w < warp; ++w) earlier += sh.warp_count[w];
+      if (j >= earlier && j - earlier < n) {
+        j -= earlier;
+        for (uint32_t p = from; p < to; p += 32) {
+          const uint32_t mask = matches(p + lane);
+          uint32_t inc = __popc(mask);
+#pragma unroll
+          for (uint32_t o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
+            if (lane >= o) inc += up;
+          }
+          const uint32_t many = __shfl_sync(kFullMask, inc, 31), before = inc - __popc(mask);
+          if (j < many) {
+            if (j >= before && j < inc) {
+              uint32_t left = mask;
+              for (uint32_t skip = j - before; skip; --skip) left &= left - 1;
+              tokens[row] = static_cast<int32_t>(8 * (p + lane) + __ffs(left) - 1 - r.skipped);
+            }
+            break;
+          }
+          j -= many;
+        }
+      }
+    }
+  }
+  if (SIZE > 1) cluster_sync();  // no block leaves while another may read its counters
+}
+
+template <typename T, int SIZE>
+cudaError_t launch(const SampleArgs &a, cudaStream_t s) {
+  const auto kernel = k_sample<T, SIZE>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = SIZE;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(a.rows * SIZE);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = SIZE > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a.logits, a.stride, a.temperature, a.top_k, a.top_p, a.min_p, a.u, a.tokens, a.logprobs,
+                            a.vocabulary);
+}
+
+}  // namespace
+
+cudaError_t sample_launch(bool fp16, const SampleArgs &a, cudaStream_t s) {
+  return fp16 ? launch<__half, 1>(a, s) : launch<__nv_bfloat16, 1>(a, s);
+}
+
+}  // namespace xpu

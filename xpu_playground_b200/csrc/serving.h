@@ -1,6 +1,6 @@
 // Launchers of the serving operators (attention over packed prompts and over
-// the paged cache, and the cache's page operators), shared between their
-// kernels and the C entry points.
+// the paged cache, the cache's page operators, products of 8-bit rows and
+// sampling), shared between their kernels and the C entry points.
 #pragma once
 
 #include "xpu_internal.h"
@@ -74,5 +74,39 @@ size_t tree_workspace_bytes(uint32_t count, uint32_t nodes, uint32_t q_heads, ui
 cudaError_t tree_attention_launch(const xpu_kv_cache_t &c, uint32_t layer, const int32_t *sequences,
                                   const int32_t *starts, const uint64_t *ancestors, uint32_t count,
                                   const AttnTensors &t, void *workspace, cudaStream_t s);
+
+// ---- 8-bit rows (fp8_rows.cu) and their products (fp8_gemm.cu) ----
+// up == NULL: plain rows.
+cudaError_t fp8_rows_launch(bool fp16, const uint16_t *x, const uint16_t *up, uint64_t stride, uint8_t *q, float *scales,
+                            uint32_t rows, uint32_t width, cudaStream_t s);
+struct Fp8Norm {
+  const uint16_t *x, *residual, *weight;  // residual may be NULL
+  uint16_t *total;                        // may be NULL
+  uint64_t x_stride, residual_stride, total_stride;
+  uint8_t *q;
+  float *scales;
+  uint32_t rows, width;
+  float epsilon;
+};
+cudaError_t fp8_rms_norm_launch(bool fp16, const Fp8Norm &n, cudaStream_t s);
+struct Fp8Product {
+  const uint8_t *a, *w;
+  const float *a_scales, *w_scales;
+  void *c;
+  uint32_t m, n, k;
+};
+cudaError_t fp8_gemm_launch(bool fp16, const Fp8Product &p, cudaStream_t s);
+
+// ---- sampling (sample.cu) ----
+struct SampleArgs {
+  const uint16_t *logits;
+  uint64_t stride;
+  const float *temperature, *top_p, *min_p, *u;  // all but u may be NULL
+  const int32_t *top_k;
+  int32_t *tokens;
+  float *logprobs;  // may be NULL
+  uint32_t rows, vocabulary;
+};
+cudaError_t sample_launch(bool fp16, const SampleArgs &a, cudaStream_t s);
 
 }  // namespace xpu

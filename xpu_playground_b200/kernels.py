@@ -297,3 +297,157 @@ def tree_attention(cache, layer: int, sequences: torch.Tensor, starts: torch.Ten
          q.shape[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), q.shape[1], q_stride, kv_stride,
          out_stride, scale, _ptr(workspace), workspace.numel(), _stream(stream))
     return out, lse
+
+
+# ------------------------------------- 8-bit rows, their products, sampling ----
+
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128  # columns of a row, and rows and columns of a weight, that share a scale
+
+
+def _here(first: torch.Tensor, *others) -> None:
+    """Refuses tensors that are not on the current device."""
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError("tensors must be on one device")
+    if device < 0:
+        raise ValueError("libxpu_cuda entry points take CUDA tensors")
+    if device != torch._C._cuda_getDevice():
+        raise ValueError("tensors must be on the current device")
+
+
+def _rows(name: str, t: torch.Tensor, width: int) -> int:
+    """Row stride of [rows, width] whose rows may stand apart."""
+    rows, columns = t.shape
+    if columns != width:
+        raise ValueError(f"{name} must have {width} columns, not {columns}")
+    row, column = t.stride()
+    if column != 1:
+        raise ValueError(f"{name}: a row must be contiguous")
+    return row if rows > 1 else max(width, row)
+
+
+def _fp8_outputs(rows: int, width: int, device, q, scales, stream):
+    shape = (rows, width)
+    if q is None:
+        q = _allocate(torch.empty, stream, shape, dtype=FP8, device=device)
+    elif q.dtype != FP8 or q.shape != shape or not q.is_contiguous():
+        raise ValueError(f"q must be a contiguous float8_e4m3fn tensor {shape}")
+    shape = (-(-width // FP8_BLOCK), rows)
+    if scales is None:
+        scales = _allocate(torch.empty, stream, shape, dtype=torch.float32, device=device)
+    elif scales.dtype != torch.float32 or scales.shape != shape or not scales.is_contiguous():
+        raise ValueError(f"scales must be a contiguous float32 tensor {shape}")
+    return q, scales
+
+
+def fp8_quantize(x: torch.Tensor, q: torch.Tensor | None = None, scales: torch.Tensor | None = None, stream=None):
+    """Rows x [rows, width] in 8 bits (xpu_fp8_quantize): q [rows, width] and a
+    scale for each 128 columns, scales [blocks, rows]. Returns (q, scales)."""
+    rows, width = x.shape
+    dtype, stride = _dtype_code(x), _rows("x", x, width)
+    q, scales = _fp8_outputs(rows, width, x.device, q, scales, stream)
+    _here(x, q, scales)
+    call("xpu_fp8_quantize", dtype, x.data_ptr(), stride, q.data_ptr(), scales.data_ptr(), rows, width, _stream(stream))
+    return q, scales
+
+
+def fp8_silu_multiply(gate_up: torch.Tensor, q: torch.Tensor | None = None, scales: torch.Tensor | None = None, stream=None):
+    """silu(gate) * up of a fused projection's rows [gate | up] in 8 bits
+    (xpu_fp8_silu_multiply). Returns (q, scales)."""
+    rows, both = gate_up.shape
+    if both % 2:
+        raise ValueError("gate_up holds gate and up side by side")
+    width = both // 2
+    dtype, stride, at = _dtype_code(gate_up), _rows("gate_up", gate_up, both), gate_up.data_ptr()
+    q, scales = _fp8_outputs(rows, width, gate_up.device, q, scales, stream)
+    _here(gate_up, q, scales)
+    call("xpu_fp8_silu_multiply", dtype, at, at + 2 * width, stride, q.data_ptr(), scales.data_ptr(), rows, width, _stream(stream))
+    return q, scales
+
+
+def fp8_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, epsilon: float = 1e-6,
+                 total: torch.Tensor | None = None, q: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                 stream=None):
+    """The residual's addition and the root-mean-square norm of the sum, the
+    norm's rows in 8 bits (xpu_fp8_rms_norm). Returns (total, q, scales) with
+    total = x + residual; `total` may be x or residual, to be updated in place.
+    Without a residual total is x."""
+    rows, width = x.shape
+    dtype, stride = _dtype_code(x), _rows("x", x, width)
+    if weight.dtype != x.dtype or weight.shape != (width,) or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous tensor [{width}] of x's dtype")
+    residual_at = residual_stride = total_at = total_stride = 0
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape:
+            raise ValueError("residual must have x's shape and dtype")
+        residual_at, residual_stride = residual.data_ptr(), _rows("residual", residual, width)
+        if total is None:
+            total = _allocate(torch.empty, stream, rows, width, dtype=x.dtype, device=x.device)
+    if total is not None:
+        if total.dtype != x.dtype or total.shape != x.shape:
+            raise ValueError("total must have x's shape and dtype")
+        total_at, total_stride = total.data_ptr(), _rows("total", total, width)
+    q, scales = _fp8_outputs(rows, width, x.device, q, scales, stream)
+    _here(x, weight, residual, total, q, scales)
+    call("xpu_fp8_rms_norm", dtype, x.data_ptr(), stride, residual_at, residual_stride, weight.data_ptr(), epsilon, total_at,
+         total_stride, q.data_ptr(), scales.data_ptr(), rows, width, _stream(stream))
+    return (x if total is None else total), q, scales
+
+
+def fp8_gemm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+             out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
+    """C[m, n] = A[m, k] . W[n, k]^T of 8-bit rows (with scales [blocks of k, m])
+    and 8-bit weights (scales [blocks of n, blocks of k]), in `dtype` or out's
+    (xpu_fp8_gemm)."""
+    m, k = a.shape
+    n, k2 = w.shape
+    blocks = -(-k // FP8_BLOCK)
+    if k2 != k or a.dtype != FP8 or w.dtype != FP8:
+        raise ValueError("fp8_gemm: a is [m, k] and w is [n, k], both float8_e4m3fn")
+    if a_scales.shape != (blocks, m) or w_scales.shape != (-(-n // FP8_BLOCK), blocks):
+        raise ValueError("fp8_gemm: a_scales is [blocks of k, m], w_scales [blocks of n, blocks of k]")
+    if a_scales.dtype != torch.float32 or w_scales.dtype != torch.float32:
+        raise ValueError("fp8_gemm: scales are float32")
+    if not (a.is_contiguous() and w.is_contiguous() and a_scales.is_contiguous() and w_scales.is_contiguous()):
+        raise ValueError("tensor must be contiguous")
+    if out is None:
+        out = _allocate(torch.empty, stream, m, n, dtype=dtype, device=a.device)
+    elif out.shape != (m, n) or not out.is_contiguous():
+        raise ValueError("fp8_gemm: out must be a contiguous tensor [m, n]")
+    _here(a, a_scales, w, w_scales, out)
+    call("xpu_fp8_gemm", _dtype_code(out), a.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), m, n, k,
+         _stream(stream))
+    return out
+
+
+def _settings(name: str, t: torch.Tensor | None, dtype: torch.dtype, rows: int) -> int:
+    if t is None:
+        return 0
+    if t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor with an entry a row")
+    return t.data_ptr()
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+           top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None, tokens: torch.Tensor | None = None,
+           logprobs: torch.Tensor | None = None, stream=None):
+    """A token for each row of logits [rows, vocabulary] from random numbers u
+    in [0, 1), with each row's settings (xpu_sample): float32 temperature, top_p,
+    min_p and int32 top_k of one entry a row. Returns (tokens, logprobs)."""
+    rows, vocabulary = logits.shape
+    dtype, stride = _dtype_code(logits), _rows("logits", logits, vocabulary)
+    if tokens is None:
+        tokens = _allocate(torch.empty, stream, rows, dtype=torch.int32, device=logits.device)
+    if logprobs is None:
+        logprobs = _allocate(torch.empty, stream, rows, dtype=torch.float32, device=logits.device)
+    f, i = torch.float32, torch.int32
+    if u is None:
+        raise ValueError("u needs a random number a row")
+    _here(logits, u, temperature, top_k, top_p, min_p, tokens, logprobs)
+    call("xpu_sample", dtype, logits.data_ptr(), stride, _settings("temperature", temperature, f, rows),
+         _settings("top_k", top_k, i, rows), _settings("top_p", top_p, f, rows), _settings("min_p", min_p, f, rows),
+         _settings("u", u, f, rows), _settings("tokens", tokens, i, rows), _settings("logprobs", logprobs, f, rows), rows,
+         vocabulary, _stream(stream))
+    return tokens, logprobs
