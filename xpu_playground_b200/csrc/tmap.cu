@@ -64,6 +64,22 @@ cudaError_t make_tmap_2d_u16_swizzled(CUtensorMap *map, const void *base, uint64
   return encode_2d_u16(map, base, cols, rows, pitch_elems, box_cols, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Row-major [rows][cols] matrix of bytes (cols a multiple of 16), 128-byte swizzled boxes of box_rows x 128 bytes.
+// Elements outside the matrix read as zero.
+cudaError_t make_tmap_2d_u8_swizzled(CUtensorMap *map, const void *base, uint64_t cols, uint64_t rows, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) || cols % 16 || box_rows > 256) return cudaErrorInvalidValue;
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {cols};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t estride[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estride,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // 3D view [d2][d1][d0] of 16-bit elements (strides in elements: dimension 1
 // every stride1, dimension 2 every stride2), 128-byte swizzled boxes of
 // box_rows x 1 x box_cols. The split GEMM reads a row-major [rows][chunks x

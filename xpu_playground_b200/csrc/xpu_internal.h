@@ -30,6 +30,8 @@ cudaError_t make_tmap_2d_u16(struct CUtensorMap_st *map, const void *base, uint6
                              uint64_t pitch_elems, uint32_t box_cols, uint32_t box_rows);
 cudaError_t make_tmap_2d_u16_swizzled(struct CUtensorMap_st *map, const void *base, uint64_t cols, uint64_t rows,
                                       uint64_t pitch_elems, uint32_t box_cols, uint32_t box_rows);
+cudaError_t make_tmap_2d_u8_swizzled(struct CUtensorMap_st *map, const void *base, uint64_t cols, uint64_t rows,
+                                     uint32_t box_rows);
 
 cudaError_t make_tmap_3d_u16_swizzled(struct CUtensorMap_st *map, const void *base, uint64_t d0, uint64_t d1,
                                       uint64_t d2, uint64_t stride1, uint64_t stride2, uint32_t box_cols,
@@ -57,6 +59,8 @@ unsigned take_device_error();
 unsigned take_peak_error();
 // And for the serving attention (serving_attention.cu; bit 2).
 unsigned take_attention_error();
+// And for the products of 8-bit rows (fp8_gemm.cu; bit 0 too).
+unsigned take_fp8_error();
 
 // ---- dense prefill (prefill.cu): bf16 [M][width] row-major activations ----
 cudaError_t prefill_embed(const uint16_t *embed, const uint32_t *tokens, uint16_t *x, uint32_t M, uint32_t H,
