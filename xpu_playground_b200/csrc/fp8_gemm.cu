@@ -12,6 +12,13 @@
 // as the M side of its products and NT rows of a as the N side, so that a tile of
 // weights is read once; the blocks of a cluster share the groups of one
 // tile and add their sums up through distributed shared memory, in a fixed order.
+//
+// Many rows (k_wide): the tensor cores bound it. Two blocks of a cluster work as a pair
+// (cta_group::2) on 256 x 256 outputs, each with 128 rows of a and 128 of w in its shared
+// memory and 128 x 256 sums in its TMEM, twice. Eight warps a block hold the tile's
+// FP32 sums in registers: a thread has one row and the 128 columns of one scale block, so
+// that a group's scale is one number a thread. The finished tile leaves through shared
+// memory while the next one's products run.
 #include <cuda.h>
 
 #include <algorithm>
@@ -44,6 +51,40 @@ __device__ __forceinline__ void mma1_f8(uint32_t tmem_d, uint64_t a, uint64_t b,
 }
 
 __device__ __forceinline__ bool has_failed(const int *flag) { return *reinterpret_cast<const volatile int *>(flag) != 0; }
+
+// sums (two of them) += {lo, hi} * scale (twice the same).
+__device__ __forceinline__ void fma2(uint64_t &sums, uint32_t lo, uint32_t hi, uint64_t scale) {
+  asm("{\n .reg .b64 d;\n mov.b64 d, {%1, %2};\n fma.rn.f32x2 %0, d, %3, %0;\n}" : "+l"(sums) : "r"(lo), "r"(hi), "l"(scale));
+}
+
+// The same answer for the whole warp, so that its lanes stay together.
+__device__ __forceinline__ bool warp_wait(int *failed, uint64_t *bar, uint32_t parity) {
+  if (__all_sync(kFullMask, mbar_wait(bar, parity))) return true;
+  *failed = 1;
+  return false;
+}
+
+// Waits for the TMEM loads in flight, whose registers are usable from here on.
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+// Arrives on a barrier of the even block. Not with a release at cluster scope: that one waits for every access of the warp,
+// 1000 cycles a group here, where what is passed on is TMEM that has been read, or shared memory of the same block.
+__device__ __forceinline__ void pair_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(uint64_t pair) {
+  const T lo = Elem<T>::from_float(__uint_as_float(static_cast<uint32_t>(pair)));
+  const T hi = Elem<T>::from_float(__uint_as_float(static_cast<uint32_t>(pair >> 32)));
+  return *reinterpret_cast<const uint16_t *>(&lo) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&hi)) << 16;
+}
 
 // A float that the kernel before may have written.
 __device__ __forceinline__ float ld_f32(const float *p) {
@@ -279,12 +320,312 @@ cudaError_t skinny_launch(const Fp8Product &p, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kernel, map_w, map_a, p.a_scales, p.w_scales, static_cast<T *>(p.c), p.m, p.n, groups, split);
 }
 
+// --------------------------------------------------------------- many rows ----
+
+constexpr uint32_t kPair = 256;                     // rows and columns of a pair's tile
+constexpr uint32_t kWideStages = 4, kWideStage = 2 * kTileBytes;
+constexpr uint32_t kSumWarps = 8, kWideThreads = 128 + 32 * kSumWarps;
+constexpr uint32_t kOutBox = 32 * 128;              // bytes of 32 rows x 64 outputs, swizzled; two a warp
+constexpr uint32_t kScaleSlots = 8;                 // groups whose scales are held, 256 each
+constexpr uint32_t kScalesAt = kWideStages * kWideStage + kSumWarps * 2 * kOutBox;
+constexpr uint32_t kWideSmem = 1024 + kScalesAt + kScaleSlots * kPair * 4;
+constexpr uint32_t kGroupRows = 8;                  // tile rows whose tiles follow one another, for the L2
+
+// Into this block's shared memory, completing on the even block's barrier.
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_addr(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma2_f8(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrives on the barrier of this offset in both blocks when the products issued so far are done.
+__device__ __forceinline__ void mma2_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+
+struct WideTile {
+  uint32_t m, n;
+};
+
+__device__ __forceinline__ WideTile wide_tile(uint32_t t, uint32_t tiles_m, uint32_t tiles_n) {
+  const uint32_t in_group = kGroupRows * tiles_n, group = t / in_group, first = group * kGroupRows;
+  const uint32_t rows = min(kGroupRows, tiles_m - first), local = t - group * in_group;
+  return {first + local % rows, local / rows};
+}
+
+// Warp 0 loads, warp 1 (of the even block) issues the products, warps 2 and 3 bring the scales, warps 4 to 11 add up and have
+// most of the registers. TMA_OUT: rows of c are 16-byte aligned.
+//
+// The sums of a group can only be taken out of TMEM when they are complete, and TMEM holds two groups: a group's time is half of
+// its products (512 cycles) and of the way round: their completion seen (200), 128 columns read and added up (450), the buffer
+// known to be free (150), the next products issued. So the loop of the adding warps has nothing in it that can stand elsewhere:
+// another pair of warps multiplies the scales of row and block and says through the barrier of the operands that they are
+// there. The issuing warp stays converged and an elected lane issues, so that operands are in uniform registers: from one
+// lane's branch a group took 1.3 times as long.
+template <typename T, bool TMA_OUT>
+__global__ void __launch_bounds__(kWideThreads, 1)
+k_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
+       const float *a_scales, const float *w_scales, T *c, uint32_t m, uint32_t n, uint32_t groups) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ uint64_t full[kWideStages], empty[kWideStages], sum_full[2], sum_empty[2], drain;
+  __shared__ uint32_t tmem_base;
+  __shared__ int failed;
+  const uint32_t a0 = smem_addr(smem_raw);
+  uint8_t *const ring = smem_raw + ((a0 + 1023u) / 1024u * 1024u - a0);
+  float *const scales = reinterpret_cast<float *>(ring + kScalesAt);  // [slot][column half][row]
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t tiles_m = (m + kPair - 1) / kPair, tiles_n = (n + kPair - 1) / kPair, tiles = tiles_m * tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < kWideStages; ++i) {
+      mbar_init(&full[i], 1 + 2 * 2);  // both blocks' operands, and their scale warps
+      mbar_init(&empty[i], 1);
+    }
+    for (uint32_t i = 0; i < 2; ++i) {
+      mbar_init(&sum_full[i], 1);
+      mbar_init(&sum_empty[i], 2 * kSumWarps);
+    }
+    mbar_init(&drain, 1);
+    fence_mbar_init();
+    failed = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  grid_dep_launch();
+  grid_dep_wait();
+
+  const uint32_t full_bars = cluster_addr(&full[0], 0);
+  // 384 threads x 168 registers at launch = 128 x 72 + 256 x 216.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      if (lane == 0) {
+        uint32_t i = 0;
+        for (uint32_t t = pair; t < tiles && !has_failed(&failed); t += pairs) {
+          const WideTile tile = wide_tile(t, tiles_m, tiles_n);
+          const int32_t ya = static_cast<int32_t>(tile.m * kPair + rank * 128), yw = static_cast<int32_t>(tile.n * kPair + rank * 128);
+          for (uint32_t g = 0; g < groups; ++g, ++i) {
+            const uint32_t s = i % kWideStages, use = i / kWideStages;
+            if (use > 0 && !mbar_wait(&empty[s], (use - 1) & 1)) { failed = 1; break; }
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * kWideStage);
+            uint8_t *const st = ring + s * kWideStage;
+            tma_load_pair(st, &map_a, static_cast<int32_t>(g * kGroup), ya, full_bars + 8 * s);
+            tma_load_pair(st + kTileBytes, &map_w, static_cast<int32_t>(g * kGroup), yw, full_bars + 8 * s);
+          }
+        }
+        if (has_failed(&failed) && rank == 0)  // no copy may land once this shared memory is another block's
+          for (uint32_t back = 0; back < kWideStages && back < i; ++back)
+            mbar_wait(&full[(i - 1 - back) % kWideStages], (i - 1 - back) / kWideStages & 1);
+      }
+    } else if (warp == 1) {
+      if (rank == 0) {
+        constexpr uint32_t idesc = instr_desc(kPair, kPair);
+        uint32_t i = 0;
+        bool ok = true;
+        for (uint32_t t = pair; ok && t < tiles; t += pairs) {
+          for (uint32_t g = 0; g < groups; ++g, ++i) {
+            const uint32_t s = i % kWideStages, b = i & 1, use = i >> 1;
+            if (!(ok = warp_wait(&failed, &full[s], i / kWideStages & 1))) break;
+            if (!(ok = use == 0 || warp_wait(&failed, &sum_empty[b], (use - 1) & 1))) break;
+            tc_fence_after();
+            const uint32_t st = smem_addr(ring + s * kWideStage);
+            const uint64_t da = smem_desc(st, 16, 1024), dw = smem_desc(st + kTileBytes, 16, 1024);
+            if (elect_one()) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < 4; ++kk) mma2_f8(tmem + b * kPair, da + 2 * kk, dw + 2 * kk, idesc, kk != 0);
+              mma2_commit(&empty[s]);
+              mma2_commit(&sum_full[b]);
+            }
+            __syncwarp();
+          }
+        }
+        if (elect_one()) mma2_commit(&drain);
+        warp_wait(&failed, &drain, 0);
+      }
+    } else {
+      // A stage's scales are written when its operands' place is free: then the group four before it has been multiplied, hence
+      // the one six before it added up, and its slot is free too.
+      static_assert(kScaleSlots >= kWideStages + 2, "scales are held until they are used");
+      const uint32_t half = warp - 2;
+      uint32_t i = 0;
+      bool ok = true;
+      for (uint32_t t = pair; ok && t < tiles; t += pairs) {
+        const WideTile tile = wide_tile(t, tiles_m, tiles_n);
+        const uint32_t row0 = tile.m * kPair + rank * 128 + lane, block = tile.n * 2 + half;
+        const bool real = block * kGroup < n;
+        const float *const sw = w_scales + static_cast<uint64_t>(block) * groups;
+        float row_scale[4][4], block_scale[4];  // of four groups on their way
+        const auto bring = [&](uint32_t g, int at) {
+          block_scale[at] = real && g < groups ? ld_f32(sw + g) : 0.f;
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q)
+            row_scale[at][q] = real && g < groups && row0 + 32 * q < m ? ld_f32(a_scales + static_cast<uint64_t>(g) * m + row0 + 32 * q) : 0.f;
+        };
+#pragma unroll
+        for (int at = 0; at < 4; ++at) bring(at, at);
+        for (uint32_t g0 = 0; ok && g0 < groups; g0 += 4) {
+#pragma unroll
+          for (int at = 0; at < 4; ++at) {
+            if (g0 + at >= groups) break;
+            const uint32_t s = i % kWideStages, use = i / kWideStages;
+            if (!(ok = use == 0 || warp_wait(&failed, &empty[s], (use - 1) & 1))) break;
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q)
+              scales[i % kScaleSlots * kPair + half * 128 + 32 * q + lane] = row_scale[at][q] * block_scale[at];
+            __syncwarp();
+            if (lane == 0) pair_arrive(full_bars + 8 * s);
+            bring(g0 + at + 4, at);
+            ++i;
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const uint32_t quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t release = cluster_addr(&sum_empty[0], 0), taddr = tmem + (quarter * 32u << 16) + half * 128;
+    const uint32_t scale_at = smem_addr(scales + half * 128 + quarter * 32 + lane);
+    uint8_t *const stage = ring + kWideStages * kWideStage + (warp - 4) * 2 * kOutBox;
+    bool ok = true;  // a warp that gives up goes on without waiting, to the end of its tile
+    uint32_t i = 0;
+    for (uint32_t t = pair; t < tiles; t += pairs) {
+      if (__any_sync(kFullMask, has_failed(&failed))) break;
+      const WideTile tile = wide_tile(t, tiles_m, tiles_n);
+      const uint32_t row0 = tile.m * kPair + rank * 128 + quarter * 32, col0 = tile.n * kPair + half * 128;
+      uint64_t sums[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) sums[j] = 0;
+      for (uint32_t g = 0; g < groups; ++g, ++i) {
+        const uint32_t b = i & 1;
+        if (ok && !mbar_wait(&sum_full[b], i >> 1 & 1)) failed = 1, ok = false;
+        __syncwarp();
+        tc_fence_after();
+        uint32_t scale;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(scale) : "r"(scale_at + i % kScaleSlots * (kPair * 4)) : "memory");
+        uint32_t d[2][16];
+        tmem_ld16_nowait(taddr + b * kPair, d[0]);
+        const uint64_t both = static_cast<uint64_t>(scale) << 32 | scale;
+#pragma unroll
+        for (int piece = 0; piece < 8; ++piece) {
+          uint32_t(&now)[16] = d[piece & 1];
+          tmem_landed(now);
+          if (piece < 7) {
+            tmem_ld16_nowait(taddr + b * kPair + 16 * (piece + 1), d[(piece + 1) & 1]);
+          } else {  // all read: the products after next may overwrite them
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) pair_arrive(release + 8 * b);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fma2(sums[8 * piece + j], now[2 * j], now[2 * j + 1], both);
+        }
+      }
+      if (row0 >= m || col0 >= n) continue;
+      if (TMA_OUT) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile has left
+        __syncwarp();
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 16; ++j) {
+        const uint4 v = make_uint4(pack2<T>(sums[4 * j]), pack2<T>(sums[4 * j + 1]), pack2<T>(sums[4 * j + 2]), pack2<T>(sums[4 * j + 3]));
+        *reinterpret_cast<uint4 *>(stage + j / 8 * kOutBox + lane * 128 + ((j % 8 ^ (lane & 7)) * 16)) = v;
+      }
+      if (TMA_OUT) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+#pragma unroll
+          for (uint32_t box = 0; box < 2; ++box)
+            if (col0 + 64 * box < n)
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&map_c),
+                           "r"(static_cast<int32_t>(col0 + 64 * box)), "r"(static_cast<int32_t>(row0)), "r"(smem_addr(stage + box * kOutBox))
+                           : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      } else {
+        __syncwarp();
+        const uint32_t rows = min(32u, m - row0);
+        for (uint32_t r = 0; r < rows; ++r)
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q) {
+            const uint32_t col = 32 * q + lane, in = col % 64;
+            if (col0 + col < n)
+              c[static_cast<uint64_t>(row0 + r) * n + col0 + col] =
+                  *reinterpret_cast<const T *>(stage + col / 64 * kOutBox + r * 128 + ((in / 8 ^ (r & 7)) * 16) + in % 8 * 2);
+          }
+        __syncwarp();
+      }
+    }
+    if (TMA_OUT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && failed) atomicOr(&g_fp8_error, kErrTimeout);
+  cluster_sync();  // neither block touches the other's barriers, shared memory or TMEM after this
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+  cluster_sync();
+}
+
+template <typename T>
+cudaError_t wide_launch(const Fp8Product &p, cudaStream_t s) {
+  const bool tma_out = p.n % 8 == 0;
+  CUtensorMap map_a, map_w, map_c;
+  cudaError_t e = make_tmap_2d_u8_swizzled(&map_a, p.a, p.k, p.m, 128);
+  if (e == cudaSuccess) e = make_tmap_2d_u8_swizzled(&map_w, p.w, p.k, p.n, 128);
+  map_c = map_a;
+  if (e == cudaSuccess && tma_out) e = make_tmap_2d_u16_swizzled(&map_c, p.c, p.n, p.m, p.n, 64, 32);
+  const auto kernel = tma_out ? k_wide<T, true> : k_wide<T, false>;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+  if (e != cudaSuccess) return e;
+  const uint64_t tiles = static_cast<uint64_t>((p.m + kPair - 1) / kPair) * ((p.n + kPair - 1) / kPair);
+  if (tiles >= (1ull << 31)) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  // The pairs do not wait for one another: any number of them is right.
+  cfg.gridDim = dim3(2 * static_cast<uint32_t>(std::min<uint64_t>(tiles, sm_count() / 2)));
+  cfg.blockDim = dim3(kWideThreads);
+  cfg.dynamicSmemBytes = kWideSmem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, map_a, map_w, map_c, p.a_scales, p.w_scales, static_cast<T *>(p.c), p.m, p.n,
+                            (p.k + kGroup - 1) / kGroup);
+}
+
 template <typename T>
 cudaError_t product_launch(const Fp8Product &p, cudaStream_t s) {
   if (p.m <= 16) return skinny_launch<T, 16>(p, s);
   if (p.m <= 32) return skinny_launch<T, 32>(p, s);
   if (p.m <= 64) return skinny_launch<T, 64>(p, s);
-  return skinny_launch<T, 128>(p, s);
+  if (p.m <= 256) return skinny_launch<T, 128>(p, s);
+  return wide_launch<T>(p, s);
 }
 
 }  // namespace

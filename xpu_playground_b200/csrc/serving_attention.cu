@@ -176,11 +176,6 @@ __device__ __forceinline__ bool wait_listed(Barriers &b, uint32_t segment) {
 
 // A value that all lanes hold, in a form the compiler knows to be uniform.
 __device__ __forceinline__ uint32_t same(uint32_t v) { return __shfl_sync(kFullMask, v, 0); }
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
-  return p != 0;
-}
 
 __host__ __device__ constexpr uint32_t attn_idesc(bool fp16, uint32_t n, bool b_kmajor) {
   return (1u << 4) | ((fp16 ? 0u : 1u) << 7) | ((fp16 ? 0u : 1u) << 10) | ((b_kmajor ? 0u : 1u) << 16) | ((n >> 3) << 17) |
