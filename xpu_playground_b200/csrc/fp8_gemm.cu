@@ -22,6 +22,8 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "serving.h"
@@ -97,19 +99,19 @@ __device__ __forceinline__ float ld_f32(const float *p) {
 
 template <int NT>
 struct Skinny {
-  static constexpr uint32_t kBuffers = NT <= 64 ? 4 : 2, kColumns = NT * kBuffers;
+  static constexpr uint32_t kBuffers = 4, kColumns = NT * kBuffers;
   static constexpr uint32_t kStageBytes = kTileBytes + NT * kGroup;
-  static constexpr uint32_t kStages = NT <= 32 ? 5 : NT == 64 ? 4 : 3;  // two blocks an SM
-  static constexpr uint32_t kChunk = 8;                                 // groups whose scales are held
-  static constexpr uint32_t kScales = 2 * kChunk * NT;
-  static constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + 4 * kScales;
+  static constexpr uint32_t kStages = NT <= 32 ? 5 : 4;  // two blocks an SM
+  static constexpr uint32_t kChunk = 8;                  // groups whose scales are held, twice
+  static constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + 2 * kChunk * NT * 4;
   static_assert(NT * kTileN * 4 <= kStages * kStageBytes, "the sums of a tile take the ring's place");
 };
-constexpr uint32_t kSkinnyThreads = 192;
+constexpr uint32_t kSkinnyThreads = 192, kSkinnyBlocks = 2;
 
-// Warp 0 loads, warp 1 issues the products, warps 2 to 5 add up: a thread has one row of w and NT sums.
+// Warp 0 loads, warp 1 issues the products (converged, as in k_wide), warps 2 to 5 add up: a thread has one row of w and NT
+// sums.
 template <typename T, int NT>
-__global__ void __launch_bounds__(kSkinnyThreads, 2)
+__global__ void __launch_bounds__(kSkinnyThreads, kSkinnyBlocks)
 k_skinny(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float *a_scales,
          const float *w_scales, T *c, uint32_t m, uint32_t n, uint32_t groups, uint32_t split) {
   using S = Skinny<NT>;
@@ -139,6 +141,10 @@ k_skinny(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUte
     fence_mbar_init();
     failed = 0;
   }
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+  }
   if (warp == 1) tmem_alloc1(&tmem_base, S::kColumns);
   tc_fence_before();
   __syncthreads();
@@ -147,7 +153,7 @@ k_skinny(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUte
   grid_dep_launch();  // with the TMEM held: a block of the next kernel cannot take it from one of this
   grid_dep_wait();
 
-  float sums[NT];
+  uint64_t sums[NT / 2];
   const uint32_t row = (warp & 3) * 32 + lane;  // of the tile; warps 2 to 5 have the TMEM quarters 2, 3, 0, 1
   const uint32_t held = min(static_cast<uint32_t>(NT), m - tile_m * NT);
   if (warp == 0) {
@@ -166,27 +172,28 @@ k_skinny(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUte
         for (uint32_t back = 0; back < S::kStages && back < i; ++back) mbar_wait(&full[(i - 1 - back) % S::kStages], (i - 1 - back) / S::kStages & 1);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = instr_desc(kTileN, NT);
-      for (uint32_t i = 0; i < count && !has_failed(&failed); ++i) {
-        const uint32_t s = i % S::kStages, b = i % S::kBuffers, use = i / S::kBuffers;
-        if (use > 0 && !mbar_wait(&sum_empty[b], (use - 1) & 1)) { failed = 1; break; }
-        if (!mbar_wait(&full[s], i / S::kStages & 1)) { failed = 1; break; }
-        tc_fence_after();
-        const uint32_t st = smem_addr(ring + s * S::kStageBytes);
-        const uint64_t dw = smem_desc(st, 16, 1024), da = smem_desc(st + kTileBytes, 16, 1024);
+    constexpr uint32_t idesc = instr_desc(kTileN, NT);
+    for (uint32_t i = 0; i < count; ++i) {
+      const uint32_t s = i % S::kStages, b = i % S::kBuffers, use = i / S::kBuffers;
+      if (!warp_wait(&failed, &full[s], i / S::kStages & 1)) break;
+      if (use > 0 && !warp_wait(&failed, &sum_empty[b], (use - 1) & 1)) break;
+      tc_fence_after();
+      const uint32_t st = smem_addr(ring + s * S::kStageBytes);
+      const uint64_t dw = smem_desc(st, 16, 1024), da = smem_desc(st + kTileBytes, 16, 1024);
+      if (elect_one()) {
 #pragma unroll
         for (uint32_t kk = 0; kk < 4; ++kk) mma1_f8(tmem + b * NT, dw + 2 * kk, da + 2 * kk, idesc, kk != 0);
         mma1_commit(&empty[s]);
         mma1_commit(&sum_full[b]);
       }
-      mma1_commit(&drain);
-      if (!mbar_wait(&drain, 0)) failed = 1;
+      __syncwarp();
     }
+    if (elect_one()) mma1_commit(&drain);
+    warp_wait(&failed, &drain, 0);
   } else {
     const uint32_t et = threadIdx.x - 64;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) sums[j] = 0.f;
+    for (int j = 0; j < NT / 2; ++j) sums[j] = 0;
     constexpr uint32_t kEach = S::kChunk * NT / 128;  // scales a thread brings
     float next[kEach];
     const auto fetch = [&](uint32_t at) {  // of groups first + at ..
@@ -213,37 +220,43 @@ k_skinny(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUte
       if (!has_failed(&failed) && !mbar_wait(&sum_full[b], i / S::kBuffers & 1)) failed = 1;
       __syncwarp();
       tc_fence_after();
-      const float4 *const by = reinterpret_cast<const float4 *>(chunk + i % S::kChunk * NT);
+      const ulonglong2 *const by = reinterpret_cast<const ulonglong2 *>(chunk + i % S::kChunk * NT);
+      const uint32_t taddr = tmem + ((warp & 3) * 32u << 16) + b * NT;
+      uint32_t d[2][16];
+      tmem_ld16_nowait(taddr, d[0]);
 #pragma unroll
-      for (int at = 0; at < NT; at += 16) {
-        float d[16];
-        tmem_ld16(tmem + ((warp & 3) * 32u << 16) + b * NT + at, d);
+      for (int piece = 0; piece < NT / 16; ++piece) {
+        uint32_t(&now)[16] = d[piece & 1];
+        tmem_landed(now);
+        if (piece + 1 < NT / 16) {
+          tmem_ld16_nowait(taddr + 16 * (piece + 1), d[(piece + 1) & 1]);
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sum_empty[b]);
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float4 s = by[at / 4 + q];
-          sums[at + 4 * q] = fmaf(d[4 * q], s.x, sums[at + 4 * q]);
-          sums[at + 4 * q + 1] = fmaf(d[4 * q + 1], s.y, sums[at + 4 * q + 1]);
-          sums[at + 4 * q + 2] = fmaf(d[4 * q + 2], s.z, sums[at + 4 * q + 2]);
-          sums[at + 4 * q + 3] = fmaf(d[4 * q + 3], s.w, sums[at + 4 * q + 3]);
+          const ulonglong2 s = by[4 * piece + q];
+          fma2(sums[8 * piece + 2 * q], now[4 * q], now[4 * q + 1], s.x);
+          fma2(sums[8 * piece + 2 * q + 1], now[4 * q + 2], now[4 * q + 3], s.y);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sum_empty[b]);
     }
-    T *const out = c + static_cast<uint64_t>(tile_m) * NT * n + tile_n * kTileN + row;
+    const auto sum = [&](int j) { return __uint_as_float(static_cast<uint32_t>(sums[j / 2] >> (32 * (j % 2)))); };
     if (split == 1) {
+      T *const out = c + static_cast<uint64_t>(tile_m) * NT * n + tile_n * kTileN + row;
       if (tile_n * kTileN + row < n) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-          if (static_cast<uint32_t>(j) < held) out[static_cast<uint64_t>(j) * n] = Elem<T>::from_float(sums[j]);
+          if (static_cast<uint32_t>(j) < held) out[static_cast<uint64_t>(j) * n] = Elem<T>::from_float(sum(j));
       }
     } else {
       // Every copy has landed and every product has read it: the ring is free.
       float *const part = reinterpret_cast<float *>(ring);
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        if (static_cast<uint32_t>(j) < held) part[j * kTileN + row] = sums[j];
+        if (static_cast<uint32_t>(j) < held) part[j * kTileN + row] = sum(j);
     }
   }
   tc_fence_before();
@@ -251,19 +264,29 @@ k_skinny(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUte
     __syncthreads();
   } else {
     cluster_sync();
-    if (threadIdx.x >= 64 && tile_n * kTileN + row < n) {  // rank r adds up rows r, r + split, .. of a
-      for (uint32_t j = rank; j < held; j += split) {
-        float total = 0.f;
-        for (uint32_t q = 0; q < split; ++q) {
-          float v;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                       : "=f"(v)
-                       : "r"(cluster_addr(reinterpret_cast<float *>(ring) + j * kTileN + row, q))
+    // Four outputs of one row a thread, the blocks' sums added in their order.
+    uint32_t from[8];
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q) from[q] = cluster_addr(ring, min(q, split - 1));
+    for (uint32_t i = rank * kSkinnyThreads + threadIdx.x; i < held * (kTileN / 4); i += split * kSkinnyThreads) {
+      float4 v[8];
+#pragma unroll
+      for (uint32_t q = 0; q < 8; ++q)
+        if (q < split)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[q].x), "=f"(v[q].y), "=f"(v[q].z), "=f"(v[q].w)
+                       : "r"(from[q] + 16 * i)
                        : "memory");
-          total += v;
-        }
-        c[(static_cast<uint64_t>(tile_m) * NT + j) * n + tile_n * kTileN + row] = Elem<T>::from_float(total);
-      }
+      float4 total = v[0];
+#pragma unroll
+      for (uint32_t q = 1; q < 8; ++q)
+        if (q < split) total.x += v[q].x, total.y += v[q].y, total.z += v[q].z, total.w += v[q].w;
+      const uint32_t j = i / (kTileN / 4), col = tile_n * kTileN + 4 * (i % (kTileN / 4));
+      T *const out = c + (static_cast<uint64_t>(tile_m) * NT + j) * n + col;
+      const T r[4] = {Elem<T>::from_float(total.x), Elem<T>::from_float(total.y), Elem<T>::from_float(total.z), Elem<T>::from_float(total.w)};
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e)
+        if (col + e < n) out[e] = r[e];
     }
     cluster_sync();  // no block leaves while another reads its sums
   }
@@ -274,21 +297,27 @@ k_skinny(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUte
   }
 }
 
-// Blocks that share a tile's groups. Time in groups that one SM reads: a block's share, and about four for beginning and
-// ending; two blocks an SM share its bandwidth.
-uint32_t pick_split(uint64_t tiles, uint32_t groups) {
-  const uint64_t slots = 2ull * sm_count();
-  uint32_t best = 1;
-  uint64_t least = UINT64_MAX;
-  for (uint32_t split = 1; split <= std::min(8u, groups); ++split) {
-    const uint64_t waves = (tiles * split + slots - 1) / slots, share = (groups + split - 1) / split;
-    const uint64_t cost = waves * (2 * share + 4);
-    if (cost < least) {
-      least = cost;
-      best = split;
+// Blocks that share a tile's groups: as many as can be resident at once for all tiles, two an SM. A second wave of smaller shares
+// costs more than it brings: 16 x 24576 x 4096 (192 tiles) 19 us unsplit, 25 and 31 in two and three; 1 x 6144 x 4096
+// (48) 13.1 unsplit, 8.7, 7.9, 6.9 and 6.6 in two to five, where six no longer fit the GPCs: 10.6.
+template <typename Kernel>
+uint32_t pick_split(Kernel kernel, int kind, cudaLaunchConfig_t cfg, uint64_t tiles, uint32_t groups) {
+  static std::mutex mutex;
+  static int resident[6][64][9] = {};  // clusters of each size at once, an SM having one block: 0 not known yet, -1 none
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return 1;
+  std::lock_guard<std::mutex> lock(mutex);
+  for (uint32_t split = std::min(8u, groups); split > 1; --split) {
+    int &clusters = resident[kind][device & 63][split];
+    if (clusters == 0) {
+      cfg.gridDim = dim3(split);
+      cfg.attrs[1].val.clusterDim.x = split;
+      cfg.numAttrs = 2;
+      if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters <= 0) clusters = -1;
     }
+    if (clusters > 0 && tiles <= static_cast<uint64_t>(clusters) * kSkinnyBlocks) return split;
   }
-  return best;
+  return 1;
 }
 
 template <typename T, int NT>
@@ -302,20 +331,22 @@ cudaError_t skinny_launch(const Fp8Product &p, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   const uint32_t groups = (p.k + kGroup - 1) / kGroup;
   const uint64_t tiles = static_cast<uint64_t>((p.n + kTileN - 1) / kTileN) * ((p.m + NT - 1) / NT);
-  const uint32_t split = pick_split(tiles, groups);
-  if (tiles * split >= (1ull << 31)) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.x = 1;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(static_cast<uint32_t>(tiles) * split);
   cfg.blockDim = dim3(kSkinnyThreads);
   cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = s;
   cfg.attrs = attr;
+  const int kind = (NT == 16 ? 0 : NT == 32 ? 1 : 2) + (std::is_same<T, __half>::value ? 3 : 0);
+  const uint32_t split = pick_split(kernel, kind, cfg, tiles, groups);
+  if (tiles * split >= (1ull << 31)) return cudaErrorInvalidConfiguration;
+  attr[1].val.clusterDim.x = split;
+  cfg.gridDim = dim3(static_cast<uint32_t>(tiles) * split);
+  cfg.stream = s;
   cfg.numAttrs = split > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, map_w, map_a, p.a_scales, p.w_scales, static_cast<T *>(p.c), p.m, p.n, groups, split);
 }
@@ -619,13 +650,21 @@ cudaError_t wide_launch(const Fp8Product &p, cudaStream_t s) {
                             (p.k + kGroup - 1) / kGroup);
 }
 
+// k_skinny with 64 rows a tile takes 0.31 us for a group of as many tiles as there are SMs, k_wide 0.4 us for one of half as many
+// of its tiles, whether there are that many or not: 128 x 4096 x 12288 17.8 and 46 us, 300 x 4096 x 4096 20.0 and
+// 19.2, 256 x 24576 x 4096 57 and 39.
+bool is_wide(const Fp8Product &p) {
+  const uint64_t sms = sm_count(), small = static_cast<uint64_t>((p.n + kTileN - 1) / kTileN) * ((p.m + 63) / 64);
+  const uint64_t large = static_cast<uint64_t>((p.n + kPair - 1) / kPair) * ((p.m + kPair - 1) / kPair);
+  const uint64_t rounds = (large + sms / 2 - 1) / (sms / 2);
+  return 4 * small >= 5 * sms * rounds;
+}
+
 template <typename T>
 cudaError_t product_launch(const Fp8Product &p, cudaStream_t s) {
   if (p.m <= 16) return skinny_launch<T, 16>(p, s);
   if (p.m <= 32) return skinny_launch<T, 32>(p, s);
-  if (p.m <= 64) return skinny_launch<T, 64>(p, s);
-  if (p.m <= 256) return skinny_launch<T, 128>(p, s);
-  return wide_launch<T>(p, s);
+  return p.m > 64 && is_wide(p) ? wide_launch<T>(p, s) : skinny_launch<T, 64>(p, s);
 }
 
 }  // namespace
