@@ -11,10 +11,13 @@
 // and which of its occurrences it is, and a second look at the row finds its place.
 // Sums are in a fixed order: results repeat bit for bit.
 //
-// SIZE blocks of a cluster share a row, a run of it each: eight where there are few
-// rows. Rows with a small top-k (a temperature of 0 is top-k 1) count only what can be among
-// the k: each thread's largest logit first, and no logit below the k-th of those.
+// Rows with a small top-k (a temperature of 0 is top-k 1) need no histogram: each thread's largest
+// logit is found first, and no logit below the k-th of those can be among the k. What is left, a few times
+// k, is listed and sorted by one block, a token a thread.
+//
+// SIZE blocks of a cluster share a row, a run of it each: as many as are resident at once for all rows.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "serving.h"
@@ -27,7 +30,8 @@ namespace {
 constexpr uint32_t kThreads = 1024, kWarps = kThreads / 32;
 constexpr uint32_t kKeys = 65536, kGroups = kKeys / 32;
 constexpr uint32_t kSmem = kKeys * 2;
-constexpr uint32_t kMostPruned = 256;  // top-k up to which the largest logits are looked for first
+constexpr uint32_t kMostListed = 256;  // top-k up to which the largest logits are looked for first
+constexpr uint32_t kListed = kThreads;
 constexpr uint32_t kHeavy = 2 * XPU_SAMPLE_MAX_VOCABULARY / 32768 + 1;
 constexpr uint32_t kRound = 32768;  // logits after which counters near overflow are emptied (slow way)
 
@@ -64,25 +68,39 @@ struct Row {
     base = row - skipped;
     pieces = (skipped + count + 7) / 8;
   }
-  __device__ __forceinline__ uint4 piece(uint32_t p) const {
-    const uint32_t first = 8 * p;  // counted from base
-    if (first >= skipped && first + 8 <= skipped + count) {
-      uint4 v;
-      asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(base + first) : "memory");
-      return v;
-    }
+  // The first and last piece, places outside being -inf.
+  __device__ __noinline__ uint4 edge(uint32_t p) const {
     uint32_t u[4];
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
       u[i] = Keys<T>::kMask;
 #pragma unroll
       for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t at = first + 2 * i + h;
+        const uint32_t at = 8 * p + 2 * i + h;  // counted from base
         if (at >= skipped && at < skipped + count)
           u[i] = (u[i] & (h ? 0xffffu : 0xffff0000u)) | static_cast<uint32_t>(*reinterpret_cast<const volatile uint16_t *>(base + at)) << (16 * h);
       }
     }
     return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  __device__ __forceinline__ uint4 piece(uint32_t p) const {
+    if (p == 0 || p + 1 == pieces) return edge(p);
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(base + 8ull * p) : "memory");
+    return v;
+  }
+  // use(piece, its number) for first, first + step, .. below end, four loads in flight.
+  template <typename Use>
+  __device__ __forceinline__ void each(uint32_t first, uint32_t step, uint32_t end, Use use) const {
+    for (uint32_t p = first; p < end; p += 4 * step) {
+      uint4 v[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        if (p + i * step < end) v[i] = piece(p + i * step);
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        if (p + i * step < end) use(v[i], p + i * step);
+    }
   }
 };
 
@@ -91,16 +109,28 @@ __device__ __forceinline__ uint32_t element(const uint4 &v, int i) {
   return u[i / 2] >> (16 * (i % 2)) & 0xffffu;
 }
 
+// Two keys of a word at once, without the case of -0.
+__device__ __forceinline__ uint32_t two_keys(uint32_t word) {
+  const uint32_t negative = word >> 15 & 0x00010001u;
+  return word ^ ((negative << 16) - negative | 0x80008000u);
+}
+
 struct Shared {
   uint32_t counts[kGroups];  // of each group of 32 values; then of the groups above it
   double masses[kGroups];    // likewise their weights
+  union {
+    uint16_t groups[kGroups];  // those that are not empty
+    uint64_t list[kListed];    // key << 32 | ~id of what can be among the first k
+  };
+  uint32_t occupied[2][kWarps];  // even and odd groups that have values in this block's run
   double warp_mass[kWarps];
   uint32_t warp_count[kWarps];
   uint32_t heavy_key[kHeavy], heavy_count[kHeavy], heavies;
   uint32_t top[8], bad[8];  // of each block of the cluster
   uint32_t found[5];        // group that answers a question, in falling order of groups, plus 1
   uint32_t answer_key, answer_at;  // the token: its value, and which occurrence; kKeys: none
-  uint32_t counted, bound;
+  uint32_t counted, bound, listed;
+  double total;
 };
 
 template <int SIZE>
@@ -138,28 +168,93 @@ __device__ __forceinline__ uint32_t last_lane(bool yes) {
   return votes ? 31 - __clz(votes) : 0;
 }
 
+// Chooses among `listed` (up to kListed) tokens of sh.list, which hold all that top-k keeps: sorted, one a thread.
+template <typename T>
+__device__ void choose_listed(Shared &sh, uint32_t listed, bool none, uint32_t most, double divisor, float top_p, float min_p, float u,
+                              int32_t *token, float *logprob) {
+  const uint32_t i = threadIdx.x, lane = i & 31, warp = i >> 5;
+  if (none) {  // the same for every thread
+    if (i == 0) {
+      *token = -1;
+      if (logprob) *logprob = -INFINITY;
+    }
+    return;
+  }
+  uint32_t size = 32;
+  while (size < listed) size *= 2;
+  uint64_t mine = sh.list[i];  // 0 behind the last
+  for (uint32_t run = 2; run <= size; run *= 2) {  // bitonic, the largest first
+    for (uint32_t stride = run / 2; stride > 0; stride /= 2) {
+      uint64_t other;
+      if (stride >= 32) {
+        __syncthreads();
+        sh.list[i] = mine;
+        __syncthreads();
+        other = sh.list[i ^ stride];
+      } else {
+        other = __shfl_xor_sync(kFullMask, mine, stride);
+      }
+      const bool larger = ((i & run) == 0) == ((i & stride) == 0);
+      mine = larger == (mine > other) ? mine : other;
+    }
+  }
+  if (i == 0) sh.answer_key = static_cast<uint32_t>(mine >> 32);
+  __syncthreads();
+  const double z = (value_of<T>(static_cast<uint32_t>(mine >> 32)) - value_of<T>(sh.answer_key)) / divisor;
+  const bool counts = i < listed && i < most;
+  const double weight = counts ? exp(z) : 0.0;
+  double sum = weight;
+#pragma unroll
+  for (uint32_t o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(kFullMask, sum, o);
+    if (lane >= o) sum += up;
+  }
+  if (lane == 31) sh.warp_mass[warp] = sum;
+  const double up = __shfl_up_sync(kFullMask, sum, 1);
+  __syncthreads();
+  double all = 0.0, lower = 0.0;
+  for (uint32_t w = 0; w < kWarps; ++w) {
+    if (w == warp) lower = all;
+    all += sh.warp_mass[w];
+  }
+  sum += lower;
+  const double before = lower + (lane ? up : 0.0);
+  const bool keep = counts && (i == 0 || ((top_p >= 1.f || before < static_cast<double>(top_p) * all) && weight >= static_cast<double>(min_p) && weight > 0.0));
+  const uint32_t kept = __syncthreads_count(keep);
+  if (i + 1 == kept) sh.total = sum;
+  __syncthreads();
+  const uint32_t at = min(static_cast<uint32_t>(__syncthreads_count(keep && sum <= static_cast<double>(u) * sh.total)), kept - 1);
+  if (i == at) {
+    *token = static_cast<int32_t>(~static_cast<uint32_t>(mine));
+    if (logprob) *logprob = static_cast<float>(z - log(sh.total));
+  }
+}
+
 template <typename T, int SIZE>
 __global__ void __launch_bounds__(kThreads, 1)
 k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, const int32_t *top_ks, const float *top_ps,
-         const float *min_ps, const float *us, int32_t *tokens, float *logprobs, uint32_t vocabulary) {
+         const float *min_ps, const float *us, int32_t *tokens, float *logprobs, uint32_t vocabulary, uint32_t resident) {
   extern __shared__ __align__(16) uint16_t histogram[];
   __shared__ Shared sh;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t rank = SIZE == 1 ? 0 : cluster_rank(), row = blockIdx.x / SIZE;
   uint4 *const words = reinterpret_cast<uint4 *>(histogram);
-  for (uint32_t i = threadIdx.x; i < kSmem / 16; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
+  const auto clear_histogram = [&] {
+    for (uint32_t i = threadIdx.x; i < kSmem / 16; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
+  };
   for (uint32_t i = threadIdx.x; i < kGroups; i += kThreads) {
     sh.counts[i] = 0;
     sh.masses[i] = 0.0;
   }
+  sh.list[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
-    sh.heavies = sh.counted = sh.bound = 0;
-    sh.top[rank] = sh.bad[rank] = 0;
+    sh.heavies = sh.counted = sh.bound = sh.listed = 0;
+    for (int i = 0; i < 8; ++i) sh.top[i] = sh.bad[i] = 0;
     for (int i = 0; i < 5; ++i) sh.found[i] = 0;
   }
   grid_dep_launch();
   grid_dep_wait();
-  __syncthreads();
+  row_sync<SIZE>();
 
   const volatile float *const vt = temperatures, *const vp = top_ps, *const vm = min_ps, *const vu = us;
   const volatile int32_t *const vk = top_ks;
@@ -169,24 +264,36 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   const bool asked = temperature >= 0.f && top_p == top_p && min_p == min_p && u >= 0.f && u < 1.f && top_k >= 0;
   const bool greedy = temperature == 0.f;
   const uint32_t most = greedy ? 1 : (top_k == 0 ? UINT32_MAX : static_cast<uint32_t>(top_k));
+  const double divisor = greedy ? 1.0 : static_cast<double>(temperature);
 
   const Row<T> r(logits + row * stride, vocabulary);
   const uint32_t share = (r.pieces + SIZE - 1) / SIZE;
   const uint32_t begin = min(rank * share, r.pieces), end = min(begin + share, r.pieces);
+  if (SIZE == 1 && threadIdx.x == 0 && row + resident < gridDim.x) {
+    // The row that this block's successor will read, towards the L2 while this one is worked on.
+    const uintptr_t from = reinterpret_cast<uintptr_t>(logits + (row + resident) * stride), first = (from + 15) & ~uintptr_t(15);
+    const uintptr_t last = (from + 2ull * vocabulary) & ~uintptr_t(15);
+    if (last > first) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(first), "r"(static_cast<uint32_t>(last - first)) : "memory");
+  }
 
-  // No logit below the `most`-th largest of the threads' largest ones can be among the first `most`.
-  if (most <= kMostPruned) {
-    uint32_t top = 0;
-    for (uint32_t p = begin + threadIdx.x; p < end; p += kThreads) {
-      const uint4 v = r.piece(p);
+  if (most <= kMostListed) {
+    uint32_t most2 = 0, least2 = ~0u;
+    r.each(begin + threadIdx.x, kThreads, end, [&](const uint4 &v, uint32_t) {
+      const uint32_t u4[4] = {two_keys(v.x), two_keys(v.y), two_keys(v.z), two_keys(v.w)};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, key_of(element(v, i)));
-    }
+      for (int i = 0; i < 4; ++i) {
+        most2 = __vmaxu2(most2, u4[i]);
+        least2 = __vminu2(least2, u4[i]);
+      }
+    });
+    uint32_t top = max(most2 & 0xffffu, most2 >> 16);
+    const uint32_t least = min(least2 & 0xffffu, least2 >> 16);
+    if (top == 0x7fffu) top = 0x8000u;
+    const bool bad = top >= Keys<T>::kPlusInf || least < Keys<T>::kMinusInf;
     if (top > Keys<T>::kMinusInf) atomicAdd(&sh.counts[top / 32], 1u);
-    __syncthreads();
-    // thread i: groups 2047 - 2 i and 2046 - 2 i
-    const uint32_t hi = kGroups - 1 - 2 * threadIdx.x;
-    const uint32_t a = sh.counts[hi], b = sh.counts[hi - 1];
+    const bool any_bad = __syncthreads_or(bad);
+    // The lowest value of the group with the `most`-th of them; thread i: groups 2047 - 2 i and 2046 - 2 i.
+    const uint32_t hi = kGroups - 1 - 2 * threadIdx.x, a = sh.counts[hi], b = sh.counts[hi - 1];
     uint32_t inc = a + b;
 #pragma unroll
     for (uint32_t o = 1; o < 32; o <<= 1) {
@@ -195,44 +302,81 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     }
     if (lane == 31) sh.warp_count[warp] = inc;
     __syncthreads();
-    uint32_t before = 0;
-    for (uint32_t w = 0; w < warp; ++w) before += sh.warp_count[w];
-    before += inc - a - b;
+    uint32_t before = lane < warp ? sh.warp_count[lane] : 0;
+    before = __reduce_add_sync(kFullMask, before) + inc - a - b;
     if (before < most && before + a >= most) sh.bound = 32 * hi;
     else if (before + a < most && before + a + b >= most) sh.bound = 32 * (hi - 1);
     sh.counts[hi] = sh.counts[hi - 1] = 0;
     __syncthreads();
+    const uint32_t bound = max(sh.bound, Keys<T>::kMinusInf + 1);
+    const uint32_t list = SIZE == 1 ? 0 : cluster_addr(sh.list, 0), counter = SIZE == 1 ? 0 : cluster_addr(&sh.listed, 0);
+    if (top >= bound) {
+      r.each(begin + threadIdx.x, kThreads, end, [&](const uint4 &v, uint32_t p) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t key = key_of(element(v, i));
+          if (key < bound) continue;
+          const uint64_t entry = static_cast<uint64_t>(key) << 32 | ~(8 * p + i - r.skipped);
+          uint32_t at;
+          if (SIZE == 1) {
+            at = atomicAdd(&sh.listed, 1u);
+            if (at < kListed) sh.list[at] = entry;
+          } else {
+            asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
+            if (at < kListed) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(entry) : "memory");
+          }
+        }
+      });
+    }
+    if (threadIdx.x == 0 && any_bad) {
+      if (SIZE == 1) sh.bad[0] = 1;
+      else asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bad[rank], 0)), "r"(1u) : "memory");
+    }
+    row_sync<SIZE>();
+    uint32_t listed = sh.listed;
+    if (SIZE > 1) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(listed) : "r"(counter) : "memory");
+    if (listed <= kListed) {  // the same for every block of the row
+      if (rank == 0) {
+        uint32_t bad_row = !asked || listed == 0;
+        for (int i = 0; i < SIZE; ++i) bad_row |= sh.bad[i];
+        choose_listed<T>(sh, listed, bad_row, most, divisor, top_p, min_p, u, tokens + row, logprobs ? logprobs + row : nullptr);
+      }
+      if (SIZE > 1) cluster_sync();  // block 0 stays until its counter has been read
+      return;
+    }
+    if (threadIdx.x < 8) sh.bad[threadIdx.x] = 0;  // found again below
   }
-  const uint32_t bound = max(sh.bound, Keys<T>::kMinusInf + 1);
+
+  clear_histogram();
+  if (threadIdx.x < kWarps) sh.occupied[0][threadIdx.x] = sh.occupied[1][threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    sh.heavy_key[0] = Keys<T>::kMinusInf + 1;
+    sh.heavy_count[0] = 0;
+  }
+  row_sync<SIZE>();  // what was cleared is, before another block writes there
   constexpr uint32_t kLowest = Keys<T>::kMinusInf + 1;  // the lowest finite value masks too: counted without the histogram
 
   uint32_t top = 0, counted = 0, lowest = 0, bad = 0;
   const auto count = [&](uint32_t from, uint32_t to) {
-    for (uint32_t p = from + threadIdx.x; p < to; p += kThreads) {
-      const uint4 v = r.piece(p);
+    r.each(from + threadIdx.x, kThreads, to, [&](const uint4 &v, uint32_t) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t key = key_of(element(v, i));
         bad |= key >= Keys<T>::kPlusInf || key < Keys<T>::kMinusInf;
         top = max(top, key);
-        if (key < bound) continue;
+        if (key <= Keys<T>::kMinusInf) continue;
         ++counted;
         if (key == kLowest) ++lowest;
         else atomicAdd(reinterpret_cast<uint32_t *>(histogram) + key / 2, 1u << (16 * (key & 1)));
       }
-    }
+    });
   };
   count(begin, end);
-  const auto add_lowest = [&] {
+  __syncthreads();
+  {
     const uint32_t n = __reduce_add_sync(kFullMask, lowest);
     if (lane == 0 && n) atomicAdd(&sh.heavy_count[0], n);
-  };
-  if (threadIdx.x == 0) {
-    sh.heavy_key[0] = kLowest;
-    sh.heavy_count[0] = 0;
   }
-  __syncthreads();
-  add_lowest();
   if (8 * (end - begin) > 65535) {
     // A counter may have passed 65535: then the sum of all is too small by a multiple of 65535 or 65536.
     uint32_t sum = 0;
@@ -241,14 +385,11 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum += element(v, e);
     }
-    if (__syncthreads_or(bad) == 0) {
-      const uint32_t missing = __reduce_add_sync(kFullMask, counted - lowest - sum);
-      if (lane == 0) atomicAdd(&sh.counted, missing);
-    }
+    const uint32_t missing = __reduce_add_sync(kFullMask, counted - lowest - sum);
+    if (lane == 0) atomicAdd(&sh.counted, missing);
     __syncthreads();
     if (sh.counted) {  // once more, emptying counters of 32768 and more after every 32768 logits
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < kSmem / 16; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
+      clear_histogram();
       if (threadIdx.x == 0) sh.heavies = 1;
       __syncthreads();
       for (uint32_t from = begin; from < end; from += kRound / 8) {
@@ -260,6 +401,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
           sh.heavy_key[at] = i;
           sh.heavy_count[at] = histogram[i];
           histogram[i] = 0;
+          atomicOr(&sh.occupied[i / 32 & 1][i / 64 / 32], 1u << (i / 64 & 31));
         }
         __syncthreads();
       }
@@ -271,8 +413,28 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     atomicMax(&sh.top[rank], top);
     atomicOr(&sh.bad[rank], bad);
   }
+  {
+    // Groups with values: thread i looks at groups 2 i and 2 i + 1, from another 16 bytes on in each lane (banks).
+    uint32_t has[2] = {0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t slot = (i + lane) & 7;
+      const uint4 v = words[8 * threadIdx.x + slot];
+      const uint32_t any = v.x | v.y | v.z | v.w;
+      has[0] |= slot < 4 ? any : 0;
+      has[1] |= slot < 4 ? 0 : any;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+      const uint32_t votes = __ballot_sync(kFullMask, has[i]);
+      if (lane == 0 && votes) atomicOr(&sh.occupied[i][warp], votes);
+    }
+  }
   __syncthreads();
-  if (threadIdx.x == 0 && sh.heavies == 0 && sh.heavy_count[0]) sh.heavies = 1;
+  if (threadIdx.x == 0 && sh.heavy_count[0]) {
+    sh.heavies = max(sh.heavies, 1u);
+    sh.occupied[kLowest / 32 & 1][kLowest / 64 / 32] |= 1u << (kLowest / 64 & 31);
+  }
   if (SIZE > 1 && threadIdx.x < SIZE && threadIdx.x != rank) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.top[rank], threadIdx.x)), "r"(sh.top[rank]) : "memory");
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bad[rank], threadIdx.x)), "r"(sh.bad[rank]) : "memory");
@@ -281,19 +443,27 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
 
   uint32_t any_heavy = 0;
   top = bad = 0;
+  uint32_t has[2] = {0, 0};
+#pragma unroll
   for (int i = 0; i < SIZE; ++i) {
     top = max(top, sh.top[i]);
     bad |= sh.bad[i];
     if (SIZE == 1) {
       any_heavy = sh.heavies;
+      has[0] = sh.occupied[0][warp];
+      has[1] = sh.occupied[1][warp];
     } else {
-      uint32_t h;
+      uint32_t h, a, b;
       asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(h) : "r"(cluster_addr(&sh.heavies, i)) : "memory");
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(a) : "r"(cluster_addr(&sh.occupied[0][warp], i)) : "memory");
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(b) : "r"(cluster_addr(&sh.occupied[1][warp], i)) : "memory");
       any_heavy |= h;
+      has[0] |= a;
+      has[1] |= b;
     }
   }
   const bool none = bad || !asked || top <= Keys<T>::kMinusInf;
-  const double largest = none ? 0.0 : value_of<T>(top), divisor = greedy ? 1.0 : static_cast<double>(temperature);
+  const double largest = none ? 0.0 : value_of<T>(top);
   const auto log_weight = [&](uint32_t key) { return (value_of<T>(key) - largest) / divisor; };
 
   if (none || greedy) {  // the same for every block of the row
@@ -305,13 +475,27 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     }
     __syncthreads();
   } else {
-    // Each block's share of the groups, their sums to block 0.
-    for (uint32_t i = warp; i < kGroups / SIZE; i += kWarps) {
-      const uint32_t g = i * SIZE + rank, key = 32 * g + lane;
-      if (g > top / 32) break;
+    // The groups with values, and each block's share of them, their sums to block 0.
+    const uint32_t first = has[0] >> lane & 1, second = has[1] >> lane & 1;
+    uint32_t inc = first + second;
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) sh.warp_count[warp] = inc;
+    __syncthreads();
+    const uint32_t of_warp = sh.warp_count[lane];
+    const uint32_t groups = __reduce_add_sync(kFullMask, of_warp);
+    uint32_t at = __reduce_add_sync(kFullMask, lane < warp ? of_warp : 0) + inc - first - second;
+    if (first) sh.groups[at++] = 2 * threadIdx.x;
+    if (second) sh.groups[at] = 2 * threadIdx.x + 1;
+    __syncthreads();
+    for (uint32_t i = warp * SIZE + rank; i < groups; i += kWarps * SIZE) {
+      const uint32_t g = sh.groups[i], key = 32 * g + lane;
       uint32_t n = 0;
+#pragma unroll
       for (int b = 0; b < SIZE; ++b) n += occurrences<SIZE>(histogram, &sh, key, b, any_heavy);
-      if (!__any_sync(kFullMask, n)) continue;
       double mass = n ? n * exp(log_weight(key)) : 0.0;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
@@ -465,21 +649,18 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   }
   if (mine) {
     const uint32_t run = (end - begin + kWarps - 1) / kWarps, from = begin + warp * run, to = min(from + run, end);
-    const auto matches = [&](uint32_t p) {
+    const auto matches = [&](const uint4 &v) {
       uint32_t mask = 0;
-      if (p < to) {
-        const uint4 v = r.piece(p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mask |= static_cast<uint32_t>(key_of(element(v, i)) == key) << i;
-      }
+      for (int i = 0; i < 8; ++i) mask |= static_cast<uint32_t>(key_of(element(v, i)) == key) << i;
       return mask;
     };
     uint32_t n = 0;
-    for (uint32_t p = from + lane; p < to; p += 32) {
-      const uint32_t mask = matches(p);
+    r.each(from + lane, 32, to, [&](const uint4 &v, uint32_t p) {
+      const uint32_t mask = matches(v);
       if (mask && here == 1) tokens[row] = static_cast<int32_t>(8 * p + __ffs(mask) - 1 - r.skipped);
       n += __popc(mask);
-    }
+    });
     if (here > 1) {
       n = __reduce_add_sync(kFullMask, n);
       if (lane == 0) sh.warp_count[warp] = n;
@@ -489,7 +670,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       if (j >= earlier && j - earlier < n) {
         j -= earlier;
         for (uint32_t p = from; p < to; p += 32) {
-          const uint32_t mask = matches(p + lane);
+          const uint32_t mask = p + lane < to ? matches(r.piece(p + lane)) : 0;
           uint32_t inc = __popc(mask);
 #pragma unroll
           for (uint32_t o = 1; o < 32; o <<= 1) {
@@ -514,7 +695,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
 }
 
 template <typename T, int SIZE>
-cudaError_t launch(const SampleArgs &a, cudaStream_t s) {
+cudaError_t launch(const SampleArgs &a, cudaStream_t s, bool *fits) {
   const auto kernel = k_sample<T, SIZE>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
@@ -531,14 +712,38 @@ cudaError_t launch(const SampleArgs &a, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = SIZE > 1 ? 2 : 1;
+  if (SIZE > 1) {
+    int device = 0;
+    if ((e = cudaGetDevice(&device)) != cudaSuccess) return e;
+    static std::atomic<int> resident[64];  // clusters at once
+    int clusters = resident[device & 63].load(std::memory_order_relaxed);
+    if (clusters == 0) {
+      if ((e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg)) != cudaSuccess) return e;
+      resident[device & 63].store(clusters = std::max(clusters, 1), std::memory_order_relaxed);
+    }
+    if (!(*fits = a.rows <= static_cast<uint32_t>(clusters))) return cudaSuccess;
+  }
+  *fits = true;
   return cudaLaunchKernelEx(&cfg, kernel, a.logits, a.stride, a.temperature, a.top_k, a.top_p, a.min_p, a.u, a.tokens, a.logprobs,
-                            a.vocabulary);
+                            a.vocabulary, sm_count());
+}
+
+// The most blocks a row with which all rows are resident at once; a run of fewer than 4096 logits a block would not pay for
+// the cluster's barriers.
+template <typename T>
+cudaError_t best_launch(const SampleArgs &a, cudaStream_t s) {
+  bool done = false;
+  cudaError_t e = cudaSuccess;
+  if (a.vocabulary >= 8 * 4096) e = launch<T, 8>(a, s, &done);
+  if (e == cudaSuccess && !done && a.vocabulary >= 4 * 4096) e = launch<T, 4>(a, s, &done);
+  if (e == cudaSuccess && !done && a.vocabulary >= 2 * 4096) e = launch<T, 2>(a, s, &done);
+  return e != cudaSuccess || done ? e : launch<T, 1>(a, s, &done);
 }
 
 }  // namespace
 
 cudaError_t sample_launch(bool fp16, const SampleArgs &a, cudaStream_t s) {
-  return fp16 ? launch<__half, 1>(a, s) : launch<__nv_bfloat16, 1>(a, s);
+  return fp16 ? best_launch<__half>(a, s) : best_launch<__nv_bfloat16>(a, s);
 }
 
 }  // namespace xpu
