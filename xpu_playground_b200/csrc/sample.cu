@@ -15,7 +15,8 @@
 // logit is found first, and no logit below the k-th of those can be among the k. What is left, a few times
 // k, is listed and sorted by one block, a token a thread.
 //
-// SIZE blocks of a cluster share a row, a run of it each: as many as are resident at once for all rows.
+// SIZE blocks of a cluster share a row, a run of it each: as many as are resident at once for all rows. Four and eight
+// blocks hold their runs in registers, one and two read theirs again from the L2.
 #include <algorithm>
 #include <atomic>
 
@@ -32,6 +33,8 @@ constexpr uint32_t kKeys = 65536, kGroups = kKeys / 32;
 constexpr uint32_t kSmem = kKeys * 2;
 constexpr uint32_t kMostListed = 256;  // top-k up to which the largest logits are looked for first
 constexpr uint32_t kListed = kThreads;
+constexpr int kHeld = 5, kBatch = 8;  // pieces of 8 logits a thread holds of its block's run, or has in flight
+static_assert(kHeld * kThreads * 8 < 65536, "counters of a held run do not overflow");
 constexpr uint32_t kHeavy = 2 * XPU_SAMPLE_MAX_VOCABULARY / 32768 + 1;
 constexpr uint32_t kRound = 32768;  // logits after which counters near overflow are emptied (slow way)
 
@@ -58,6 +61,23 @@ __device__ __forceinline__ double value_of(uint32_t key) {
   return static_cast<double>(Elem<T>::lo(bits));
 }
 
+// Piece p of a row whose logits are [skipped, skipped + count) from base on; places outside are -inf.
+template <typename T>
+__device__ __noinline__ uint4 edge_piece(const uint16_t *base, uint32_t skipped, uint32_t count, uint32_t p) {
+  uint32_t u[4];
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    u[i] = Keys<T>::kMask;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t at = 8 * p + 2 * i + h;
+      if (at >= skipped && at < skipped + count)
+        u[i] = (u[i] & (h ? 0xffffu : 0xffff0000u)) | static_cast<uint32_t>(*reinterpret_cast<const volatile uint16_t *>(base + at)) << (16 * h);
+    }
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
 // A row of logits at any 2-byte aligned address, in pieces of 8 from a 16-byte boundary on; places outside are -inf.
 template <typename T>
 struct Row {
@@ -68,38 +88,49 @@ struct Row {
     base = row - skipped;
     pieces = (skipped + count + 7) / 8;
   }
-  // The first and last piece, places outside being -inf.
-  __device__ __noinline__ uint4 edge(uint32_t p) const {
-    uint32_t u[4];
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      u[i] = Keys<T>::kMask;
-#pragma unroll
-      for (uint32_t h = 0; h < 2; ++h) {
-        const uint32_t at = 8 * p + 2 * i + h;  // counted from base
-        if (at >= skipped && at < skipped + count)
-          u[i] = (u[i] & (h ? 0xffffu : 0xffff0000u)) | static_cast<uint32_t>(*reinterpret_cast<const volatile uint16_t *>(base + at)) << (16 * h);
-      }
-    }
-    return make_uint4(u[0], u[1], u[2], u[3]);
-  }
   __device__ __forceinline__ uint4 piece(uint32_t p) const {
-    if (p == 0 || p + 1 == pieces) return edge(p);
+    if (p == 0 || p + 1 == pieces) return edge_piece<T>(base, skipped, count, p);
     uint4 v;
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(base + 8ull * p) : "memory");
     return v;
   }
-  // use(piece, its number) for first, first + step, .. below end, four loads in flight.
+};
+
+// The pieces begin .. end of a row that a block has, one a thread a turn.
+template <typename T, bool HELD>
+struct Run {
+  Row<T> row;
+  uint32_t begin, end;
+  uint4 held[HELD ? kHeld : 1];
+  __device__ Run(const uint16_t *logits, uint32_t vocabulary, uint32_t rank, uint32_t size) : row(logits, vocabulary) {
+    const uint32_t share = (row.pieces + size - 1) / size;
+    begin = min(rank * share, row.pieces);
+    end = min(begin + share, row.pieces);
+    if (HELD) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const uint32_t p = begin + threadIdx.x + i * kThreads;
+        held[i] = make_uint4(Keys<T>::kMask, Keys<T>::kMask, Keys<T>::kMask, Keys<T>::kMask);
+        if (p < end) held[i] = row.piece(p);
+      }
+    }
+  }
+  // use(piece, its number) for this thread's pieces from `from` on and below `to`; both at whole turns.
   template <typename Use>
-  __device__ __forceinline__ void each(uint32_t first, uint32_t step, uint32_t end, Use use) const {
-    for (uint32_t p = first; p < end; p += 4 * step) {
-      uint4 v[4];
+  __device__ __forceinline__ void each(uint32_t from, uint32_t to, Use use) const {
+    if (HELD) {
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-        if (p + i * step < end) v[i] = piece(p + i * step);
+      for (int i = 0; i < kHeld; ++i) use(held[i], begin + threadIdx.x + i * kThreads);
+      return;
+    }
+    for (uint32_t p = from + threadIdx.x; p < to; p += kBatch * kThreads) {
+      uint4 v[kBatch];
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-        if (p + i * step < end) use(v[i], p + i * step);
+      for (uint32_t i = 0; i < kBatch; ++i)
+        if (p + i * kThreads < to) v[i] = row.piece(p + i * kThreads);
+#pragma unroll
+      for (uint32_t i = 0; i < kBatch; ++i)
+        if (p + i * kThreads < to) use(v[i], p + i * kThreads);
     }
   }
 };
@@ -129,7 +160,7 @@ struct Shared {
   uint32_t top[8], bad[8];  // of each block of the cluster
   uint32_t found[5];        // group that answers a question, in falling order of groups, plus 1
   uint32_t answer_key, answer_at;  // the token: its value, and which occurrence; kKeys: none
-  uint32_t counted, bound, listed;
+  uint32_t counted, listed, bounds[2][8];
   double total;
 };
 
@@ -158,6 +189,18 @@ __device__ __forceinline__ uint32_t occurrences(const uint16_t *histogram, const
   return n;
 }
 
+// Inclusive sum over a warp, in a fixed order.
+template <typename V>
+__device__ __forceinline__ V warp_scan(V v) {
+  const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+  for (uint32_t o = 1; o < 32; o <<= 1) {
+    const V up = __shfl_up_sync(kFullMask, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+
 struct Bin {  // one value of a group, a lane each, the largest in lane 0
   uint32_t key, count, before;  // occurrences, and tokens before them in the order
   double weight, mass;          // of one, and of all before
@@ -168,21 +211,14 @@ __device__ __forceinline__ uint32_t last_lane(bool yes) {
   return votes ? 31 - __clz(votes) : 0;
 }
 
-// Chooses among `listed` (up to kListed) tokens of sh.list, which hold all that top-k keeps: sorted, one a thread.
+// Chooses among `listed` (up to kListed) tokens, thread i's being `mine` (key << 32 | ~id, 0 behind the last), which hold all
+// that top-k keeps: sorted, one a thread.
 template <typename T>
-__device__ void choose_listed(Shared &sh, uint32_t listed, bool none, uint32_t most, double divisor, float top_p, float min_p, float u,
-                              int32_t *token, float *logprob) {
+__device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32_t most, double divisor, float top_p, float min_p,
+                              float u, int32_t *token, float *logprob) {
   const uint32_t i = threadIdx.x, lane = i & 31, warp = i >> 5;
-  if (none) {  // the same for every thread
-    if (i == 0) {
-      *token = -1;
-      if (logprob) *logprob = -INFINITY;
-    }
-    return;
-  }
   uint32_t size = 32;
   while (size < listed) size *= 2;
-  uint64_t mine = sh.list[i];  // 0 behind the last
   for (uint32_t run = 2; run <= size; run *= 2) {  // bitonic, the largest first
     for (uint32_t stride = run / 2; stride > 0; stride /= 2) {
       uint64_t other;
@@ -198,28 +234,28 @@ __device__ void choose_listed(Shared &sh, uint32_t listed, bool none, uint32_t m
       mine = larger == (mine > other) ? mine : other;
     }
   }
+  if (most == 1) {  // temperature 0, or top-k 1: nothing else is kept
+    if (i == 0) {
+      *token = static_cast<int32_t>(~static_cast<uint32_t>(mine));
+      if (logprob) *logprob = 0.f;
+    }
+    return;
+  }
   if (i == 0) sh.answer_key = static_cast<uint32_t>(mine >> 32);
   __syncthreads();
   const double z = (value_of<T>(static_cast<uint32_t>(mine >> 32)) - value_of<T>(sh.answer_key)) / divisor;
   const bool counts = i < listed && i < most;
   const double weight = counts ? exp(z) : 0.0;
-  double sum = weight;
-#pragma unroll
-  for (uint32_t o = 1; o < 32; o <<= 1) {
-    const double up = __shfl_up_sync(kFullMask, sum, o);
-    if (lane >= o) sum += up;
-  }
+  double sum = warp_scan(weight);
   if (lane == 31) sh.warp_mass[warp] = sum;
   const double up = __shfl_up_sync(kFullMask, sum, 1);
   __syncthreads();
-  double all = 0.0, lower = 0.0;
-  for (uint32_t w = 0; w < kWarps; ++w) {
-    if (w == warp) lower = all;
-    all += sh.warp_mass[w];
-  }
+  const double warps = warp_scan(sh.warp_mass[lane]), all = __shfl_sync(kFullMask, warps, 31);
+  const double lower = warp ? __shfl_sync(kFullMask, warps, warp - 1) : 0.0;
   sum += lower;
   const double before = lower + (lane ? up : 0.0);
-  const bool keep = counts && (i == 0 || ((top_p >= 1.f || before < static_cast<double>(top_p) * all) && weight >= static_cast<double>(min_p) && weight > 0.0));
+  const bool keep = counts && (i == 0 || ((top_p >= 1.f || before < static_cast<double>(top_p) * all) &&
+                                          weight >= static_cast<double>(min_p) && weight > 0.0));
   const uint32_t kept = __syncthreads_count(keep);
   if (i + 1 == kept) sh.total = sum;
   __syncthreads();
@@ -246,10 +282,9 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     sh.counts[i] = 0;
     sh.masses[i] = 0.0;
   }
-  sh.list[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
-    sh.heavies = sh.counted = sh.bound = sh.listed = 0;
-    for (int i = 0; i < 8; ++i) sh.top[i] = sh.bad[i] = 0;
+    sh.heavies = sh.counted = sh.listed = 0;
+    for (int i = 0; i < 8; ++i) sh.top[i] = sh.bad[i] = sh.bounds[0][i] = sh.bounds[1][i] = 0;
     for (int i = 0; i < 5; ++i) sh.found[i] = 0;
   }
   grid_dep_launch();
@@ -261,14 +296,13 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   const float temperature = temperatures ? vt[row] : 1.f, top_p = top_ps ? vp[row] : 1.f, min_p = min_ps ? vm[row] : 0.f;
   const int32_t top_k = top_ks ? vk[row] : 0;
   const float u = vu[row];
+  const Run<T, (SIZE >= 4)> r(logits + row * stride, vocabulary, rank, SIZE);
   const bool asked = temperature >= 0.f && top_p == top_p && min_p == min_p && u >= 0.f && u < 1.f && top_k >= 0;
   const bool greedy = temperature == 0.f;
   const uint32_t most = greedy ? 1 : (top_k == 0 ? UINT32_MAX : static_cast<uint32_t>(top_k));
   const double divisor = greedy ? 1.0 : static_cast<double>(temperature);
+  const uint32_t begin = r.begin, end = r.end;
 
-  const Row<T> r(logits + row * stride, vocabulary);
-  const uint32_t share = (r.pieces + SIZE - 1) / SIZE;
-  const uint32_t begin = min(rank * share, r.pieces), end = min(begin + share, r.pieces);
   if (SIZE == 1 && threadIdx.x == 0 && row + resident < gridDim.x) {
     // The row that this block's successor will read, towards the L2 while this one is worked on.
     const uintptr_t from = reinterpret_cast<uintptr_t>(logits + (row + resident) * stride), first = (from + 15) & ~uintptr_t(15);
@@ -276,75 +310,119 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     if (last > first) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(first), "r"(static_cast<uint32_t>(last - first)) : "memory");
   }
 
-  if (most <= kMostListed) {
-    uint32_t most2 = 0, least2 = ~0u;
-    r.each(begin + threadIdx.x, kThreads, end, [&](const uint4 &v, uint32_t) {
-      const uint32_t u4[4] = {two_keys(v.x), two_keys(v.y), two_keys(v.z), two_keys(v.w)};
+  // Largest and smallest key of two, over this thread's pieces.
+  uint32_t most2 = 0, least2 = ~0u;
+  const auto look = [&](const uint4 &v, uint32_t (&keys)[4]) {
+    keys[0] = two_keys(v.x), keys[1] = two_keys(v.y), keys[2] = two_keys(v.z), keys[3] = two_keys(v.w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        most2 = __vmaxu2(most2, u4[i]);
-        least2 = __vminu2(least2, u4[i]);
-      }
-    });
-    uint32_t top = max(most2 & 0xffffu, most2 >> 16);
-    const uint32_t least = min(least2 & 0xffffu, least2 >> 16);
-    if (top == 0x7fffu) top = 0x8000u;
-    const bool bad = top >= Keys<T>::kPlusInf || least < Keys<T>::kMinusInf;
-    if (top > Keys<T>::kMinusInf) atomicAdd(&sh.counts[top / 32], 1u);
-    const bool any_bad = __syncthreads_or(bad);
-    // The lowest value of the group with the `most`-th of them; thread i: groups 2047 - 2 i and 2046 - 2 i.
-    const uint32_t hi = kGroups - 1 - 2 * threadIdx.x, a = sh.counts[hi], b = sh.counts[hi - 1];
-    uint32_t inc = a + b;
-#pragma unroll
-    for (uint32_t o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
-      if (lane >= o) inc += up;
+    for (int i = 0; i < 4; ++i) {
+      most2 = __vmaxu2(most2, keys[i]);
+      least2 = __vminu2(least2, keys[i]);
     }
+  };
+  const auto top_of = [&] {
+    const uint32_t top = max(most2 & 0xffffu, most2 >> 16);
+    return top == 0x7fffu ? 0x8000u : top;  // -0 is 0
+  };
+  const auto is_bad = [&] { return top_of() >= Keys<T>::kPlusInf || min(least2 & 0xffffu, least2 >> 16) < Keys<T>::kMinusInf; };
+
+  if (most <= kMostListed) {
+    r.each(begin, end, [&](const uint4 &v, uint32_t) {
+      uint32_t keys[4];
+      look(v, keys);
+    });
+    const uint32_t mine = top_of();
+    if (mine > Keys<T>::kMinusInf) atomicAdd(&sh.counts[mine / 32], 1u);
+    const bool any_bad = __syncthreads_or(is_bad());
+    // Lower bounds of the `most`-th largest logit: the lowest value of the group that holds this block's `most`-th of the
+    // threads' largest; and the least of all blocks' such values for their part of `most`. Thread i: groups
+    // 2047 - 2 i and 2046 - 2 i.
+    const uint32_t hi = kGroups - 1 - 2 * threadIdx.x, a = sh.counts[hi], b = sh.counts[hi - 1];
+    const uint32_t inc = warp_scan(a + b);
     if (lane == 31) sh.warp_count[warp] = inc;
     __syncthreads();
-    uint32_t before = lane < warp ? sh.warp_count[lane] : 0;
-    before = __reduce_add_sync(kFullMask, before) + inc - a - b;
-    if (before < most && before + a >= most) sh.bound = 32 * hi;
-    else if (before + a < most && before + a + b >= most) sh.bound = 32 * (hi - 1);
-    sh.counts[hi] = sh.counts[hi - 1] = 0;
-    __syncthreads();
-    const uint32_t bound = max(sh.bound, Keys<T>::kMinusInf + 1);
-    const uint32_t list = SIZE == 1 ? 0 : cluster_addr(sh.list, 0), counter = SIZE == 1 ? 0 : cluster_addr(&sh.listed, 0);
-    if (top >= bound) {
-      r.each(begin + threadIdx.x, kThreads, end, [&](const uint4 &v, uint32_t p) {
+    const uint32_t before = __reduce_add_sync(kFullMask, lane < warp ? sh.warp_count[lane] : 0) + inc - a - b;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t key = key_of(element(v, i));
-          if (key < bound) continue;
-          const uint64_t entry = static_cast<uint64_t>(key) << 32 | ~(8 * p + i - r.skipped);
-          uint32_t at;
-          if (SIZE == 1) {
-            at = atomicAdd(&sh.listed, 1u);
-            if (at < kListed) sh.list[at] = entry;
-          } else {
-            asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
-            if (at < kListed) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list + 8 * at), "l"(entry) : "memory");
-          }
+    for (uint32_t part = 0; part < (SIZE == 1 ? 1 : 2); ++part) {
+      const uint32_t n = part ? (most + SIZE - 1) / SIZE : most;
+      const bool first = before < n && before + a >= n, second = before + a < n && before + a + b >= n;
+      if (first || second) {
+        const uint32_t bound = 32 * (first ? hi : hi - 1);
+        if (SIZE == 1) {
+          sh.bounds[0][0] = bound;
+        } else {
+#pragma unroll
+          for (uint32_t q = 0; q < SIZE; ++q)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bounds[part][rank], q)), "r"(bound) : "memory");
         }
-      });
-    }
-    if (threadIdx.x == 0 && any_bad) {
-      if (SIZE == 1) sh.bad[0] = 1;
-      else asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bad[rank], 0)), "r"(1u) : "memory");
-    }
-    row_sync<SIZE>();
-    uint32_t listed = sh.listed;
-    if (SIZE > 1) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(listed) : "r"(counter) : "memory");
-    if (listed <= kListed) {  // the same for every block of the row
-      if (rank == 0) {
-        uint32_t bad_row = !asked || listed == 0;
-        for (int i = 0; i < SIZE; ++i) bad_row |= sh.bad[i];
-        choose_listed<T>(sh, listed, bad_row, most, divisor, top_p, min_p, u, tokens + row, logprobs ? logprobs + row : nullptr);
       }
-      if (SIZE > 1) cluster_sync();  // block 0 stays until its counter has been read
+    }
+    sh.counts[hi] = sh.counts[hi - 1] = 0;
+    row_sync<SIZE>();
+    uint32_t bound = Keys<T>::kMinusInf + 1, least = ~0u;
+#pragma unroll
+    for (int q = 0; q < SIZE; ++q) {
+      bound = max(bound, sh.bounds[0][q]);
+      least = min(least, sh.bounds[1][q]);
+    }
+    if (SIZE > 1) bound = max(bound, least);
+    const auto list = [&](const uint4 &v, uint32_t p) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t key = key_of(element(v, i));
+        if (key < bound) continue;
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kListed) sh.list[at] = static_cast<uint64_t>(key) << 32 | ~(8 * p + i - r.row.skipped);
+      }
+    };
+    if (SIZE >= 4) {
+      if (mine >= bound) r.each(begin, end, list);
+    } else {  // the pieces of the warp's threads that have such a logit, over its lanes
+      uint32_t threads = __ballot_sync(kFullMask, mine >= bound);
+      const uint32_t turns = (end - begin + kThreads - 1) / kThreads, items = __popc(threads) * turns;
+      for (uint32_t item = lane; item < items; item += 32) {
+        uint32_t left = threads;
+        for (uint32_t skip = item / turns; skip; --skip) left &= left - 1;
+        const uint32_t p = begin + 32 * warp + __ffs(left) - 1 + item % turns * kThreads;
+        if (p < end) list(r.row.piece(p), p);
+      }
+    }
+    if (threadIdx.x == 0) sh.bad[0] = any_bad;
+    row_sync<SIZE>();
+    uint32_t listed = 0, none = !asked, from = 0, at = threadIdx.x;
+#pragma unroll
+    for (uint32_t q = 0; q < SIZE; ++q) {
+      uint32_t n = sh.listed, bad = sh.bad[0];
+      if (SIZE > 1) {
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(cluster_addr(&sh.listed, q)) : "memory");
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(bad) : "r"(cluster_addr(&sh.bad[0], q)) : "memory");
+      }
+      if (threadIdx.x >= listed && threadIdx.x < listed + n) from = q, at = threadIdx.x - listed;
+      listed += n;
+      none |= bad;
+    }
+    none |= listed == 0;
+    if (none || listed <= kListed) {  // the same for every block of the row
+      if (rank == 0) {
+        if (none) {
+          if (threadIdx.x == 0) {
+            tokens[row] = -1;
+            if (logprobs) logprobs[row] = -INFINITY;
+          }
+        } else {
+          uint64_t entry = 0;
+          if (threadIdx.x < listed) {
+            if (SIZE == 1) entry = sh.list[at];
+            else asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(entry) : "r"(cluster_addr(&sh.list[at], from)) : "memory");
+          }
+          choose_listed<T>(sh, entry, listed, most, divisor, top_p, min_p, u, tokens + row, logprobs ? logprobs + row : nullptr);
+        }
+      }
+      if (SIZE > 1) cluster_sync();  // no block leaves while its list is read
       return;
     }
-    if (threadIdx.x < 8) sh.bad[threadIdx.x] = 0;  // found again below
+    row_sync<SIZE>();  // every block has seen the others' numbers
+    if (threadIdx.x == 0) sh.bad[0] = 0;
   }
 
   clear_histogram();
@@ -356,18 +434,20 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   row_sync<SIZE>();  // what was cleared is, before another block writes there
   constexpr uint32_t kLowest = Keys<T>::kMinusInf + 1;  // the lowest finite value masks too: counted without the histogram
 
-  uint32_t top = 0, counted = 0, lowest = 0, bad = 0;
+  uint32_t counted = 0, lowest = 0;
   const auto count = [&](uint32_t from, uint32_t to) {
-    r.each(from + threadIdx.x, kThreads, to, [&](const uint4 &v, uint32_t) {
+    r.each(from, to, [&](const uint4 &v, uint32_t) {
+      uint32_t keys[4];
+      look(v, keys);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t key = key_of(element(v, i));
-        bad |= key >= Keys<T>::kPlusInf || key < Keys<T>::kMinusInf;
-        top = max(top, key);
-        if (key <= Keys<T>::kMinusInf) continue;
-        ++counted;
-        if (key == kLowest) ++lowest;
-        else atomicAdd(reinterpret_cast<uint32_t *>(histogram) + key / 2, 1u << (16 * (key & 1)));
+        const uint32_t key = keys[i / 2] >> (16 * (i % 2)) & 0xffffu;
+        if (key > kLowest) {
+          ++counted;
+          atomicAdd(reinterpret_cast<uint32_t *>(histogram) + key / 2, 1u << (16 * (key & 1)));
+        } else if (key == kLowest) {
+          ++lowest;
+        }
       }
     });
   };
@@ -385,14 +465,14 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum += element(v, e);
     }
-    const uint32_t missing = __reduce_add_sync(kFullMask, counted - lowest - sum);
+    const uint32_t missing = __reduce_add_sync(kFullMask, counted - sum);
     if (lane == 0) atomicAdd(&sh.counted, missing);
     __syncthreads();
     if (sh.counted) {  // once more, emptying counters of 32768 and more after every 32768 logits
       clear_histogram();
       if (threadIdx.x == 0) sh.heavies = 1;
       __syncthreads();
-      for (uint32_t from = begin; from < end; from += kRound / 8) {
+      for (uint32_t from = begin; from < end; from += kRound / 8) {  // four whole turns
         count(from, min(end, from + kRound / 8));
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < kKeys; i += kThreads) {
@@ -401,18 +481,33 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
           sh.heavy_key[at] = i;
           sh.heavy_count[at] = histogram[i];
           histogram[i] = 0;
-          atomicOr(&sh.occupied[i / 32 & 1][i / 64 / 32], 1u << (i / 64 & 31));
+          const uint32_t key = i == 0x7fff ? 0x8000 : i;
+          atomicOr(&sh.occupied[key / 32 & 1][key / 64 / 32], 1u << (key / 64 & 31));
         }
         __syncthreads();
       }
     }
   }
-  top = __reduce_max_sync(kFullMask, top);
-  bad = __any_sync(kFullMask, bad);
+  uint32_t top = __reduce_max_sync(kFullMask, top_of()), bad = __any_sync(kFullMask, is_bad());
   if (lane == 0) {
     atomicMax(&sh.top[rank], top);
     atomicOr(&sh.bad[rank], bad);
   }
+  __syncthreads();
+  if (threadIdx.x == 0 && histogram[0x7fff]) {  // -0 is 0; a sum of more than 16 bits becomes a heavy one
+    const uint32_t zeros = static_cast<uint32_t>(histogram[0x8000]) + histogram[0x7fff];
+    histogram[0x7fff] = 0;
+    if (zeros < 65536) {
+      histogram[0x8000] = static_cast<uint16_t>(zeros);
+    } else {
+      sh.heavies = max(sh.heavies, 1u);
+      sh.heavy_key[sh.heavies] = 0x8000;
+      sh.heavy_count[sh.heavies++] = zeros - 65535;
+      histogram[0x8000] = 65535;
+    }
+  }
+  if (sh.heavies && threadIdx.x < sh.heavies && sh.heavy_key[threadIdx.x] == 0x7fff) sh.heavy_key[threadIdx.x] = 0x8000;
+  __syncthreads();
   {
     // Groups with values: thread i looks at groups 2 i and 2 i + 1, from another 16 bytes on in each lane (banks).
     uint32_t has[2] = {0, 0};
@@ -477,12 +572,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   } else {
     // The groups with values, and each block's share of them, their sums to block 0.
     const uint32_t first = has[0] >> lane & 1, second = has[1] >> lane & 1;
-    uint32_t inc = first + second;
-#pragma unroll
-    for (uint32_t o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
-      if (lane >= o) inc += up;
-    }
+    const uint32_t inc = warp_scan(first + second);
     if (lane == 31) sh.warp_count[warp] = inc;
     __syncthreads();
     const uint32_t of_warp = sh.warp_count[lane];
@@ -517,32 +607,17 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       uint32_t before[2];
       double mass[2];
       const double m0 = sh.masses[hi], m1 = sh.masses[hi - 1];
-      uint32_t inc = own[0] + own[1];
-      double minc = m0 + m1;
-#pragma unroll
-      for (uint32_t o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
-        const double mup = __shfl_up_sync(kFullMask, minc, o);
-        if (lane >= o) {
-          inc += up;
-          minc += mup;
-        }
-      }
+      const uint32_t inc = warp_scan(own[0] + own[1]);
+      const double minc = warp_scan(m0 + m1);
       if (lane == 31) {
         sh.warp_count[warp] = inc;
         sh.warp_mass[warp] = minc;
       }
       __syncthreads();
-      uint32_t all = 0, lower = 0;
-      double all_mass = 0.0, lower_mass = 0.0;
-      for (uint32_t w = 0; w < kWarps; ++w) {
-        if (w == warp) {
-          lower = all;
-          lower_mass = all_mass;
-        }
-        all += sh.warp_count[w];
-        all_mass += sh.warp_mass[w];
-      }
+      const uint32_t counts = warp_scan(sh.warp_count[lane]), all = __shfl_sync(kFullMask, counts, 31);
+      const double masses = warp_scan(sh.warp_mass[lane]), all_mass = __shfl_sync(kFullMask, masses, 31);
+      const uint32_t lower = warp ? __shfl_sync(kFullMask, counts, warp - 1) : 0;
+      const double lower_mass = warp ? __shfl_sync(kFullMask, masses, warp - 1) : 0.0;
       const uint32_t up1 = __shfl_up_sync(kFullMask, inc, 1);
       const double mup1 = __shfl_up_sync(kFullMask, minc, 1);
       before[0] = lower + (lane ? up1 : 0);
@@ -568,17 +643,8 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
         bin.count = 0;
         for (int b = 0; b < SIZE; ++b) bin.count += occurrences<SIZE>(histogram, &sh, bin.key, b, any_heavy);
         bin.weight = bin.count ? exp(log_weight(bin.key)) : 0.0;
-        uint32_t n = bin.count;
-        double m = bin.count * bin.weight;
-#pragma unroll
-        for (uint32_t o = 1; o < 32; o <<= 1) {
-          const uint32_t up = __shfl_up_sync(kFullMask, n, o);
-          const double mup = __shfl_up_sync(kFullMask, m, o);
-          if (lane >= o) {
-            n += up;
-            m += mup;
-          }
-        }
+        const uint32_t n = warp_scan(bin.count);
+        const double m = warp_scan(bin.count * bin.weight);
         const double mup = __shfl_up_sync(kFullMask, m, 1);
         bin.before = sh.counts[g] + n - bin.count;
         bin.mass = sh.masses[g] + (lane ? mup : 0.0);
@@ -647,21 +713,30 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       j -= n;
     }
   }
-  if (mine) {
-    const uint32_t run = (end - begin + kWarps - 1) / kWarps, from = begin + warp * run, to = min(from + run, end);
-    const auto matches = [&](const uint4 &v) {
-      uint32_t mask = 0;
+  const auto matches = [&](const uint4 &v) {
+    uint32_t mask = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mask |= static_cast<uint32_t>(key_of(element(v, i)) == key) << i;
-      return mask;
-    };
-    uint32_t n = 0;
-    r.each(from + lane, 32, to, [&](const uint4 &v, uint32_t p) {
+    for (int i = 0; i < 8; ++i) mask |= static_cast<uint32_t>(key_of(element(v, i)) == key) << i;
+    return mask;
+  };
+  if (mine && here == 1) {
+    r.each(begin, end, [&](const uint4 &v, uint32_t p) {
       const uint32_t mask = matches(v);
-      if (mask && here == 1) tokens[row] = static_cast<int32_t>(8 * p + __ffs(mask) - 1 - r.skipped);
-      n += __popc(mask);
+      if (mask) tokens[row] = static_cast<int32_t>(8 * p + __ffs(mask) - 1 - r.row.skipped);
     });
-    if (here > 1) {
+  } else if (mine) {  // a run of pieces a warp, whose occurrences are counted first
+    const uint32_t run = (end - begin + kWarps - 1) / kWarps, from = begin + warp * run, to = min(from + run, end);
+    uint32_t n = 0;
+    for (uint32_t p = from + lane; p < to; p += 4 * 32) {
+      uint4 v[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        if (p + 32 * i < to) v[i] = r.row.piece(p + 32 * i);
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        if (p + 32 * i < to) n += __popc(matches(v[i]));
+    }
+    {
       n = __reduce_add_sync(kFullMask, n);
       if (lane == 0) sh.warp_count[warp] = n;
       __syncthreads();
@@ -670,19 +745,14 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       if (j >= earlier && j - earlier < n) {
         j -= earlier;
         for (uint32_t p = from; p < to; p += 32) {
-          const uint32_t mask = p + lane < to ? matches(r.piece(p + lane)) : 0;
-          uint32_t inc = __popc(mask);
-#pragma unroll
-          for (uint32_t o = 1; o < 32; o <<= 1) {
-            const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
-            if (lane >= o) inc += up;
-          }
+          const uint32_t mask = p + lane < to ? matches(r.row.piece(p + lane)) : 0;
+          const uint32_t inc = warp_scan(static_cast<uint32_t>(__popc(mask)));
           const uint32_t many = __shfl_sync(kFullMask, inc, 31), before = inc - __popc(mask);
           if (j < many) {
             if (j >= before && j < inc) {
               uint32_t left = mask;
               for (uint32_t skip = j - before; skip; --skip) left &= left - 1;
-              tokens[row] = static_cast<int32_t>(8 * (p + lane) + __ffs(left) - 1 - r.skipped);
+              tokens[row] = static_cast<int32_t>(8 * (p + lane) + __ffs(left) - 1 - r.row.skipped);
             }
             break;
           }
@@ -734,8 +804,10 @@ template <typename T>
 cudaError_t best_launch(const SampleArgs &a, cudaStream_t s) {
   bool done = false;
   cudaError_t e = cudaSuccess;
-  if (a.vocabulary >= 8 * 4096) e = launch<T, 8>(a, s, &done);
-  if (e == cudaSuccess && !done && a.vocabulary >= 4 * 4096) e = launch<T, 4>(a, s, &done);
+  // up to 8 blocks x kHeld x 1024 pieces, one piece more where the row's address is odd
+  const uint32_t pieces = (a.vocabulary + 14) / 8;
+  if (a.vocabulary >= 8 * 4096 && (pieces + 7) / 8 <= kHeld * kThreads) e = launch<T, 8>(a, s, &done);
+  if (e == cudaSuccess && !done && a.vocabulary >= 4 * 4096 && (pieces + 3) / 4 <= kHeld * kThreads) e = launch<T, 4>(a, s, &done);
   if (e == cudaSuccess && !done && a.vocabulary >= 2 * 4096) e = launch<T, 2>(a, s, &done);
   return e != cudaSuccess || done ? e : launch<T, 1>(a, s, &done);
 }
