@@ -33,7 +33,7 @@ constexpr uint32_t kKeys = 65536, kGroups = kKeys / 32;
 constexpr uint32_t kSmem = kKeys * 2;
 constexpr uint32_t kMostListed = 256;  // top-k up to which the largest logits are looked for first
 constexpr uint32_t kListed = kThreads;
-constexpr int kHeld = 5, kBatch = 8;  // pieces of 8 logits a thread holds of its block's run, or has in flight
+constexpr int kHeld = 5, kBatch = 4;  // pieces of 8 logits a thread holds of its block's run, or has in flight
 static_assert(kHeld * kThreads * 8 < 65536, "counters of a held run do not overflow");
 constexpr uint32_t kHeavy = 2 * XPU_SAMPLE_MAX_VOCABULARY / 32768 + 1;
 constexpr uint32_t kRound = 32768;  // logits after which counters near overflow are emptied (slow way)
@@ -147,20 +147,20 @@ __device__ __forceinline__ uint32_t two_keys(uint32_t word) {
 }
 
 struct Shared {
-  uint32_t counts[kGroups];  // of each group of 32 values; then of the groups above it
+  uint32_t counts[kGroups];  // logits of each group that is not empty, falling; then of the groups before it
   double masses[kGroups];    // likewise their weights
   union {
     uint16_t groups[kGroups];  // those that are not empty
     uint64_t list[kListed];    // key << 32 | ~id of what can be among the first k
   };
-  uint32_t occupied[2][kWarps];  // even and odd groups that have values in this block's run
+  uint32_t occupied[2][kWarps];  // groups that have values in this block's run: of negative ones, of the others
   double warp_mass[kWarps];
   uint32_t warp_count[kWarps];
   uint32_t heavy_key[kHeavy], heavy_count[kHeavy], heavies;
   uint32_t top[8], bad[8];  // of each block of the cluster
-  uint32_t found[5];        // group that answers a question, in falling order of groups, plus 1
   uint32_t answer_key, answer_at;  // the token: its value, and which occurrence; kKeys: none
   uint32_t counted, listed, bounds[2][8];
+  uint32_t coarse[2], wanted[2], fine[2][32];  // group of a bound, how many of its threads, their values
   double total;
 };
 
@@ -170,12 +170,15 @@ __device__ __forceinline__ void row_sync() {
   else cluster_sync();
 }
 
+// Place of a value's 16-bit counter: neighbours in words of their own.
+__device__ __forceinline__ uint32_t counter(uint32_t key) { return (key & 0x7fffu) << 1 | key >> 15; }
+
 // Occurrences of a value in block r's run.
 template <int SIZE>
 __device__ __forceinline__ uint32_t occurrences(const uint16_t *histogram, const Shared *sh, uint32_t key, uint32_t r, bool any_heavy) {
   uint32_t n;
-  if (SIZE == 1) n = histogram[key];
-  else asm volatile("{\n .reg .u16 t;\n ld.shared::cluster.u16 t, [%1];\n cvt.u32.u16 %0, t;\n}" : "=r"(n) : "r"(cluster_addr(histogram + key, r)) : "memory");
+  if (SIZE == 1) n = histogram[counter(key)];
+  else asm volatile("{\n .reg .u16 t;\n ld.shared::cluster.u16 t, [%1];\n cvt.u32.u16 %0, t;\n}" : "=r"(n) : "r"(cluster_addr(histogram + counter(key), r)) : "memory");
   if (any_heavy) {
     for (uint32_t i = 0; i < kHeavy; ++i) {
       uint32_t k, c, many;
@@ -243,9 +246,12 @@ __device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32
   }
   if (i == 0) sh.answer_key = static_cast<uint32_t>(mine >> 32);
   __syncthreads();
-  const double z = (value_of<T>(static_cast<uint32_t>(mine >> 32)) - value_of<T>(sh.answer_key)) / divisor;
   const bool counts = i < listed && i < most;
-  const double weight = counts ? exp(z) : 0.0;
+  double z = 0.0, weight = 0.0;
+  if (counts) {
+    z = (value_of<T>(static_cast<uint32_t>(mine >> 32)) - value_of<T>(sh.answer_key)) / divisor;
+    weight = exp(z);
+  }
   double sum = warp_scan(weight);
   if (lane == 31) sh.warp_mass[warp] = sum;
   const double up = __shfl_up_sync(kFullMask, sum, 1);
@@ -269,7 +275,7 @@ __device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32
 template <typename T, int SIZE>
 __global__ void __launch_bounds__(kThreads, 1)
 k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, const int32_t *top_ks, const float *top_ps,
-         const float *min_ps, const float *us, int32_t *tokens, float *logprobs, uint32_t vocabulary, uint32_t resident) {
+         const float *min_ps, const float *us, int32_t *tokens, float *logprobs, uint32_t vocabulary) {
   extern __shared__ __align__(16) uint16_t histogram[];
   __shared__ Shared sh;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -285,8 +291,9 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   if (threadIdx.x == 0) {
     sh.heavies = sh.counted = sh.listed = 0;
     for (int i = 0; i < 8; ++i) sh.top[i] = sh.bad[i] = sh.bounds[0][i] = sh.bounds[1][i] = 0;
-    for (int i = 0; i < 5; ++i) sh.found[i] = 0;
+    sh.coarse[0] = sh.coarse[1] = kGroups;
   }
+  if (threadIdx.x < 64) sh.fine[threadIdx.x / 32][lane] = 0;
   grid_dep_launch();
   grid_dep_wait();
   row_sync<SIZE>();
@@ -302,13 +309,6 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   const uint32_t most = greedy ? 1 : (top_k == 0 ? UINT32_MAX : static_cast<uint32_t>(top_k));
   const double divisor = greedy ? 1.0 : static_cast<double>(temperature);
   const uint32_t begin = r.begin, end = r.end;
-
-  if (SIZE == 1 && threadIdx.x == 0 && row + resident < gridDim.x) {
-    // The row that this block's successor will read, towards the L2 while this one is worked on.
-    const uintptr_t from = reinterpret_cast<uintptr_t>(logits + (row + resident) * stride), first = (from + 15) & ~uintptr_t(15);
-    const uintptr_t last = (from + 2ull * vocabulary) & ~uintptr_t(15);
-    if (last > first) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(first), "r"(static_cast<uint32_t>(last - first)) : "memory");
-  }
 
   // Largest and smallest key of two, over this thread's pieces.
   uint32_t most2 = 0, least2 = ~0u;
@@ -334,27 +334,36 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     const uint32_t mine = top_of();
     if (mine > Keys<T>::kMinusInf) atomicAdd(&sh.counts[mine / 32], 1u);
     const bool any_bad = __syncthreads_or(is_bad());
-    // Lower bounds of the `most`-th largest logit: the lowest value of the group that holds this block's `most`-th of the
-    // threads' largest; and the least of all blocks' such values for their part of `most`. Thread i: groups
-    // 2047 - 2 i and 2046 - 2 i.
+    // Lower bounds of the `most`-th largest logit: this block's `most`-th of the threads' largest; and the least of all blocks'
+    // such values for their part of `most`. First the group of 32 values, thread i looking at groups 2047 - 2 i and
+    // 2046 - 2 i, then the value.
     const uint32_t hi = kGroups - 1 - 2 * threadIdx.x, a = sh.counts[hi], b = sh.counts[hi - 1];
     const uint32_t inc = warp_scan(a + b);
     if (lane == 31) sh.warp_count[warp] = inc;
     __syncthreads();
     const uint32_t before = __reduce_add_sync(kFullMask, lane < warp ? sh.warp_count[lane] : 0) + inc - a - b;
+    constexpr uint32_t kParts = SIZE == 1 ? 1 : 2;
 #pragma unroll
-    for (uint32_t part = 0; part < (SIZE == 1 ? 1 : 2); ++part) {
+    for (uint32_t part = 0; part < kParts; ++part) {
       const uint32_t n = part ? (most + SIZE - 1) / SIZE : most;
       const bool first = before < n && before + a >= n, second = before + a < n && before + a + b >= n;
       if (first || second) {
-        const uint32_t bound = 32 * (first ? hi : hi - 1);
-        if (SIZE == 1) {
-          sh.bounds[0][0] = bound;
-        } else {
+        sh.coarse[part] = first ? hi : hi - 1;
+        sh.wanted[part] = n - before - (first ? 0 : a);
+      }
+    }
+    __syncthreads();
 #pragma unroll
-          for (uint32_t q = 0; q < SIZE; ++q)
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bounds[part][rank], q)), "r"(bound) : "memory");
-        }
+    for (uint32_t part = 0; part < kParts; ++part)
+      if (mine / 32 == sh.coarse[part]) atomicAdd(&sh.fine[part][31 - mine % 32], 1u);
+    __syncthreads();
+    if (warp < kParts && sh.coarse[warp] < kGroups) {
+      const uint32_t votes = __ballot_sync(kFullMask, warp_scan(sh.fine[warp][lane]) >= sh.wanted[warp]);
+      const uint32_t bound = 32 * sh.coarse[warp] + 32 - __ffs(votes);
+      if (SIZE == 1) {
+        if (lane == 0) sh.bounds[0][0] = bound;
+      } else if (lane < SIZE) {
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bounds[warp][rank], lane)), "r"(bound) : "memory");
       }
     }
     sh.counts[hi] = sh.counts[hi - 1] = 0;
@@ -435,16 +444,30 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   constexpr uint32_t kLowest = Keys<T>::kMinusInf + 1;  // the lowest finite value masks too: counted without the histogram
 
   uint32_t counted = 0, lowest = 0;
+  const auto add = [&](uint32_t key_at_top) {  // a key in the upper half of a word
+    atomicAdd(reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(histogram) + (key_at_top >> 14 & 0x1fffcu)),
+              static_cast<int32_t>(key_at_top) < 0 ? 0x10000u : 1u);
+  };
   const auto count = [&](uint32_t from, uint32_t to) {
     r.each(from, to, [&](const uint4 &v, uint32_t) {
       uint32_t keys[4];
       look(v, keys);
+      const uint32_t least = __vminu2(__vminu2(keys[0], keys[1]), __vminu2(keys[2], keys[3]));
+      if (min(least & 0xffffu, least >> 16) > kLowest) {
+        counted += 8;
 #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          add(keys[i] << 16);
+          add(keys[i]);
+        }
+        return;
+      }
+#pragma unroll 1
       for (int i = 0; i < 8; ++i) {
-        const uint32_t key = keys[i / 2] >> (16 * (i % 2)) & 0xffffu;
+        const uint32_t word = i < 4 ? (i < 2 ? keys[0] : keys[1]) : (i < 6 ? keys[2] : keys[3]), key = word >> (16 * (i % 2)) & 0xffffu;
         if (key > kLowest) {
           ++counted;
-          atomicAdd(reinterpret_cast<uint32_t *>(histogram) + key / 2, 1u << (16 * (key & 1)));
+          add(key << 16);
         } else if (key == kLowest) {
           ++lowest;
         }
@@ -476,13 +499,14 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
         count(from, min(end, from + kRound / 8));
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < kKeys; i += kThreads) {
-          if (histogram[i] < kRound) continue;
+          uint16_t *const held = histogram + counter(i);
+          if (*held < kRound) continue;
           const uint32_t at = atomicAdd(&sh.heavies, 1u);
           sh.heavy_key[at] = i;
-          sh.heavy_count[at] = histogram[i];
-          histogram[i] = 0;
+          sh.heavy_count[at] = *held;
+          *held = 0;
           const uint32_t key = i == 0x7fff ? 0x8000 : i;
-          atomicOr(&sh.occupied[key / 32 & 1][key / 64 / 32], 1u << (key / 64 & 31));
+          atomicOr(&sh.occupied[key >> 15][key / 1024 & 31], 1u << (key / 32 & 31));
         }
         __syncthreads();
       }
@@ -494,30 +518,28 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     atomicOr(&sh.bad[rank], bad);
   }
   __syncthreads();
-  if (threadIdx.x == 0 && histogram[0x7fff]) {  // -0 is 0; a sum of more than 16 bits becomes a heavy one
-    const uint32_t zeros = static_cast<uint32_t>(histogram[0x8000]) + histogram[0x7fff];
-    histogram[0x7fff] = 0;
-    if (zeros < 65536) {
-      histogram[0x8000] = static_cast<uint16_t>(zeros);
-    } else {
+  if (threadIdx.x == 0 && histogram[counter(0x7fff)]) {  // -0 is 0; a sum of more than 16 bits becomes a heavy one
+    uint16_t *const zero = histogram + counter(0x8000), *const minus = histogram + counter(0x7fff);
+    const uint32_t zeros = static_cast<uint32_t>(*zero) + *minus;
+    *minus = 0;
+    *zero = static_cast<uint16_t>(min(zeros, 65535u));
+    if (zeros > 65535) {
       sh.heavies = max(sh.heavies, 1u);
       sh.heavy_key[sh.heavies] = 0x8000;
       sh.heavy_count[sh.heavies++] = zeros - 65535;
-      histogram[0x8000] = 65535;
     }
   }
   if (sh.heavies && threadIdx.x < sh.heavies && sh.heavy_key[threadIdx.x] == 0x7fff) sh.heavy_key[threadIdx.x] = 0x8000;
   __syncthreads();
   {
-    // Groups with values: thread i looks at groups 2 i and 2 i + 1, from another 16 bytes on in each lane (banks).
+    // Groups with values: thread i looks at groups i (lower halves) and 1024 + i, from another 16 bytes on in each lane (banks).
     uint32_t has[2] = {0, 0};
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t slot = (i + lane) & 7;
-      const uint4 v = words[8 * threadIdx.x + slot];
+      const uint4 v = words[8 * threadIdx.x + ((i + lane) & 7)];
       const uint32_t any = v.x | v.y | v.z | v.w;
-      has[0] |= slot < 4 ? any : 0;
-      has[1] |= slot < 4 ? 0 : any;
+      has[0] |= any & 0xffffu;
+      has[1] |= any >> 16;
     }
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
@@ -528,7 +550,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   __syncthreads();
   if (threadIdx.x == 0 && sh.heavy_count[0]) {
     sh.heavies = max(sh.heavies, 1u);
-    sh.occupied[kLowest / 32 & 1][kLowest / 64 / 32] |= 1u << (kLowest / 64 & 31);
+    sh.occupied[0][kLowest / 1024] |= 1u << (kLowest / 32 & 31);
   }
   if (SIZE > 1 && threadIdx.x < SIZE && threadIdx.x != rank) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.top[rank], threadIdx.x)), "r"(sh.top[rank]) : "memory");
@@ -571,15 +593,13 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     __syncthreads();
   } else {
     // The groups with values, and each block's share of them, their sums to block 0.
-    const uint32_t first = has[0] >> lane & 1, second = has[1] >> lane & 1;
-    const uint32_t inc = warp_scan(first + second);
-    if (lane == 31) sh.warp_count[warp] = inc;
+    const uint32_t below[2] = {__popc(has[0] & ((1u << lane) - 1)), __popc(has[1] & ((1u << lane) - 1))};
+    if (lane == 0) sh.warp_count[warp] = __popc(has[0]) | __popc(has[1]) << 16;
     __syncthreads();
-    const uint32_t of_warp = sh.warp_count[lane];
-    const uint32_t groups = __reduce_add_sync(kFullMask, of_warp);
-    uint32_t at = __reduce_add_sync(kFullMask, lane < warp ? of_warp : 0) + inc - first - second;
-    if (first) sh.groups[at++] = 2 * threadIdx.x;
-    if (second) sh.groups[at] = 2 * threadIdx.x + 1;
+    const uint32_t of_warp = sh.warp_count[lane], earlier = __reduce_add_sync(kFullMask, lane < warp ? of_warp : 0);
+    const uint32_t both = __reduce_add_sync(kFullMask, of_warp), groups = (both & 0xffffu) + (both >> 16);
+    if (has[0] >> lane & 1) sh.groups[(earlier & 0xffffu) + below[0]] = static_cast<uint16_t>(threadIdx.x);
+    if (has[1] >> lane & 1) sh.groups[(both & 0xffffu) + (earlier >> 16) + below[1]] = static_cast<uint16_t>(1024 + threadIdx.x);
     __syncthreads();
     for (uint32_t i = warp * SIZE + rank; i < groups; i += kWarps * SIZE) {
       const uint32_t g = sh.groups[i], key = 32 * g + lane;
@@ -592,22 +612,20 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       n = __reduce_add_sync(kFullMask, n);
       if (lane == 0) {
         if (SIZE == 1) {
-          sh.counts[g] = n;
-          sh.masses[g] = mass;
+          sh.counts[groups - 1 - i] = n;
+          sh.masses[groups - 1 - i] = mass;
         } else {
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.counts[g], 0)), "r"(n) : "memory");
-          asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&sh.masses[g], 0)), "d"(mass) : "memory");
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.counts[groups - 1 - i], 0)), "r"(n) : "memory");
+          asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&sh.masses[groups - 1 - i], 0)), "d"(mass) : "memory");
         }
       }
     }
     row_sync<SIZE>();
     if (rank == 0) {
-      // Sums over the groups above each; thread i has groups 2047 - 2 i and 2046 - 2 i.
-      const uint32_t hi = kGroups - 1 - 2 * threadIdx.x, own[2] = {sh.counts[hi], sh.counts[hi - 1]};
-      uint32_t before[2];
-      double mass[2];
-      const double m0 = sh.masses[hi], m1 = sh.masses[hi - 1];
-      const uint32_t inc = warp_scan(own[0] + own[1]);
+      // Sums over the groups before each; thread i has groups 2 i and 2 i + 1.
+      const uint32_t e = 2 * threadIdx.x, n0 = e < groups ? sh.counts[e] : 0, n1 = e + 1 < groups ? sh.counts[e + 1] : 0;
+      const double m0 = e < groups ? sh.masses[e] : 0.0, m1 = e + 1 < groups ? sh.masses[e + 1] : 0.0;
+      const uint32_t inc = warp_scan(n0 + n1);
       const double minc = warp_scan(m0 + m1);
       if (lane == 31) {
         sh.warp_count[warp] = inc;
@@ -616,81 +634,107 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       __syncthreads();
       const uint32_t counts = warp_scan(sh.warp_count[lane]), all = __shfl_sync(kFullMask, counts, 31);
       const double masses = warp_scan(sh.warp_mass[lane]), all_mass = __shfl_sync(kFullMask, masses, 31);
-      const uint32_t lower = warp ? __shfl_sync(kFullMask, counts, warp - 1) : 0;
-      const double lower_mass = warp ? __shfl_sync(kFullMask, masses, warp - 1) : 0.0;
-      const uint32_t up1 = __shfl_up_sync(kFullMask, inc, 1);
-      const double mup1 = __shfl_up_sync(kFullMask, minc, 1);
-      before[0] = lower + (lane ? up1 : 0);
-      mass[0] = lower_mass + (lane ? mup1 : 0.0);
-      before[1] = before[0] + own[0];
-      mass[1] = mass[0] + m0;
-      sh.counts[hi] = before[0];
-      sh.counts[hi - 1] = before[1];
-      sh.masses[hi] = mass[0];
-      sh.masses[hi - 1] = mass[1];
-
-      // The values of the last group that is not empty and of which yes(tokens before it, their weight, the group).
-      const auto ask = [&](int question, auto yes) {
-        uint32_t last = 0;  // place in falling order, plus 1
-        if (own[0] && yes(before[0], mass[0], hi)) last = 2 * threadIdx.x + 1;
-        if (own[1] && yes(before[1], mass[1], hi - 1)) last = 2 * threadIdx.x + 2;
-        last = __reduce_max_sync(kFullMask, last);
-        if (lane == 0 && last) atomicMax(&sh.found[question], last);
-        __syncthreads();
-        const uint32_t g = kGroups - max(sh.found[question], 1u);
-        Bin bin;
-        bin.key = 32 * g + 31 - lane;
-        bin.count = 0;
-        for (int b = 0; b < SIZE; ++b) bin.count += occurrences<SIZE>(histogram, &sh, bin.key, b, any_heavy);
-        bin.weight = bin.count ? exp(log_weight(bin.key)) : 0.0;
-        const uint32_t n = warp_scan(bin.count);
-        const double m = warp_scan(bin.count * bin.weight);
-        const double mup = __shfl_up_sync(kFullMask, m, 1);
-        bin.before = sh.counts[g] + n - bin.count;
-        bin.mass = sh.masses[g] + (lane ? mup : 0.0);
-        return bin;
-      };
-      // Weight of the first n tokens.
-      const auto weight_of_first = [&](int question, uint32_t n) {
-        const Bin b = ask(question, [&](uint32_t c, double, uint32_t) { return c < n; });
-        const uint32_t at = last_lane(b.count && b.before < n);
-        return __shfl_sync(kFullMask, b.mass + min(n - b.before, b.count) * b.weight, at);
-      };
-      uint32_t kept = min(most, all);
-      double total = kept == all ? all_mass : weight_of_first(0, kept);
-      uint32_t fewer = kept;
-      if (top_p < 1.f) {
-        const double wanted = static_cast<double>(top_p) * total;
-        const Bin b = ask(1, [&](uint32_t, double m, uint32_t) { return m < wanted; });
-        const uint32_t at = last_lane(b.count && b.mass < wanted);
-        const double need = fmin(fmax(ceil((wanted - b.mass) / b.weight), 1.0), static_cast<double>(b.count));
-        fewer = min(fewer, __shfl_sync(kFullMask, b.before + (b.count ? static_cast<uint32_t>(need) : 0), at));
+      uint32_t before = __shfl_up_sync(kFullMask, inc, 1);
+      double mass = __shfl_up_sync(kFullMask, minc, 1);
+      const uint32_t lower = __shfl_sync(kFullMask, counts, warp ? warp - 1 : 0);
+      const double lower_mass = __shfl_sync(kFullMask, masses, warp ? warp - 1 : 0);
+      before = (lane ? before : 0) + (warp ? lower : 0);
+      mass = (lane ? mass : 0.0) + (warp ? lower_mass : 0.0);
+      if (e < groups) {
+        sh.counts[e] = before;
+        sh.masses[e] = mass;
       }
-      if (min_p > 0.f) {
-        // of the last group with values that would be heavy enough, those that are; all above it are
-        const double least = static_cast<double>(min_p);
-        const Bin b = ask(2, [&](uint32_t, double, uint32_t g) { return exp(log_weight(min(32 * g + 31, top))) >= least; });
-        const uint32_t at = last_lane(b.count && b.weight >= least);
-        const uint32_t heavy = __shfl_sync(kFullMask, b.count && b.weight >= least ? b.before + b.count : b.before, at);
-        fewer = min(fewer, heavy);
+      if (e + 1 < groups) {
+        sh.counts[e + 1] = before + n0;
+        sh.masses[e + 1] = mass + m0;
       }
-      fewer = max(fewer, 1u);
-      if (fewer < kept) total = weight_of_first(3, kept = fewer);
-      const double wanted = static_cast<double>(u) * total;
-      const Bin b = ask(4, [&](uint32_t c, double m, uint32_t) { return c < kept && m <= wanted; });
-      const uint32_t at = last_lane(b.count && b.weight > 0.0 && b.before < kept && b.mass <= wanted);
-      if (warp == 0 && lane == at) {
-        const uint32_t in = min(b.count, kept - b.before);  // of its occurrences are kept
-        const double which = floor((wanted - b.mass) / b.weight);
-        const uint32_t j = which < in ? static_cast<uint32_t>(which) : in - 1;
-        if (logprobs) logprobs[row] = static_cast<float>(log_weight(b.key) - log(total));
-        for (int i = 0; i < SIZE; ++i) {
-          if (SIZE == 1) {
-            sh.answer_key = b.key;
-            sh.answer_at = j;
-          } else {
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_key, i)), "r"(b.key) : "memory");
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_at, i)), "r"(j) : "memory");
+      __syncthreads();
+      if (warp == 0) {
+        // The last group of which yes(tokens before it, their weight); the first if there is none.
+        const auto last_group = [&](auto yes) {
+          uint32_t low = 0, many = groups;
+          while (many > 1) {  // 32 places of [low, low + many) at once
+            const uint32_t step = (many + 31) / 32, at = low + min(lane * step, many - 1);
+            const uint32_t votes = __ballot_sync(kFullMask, yes(sh.counts[at], sh.masses[at]));
+            const uint32_t run = votes == kFullMask ? 32 : __ffs(~votes) - 1, from = min((run ? run - 1 : 0) * step, many - 1);
+            low += from;
+            many = min(step, many - from);
+          }
+          return low;
+        };
+        const auto bins_of = [&](uint32_t group) {
+          Bin bin;
+          bin.key = 32 * sh.groups[groups - 1 - group] + 31 - lane;
+          bin.count = 0;
+#pragma unroll
+          for (int b = 0; b < SIZE; ++b) bin.count += occurrences<SIZE>(histogram, &sh, bin.key, b, any_heavy);
+          bin.weight = bin.count ? exp(log_weight(bin.key)) : 0.0;
+          const double m = warp_scan(bin.count * bin.weight);
+          const double up = __shfl_up_sync(kFullMask, m, 1);
+          bin.before = sh.counts[group] + warp_scan(bin.count) - bin.count;
+          bin.mass = sh.masses[group] + (lane ? up : 0.0);
+          return bin;
+        };
+        // Weight of the first n tokens.
+        const auto weight_of_first = [&](uint32_t n) {
+          const Bin b = bins_of(last_group([&](uint32_t c, double) { return c < n; }));
+          const uint32_t at = last_lane(b.count && b.before < n);
+          return __shfl_sync(kFullMask, b.mass + min(n - b.before, b.count) * b.weight, at);
+        };
+        uint32_t kept = min(most, all);
+        double total = kept == all ? all_mass : weight_of_first(kept);
+        uint32_t fewer = kept;
+        if (top_p < 1.f) {
+          const double wanted = static_cast<double>(top_p) * total;
+          const Bin b = bins_of(last_group([&](uint32_t, double m) { return m < wanted; }));
+          const uint32_t at = last_lane(b.count && b.mass < wanted);
+          const double need = fmin(fmax(ceil((wanted - b.mass) / b.weight), 1.0), static_cast<double>(b.count));
+          fewer = min(fewer, __shfl_sync(kFullMask, b.before + (b.count ? static_cast<uint32_t>(need) : 0), at));
+        }
+        if (min_p > 1.f) {
+          fewer = 1;
+        } else if (min_p > 0.f) {  // the lowest value that is heavy enough: one of the keys [low, low + many)
+          uint32_t low = 0, many = top + 1;
+          while (many > 1) {
+            const uint32_t step = (many + 31) / 32, at = low + min((lane + 1) * step, many) - 1;
+            const double weight = at > Keys<T>::kMinusInf ? exp(log_weight(at)) : 0.0;
+            const uint32_t votes = __ballot_sync(kFullMask, weight >= static_cast<double>(min_p));
+            const uint32_t chosen = votes ? __ffs(votes) - 1 : 31, from = min(chosen * step, many - 1);
+            low += from;
+            many = min(step, many - from);
+          }
+          // tokens of that value and above
+          uint32_t found = 0, place = groups;  // the first group whose highest value is below it
+          for (uint32_t from = 0; from < groups && place == groups; from += 32) {
+            const uint32_t at = from + lane;
+            const uint32_t votes = __ballot_sync(kFullMask, at < groups && 32u * sh.groups[groups - 1 - at] + 31 < low);
+            if (votes) place = from + __ffs(votes) - 1;
+          }
+          if (place > 0) {
+            const Bin b = bins_of(place - 1);
+            const uint32_t in = __reduce_add_sync(kFullMask, b.key >= low ? b.count : 0);
+            found = sh.counts[place - 1] + in;
+          }
+          fewer = min(fewer, found);
+        }
+        fewer = max(fewer, 1u);
+        if (fewer < kept) total = weight_of_first(kept = fewer);
+        const double wanted = static_cast<double>(u) * total;
+        const Bin b = bins_of(last_group([&](uint32_t c, double m) { return c < kept && m <= wanted; }));
+        const uint32_t at = last_lane(b.count && b.weight > 0.0 && b.before < kept && b.mass <= wanted);
+        if (lane == at) {
+          const uint32_t in = max(min(b.count, kept - b.before), 1u);  // of its occurrences are kept
+          const double which = floor((wanted - b.mass) / b.weight);
+          const uint32_t j = which < in ? static_cast<uint32_t>(which) : in - 1;
+          if (logprobs) logprobs[row] = static_cast<float>(log_weight(b.key) - log(total));
+          for (int i = 0; i < SIZE; ++i) {
+            if (SIZE == 1) {
+              sh.answer_key = b.key;
+              sh.answer_at = j;
+            } else {
+              asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_key, i)), "r"(b.key) : "memory");
+              asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_at, i)), "r"(j) : "memory");
+            }
           }
         }
       }
@@ -713,10 +757,20 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       j -= n;
     }
   }
+  // A bit for each of a piece's logits that has the value; 0 has two forms.
+  const uint32_t form = key & 0x8000u ? key & 0x7fffu : key ^ 0xffffu, form2 = form << 16 | form, other2 = form ? form2 : 0x80008000u;
   const auto matches = [&](const uint4 &v) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    uint32_t equal[4], any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      equal[i] = __vcmpeq2(u[i], form2) | __vcmpeq2(u[i], other2);
+      any |= equal[i];
+    }
+    if (any == 0) return 0u;
     uint32_t mask = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mask |= static_cast<uint32_t>(key_of(element(v, i)) == key) << i;
+    for (int i = 0; i < 4; ++i) mask |= (equal[i] & 1u) << 2 * i | (equal[i] >> 31) << (2 * i + 1);
     return mask;
   };
   if (mine && here == 1) {
@@ -795,7 +849,7 @@ cudaError_t launch(const SampleArgs &a, cudaStream_t s, bool *fits) {
   }
   *fits = true;
   return cudaLaunchKernelEx(&cfg, kernel, a.logits, a.stride, a.temperature, a.top_k, a.top_p, a.min_p, a.u, a.tokens, a.logprobs,
-                            a.vocabulary, sm_count());
+                            a.vocabulary);
 }
 
 // The most blocks a row with which all rows are resident at once; a run of fewer than 4096 logits a block would not pay for
