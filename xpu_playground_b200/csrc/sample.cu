@@ -120,7 +120,8 @@ struct Run {
   __device__ __forceinline__ void each(uint32_t from, uint32_t to, Use use) const {
     if (HELD) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) use(held[i], begin + threadIdx.x + i * kThreads);
+      for (int i = 0; i < kHeld; ++i)
+        if (begin + threadIdx.x + i * kThreads < end) use(held[i], begin + threadIdx.x + i * kThreads);
       return;
     }
     for (uint32_t p = from + threadIdx.x; p < to; p += kBatch * kThreads) {
@@ -217,7 +218,7 @@ __device__ __forceinline__ uint32_t last_lane(bool yes) {
 // Chooses among `listed` (up to kListed) tokens, thread i's being `mine` (key << 32 | ~id, 0 behind the last), which hold all
 // that top-k keeps: sorted, one a thread.
 template <typename T>
-__device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32_t most, double divisor, float top_p, float min_p,
+__device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32_t most, double slope, float top_p, float min_p,
                               float u, int32_t *token, float *logprob) {
   const uint32_t i = threadIdx.x, lane = i & 31, warp = i >> 5;
   uint32_t size = 32;
@@ -249,7 +250,7 @@ __device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32
   const bool counts = i < listed && i < most;
   double z = 0.0, weight = 0.0;
   if (counts) {
-    z = (value_of<T>(static_cast<uint32_t>(mine >> 32)) - value_of<T>(sh.answer_key)) / divisor;
+    z = (value_of<T>(static_cast<uint32_t>(mine >> 32)) - value_of<T>(sh.answer_key)) * slope;
     weight = exp(z);
   }
   double sum = warp_scan(weight);
@@ -307,7 +308,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   const bool asked = temperature >= 0.f && top_p == top_p && min_p == min_p && u >= 0.f && u < 1.f && top_k >= 0;
   const bool greedy = temperature == 0.f;
   const uint32_t most = greedy ? 1 : (top_k == 0 ? UINT32_MAX : static_cast<uint32_t>(top_k));
-  const double divisor = greedy ? 1.0 : static_cast<double>(temperature);
+  const double slope = greedy ? 1.0 : 1.0 / static_cast<double>(temperature);
   const uint32_t begin = r.begin, end = r.end;
 
   // Largest and smallest key of two, over this thread's pieces.
@@ -323,6 +324,16 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   const auto top_of = [&] {
     const uint32_t top = max(most2 & 0xffffu, most2 >> 16);
     return top == 0x7fffu ? 0x8000u : top;  // -0 is 0
+  };
+  // use(piece, its number) for the pieces of some of the warp's threads, spread over its lanes.
+  const auto over_lanes = [&](uint32_t threads, auto use) {
+    const uint32_t turns = (end - begin + kThreads - 1) / kThreads, items = __popc(threads) * turns;
+    for (uint32_t item = lane; item < items; item += 32) {
+      uint32_t left = threads;
+      for (uint32_t skip = item / turns; skip; --skip) left &= left - 1;
+      const uint32_t p = begin + 32 * warp + __ffs(left) - 1 + item % turns * kThreads;
+      if (p < end) use(r.row.piece(p), p);
+    }
   };
   const auto is_bad = [&] { return top_of() >= Keys<T>::kPlusInf || min(least2 & 0xffffu, least2 >> 16) < Keys<T>::kMinusInf; };
 
@@ -386,15 +397,8 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     };
     if (SIZE >= 4) {
       if (mine >= bound) r.each(begin, end, list);
-    } else {  // the pieces of the warp's threads that have such a logit, over its lanes
-      uint32_t threads = __ballot_sync(kFullMask, mine >= bound);
-      const uint32_t turns = (end - begin + kThreads - 1) / kThreads, items = __popc(threads) * turns;
-      for (uint32_t item = lane; item < items; item += 32) {
-        uint32_t left = threads;
-        for (uint32_t skip = item / turns; skip; --skip) left &= left - 1;
-        const uint32_t p = begin + 32 * warp + __ffs(left) - 1 + item % turns * kThreads;
-        if (p < end) list(r.row.piece(p), p);
-      }
+    } else {
+      over_lanes(__ballot_sync(kFullMask, mine >= bound), list);
     }
     if (threadIdx.x == 0) sh.bad[0] = any_bad;
     row_sync<SIZE>();
@@ -424,7 +428,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
             if (SIZE == 1) entry = sh.list[at];
             else asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(entry) : "r"(cluster_addr(&sh.list[at], from)) : "memory");
           }
-          choose_listed<T>(sh, entry, listed, most, divisor, top_p, min_p, u, tokens + row, logprobs ? logprobs + row : nullptr);
+          choose_listed<T>(sh, entry, listed, most, slope, top_p, min_p, u, tokens + row, logprobs ? logprobs + row : nullptr);
         }
       }
       if (SIZE > 1) cluster_sync();  // no block leaves while its list is read
@@ -581,7 +585,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   }
   const bool none = bad || !asked || top <= Keys<T>::kMinusInf;
   const double largest = none ? 0.0 : value_of<T>(top);
-  const auto log_weight = [&](uint32_t key) { return (value_of<T>(key) - largest) / divisor; };
+  const auto log_weight = [&](uint32_t key) { return (value_of<T>(key) - largest) * slope; };
 
   if (none || greedy) {  // the same for every block of the row
     if (threadIdx.x == 0) {
@@ -744,17 +748,18 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
 
   // The answer's place in the row: which block's run has that occurrence, then which warp's.
   const uint32_t key = sh.answer_key;
-  uint32_t j = sh.answer_at, here = 0;
+  uint32_t j = sh.answer_at, here = 0, of_block[SIZE];
+#pragma unroll
+  for (uint32_t b = 0; b < SIZE; ++b) of_block[b] = key < kKeys ? occurrences<SIZE>(histogram, &sh, key, b, any_heavy) : 0;
   bool mine = key < kKeys;
-  for (uint32_t b = 0; mine && b <= rank; ++b) {
-    const uint32_t n = occurrences<SIZE>(histogram, &sh, key, b, any_heavy);
+#pragma unroll
+  for (uint32_t b = 0; b < SIZE; ++b) {
     if (b == rank) {
-      here = n;
-      mine = j < n;
-    } else if (j < n) {
-      mine = false;
-    } else {
-      j -= n;
+      here = of_block[b];
+      mine = mine && j < here;
+    } else if (b < rank) {
+      mine = mine && j >= of_block[b];
+      j -= of_block[b];
     }
   }
   // A bit for each of a piece's logits that has the value; 0 has two forms.
@@ -773,11 +778,29 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     for (int i = 0; i < 4; ++i) mask |= (equal[i] & 1u) << 2 * i | (equal[i] >> 31) << (2 * i + 1);
     return mask;
   };
-  if (mine && here == 1) {
-    r.each(begin, end, [&](const uint4 &v, uint32_t p) {
-      const uint32_t mask = matches(v);
-      if (mask) tokens[row] = static_cast<int32_t>(8 * p + __ffs(mask) - 1 - r.row.skipped);
-    });
+  if (mine && here <= kListed) {  // listed by the threads whose largest logit is not below it, then the j-th in the order of ids
+    uint32_t *const ids = reinterpret_cast<uint32_t *>(sh.list);
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    const auto list = [&](const uint4 &v, uint32_t p) {
+      for (uint32_t mask = matches(v); mask; mask &= mask - 1) {
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kListed) ids[at] = 8 * p + __ffs(mask) - 1 - r.row.skipped;
+      }
+    };
+    const bool may = top_of() >= key;
+    const uint32_t threads = __ballot_sync(kFullMask, may);
+    if (SIZE >= 4 || __popc(threads) > 4) {
+      if (may) r.each(begin, end, list);
+    } else {
+      over_lanes(threads, list);
+    }
+    __syncthreads();
+    const uint32_t id = threadIdx.x < here ? ids[threadIdx.x] : 0;
+    uint32_t lower = 0;
+    if (threadIdx.x < here)
+      for (uint32_t i = 0; i < here; ++i) lower += ids[i] < id;
+    if (threadIdx.x < here && lower == j) tokens[row] = static_cast<int32_t>(id);
   } else if (mine) {  // a run of pieces a warp, whose occurrences are counted first
     const uint32_t run = (end - begin + kWarps - 1) / kWarps, from = begin + warp * run, to = min(from + run, end);
     uint32_t n = 0;
