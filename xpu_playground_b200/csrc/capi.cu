@@ -115,7 +115,8 @@ static int check_fp8_rows(int dtype, const void *x, const void *other, uint64_t 
   XPU_REQUIRE(aligned4(scales), at + "scales must be 4-byte aligned");
   XPU_REQUIRE(dtype == XPU_BF16 || dtype == XPU_FP16, at + "dtype must be XPU_BF16 or XPU_FP16");
   XPU_REQUIRE(width > 0 && width % 16 == 0, at + "width must be a positive multiple of 16");
-  XPU_REQUIRE(rows < (1u << 31) && width < (1u << 31), at + "too many rows or columns");
+  XPU_REQUIRE(width < (1u << 31) && (static_cast<uint64_t>(width) + XPU_FP8_BLOCK - 1) / XPU_FP8_BLOCK * rows < (1ull << 31),
+              at + "too many rows or columns");
   XPU_REQUIRE(stride % 8 == 0 && stride >= width && stride < (1ull << 32), at + "row strides must be multiples of 8 elements and hold a row");
   return XPU_OK;
 }
