@@ -303,6 +303,14 @@ def tree_attention(cache, layer: int, sequences: torch.Tensor, starts: torch.Ten
 
 FP8 = torch.float8_e4m3fn
 FP8_BLOCK = 128  # columns of a row, and rows and columns of a weight, that share a scale
+_CODES = {torch.bfloat16: XPU_BF16, torch.float16: XPU_FP16}
+
+
+def _code(dtype: torch.dtype) -> int:
+    code = _CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {dtype}")
+    return code
 
 
 def _here(first: torch.Tensor, *others) -> None:
@@ -317,28 +325,26 @@ def _here(first: torch.Tensor, *others) -> None:
         raise ValueError("tensors must be on the current device")
 
 
-def _rows(name: str, t: torch.Tensor, width: int) -> int:
+def _row_stride(name: str, t: torch.Tensor, width: int) -> int:
     """Row stride of [rows, width] whose rows may stand apart."""
-    rows, columns = t.shape
-    if columns != width:
-        raise ValueError(f"{name} must have {width} columns, not {columns}")
+    if t.is_contiguous():
+        return width
     row, column = t.stride()
     if column != 1:
         raise ValueError(f"{name}: a row must be contiguous")
-    return row if rows > 1 else max(width, row)
+    return row if t.shape[0] > 1 else max(width, row)
 
 
-def _fp8_outputs(rows: int, width: int, device, q, scales, stream):
-    shape = (rows, width)
+def _fp8_outputs(rows: int, width: int, x, q, scales, stream):
     if q is None:
-        q = _allocate(torch.empty, stream, shape, dtype=FP8, device=device)
-    elif q.dtype != FP8 or q.shape != shape or not q.is_contiguous():
-        raise ValueError(f"q must be a contiguous float8_e4m3fn tensor {shape}")
-    shape = (-(-width // FP8_BLOCK), rows)
+        q = _allocate(torch.empty, stream, (rows, width), dtype=FP8, device=x.device)
+    elif q.dtype != FP8 or q.shape != (rows, width) or not q.is_contiguous():
+        raise ValueError(f"q must be a contiguous float8_e4m3fn tensor {(rows, width)}")
+    blocks = -(-width // FP8_BLOCK)
     if scales is None:
-        scales = _allocate(torch.empty, stream, shape, dtype=torch.float32, device=device)
-    elif scales.dtype != torch.float32 or scales.shape != shape or not scales.is_contiguous():
-        raise ValueError(f"scales must be a contiguous float32 tensor {shape}")
+        scales = _allocate(torch.empty, stream, (blocks, rows), dtype=torch.float32, device=x.device)
+    elif scales.dtype != torch.float32 or scales.shape != (blocks, rows) or not scales.is_contiguous():
+        raise ValueError(f"scales must be a contiguous float32 tensor {(blocks, rows)}")
     return q, scales
 
 
@@ -346,10 +352,10 @@ def fp8_quantize(x: torch.Tensor, q: torch.Tensor | None = None, scales: torch.T
     """Rows x [rows, width] in 8 bits (xpu_fp8_quantize): q [rows, width] and a
     scale for each 128 columns, scales [blocks, rows]. Returns (q, scales)."""
     rows, width = x.shape
-    dtype, stride = _dtype_code(x), _rows("x", x, width)
-    q, scales = _fp8_outputs(rows, width, x.device, q, scales, stream)
+    code, stride = _code(x.dtype), _row_stride("x", x, width)
+    q, scales = _fp8_outputs(rows, width, x, q, scales, stream)
     _here(x, q, scales)
-    call("xpu_fp8_quantize", dtype, x.data_ptr(), stride, q.data_ptr(), scales.data_ptr(), rows, width, _stream(stream))
+    call("xpu_fp8_quantize", code, x.data_ptr(), stride, q.data_ptr(), scales.data_ptr(), rows, width, _stream(stream))
     return q, scales
 
 
@@ -360,10 +366,11 @@ def fp8_silu_multiply(gate_up: torch.Tensor, q: torch.Tensor | None = None, scal
     if both % 2:
         raise ValueError("gate_up holds gate and up side by side")
     width = both // 2
-    dtype, stride, at = _dtype_code(gate_up), _rows("gate_up", gate_up, both), gate_up.data_ptr()
-    q, scales = _fp8_outputs(rows, width, gate_up.device, q, scales, stream)
+    code, stride = _code(gate_up.dtype), _row_stride("gate_up", gate_up, both)
+    q, scales = _fp8_outputs(rows, width, gate_up, q, scales, stream)
     _here(gate_up, q, scales)
-    call("xpu_fp8_silu_multiply", dtype, at, at + 2 * width, stride, q.data_ptr(), scales.data_ptr(), rows, width, _stream(stream))
+    at = gate_up.data_ptr()
+    call("xpu_fp8_silu_multiply", code, at, at + 2 * width, stride, q.data_ptr(), scales.data_ptr(), rows, width, _stream(stream))
     return q, scales
 
 
@@ -374,24 +381,25 @@ def fp8_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     norm's rows in 8 bits (xpu_fp8_rms_norm). Returns (total, q, scales) with
     total = x + residual; `total` may be x or residual, to be updated in place.
     Without a residual total is x."""
-    rows, width = x.shape
-    dtype, stride = _dtype_code(x), _rows("x", x, width)
-    if weight.dtype != x.dtype or weight.shape != (width,) or not weight.is_contiguous():
+    shape, dtype = x.shape, x.dtype
+    rows, width = shape
+    code, stride = _code(dtype), _row_stride("x", x, width)
+    if weight.dtype != dtype or weight.shape != (width,) or not weight.is_contiguous():
         raise ValueError(f"weight must be a contiguous tensor [{width}] of x's dtype")
     residual_at = residual_stride = total_at = total_stride = 0
     if residual is not None:
-        if residual.dtype != x.dtype or residual.shape != x.shape:
+        if residual.dtype != dtype or residual.shape != shape:
             raise ValueError("residual must have x's shape and dtype")
-        residual_at, residual_stride = residual.data_ptr(), _rows("residual", residual, width)
+        residual_at, residual_stride = residual.data_ptr(), _row_stride("residual", residual, width)
         if total is None:
-            total = _allocate(torch.empty, stream, rows, width, dtype=x.dtype, device=x.device)
+            total = _allocate(torch.empty, stream, rows, width, dtype=dtype, device=x.device)
     if total is not None:
-        if total.dtype != x.dtype or total.shape != x.shape:
+        if total.dtype != dtype or total.shape != shape:
             raise ValueError("total must have x's shape and dtype")
-        total_at, total_stride = total.data_ptr(), _rows("total", total, width)
-    q, scales = _fp8_outputs(rows, width, x.device, q, scales, stream)
+        total_at, total_stride = total.data_ptr(), _row_stride("total", total, width)
+    q, scales = _fp8_outputs(rows, width, x, q, scales, stream)
     _here(x, weight, residual, total, q, scales)
-    call("xpu_fp8_rms_norm", dtype, x.data_ptr(), stride, residual_at, residual_stride, weight.data_ptr(), epsilon, total_at,
+    call("xpu_fp8_rms_norm", code, x.data_ptr(), stride, residual_at, residual_stride, weight.data_ptr(), epsilon, total_at,
          total_stride, q.data_ptr(), scales.data_ptr(), rows, width, _stream(stream))
     return (x if total is None else total), q, scales
 
@@ -416,13 +424,14 @@ def fp8_gemm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales:
         out = _allocate(torch.empty, stream, m, n, dtype=dtype, device=a.device)
     elif out.shape != (m, n) or not out.is_contiguous():
         raise ValueError("fp8_gemm: out must be a contiguous tensor [m, n]")
+    code = _code(out.dtype)
     _here(a, a_scales, w, w_scales, out)
-    call("xpu_fp8_gemm", _dtype_code(out), a.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), m, n, k,
+    call("xpu_fp8_gemm", code, a.data_ptr(), a_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), m, n, k,
          _stream(stream))
     return out
 
 
-def _settings(name: str, t: torch.Tensor | None, dtype: torch.dtype, rows: int) -> int:
+def _per_row(name: str, t: torch.Tensor | None, dtype: torch.dtype, rows: int) -> int:
     if t is None:
         return 0
     if t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous():
@@ -437,17 +446,17 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | No
     in [0, 1), with each row's settings (xpu_sample): float32 temperature, top_p,
     min_p and int32 top_k of one entry a row. Returns (tokens, logprobs)."""
     rows, vocabulary = logits.shape
-    dtype, stride = _dtype_code(logits), _rows("logits", logits, vocabulary)
-    if tokens is None:
-        tokens = _allocate(torch.empty, stream, rows, dtype=torch.int32, device=logits.device)
-    if logprobs is None:
-        logprobs = _allocate(torch.empty, stream, rows, dtype=torch.float32, device=logits.device)
-    f, i = torch.float32, torch.int32
+    code, stride = _code(logits.dtype), _row_stride("logits", logits, vocabulary)
     if u is None:
         raise ValueError("u needs a random number a row")
+    f, i = torch.float32, torch.int32
+    settings = (_per_row("temperature", temperature, f, rows), _per_row("top_k", top_k, i, rows), _per_row("top_p", top_p, f, rows),
+                _per_row("min_p", min_p, f, rows), _per_row("u", u, f, rows))
+    if tokens is None:
+        tokens = _allocate(torch.empty, stream, rows, dtype=i, device=logits.device)
+    if logprobs is None:
+        logprobs = _allocate(torch.empty, stream, rows, dtype=f, device=logits.device)
+    outputs = _per_row("tokens", tokens, i, rows), _per_row("logprobs", logprobs, f, rows)
     _here(logits, u, temperature, top_k, top_p, min_p, tokens, logprobs)
-    call("xpu_sample", dtype, logits.data_ptr(), stride, _settings("temperature", temperature, f, rows),
-         _settings("top_k", top_k, i, rows), _settings("top_p", top_p, f, rows), _settings("min_p", min_p, f, rows),
-         _settings("u", u, f, rows), _settings("tokens", tokens, i, rows), _settings("logprobs", logprobs, f, rows), rows,
-         vocabulary, _stream(stream))
+    call("xpu_sample", code, logits.data_ptr(), stride, *settings, *outputs, rows, vocabulary, _stream(stream))
     return tokens, logprobs
