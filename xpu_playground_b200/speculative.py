@@ -1,4 +1,4 @@
-"""Speculative greedy decoding over the paged cache: the serving operators together.
+"""Speculative decoding over the paged cache: the serving operators together.
 
 A Qwen3 of any preset, with the engine's seeded synthetic weights, serves several
 prompts at once: the prompts go through each layer packed
@@ -11,9 +11,17 @@ frees sequences that are done (``KvCache.trim``, ``KvCache.compact``). Drafts co
 from the sequence's own text: what followed the last occurrences of its newest
 token. With ``width`` 0 a tree is one node and the loop is plain greedy decoding;
 drafts change how many steps it takes, not the tokens (up to logits that differ
-by no more than their rounding).
+by no more than their rounding). With a ``Sampling`` every token is drawn
+(``kernels.sample``) instead, from a random number of its own sequence and position, so
+that drafts do not change it either: a drafted token stands where it is the one drawn.
+
+With ``eight_bits`` the projections are held and multiplied in 8 bits: the residual's
+addition and the norm (``kernels.fp8_rms_norm``), the attention's output
+(``kernels.fp8_quantize``) and the gated activation (``kernels.fp8_silu_multiply``) leave
+as 8-bit rows, which enter ``kernels.fp8_gemm``.
 
     python -m xpu_playground_b200.speculative --preset tiny --prompts 3 --new-tokens 48
+    python -m xpu_playground_b200.speculative --eight-bits --temperature 0.7 --top-k 20 --top-p 0.95
 """
 
 from __future__ import annotations
@@ -26,6 +34,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _lib, kernels
+from .fp8 import Fp8Weight
 from .kv_cache import KvCache
 from .qwen3_config import HEAD_DIM, PRESETS, WEIGHT_STD, Qwen3Shape
 
@@ -45,9 +54,10 @@ def synthetic_weights(shape: Qwen3Shape, seed: int, std: float = WEIGHT_STD) -> 
 
 
 class PagedQwen3:
-    """The decoder over packed tokens, its attention given by the caller."""
+    """The decoder over packed tokens, its attention given by the caller. eight_bits:
+    projections in 8 bits (embedding, norms, rotation and attention stay bf16)."""
 
-    def __init__(self, shape: Qwen3Shape, weights: dict[str, torch.Tensor], max_positions: int):
+    def __init__(self, shape: Qwen3Shape, weights: dict[str, torch.Tensor], max_positions: int, eight_bits: bool = False):
         self.shape, self.embed = shape, weights["model.embed_tokens.weight"]
         self.norm = weights["model.norm.weight"]
         self.lm_head = self.embed if shape.tied else weights["lm_head.weight"]
@@ -58,7 +68,12 @@ class PagedQwen3:
                 "self_attn.o_proj", "self_attn.q_norm", "self_attn.k_norm", "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")}
             w["qkv"] = torch.cat([w.pop(f"self_attn.{x}_proj") for x in "qkv"])
             w["gate_up"] = torch.cat([w.pop("mlp.gate_proj"), w.pop("mlp.up_proj")])
+            if eight_bits:
+                w |= {k: Fp8Weight(w[k]) for k in ("qkv", "self_attn.o_proj", "gate_up", "mlp.down_proj")}
             self.layers.append(w)
+        self.eight_bits = eight_bits
+        if eight_bits:
+            self.lm_head = Fp8Weight(self.lm_head)
         inverse = 1.0 / shape.rope_theta ** (torch.arange(0, HEAD_DIM, 2, device="cuda").float() / HEAD_DIM)
         angle = torch.arange(max_positions, device="cuda").float()[:, None] * inverse
         self.cos, self.sin = (torch.cat([f(angle)] * 2, 1).bfloat16() for f in (torch.cos, torch.sin))
@@ -73,19 +88,47 @@ class PagedQwen3:
 
     def forward(self, tokens, positions, attend):
         """Logits of packed tokens; attend(layer, q, k, v) -> [tokens, q_heads, head_dim]."""
+        if self.eight_bits:
+            return self._forward_eight_bits(tokens, positions, attend)
         s = self.shape
         x = self.embed[tokens]
         for i, w in enumerate(self.layers):
-            qkv = kernels.gemm_bt(self._rms(x, w["input_layernorm"]), w["qkv"]).view(-1, s.q_heads + 2 * s.kv_heads, HEAD_DIM)
-            q, k, v = qkv.split([s.q_heads, s.kv_heads, s.kv_heads], 1)
-            q = self._rope(self._rms(q, w["self_attn.q_norm"]), positions)
-            k = self._rope(self._rms(k, w["self_attn.k_norm"]), positions)
-            out = attend(i, q, k, v.contiguous())
-            x = x + kernels.gemm_bt(out.reshape(len(tokens), -1), w["self_attn.o_proj"])
+            qkv = kernels.gemm_bt(self._rms(x, w["input_layernorm"]), w["qkv"])
+            out = self._heads(i, w, qkv, positions, attend)
+            x = x + kernels.gemm_bt(out, w["self_attn.o_proj"])
             gate, up = kernels.gemm_bt(self._rms(x, w["post_attention_layernorm"]), w["gate_up"]).chunk(2, 1)
             h = (torch.nn.functional.silu(gate.float()).bfloat16() * up).contiguous()
             x = x + kernels.gemm_bt(h, w["mlp.down_proj"])
         return kernels.gemm_bt(self._rms(x, self.norm), self.lm_head)
+
+    def _heads(self, layer, w, qkv, positions, attend):
+        """Norms and rotation of the heads, and their attention: [tokens, q_heads * head_dim]."""
+        s = self.shape
+        q, k, v = qkv.view(-1, s.q_heads + 2 * s.kv_heads, HEAD_DIM).split([s.q_heads, s.kv_heads, s.kv_heads], 1)
+        q = self._rope(self._rms(q, w["self_attn.q_norm"]), positions)
+        k = self._rope(self._rms(k, w["self_attn.k_norm"]), positions)
+        return attend(layer, q, k, v.contiguous()).reshape(len(qkv), -1)
+
+    def _forward_eight_bits(self, tokens, positions, attend):
+        eps, x, residual = self.shape.eps, self.embed[tokens], None
+        for i, w in enumerate(self.layers):
+            residual, *rows = kernels.fp8_rms_norm(x, w["input_layernorm"], residual, eps, total=residual)
+            out = self._heads(i, w, w["qkv"](rows), positions, attend)
+            x = w["self_attn.o_proj"](kernels.fp8_quantize(out))
+            residual, *rows = kernels.fp8_rms_norm(x, w["post_attention_layernorm"], residual, eps, total=residual)
+            x = w["mlp.down_proj"](kernels.fp8_silu_multiply(w["gate_up"](rows)))
+        return self.lm_head(kernels.fp8_rms_norm(x, self.norm, residual, eps, total=residual)[1:])
+
+
+@dataclass
+class Sampling:
+    """How tokens are drawn (kernels.sample), for every sequence of a server."""
+
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int = 0
 
 
 @dataclass
@@ -149,10 +192,28 @@ def _starts(counts) -> list[int]:
 
 
 class Server:
-    def __init__(self, model: PagedQwen3, pages: int, page_size: int, sequences: int, max_positions: int):
+    def __init__(self, model: PagedQwen3, pages: int, page_size: int, sequences: int, max_positions: int,
+                 sampling: Sampling | None = None):
         s = model.shape
-        self.model, self.steps, self.emitted = model, 0, 0
+        self.model, self.steps, self.emitted, self.sampling = model, 0, 0, sampling
+        if sampling is not None:  # one random number for what follows each position of each sequence
+            g = torch.Generator(device="cuda").manual_seed(sampling.seed)
+            self.u = torch.rand(sequences, max_positions, device="cuda", generator=g)
         self.cache = KvCache(s.layers, pages, page_size, s.kv_heads, HEAD_DIM, sequences, max_positions)
+
+    def choose(self, logits: torch.Tensor, sequences: list[int], positions: list[int]) -> list[int]:
+        """The token after each row's position: the likeliest, or one drawn."""
+        if self.sampling is None:
+            return logits.argmax(-1).tolist()
+        a, rows = self.sampling, len(sequences)
+        last = self.u.shape[1] - 1  # a tree may be drafted past the room there is; the cache refuses such tokens
+        u = self.u[torch.tensor(sequences, device="cuda"), torch.tensor([min(p, last) for p in positions], device="cuda")]
+        full = lambda v, dtype=torch.float32: torch.full((rows,), v, dtype=dtype, device="cuda")  # noqa: E731
+        tokens, _ = kernels.sample(logits, u, full(a.temperature), full(a.top_k, torch.int32), full(a.top_p), full(a.min_p))
+        chosen = tokens.tolist()
+        if min(chosen) < 0:
+            raise RuntimeError("a row of logits has nothing to choose from, or the sampling's settings are out of range")
+        return chosen
 
     def prefill(self, prompts: list[list[int]], sequences: list[int]) -> torch.Tensor:
         """Packed prompts into empty sequences; the logits after each."""
@@ -172,7 +233,7 @@ class Server:
         return self.model.forward(tokens, positions, attend)[torch.tensor(starts[1:], device="cuda") - 1]
 
     def verify(self, texts: list[list[int]], sequences: list[int], trees: list[Tree], workspace) -> list[list[int]]:
-        """One forward pass of every sequence's tree; appends what greedy decoding would have
+        """One forward pass of every sequence's tree; appends what plain decoding would have
         taken to cache and texts, and returns the new tokens."""
         s, cache = self.model.shape, self.cache
         counts = [len(t.tokens) for t in trees]
@@ -185,14 +246,15 @@ class Server:
             return kernels.tree_attention(cache, layer, ids, offsets, sets, q, k, v, workspace)[0]
 
         tokens = torch.tensor([x for t in trees for x in t.tokens], device="cuda")
-        positions = torch.tensor([len(text) - 1 + d for text, t in zip(texts, trees) for d in t.depths()], device="cuda")
-        greedy = self.model.forward(tokens, positions, attend).argmax(-1).tolist()
+        places = [len(text) - 1 + d for text, t in zip(texts, trees) for d in t.depths()]
+        logits = self.model.forward(tokens, torch.tensor(places, device="cuda"), attend)
+        chosen = self.choose(logits, [i for i, n in zip(sequences, counts) for _ in range(n)], places)
         rows, taken, new = [], [], []
         for begin, text, tree in zip(starts, texts, trees):
             node, out, path = 0, [], []
             while node is not None:  # node's token stands; what follows it is known now
                 path.append(begin + node)
-                out.append(greedy[begin + node])
+                out.append(chosen[begin + node])
                 node = tree.child(node, out[-1])
             rows += path
             taken.append(len(path))
@@ -205,18 +267,22 @@ class Server:
 
     def generate(self, prompts: list[list[int]], new_tokens: int, samples: int = 1, width: int = 4,
                  depth: int = 6) -> list[list[list[int]]]:
-        """`samples` continuations of each prompt, of new_tokens tokens: sample i begins with the
-        prompt's i-th most likely next token and goes on greedily."""
+        """`samples` continuations of each prompt, of new_tokens tokens: drawn ones with a Sampling; else
+        sample i begins with the prompt's i-th most likely next token and goes on greedily."""
         if not all(prompts):
             raise ValueError("a prompt needs at least one token")
         s, cache, many = self.model.shape, self.cache, len(prompts)
-        first = self.prefill(prompts, list(range(many))).topk(samples, -1).indices.tolist()
+        logits = self.prefill(prompts, list(range(many)))
         owners = [p for p in range(many) for _ in range(samples)]
         if samples > 1:
             children = [many + i for i in range(many * (samples - 1))]
             cache.fork(_ints(p for p in range(many) for _ in range(samples - 1)), _ints(children))
         slots = [p if i == 0 else many + p * (samples - 1) + i - 1 for p in range(many) for i in range(samples)]
-        texts = [list(prompts[p]) + [first[p][i % samples]] for i, p in enumerate(owners)]
+        if self.sampling is None:
+            first = logits.topk(samples, -1).indices.flatten().tolist()
+        else:
+            first = self.choose(logits.repeat_interleave(samples, 0), slots, [len(prompts[p]) - 1 for p in owners])
+        texts = [list(prompts[p]) + [first[i]] for i, p in enumerate(owners)]
         live = list(range(len(texts)))
         workspace = kernels.tree_attention_workspace(len(texts), 64 * len(texts), s.q_heads, s.kv_heads, HEAD_DIM)
         while live:
@@ -246,12 +312,18 @@ def main(argv=None) -> int:
     ap.add_argument("--width", type=int, default=4, help="drafted continuations a step, 0: plain decoding")
     ap.add_argument("--depth", type=int, default=6, help="tokens of each")
     ap.add_argument("--page-size", type=int, default=16)
+    ap.add_argument("--eight-bits", action="store_true", help="projections in 8 bits")
+    ap.add_argument("--temperature", type=float, help="draw tokens (default: the likeliest)")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     a = ap.parse_args(argv)
     shape = PRESETS[a.preset]
     room = a.prompt_len + a.new_tokens + a.depth + 2
-    model = PagedQwen3(shape, synthetic_weights(shape, a.seed), room)
+    model = PagedQwen3(shape, synthetic_weights(shape, a.seed), room, a.eight_bits)
+    sampling = None if a.temperature is None else Sampling(a.temperature, a.top_k, a.top_p, a.min_p, a.seed)
     sequences = a.prompts * a.samples
-    server = Server(model, sequences * -(-room // a.page_size), a.page_size, sequences, room)
+    server = Server(model, sequences * -(-room // a.page_size), a.page_size, sequences, room, sampling)
     g = torch.Generator().manual_seed(a.seed)
     prompts = [torch.randint(shape.vocab, (max(1, a.prompt_len - 7 * i),), generator=g).tolist() for i in range(a.prompts)]
     torch.cuda.synchronize()
