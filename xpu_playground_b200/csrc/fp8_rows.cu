@@ -17,7 +17,8 @@ namespace xpu {
 namespace {
 
 constexpr uint32_t kGroup = XPU_FP8_BLOCK, kLanes = kGroup / 8;  // lanes of a group
-constexpr uint32_t kAtOnce = 3, kHalves = 16;           // groups a half warp takes at once, half warps a block
+constexpr uint32_t kHalves = 16;                        // half warps a block
+__host__ __device__ constexpr uint32_t at_once(bool gated) { return gated ? 2 : 3; }  // groups a half warp takes at once
 constexpr float kLargest = 448.f, kSmallestScale = 1.17549435e-38f;
 
 // 16 bytes of a row that is read once, behind the wait for the kernel before.
@@ -40,15 +41,42 @@ __device__ __forceinline__ void widen(const uint4 &v, float (&y)[8]) {
   }
 }
 
-// Scale and 8-bit values of a group that 16 lanes hold, 8 columns each. One true division for the
-// scale and one for its reciprocal; y * (1 / s) is within 2^-23 of y / s.
+// Two FP32 values rounded to T, side by side.
+template <typename T>
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t narrow2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t narrow2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+// The special function unit's reciprocal and power of two, off by 2^-23 and 2^-22; subnormal numbers are 0.
+__device__ __forceinline__ float fast_reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Scale and 8-bit values of a group that 16 lanes hold, 8 columns each. The instructions bound these kernels beside the memory
+// (24 a value with true divisions), so the scale is a product with 1 / 448, within 2^-23 of the quotient, and a value a product
+// with the scale's fast reciprocal, within 2^-22 of its quotient; e4m3 keeps 2^-4.
 __device__ __forceinline__ float encode(const float (&y)[8], uint2 *q) {
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(y[i]));
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-  const float scale = fmaxf(top / kLargest, kSmallestScale), inverse = 1.f / scale;
+  const float scale = fmaxf(top * (1.f / kLargest), kSmallestScale), inverse = fast_reciprocal(scale);
   uint32_t half[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -59,17 +87,18 @@ __device__ __forceinline__ float encode(const float (&y)[8], uint2 *q) {
 
 // ------------------------------------------------- plain and gated rows ----
 
-// silu(g) u. The fast exponential and division are within 2^-16 for every g whose result is not below the
-// smallest normal number; the 8 bits keep 2^-4, the scales' use of it 2^-16 too.
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// silu(g) u = g u / (1 + 2^(-g log2 e)). The exponent's rounding is 2^-24 of itself, so results are within 2^-16 down to g =
+// -87, below which 1 + 2^x passes 2^126 and its reciprocal is 0: then so is the result, less than 1e-36 u.
+__device__ __forceinline__ float gated(float g, float u) { return g * fast_reciprocal(1.f + fast_exp2(g * -1.4426950408889634f)) * u; }
 
 // A half warp takes kAtOnce groups, so that as many loads are in flight, a block 16 kAtOnce in the order of rows and columns.
-// 8192 x 12288 gated 89 us (5.7 TB/s; 91 with two groups, 99 with one; 114 with a loop over resident blocks, whose
-// last turn leaves some idle), plain 8192 x 4096 20.5 us (4.9 TB/s, from the L2 in part). Blocks of 16 rows, whose
-// scales are side by side, were no faster.
+// 8192 x 12288 gated: fp16 80 us (6.3 TB/s), bf16 83; 84 with three groups, 85 with four, 99 with one; 114 with a loop over
+// resident blocks, whose last turn leaves some idle. Plain 8192 x 4096: 17.6 us (5.7 TB/s, from the L2 in part).
+// Blocks of 16 rows, whose scales are side by side, were no faster.
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(16 * kHalves) k_fp8_rows(const uint16_t *x, const uint16_t *up, uint64_t stride, uint8_t *q,
                                                   float *scales, uint32_t rows, uint32_t width) {
+  constexpr uint32_t kAtOnce = at_once(GATED);
   grid_dep_launch();
   grid_dep_wait();
   const uint32_t groups = (width + kGroup - 1) / kGroup, lane = threadIdx.x % kLanes, half = threadIdx.x / kLanes;
@@ -149,8 +178,7 @@ __global__ void __launch_bounds__(1024) k_fp8_rms_norm(const uint16_t *x, uint64
       uint32_t u[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const T lo = Elem<T>::from_float(a[2 * i] + b[2 * i]), hi = Elem<T>::from_float(a[2 * i + 1] + b[2 * i + 1]);
-        u[i] = *reinterpret_cast<const uint16_t *>(&lo) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&hi)) << 16;
+        u[i] = narrow2<T>(a[2 * i] + b[2 * i], a[2 * i + 1] + b[2 * i + 1]);
       }
       t[c] = make_uint4(u[0], u[1], u[2], u[3]);
     }
@@ -203,8 +231,8 @@ cudaError_t norm_launch(const Fp8Norm &n, cudaStream_t s) {
                         n.total_stride, n.q, n.scales, n.rows, n.width, n.epsilon);
   };
   // Few rows: the most threads, for the latency (64 x 4096 2.5 us, 2.7 with two pieces a thread, 3.4 with four). Many: blocks of
-  // about 256 threads, so that several are resident and one's sum is another's load (8192 x 4096 40.4 us, 5.8 TB/s, with
-  // two pieces, 43.2 with one, 41.0 with four; 2048 x 12288 36.5 with four, 43.8 with two).
+  // about 256 threads, so that several are resident and one's sum is another's load (8192 x 4096 39.5 us, 5.9 TB/s, with
+  // two pieces, 3 more with one; 2048 x 12288 33.4 with four, 7 more with two).
   const bool many = n.rows > 2 * sm_count();
   if (pieces <= 256 || (!many && pieces <= 1024)) return go(k_fp8_rms_norm<T, 1>, 1);
   if (pieces <= 512 || (!many && pieces <= 2048)) return go(k_fp8_rms_norm<T, 2>, 2);
@@ -215,7 +243,7 @@ cudaError_t norm_launch(const Fp8Norm &n, cudaStream_t s) {
 
 cudaError_t fp8_rows_launch(bool fp16, const uint16_t *x, const uint16_t *up, uint64_t stride, uint8_t *q, float *scales,
                             uint32_t rows, uint32_t width, cudaStream_t s) {
-  const uint32_t halves = (width + kGroup - 1) / kGroup * rows, each = kHalves * kAtOnce;
+  const uint32_t halves = (width + kGroup - 1) / kGroup * rows, each = kHalves * at_once(up != nullptr);
   const uint32_t blocks = halves / each + (halves % each != 0);
   const auto go = [&](auto kernel) { return launch_after(kernel, blocks, 16 * kHalves, 0, s, x, up, stride, q, scales, rows, width); };
   if (fp16) return up ? go(k_fp8_rows<__half, true>) : go(k_fp8_rows<__half, false>);
