@@ -33,6 +33,9 @@ constexpr uint32_t kKeys = 65536, kGroups = kKeys / 32;
 constexpr uint32_t kSmem = kKeys * 2;
 constexpr uint32_t kMostListed = 256;  // top-k up to which the largest logits are looked for first
 constexpr uint32_t kListed = kThreads;
+// Groups up to which a warp takes one at a time: 6200 cycles for 100 (bf16), 28000 for 1000 (fp16), where a thread each takes
+// 10500 for up to 1024.
+constexpr uint32_t kMostGroups = 192;
 constexpr int kHeld = 5, kBatch = 4;  // pieces of 8 logits a thread holds of its block's run, or has in flight
 static_assert(kHeld * kThreads * 8 < 65536, "counters of a held run do not overflow");
 constexpr uint32_t kHeavy = 2 * XPU_SAMPLE_MAX_VOCABULARY / 32768 + 1;
@@ -605,23 +608,50 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     if (has[0] >> lane & 1) sh.groups[(earlier & 0xffffu) + below[0]] = static_cast<uint16_t>(threadIdx.x);
     if (has[1] >> lane & 1) sh.groups[(both & 0xffffu) + (earlier >> 16) + below[1]] = static_cast<uint16_t>(1024 + threadIdx.x);
     __syncthreads();
-    for (uint32_t i = warp * SIZE + rank; i < groups; i += kWarps * SIZE) {
-      const uint32_t g = sh.groups[i], key = 32 * g + lane;
-      uint32_t n = 0;
-#pragma unroll
-      for (int b = 0; b < SIZE; ++b) n += occurrences<SIZE>(histogram, &sh, key, b, any_heavy);
-      double mass = n ? n * exp(log_weight(key)) : 0.0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
-      n = __reduce_add_sync(kFullMask, n);
-      if (lane == 0) {
-        if (SIZE == 1) {
-          sh.counts[groups - 1 - i] = n;
-          sh.masses[groups - 1 - i] = mass;
-        } else {
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.counts[groups - 1 - i], 0)), "r"(n) : "memory");
-          asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&sh.masses[groups - 1 - i], 0)), "d"(mass) : "memory");
+    const auto put = [&](uint32_t i, uint32_t n, double mass) {
+      if (SIZE == 1) {
+        sh.counts[groups - 1 - i] = n;
+        sh.masses[groups - 1 - i] = mass;
+      } else {
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.counts[groups - 1 - i], 0)), "r"(n) : "memory");
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(cluster_addr(&sh.masses[groups - 1 - i], 0)), "d"(mass) : "memory");
+      }
+    };
+    if (SIZE == 1 && groups > kMostGroups) {
+      // A thread a group: its values are evenly spaced, its weights a geometric series, w n_e + w r n_(e-1) + .. = w (n_e + r
+      // (n_(e-1) + ..)) from its highest value e down, taken upwards from another value in each lane (banks): the part from
+      // there to e, and the part below it times its power of r. e is the largest logit in its own group, whose weight is 1.
+      for (uint32_t i = warp + kWarps * lane; i < groups; i += kThreads) {
+        const uint32_t g = sh.groups[i], last = g == top / 32 ? top % 32 : 31, highest = 32 * g + last;
+        const double ratio = exp((value_of<T>(highest - 1) - value_of<T>(highest)) * slope);
+        double sum = 0.0, upper = 0.0;
+        uint32_t many = 0;
+#pragma unroll 4
+        for (uint32_t k = 0; k < 32; ++k) {
+          const uint32_t at = (lane + k) & 31;
+          if (at == 0) upper = sum, sum = 0.0;
+          const uint32_t n = occurrences<SIZE>(histogram, &sh, 32 * g + at, 0, any_heavy);
+          many += n;
+          if (at <= last) sum = fma(sum, ratio, __hiloint2double(0x43300000, static_cast<int>(n)) - 4503599627370496.0);  // 2^52 + n
         }
+        double power = 1.0, factor = ratio;
+        for (uint32_t left = lane && lane <= last ? last + 1 - lane : 0; left; left /= 2) {
+          if (left & 1) power *= factor;
+          factor *= factor;
+        }
+        put(i, many, exp(log_weight(highest)) * fma(sum, power, upper));
+      }
+    } else {
+      for (uint32_t i = warp * SIZE + rank; i < groups; i += kWarps * SIZE) {
+        const uint32_t key = 32 * sh.groups[i] + lane;
+        uint32_t n = 0;
+#pragma unroll
+        for (int b = 0; b < SIZE; ++b) n += occurrences<SIZE>(histogram, &sh, key, b, any_heavy);
+        double mass = n ? n * exp(log_weight(key)) : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
+        n = __reduce_add_sync(kFullMask, n);
+        if (lane == 0) put(i, n, mass);
       }
     }
     row_sync<SIZE>();
