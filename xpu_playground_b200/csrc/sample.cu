@@ -51,12 +51,33 @@ template <typename T>
 struct Keys;
 template <>
 struct Keys<__nv_bfloat16> {
-  static constexpr uint32_t kMinusInf = 0x007f, kPlusInf = 0xff80, kMask = 0xff80ff80u;  // two bits patterns of -inf
+  using Two = __nv_bfloat162;
+  static constexpr uint32_t kMinusInf = 0x007f, kPlusInf = 0xff80;
+  static constexpr uint32_t kMask = 0xff80ff80u, kLowest2 = 0xff7fff7fu;  // two of -inf, and of the lowest finite value
 };
 template <>
 struct Keys<__half> {
-  static constexpr uint32_t kMinusInf = 0x03ff, kPlusInf = 0xfc00, kMask = 0xfc00fc00u;
+  using Two = __half2;
+  static constexpr uint32_t kMinusInf = 0x03ff, kPlusInf = 0xfc00;
+  static constexpr uint32_t kMask = 0xfc00fc00u, kLowest2 = 0xfbfffbffu;
 };
+
+template <typename T>
+__device__ __forceinline__ typename Keys<T>::Two as_two(uint32_t word) {
+  return *reinterpret_cast<const typename Keys<T>::Two *>(&word);
+}
+// The larger of each half; NaN if one is.
+template <typename T>
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+  const typename Keys<T>::Two v = __hmax2_nan(as_two<T>(a), as_two<T>(b));
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+// Whether all of a piece's logits are above the lowest finite value.
+template <typename T>
+__device__ __forceinline__ bool all_above_lowest(const uint4 &v) {
+  const auto least = __hmin2(__hmin2(as_two<T>(v.x), as_two<T>(v.y)), __hmin2(as_two<T>(v.z), as_two<T>(v.w)));
+  return __hbgt2(least, as_two<T>(Keys<T>::kLowest2));
+}
 
 template <typename T>
 __device__ __forceinline__ double value_of(uint32_t key) {
@@ -144,12 +165,6 @@ __device__ __forceinline__ uint32_t element(const uint4 &v, int i) {
   return u[i / 2] >> (16 * (i % 2)) & 0xffffu;
 }
 
-// Two keys of a word at once, without the case of -0.
-__device__ __forceinline__ uint32_t two_keys(uint32_t word) {
-  const uint32_t negative = word >> 15 & 0x00010001u;
-  return word ^ ((negative << 16) - negative | 0x80008000u);
-}
-
 struct Shared {
   uint32_t counts[kGroups];  // logits of each group that is not empty, falling; then of the groups before it
   double masses[kGroups];    // likewise their weights
@@ -157,7 +172,7 @@ struct Shared {
     uint16_t groups[kGroups];  // those that are not empty
     uint64_t list[kListed];    // key << 32 | ~id of what can be among the first k
   };
-  uint32_t occupied[2][kWarps];  // groups that have values in this block's run: of negative ones, of the others
+  uint32_t occupied[2][kWarps];  // 32 magnitudes each that this block's run has: of positive values, of negative ones
   double warp_mass[kWarps];
   uint32_t warp_count[kWarps];
   uint32_t heavy_key[kHeavy], heavy_count[kHeavy], heavies;
@@ -174,8 +189,9 @@ __device__ __forceinline__ void row_sync() {
   else cluster_sync();
 }
 
-// Place of a value's 16-bit counter: neighbours in words of their own.
-__device__ __forceinline__ uint32_t counter(uint32_t key) { return (key & 0x7fffu) << 1 | key >> 15; }
+// Place of a value's 16-bit counter: a word for each magnitude, its lower half for the positive value, so that values side by side
+// have words of their own and counting needs no order.
+__device__ __forceinline__ uint32_t counter(uint32_t key) { return key & 0x8000u ? (key & 0x7fffu) << 1 : (key ^ 0x7fffu) << 1 | 1; }
 
 // Occurrences of a value in block r's run.
 template <int SIZE>
@@ -314,20 +330,9 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   const double slope = greedy ? 1.0 : 1.0 / static_cast<double>(temperature);
   const uint32_t begin = r.begin, end = r.end;
 
-  // Largest and smallest key of two, over this thread's pieces.
-  uint32_t most2 = 0, least2 = ~0u;
-  const auto look = [&](const uint4 &v, uint32_t (&keys)[4]) {
-    keys[0] = two_keys(v.x), keys[1] = two_keys(v.y), keys[2] = two_keys(v.z), keys[3] = two_keys(v.w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      most2 = __vmaxu2(most2, keys[i]);
-      least2 = __vminu2(least2, keys[i]);
-    }
-  };
-  const auto top_of = [&] {
-    const uint32_t top = max(most2 & 0xffffu, most2 >> 16);
-    return top == 0x7fffu ? 0x8000u : top;  // -0 is 0
-  };
+  uint32_t most2 = Keys<T>::kMask;  // the largest of this thread's logits, in each half
+  const auto look = [&](const uint4 &v) { most2 = larger2<T>(larger2<T>(most2, larger2<T>(v.x, v.y)), larger2<T>(v.z, v.w)); };
+  const auto top_of = [&] { return max(key_of(most2 & 0xffffu), key_of(most2 >> 16)); };
   // use(piece, its number) for the pieces of some of the warp's threads, spread over its lanes.
   const auto over_lanes = [&](uint32_t threads, auto use) {
     const uint32_t turns = (end - begin + kThreads - 1) / kThreads, items = __popc(threads) * turns;
@@ -338,13 +343,10 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       if (p < end) use(r.row.piece(p), p);
     }
   };
-  const auto is_bad = [&] { return top_of() >= Keys<T>::kPlusInf || min(least2 & 0xffffu, least2 >> 16) < Keys<T>::kMinusInf; };
+  const auto is_bad = [&] { return top_of() >= Keys<T>::kPlusInf; };  // the NaN of a maximum is positive
 
   if (most <= kMostListed) {
-    r.each(begin, end, [&](const uint4 &v, uint32_t) {
-      uint32_t keys[4];
-      look(v, keys);
-    });
+    r.each(begin, end, [&](const uint4 &v, uint32_t) { look(v); });
     const uint32_t mine = top_of();
     if (mine > Keys<T>::kMinusInf) atomicAdd(&sh.counts[mine / 32], 1u);
     const bool any_bad = __syncthreads_or(is_bad());
@@ -451,30 +453,24 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   constexpr uint32_t kLowest = Keys<T>::kMinusInf + 1;  // the lowest finite value masks too: counted without the histogram
 
   uint32_t counted = 0, lowest = 0;
-  const auto add = [&](uint32_t key_at_top) {  // a key in the upper half of a word
-    atomicAdd(reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(histogram) + (key_at_top >> 14 & 0x1fffcu)),
-              static_cast<int32_t>(key_at_top) < 0 ? 0x10000u : 1u);
+  const auto add = [&](uint32_t at_top) {  // a logit in the upper half of a word
+    atomicAdd(reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(histogram) + (at_top >> 14 & 0x1fffcu)),
+              static_cast<int32_t>(at_top) < 0 ? 0x10000u : 1u);
   };
   const auto count = [&](uint32_t from, uint32_t to) {
     r.each(from, to, [&](const uint4 &v, uint32_t) {
-      uint32_t keys[4];
-      look(v, keys);
-      const uint32_t least = __vminu2(__vminu2(keys[0], keys[1]), __vminu2(keys[2], keys[3]));
-      if (min(least & 0xffffu, least >> 16) > kLowest) {
+      look(v);
+      if (all_above_lowest<T>(v)) {
         counted += 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          add(keys[i] << 16);
-          add(keys[i]);
-        }
+        add(v.x << 16), add(v.x), add(v.y << 16), add(v.y), add(v.z << 16), add(v.z), add(v.w << 16), add(v.w);
         return;
       }
 #pragma unroll 1
       for (int i = 0; i < 8; ++i) {
-        const uint32_t word = i < 4 ? (i < 2 ? keys[0] : keys[1]) : (i < 6 ? keys[2] : keys[3]), key = word >> (16 * (i % 2)) & 0xffffu;
+        const uint32_t word = i < 4 ? (i < 2 ? v.x : v.y) : (i < 6 ? v.z : v.w), bits = word >> (16 * (i % 2)) & 0xffffu, key = key_of(bits);
         if (key > kLowest) {
           ++counted;
-          add(key << 16);
+          add(bits << 16);
         } else if (key == kLowest) {
           ++lowest;
         }
@@ -513,7 +509,8 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
           sh.heavy_count[at] = *held;
           *held = 0;
           const uint32_t key = i == 0x7fff ? 0x8000 : i;
-          atomicOr(&sh.occupied[key >> 15][key / 1024 & 31], 1u << (key / 32 & 31));
+          const uint32_t magnitudes = counter(key) / 64;
+          atomicOr(&sh.occupied[counter(key) & 1][magnitudes / 32], 1u << (magnitudes & 31));
         }
         __syncthreads();
       }
@@ -539,7 +536,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   if (sh.heavies && threadIdx.x < sh.heavies && sh.heavy_key[threadIdx.x] == 0x7fff) sh.heavy_key[threadIdx.x] = 0x8000;
   __syncthreads();
   {
-    // Groups with values: thread i looks at groups i (lower halves) and 1024 + i, from another 16 bytes on in each lane (banks).
+    // Thread i looks at 32 magnitudes, from another 16 bytes on in each lane (banks).
     uint32_t has[2] = {0, 0};
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
@@ -557,7 +554,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   __syncthreads();
   if (threadIdx.x == 0 && sh.heavy_count[0]) {
     sh.heavies = max(sh.heavies, 1u);
-    sh.occupied[0][kLowest / 1024] |= 1u << (kLowest / 32 & 31);
+    sh.occupied[1][counter(kLowest) / 64 / 32] |= 1u << (counter(kLowest) / 64 & 31);
   }
   if (SIZE > 1 && threadIdx.x < SIZE && threadIdx.x != rank) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.top[rank], threadIdx.x)), "r"(sh.top[rank]) : "memory");
@@ -604,9 +601,9 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
     if (lane == 0) sh.warp_count[warp] = __popc(has[0]) | __popc(has[1]) << 16;
     __syncthreads();
     const uint32_t of_warp = sh.warp_count[lane], earlier = __reduce_add_sync(kFullMask, lane < warp ? of_warp : 0);
-    const uint32_t both = __reduce_add_sync(kFullMask, of_warp), groups = (both & 0xffffu) + (both >> 16);
-    if (has[0] >> lane & 1) sh.groups[(earlier & 0xffffu) + below[0]] = static_cast<uint16_t>(threadIdx.x);
-    if (has[1] >> lane & 1) sh.groups[(both & 0xffffu) + (earlier >> 16) + below[1]] = static_cast<uint16_t>(1024 + threadIdx.x);
+    const uint32_t both = __reduce_add_sync(kFullMask, of_warp), negative = both >> 16, groups = (both & 0xffffu) + negative;
+    if (has[1] >> lane & 1) sh.groups[negative - 1 - (earlier >> 16) - below[1]] = static_cast<uint16_t>(1023 - threadIdx.x);
+    if (has[0] >> lane & 1) sh.groups[negative + (earlier & 0xffffu) + below[0]] = static_cast<uint16_t>(1024 + threadIdx.x);
     __syncthreads();
     const auto put = [&](uint32_t i, uint32_t n, double mass) {
       if (SIZE == 1) {
