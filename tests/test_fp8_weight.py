@@ -31,3 +31,8 @@ def test_a_block_of_zeros():
 def test_columns_that_cannot_be_loaded_are_refused():
     with pytest.raises(ValueError, match="multiple of 16"):
         Fp8Weight(torch.zeros(16, 24))
+
+
+def test_a_parameter_leaves_no_graph():
+    e = Fp8Weight(torch.nn.Linear(32, 16).weight)
+    assert not e.q.requires_grad and not e.scales.requires_grad

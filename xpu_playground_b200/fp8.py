@@ -13,8 +13,9 @@ LARGEST, SMALLEST_SCALE = 448.0, 2.0 ** -126
 class Fp8Weight:
     """A Linear weight [n, k] held as e4m3 with a scale for each block of 128 x
     128: the block's largest value becomes 448. Made once, when a model is
-    loaded. k is a multiple of 16."""
+    loaded, without gradients. k is a multiple of 16."""
 
+    @torch.no_grad()
     def __init__(self, weight: torch.Tensor):
         n, k = weight.shape
         if k % 16:
