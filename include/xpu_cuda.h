@@ -302,13 +302,15 @@ int xpu_tree_attention(const xpu_kv_cache_t *cache, uint32_t layer, const int32_
  * scales side by side. A group with a NaN or an infinity stands for NaN there
  * or throughout. Arithmetic in FP32. width is a multiple of 16, pointers are 16-byte
  * aligned (scales: 4), strides in elements of `dtype` and multiples of 8. rows
- * 0: nothing is done. q and scales may not overlap the inputs.
+ * 0: nothing is done. q and scales may not overlap the inputs. Scales and quotients are products
+ * with reciprocals, within 2^-21 of the exact ones.
  *
  * xpu_fp8_quantize: y = x.
- * xpu_fp8_silu_multiply: y = gate / (1 + exp(-gate)) * up, of one row stride.
+ * xpu_fp8_silu_multiply: y = gate / (1 + exp(-gate)) * up, of one row stride; 0 for a
+ *   finite gate below -87.
  * xpu_fp8_rms_norm: t = x + residual (NULL: x) rounded to dtype and stored in
- *   total (may be NULL, and may be x or residual itself, with its stride); y = t * rsqrt(mean(t^2)
- *   + epsilon) * weight. width up to 32768. */
+ *   total (may be NULL, and may be x or residual itself, with its stride; it overlaps
+ *   nothing else); y = t * rsqrt(mean(t^2) + epsilon) * weight. width up to 32768. */
 #define XPU_FP8_BLOCK 128u
 int xpu_fp8_quantize(int dtype, const void *x, uint64_t stride, void *q, float *scales, uint32_t rows, uint32_t width,
                      void *stream);
@@ -319,9 +321,10 @@ int xpu_fp8_rms_norm(int dtype, const void *x, uint64_t x_stride, const void *re
                      uint32_t rows, uint32_t width, void *stream);
 /* c[m][n] = sum over groups g of 128 columns of a_scales[g][m] * w_scales[n / 128][g] *
  * sum_{k in g} a[m][k] w[n][k]: rows in the form above against weights w [n][k] (e4m3) with
- * a scale for each block of 128 x 128, w_scales [ceil(n / 128)][ceil(k / 128)]. FP32 sums,
- * c [m][n] rounded once to dtype. k is a multiple of 16; a, w and c are contiguous,
- * 16-byte aligned. Stands beside xpu_gemm_bt. */
+ * a scale for each block of 128 x 128, w_scales [ceil(n / 128)][ceil(k / 128)]. FP32
+ * sums, the two scales multiplied first, c [m][n] rounded once to dtype. k is a multiple of
+ * 16; a, w and c are contiguous, 16-byte aligned, and c overlaps none of the inputs. Results
+ * repeat bit for bit. Stands beside xpu_gemm_bt. */
 int xpu_fp8_gemm(int dtype, const void *a, const float *a_scales, const void *w, const float *w_scales, void *c, uint32_t m,
                  uint32_t n, uint32_t k, void *stream);
 

@@ -318,6 +318,8 @@ def main(argv=None) -> int:
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--min-p", type=float, default=0.0)
     a = ap.parse_args(argv)
+    if a.temperature is None and (a.top_k, a.top_p, a.min_p) != (0, 1.0, 0.0):
+        ap.error("--top-k, --top-p and --min-p need --temperature")
     shape = PRESETS[a.preset]
     room = a.prompt_len + a.new_tokens + a.depth + 2
     model = PagedQwen3(shape, synthetic_weights(shape, a.seed), room, a.eight_bits)
