@@ -17,6 +17,13 @@
 //
 // SIZE blocks of a cluster share a row, a run of it each: as many as are resident at once for all rows. Four and eight
 // blocks hold their runs in registers, one and two read theirs again from the L2.
+//
+// Rows of 151936 bf16 logits, us without top-k / top-k 50 / temperature 0: 1 row 16.7 / 12.3 / 8.7; 148 rows 35 / 19 / 14.5; 1024
+// rows 197 / 110 / 83, where memory would take 48. One row is a chain of latencies: 32000 cycles, of which 11000 find the token once the
+// groups' sums are known. Of many rows an SM has one at a time (its histogram), which takes 43000 cycles:
+// counting 24000 (a warp's 32 additions meet random banks, 3.5 to one of them; the memory needs 13000), finding
+// the groups 4000, their sums 6000 (11000 in fp16, which has ten times the values), prefix sums, the search and the token's place
+// 7000. With a top-k 30000: reading 17000, bounds and the list 7000, the sort 6000.
 #include <algorithm>
 #include <atomic>
 
