@@ -1,0 +1,44 @@
+"""Sampling where places are counted and where blocks' counters are joined, against a sort in 64 bits."""
+
+import pytest
+import torch
+
+from tests.test_sample_gpu import BF16, FP16, check, randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [1, 20, 40, 90])  # eight, four, two and one block a row
+@pytest.mark.parametrize("vocabulary", [31, 32, 33, 64, 65, 127, 128, 129, 255, 256, 257, 300])
+def test_as_many_tokens_as_places(rows, vocabulary):
+    """All are listed where top-k is 256: a multiple of a warp or not, to the last place."""
+    g = torch.Generator().manual_seed(vocabulary)
+    u = torch.rand(rows, generator=g)
+    u[-1] = 1 - 2.0 ** -24
+    x = randn(rows, rows, vocabulary, FP16)
+    check(x, u, top_k=[256] * rows)
+    check(x[:, :1].expand(rows, vocabulary).contiguous(), u, top_k=[min(256, i + vocabulary // 2) for i in range(rows)])
+    check(x, u, top_k=[1 + 3 * i % 256 for i in range(rows)], top_p=[0.9] * rows, temperature=[3.0] * rows)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 20, 40])
+@pytest.mark.parametrize("many", [60000, 65535, 65536, 80000, 131072])
+def test_a_value_that_blocks_share(rows, many):
+    """Groups whose joined counter holds the value's number, and one whose does not, beside one another."""
+    vocabulary = 151936
+    g = torch.Generator().manual_seed(many + rows)
+    x = randn(many, rows, vocabulary, BF16)
+    for row in x:
+        places = torch.randperm(vocabulary, generator=g)
+        row[places[:many]] = 4.0
+        row[places[many:many + 2000]] = 4.03125  # its neighbour, in the same group
+        row[places[many + 2000:many + 5000]] = 5.0
+        row[places[many + 5000:many + 5300]] = -0.0
+        row[places[many + 5300:many + 5600]] = 0.0
+    u = torch.rand(rows, generator=g)
+    u[0] = 0.999
+    check(x, u)
+    check(x, u, temperature=[0.8] * rows, top_p=[0.7] * rows, min_p=[0.05] * rows)
+    check(x, u, top_k=[1000 + 997 * i for i in range(rows)])
+    check(x, u, temperature=[20.0] * rows, min_p=[0.75] * rows)
+    check(x, u, temperature=[50.0] * rows, top_k=[140000] * rows)

@@ -13,17 +13,16 @@
 //
 // Rows with a small top-k (a temperature of 0 is top-k 1) need no histogram: each thread's largest
 // logit is found first, and no logit below the k-th of those can be among the k. What is left, a few times
-// k, is listed and sorted by one block, a token a thread.
+// k, is listed and put in order by one block, a token a thread.
 //
 // SIZE blocks of a cluster share a row, a run of it each: as many as are resident at once for all rows. Four and eight
 // blocks hold their runs in registers, one and two read theirs again from the L2.
 //
-// Rows of 151936 bf16 logits, us without top-k / top-k 50 / temperature 0: 1 row 16.7 / 12.3 / 8.7; 148 rows 35 / 19 / 14.5; 1024
-// rows 197 / 110 / 83, where memory would take 48. One row is a chain of latencies: 32000 cycles, of which 11000 find the token once the
-// groups' sums are known. Of many rows an SM has one at a time (its histogram), which takes 43000 cycles:
+// Rows of 151936 bf16 logits, us without top-k / top-k 50 / temperature 0: 1 row 15.8 / 9.3 / 7.1; 148 rows 35 / 17.4 / 13.6; 1024
+// rows 194 / 99 / 75, where memory would take 48. One row is a chain of latencies. Of many rows an SM has one at a time (its histogram), which takes 43000 cycles:
 // counting 24000 (a warp's 32 additions meet random banks, 3.5 to one of them; the memory needs 13000), finding
 // the groups 4000, their sums 6000 (11000 in fp16, which has ten times the values), prefix sums, the search and the token's place
-// 7000. With a top-k 30000: reading 17000, bounds and the list 7000, the sort 6000.
+// 7000. With a top-k 27000: reading 17000, bounds and the list 7000, the choice 3000.
 #include <algorithm>
 #include <atomic>
 
@@ -40,6 +39,11 @@ constexpr uint32_t kKeys = 65536, kGroups = kKeys / 32;
 constexpr uint32_t kSmem = kKeys * 2;
 constexpr uint32_t kMostListed = 256;  // top-k up to which the largest logits are looked for first
 constexpr uint32_t kListed = kThreads;
+constexpr uint32_t kJoined = 1u << 31;                  // a group's counters in block 0 are the row's: beside its count,
+constexpr uint16_t kJoinedGroup = 0x8000;               // and beside its number
+// Listed tokens up to which a token's place is counted, above which they are sorted: one row, top-k 200 (256 tokens) 12.3 and 14.3 us,
+// top-k 250 (512) 15.7 and 15.1; top-k 50 (64 or 128) 9.3 and 12.2.
+constexpr uint32_t kRanked = 256;
 // Groups up to which a warp takes one at a time: 6200 cycles for 100 (bf16), 28000 for 1000 (fp16), where a thread each takes
 // 10500 for up to 1024.
 constexpr uint32_t kMostGroups = 192;
@@ -185,8 +189,10 @@ struct Shared {
   uint32_t heavy_key[kHeavy], heavy_count[kHeavy], heavies;
   uint32_t top[8], bad[8];  // of each block of the cluster
   uint32_t answer_key, answer_at;  // the token: its value, and which occurrence; kKeys: none
+  uint32_t answer_joined;          // whether block 0's counter of that value is the row's
   uint32_t counted, listed, bounds[2][8];
   uint32_t coarse[2], wanted[2], fine[2][32];  // group of a bound, how many of its threads, their values
+  uint32_t heavy_enough;  // tokens that min-p keeps
   double total;
 };
 
@@ -234,6 +240,7 @@ __device__ __forceinline__ V warp_scan(V v) {
 struct Bin {  // one value of a group, a lane each, the largest in lane 0
   uint32_t key, count, before;  // occurrences, and tokens before them in the order
   double weight, mass;          // of one, and of all before
+  bool joined;                  // counted in block 0 for all blocks
 };
 
 __device__ __forceinline__ uint32_t last_lane(bool yes) {
@@ -249,19 +256,34 @@ __device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32
   const uint32_t i = threadIdx.x, lane = i & 31, warp = i >> 5;
   uint32_t size = 32;
   while (size < listed) size *= 2;
-  for (uint32_t run = 2; run <= size; run *= 2) {  // bitonic, the largest first
-    for (uint32_t stride = run / 2; stride > 0; stride /= 2) {
-      uint64_t other;
-      if (stride >= 32) {
-        __syncthreads();
-        sh.list[i] = mine;
-        __syncthreads();
-        other = sh.list[i ^ stride];
-      } else {
-        other = __shfl_xor_sync(kFullMask, mine, stride);
+  if (size <= kRanked) {  // each one's place is the number of larger ones, counted by several threads
+    __syncthreads();
+    if (i < size) sh.list[i] = mine;
+    __syncthreads();
+    const uint32_t entry = i & (size - 1), each = size * size / kThreads;
+    const uint64_t own = sh.list[entry];
+    uint32_t larger = 0;
+    for (uint32_t j = i / size * each, end = j + each; j < end; ++j) larger += sh.list[j] > own;
+    if (larger) atomicAdd(&sh.counts[entry], larger);
+    __syncthreads();
+    if (i < listed) sh.list[sh.counts[i]] = mine;
+    __syncthreads();
+    mine = i < listed ? sh.list[i] : 0;
+  } else {
+    for (uint32_t run = 2; run <= size; run *= 2) {  // bitonic, the largest first
+      for (uint32_t stride = run / 2; stride > 0; stride /= 2) {
+        uint64_t other;
+        if (stride >= 32) {
+          __syncthreads();
+          sh.list[i] = mine;
+          __syncthreads();
+          other = sh.list[i ^ stride];
+        } else {
+          other = __shfl_xor_sync(kFullMask, mine, stride);
+        }
+        const bool larger = ((i & run) == 0) == ((i & stride) == 0);
+        mine = larger == (mine > other) ? mine : other;
       }
-      const bool larger = ((i & run) == 0) == ((i & stride) == 0);
-      mine = larger == (mine > other) ? mine : other;
     }
   }
   if (most == 1) {  // temperature 0, or top-k 1: nothing else is kept
@@ -455,6 +477,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   if (threadIdx.x == 0) {
     sh.heavy_key[0] = Keys<T>::kMinusInf + 1;
     sh.heavy_count[0] = 0;
+    sh.answer_joined = 0;
   }
   row_sync<SIZE>();  // what was cleared is, before another block writes there
   constexpr uint32_t kLowest = Keys<T>::kMinusInf + 1;  // the lowest finite value masks too: counted without the histogram
@@ -652,16 +675,22 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
 #pragma unroll
         for (int b = 0; b < SIZE; ++b) n += occurrences<SIZE>(histogram, &sh, key, b, any_heavy);
         double mass = n ? n * exp(log_weight(key)) : 0.0;
+        // Block 0's counters become the row's, where they hold it: the search would wait 2000 cycles for the others' each time.
+        const bool joined = SIZE > 1 && !any_heavy && __all_sync(kFullMask, n < 65536);
+        if (joined) asm volatile("st.shared::cluster.u16 [%0], %1;" ::"r"(cluster_addr(histogram + counter(key), 0)), "h"(static_cast<uint16_t>(n)) : "memory");
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(kFullMask, mass, o);
         n = __reduce_add_sync(kFullMask, n);
-        if (lane == 0) put(i, n, mass);
+        if (lane == 0) put(i, n | (joined ? kJoined : 0), mass);
       }
     }
     row_sync<SIZE>();
     if (rank == 0) {
       // Sums over the groups before each; thread i has groups 2 i and 2 i + 1.
-      const uint32_t e = 2 * threadIdx.x, n0 = e < groups ? sh.counts[e] : 0, n1 = e + 1 < groups ? sh.counts[e + 1] : 0;
+      const uint32_t e = 2 * threadIdx.x, c0 = e < groups ? sh.counts[e] : 0, c1 = e + 1 < groups ? sh.counts[e + 1] : 0;
+      const uint32_t n0 = c0 & ~kJoined, n1 = c1 & ~kJoined;
+      if (c0 & kJoined) sh.groups[groups - 1 - e] |= kJoinedGroup;
+      if (c1 & kJoined) sh.groups[groups - 2 - e] |= kJoinedGroup;
       const double m0 = e < groups ? sh.masses[e] : 0.0, m1 = e + 1 < groups ? sh.masses[e + 1] : 0.0;
       const uint32_t inc = warp_scan(n0 + n1);
       const double minc = warp_scan(m0 + m1);
@@ -687,7 +716,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
         sh.masses[e + 1] = mass + m0;
       }
       __syncthreads();
-      if (warp == 0) {
+      if (warp < 2) {
         // The last group of which yes(tokens before it, their weight); the first if there is none.
         const auto last_group = [&](auto yes) {
           uint32_t low = 0, many = groups;
@@ -702,10 +731,16 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
         };
         const auto bins_of = [&](uint32_t group) {
           Bin bin;
-          bin.key = 32 * sh.groups[groups - 1 - group] + 31 - lane;
+          const uint32_t g = sh.groups[groups - 1 - group];
+          bin.key = 32 * (g & (kGroups - 1)) + 31 - lane;
           bin.count = 0;
+          bin.joined = SIZE > 1 && (g & kJoinedGroup);
+          if (bin.joined) {
+            bin.count = histogram[counter(bin.key)];
+          } else {
 #pragma unroll
-          for (int b = 0; b < SIZE; ++b) bin.count += occurrences<SIZE>(histogram, &sh, bin.key, b, any_heavy);
+            for (int b = 0; b < SIZE; ++b) bin.count += occurrences<SIZE>(histogram, &sh, bin.key, b, any_heavy);
+          }
           bin.weight = bin.count ? exp(log_weight(bin.key)) : 0.0;
           const double m = warp_scan(bin.count * bin.weight);
           const double up = __shfl_up_sync(kFullMask, m, 1);
@@ -719,19 +754,8 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
           const uint32_t at = last_lane(b.count && b.before < n);
           return __shfl_sync(kFullMask, b.mass + min(n - b.before, b.count) * b.weight, at);
         };
-        uint32_t kept = min(most, all);
-        double total = kept == all ? all_mass : weight_of_first(kept);
-        uint32_t fewer = kept;
-        if (top_p < 1.f) {
-          const double wanted = static_cast<double>(top_p) * total;
-          const Bin b = bins_of(last_group([&](uint32_t, double m) { return m < wanted; }));
-          const uint32_t at = last_lane(b.count && b.mass < wanted);
-          const double need = fmin(fmax(ceil((wanted - b.mass) / b.weight), 1.0), static_cast<double>(b.count));
-          fewer = min(fewer, __shfl_sync(kFullMask, b.before + (b.count ? static_cast<uint32_t>(need) : 0), at));
-        }
-        if (min_p > 1.f) {
-          fewer = 1;
-        } else if (min_p > 0.f) {  // the lowest value that is heavy enough: one of the keys [low, low + many)
+        if (warp == 1 && min_p > 0.f && min_p <= 1.f) {  // what min-p keeps, while the other warp looks at top-k and top-p
+          // The lowest value that is heavy enough: one of the keys [low, low + many).
           uint32_t low = 0, many = top + 1;
           while (many > 1) {
             const uint32_t step = (many + 31) / 32, at = low + min((lane + 1) * step, many) - 1;
@@ -745,7 +769,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
           uint32_t found = 0, place = groups;  // the first group whose highest value is below it
           for (uint32_t from = 0; from < groups && place == groups; from += 32) {
             const uint32_t at = from + lane;
-            const uint32_t votes = __ballot_sync(kFullMask, at < groups && 32u * sh.groups[groups - 1 - at] + 31 < low);
+            const uint32_t votes = __ballot_sync(kFullMask, at < groups && 32u * (sh.groups[groups - 1 - at] & (kGroups - 1)) + 31 < low);
             if (votes) place = from + __ffs(votes) - 1;
           }
           if (place > 0) {
@@ -753,25 +777,45 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
             const uint32_t in = __reduce_add_sync(kFullMask, b.key >= low ? b.count : 0);
             found = sh.counts[place - 1] + in;
           }
-          fewer = min(fewer, found);
+          if (lane == 0) sh.heavy_enough = found;
+          asm volatile("bar.sync 1, 64;" ::: "memory");
         }
-        fewer = max(fewer, 1u);
-        if (fewer < kept) total = weight_of_first(kept = fewer);
-        const double wanted = static_cast<double>(u) * total;
-        const Bin b = bins_of(last_group([&](uint32_t c, double m) { return c < kept && m <= wanted; }));
-        const uint32_t at = last_lane(b.count && b.weight > 0.0 && b.before < kept && b.mass <= wanted);
-        if (lane == at) {
-          const uint32_t in = max(min(b.count, kept - b.before), 1u);  // of its occurrences are kept
-          const double which = floor((wanted - b.mass) / b.weight);
-          const uint32_t j = which < in ? static_cast<uint32_t>(which) : in - 1;
-          if (logprobs) logprobs[row] = static_cast<float>(log_weight(b.key) - log(total));
-          for (int i = 0; i < SIZE; ++i) {
-            if (SIZE == 1) {
-              sh.answer_key = b.key;
-              sh.answer_at = j;
-            } else {
-              asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_key, i)), "r"(b.key) : "memory");
-              asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_at, i)), "r"(j) : "memory");
+        if (warp == 0) {
+          uint32_t kept = min(most, all);
+          double total = kept == all ? all_mass : weight_of_first(kept);
+          uint32_t fewer = kept;
+          if (top_p < 1.f) {
+            const double wanted = static_cast<double>(top_p) * total;
+            const Bin b = bins_of(last_group([&](uint32_t, double m) { return m < wanted; }));
+            const uint32_t at = last_lane(b.count && b.mass < wanted);
+            const double need = fmin(fmax(ceil((wanted - b.mass) / b.weight), 1.0), static_cast<double>(b.count));
+            fewer = min(fewer, __shfl_sync(kFullMask, b.before + (b.count ? static_cast<uint32_t>(need) : 0), at));
+          }
+          if (min_p > 1.f) {
+            fewer = 1;
+          } else if (min_p > 0.f) {
+            asm volatile("bar.sync 1, 64;" ::: "memory");
+            fewer = min(fewer, sh.heavy_enough);
+          }
+          fewer = max(fewer, 1u);
+          if (fewer < kept) total = weight_of_first(kept = fewer);
+          const double wanted = static_cast<double>(u) * total;
+          const Bin b = bins_of(last_group([&](uint32_t c, double m) { return c < kept && m <= wanted; }));
+          const uint32_t at = last_lane(b.count && b.weight > 0.0 && b.before < kept && b.mass <= wanted);
+          if (lane == at) {
+            const uint32_t in = max(min(b.count, kept - b.before), 1u);  // of its occurrences are kept
+            const double which = floor((wanted - b.mass) / b.weight);
+            const uint32_t j = which < in ? static_cast<uint32_t>(which) : in - 1;
+            if (logprobs) logprobs[row] = static_cast<float>(log_weight(b.key) - log(total));
+            for (int i = 0; i < SIZE; ++i) {
+              if (SIZE == 1) {
+                sh.answer_key = b.key;
+                sh.answer_at = j;
+              } else {
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_key, i)), "r"(b.key) : "memory");
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_at, i)), "r"(j) : "memory");
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.answer_joined, i)), "r"(static_cast<uint32_t>(b.joined)) : "memory");
+              }
             }
           }
         }
@@ -785,6 +829,10 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   uint32_t j = sh.answer_at, here = 0, of_block[SIZE];
 #pragma unroll
   for (uint32_t b = 0; b < SIZE; ++b) of_block[b] = key < kKeys ? occurrences<SIZE>(histogram, &sh, key, b, any_heavy) : 0;
+  if (SIZE > 1 && sh.answer_joined) {
+#pragma unroll
+    for (uint32_t b = 1; b < SIZE; ++b) of_block[0] -= of_block[b];
+  }
   bool mine = key < kKeys;
 #pragma unroll
   for (uint32_t b = 0; b < SIZE; ++b) {
