@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tests.test_sample_gpu import BF16, FP16, check, randn
+from tests.test_sample_gpu import BF16, FP16, INF, NAN, check, randn, settings
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,26 @@ def test_a_value_that_blocks_share(rows, many):
     check(x, u, top_k=[1000 + 997 * i for i in range(rows)])
     check(x, u, temperature=[20.0] * rows, min_p=[0.75] * rows)
     check(x, u, temperature=[50.0] * rows, top_k=[140000] * rows)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("vocabulary", [1, 2, 63, 100, 511, 513, 1024, 2047, 2048, 2049])
+def test_short_rows(vocabulary, dtype):
+    """On both sides of the length up to which a row is sorted whole: any settings, ties, masks and rows without an answer."""
+    rows = 300
+    x = randn(vocabulary, rows, vocabulary, dtype)
+    x[:40] = (2 * x[:40]).round() / 2  # ties, zeros of both signs
+    x[40:60, 1::2] = -INF
+    x[60:70, : vocabulary - 1] = torch.finfo(dtype).min
+    x[70:74] = -INF
+    x[74:76, vocabulary // 2] = INF
+    x[76:78, vocabulary - 1] = NAN
+    x[78:80, 0] = -torch.tensor(NAN)
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(vocabulary))
+    u[::50], u[1::50] = 0.0, 1 - 2.0 ** -24
+    tokens, _ = check(x, u, **settings(vocabulary, rows))
+    assert (tokens[70:80] == -1).all()
+    check(x, u)
+    apart = torch.empty(rows, vocabulary + 3, dtype=dtype, device="cuda")[:, 1:vocabulary + 1]  # rows at odd places
+    apart.copy_(x)
+    check(apart, u, **settings(vocabulary + 1, rows))

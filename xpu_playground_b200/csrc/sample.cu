@@ -18,11 +18,13 @@
 // SIZE blocks of a cluster share a row, a run of it each: as many as are resident at once for all rows. Four and eight
 // blocks hold their runs in registers, one and two read theirs again from the L2.
 //
-// Rows of 151936 bf16 logits, us without top-k / top-k 50 / temperature 0: 1 row 15.8 / 9.3 / 7.1; 148 rows 35 / 17.4 / 13.6; 1024
-// rows 194 / 99 / 75, where memory would take 48. One row is a chain of latencies. Of many rows an SM has one at a time (its histogram), which takes 43000 cycles:
-// counting 24000 (a warp's 32 additions meet random banks, 3.5 to one of them; the memory needs 13000), finding
-// the groups 4000, their sums 6000 (11000 in fp16, which has ten times the values), prefix sums, the search and the token's place
-// 7000. With a top-k 27000: reading 17000, bounds and the list 7000, the choice 3000.
+// Rows of 151936 bf16 logits, us without top-k / top-k 50 / temperature 0: 1 row 15.7 / 9.3 / 6.2; 148 rows 35 / 17.6 / 12.4; 1024
+// rows 194 / 99 / 69, where memory would take 48. One row is a chain of latencies. Of many rows an SM has one at a time (its
+// histogram), which takes 43000 cycles: counting 24000 (a warp's 32 additions meet random banks, 3.5 to one of them; the
+// memory needs 13000), finding the groups 4000, their sums 6000 (11000 in fp16, which has ten times the values), prefix sums, the
+// search and the token's place 7000. With a top-k 27000: reading 17000, bounds and the list 7000, the choice 3000.
+//
+// Short rows need none of this: they are sorted whole.
 #include <algorithm>
 #include <atomic>
 
@@ -249,11 +251,21 @@ __device__ __forceinline__ uint32_t last_lane(bool yes) {
 }
 
 // Chooses among `listed` (up to kListed) tokens, thread i's being `mine` (key << 32 | ~id, 0 behind the last), which hold all
-// that top-k keeps: sorted, one a thread.
+// that top-k keeps: put in order, one a thread. sh.counts are 0.
 template <typename T>
 __device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32_t most, double slope, float top_p, float min_p,
                               float u, int32_t *token, float *logprob) {
   const uint32_t i = threadIdx.x, lane = i & 31, warp = i >> 5;
+  if (most == 1) {  // temperature 0, or top-k 1: all listed are the largest value
+    const uint32_t lowest = __reduce_max_sync(kFullMask, static_cast<uint32_t>(mine));
+    if (lane == 0) atomicMax(&sh.counts[0], lowest);
+    __syncthreads();
+    if (i == 0) {
+      *token = static_cast<int32_t>(~sh.counts[0]);
+      if (logprob) *logprob = 0.f;
+    }
+    return;
+  }
   uint32_t size = 32;
   while (size < listed) size *= 2;
   if (size <= kRanked) {  // each one's place is the number of larger ones, counted by several threads
@@ -285,13 +297,6 @@ __device__ void choose_listed(Shared &sh, uint64_t mine, uint32_t listed, uint32
         mine = larger == (mine > other) ? mine : other;
       }
     }
-  }
-  if (most == 1) {  // temperature 0, or top-k 1: nothing else is kept
-    if (i == 0) {
-      *token = static_cast<int32_t>(~static_cast<uint32_t>(mine));
-      if (logprob) *logprob = 0.f;
-    }
-    return;
   }
   if (i == 0) sh.answer_key = static_cast<uint32_t>(mine >> 32);
   __syncthreads();
@@ -377,41 +382,50 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   if (most <= kMostListed) {
     r.each(begin, end, [&](const uint4 &v, uint32_t) { look(v); });
     const uint32_t mine = top_of();
-    if (mine > Keys<T>::kMinusInf) atomicAdd(&sh.counts[mine / 32], 1u);
+    if (most > 1) {
+      if (mine > Keys<T>::kMinusInf) atomicAdd(&sh.counts[mine / 32], 1u);
+    } else {
+      const uint32_t warp_top = __reduce_max_sync(kFullMask, mine);
+      if (lane == 0) atomicMax(&sh.bounds[0][rank], warp_top);
+    }
     const bool any_bad = __syncthreads_or(is_bad());
-    // Lower bounds of the `most`-th largest logit: this block's `most`-th of the threads' largest; and the least of all blocks'
-    // such values for their part of `most`. First the group of 32 values, thread i looking at groups 2047 - 2 i and
-    // 2046 - 2 i, then the value.
-    const uint32_t hi = kGroups - 1 - 2 * threadIdx.x, a = sh.counts[hi], b = sh.counts[hi - 1];
-    const uint32_t inc = warp_scan(a + b);
-    if (lane == 31) sh.warp_count[warp] = inc;
-    __syncthreads();
-    const uint32_t before = __reduce_add_sync(kFullMask, lane < warp ? sh.warp_count[lane] : 0) + inc - a - b;
-    constexpr uint32_t kParts = SIZE == 1 ? 1 : 2;
+    if (most > 1) {
+      // Lower bounds of the `most`-th largest logit: this block's `most`-th of the threads' largest; and the least of all blocks'
+      // such values for their part of `most`. First the group of 32 values, thread i looking at groups 2047 - 2 i and
+      // 2046 - 2 i, then the value.
+      const uint32_t hi = kGroups - 1 - 2 * threadIdx.x, a = sh.counts[hi], b = sh.counts[hi - 1];
+      const uint32_t inc = warp_scan(a + b);
+      if (lane == 31) sh.warp_count[warp] = inc;
+      __syncthreads();
+      const uint32_t before = __reduce_add_sync(kFullMask, lane < warp ? sh.warp_count[lane] : 0) + inc - a - b;
+      constexpr uint32_t kParts = SIZE == 1 ? 1 : 2;
 #pragma unroll
-    for (uint32_t part = 0; part < kParts; ++part) {
-      const uint32_t n = part ? (most + SIZE - 1) / SIZE : most;
-      const bool first = before < n && before + a >= n, second = before + a < n && before + a + b >= n;
-      if (first || second) {
-        sh.coarse[part] = first ? hi : hi - 1;
-        sh.wanted[part] = n - before - (first ? 0 : a);
+      for (uint32_t part = 0; part < kParts; ++part) {
+        const uint32_t n = part ? (most + SIZE - 1) / SIZE : most;
+        const bool first = before < n && before + a >= n, second = before + a < n && before + a + b >= n;
+        if (first || second) {
+          sh.coarse[part] = first ? hi : hi - 1;
+          sh.wanted[part] = n - before - (first ? 0 : a);
+        }
       }
-    }
-    __syncthreads();
+      __syncthreads();
 #pragma unroll
-    for (uint32_t part = 0; part < kParts; ++part)
-      if (mine / 32 == sh.coarse[part]) atomicAdd(&sh.fine[part][31 - mine % 32], 1u);
-    __syncthreads();
-    if (warp < kParts && sh.coarse[warp] < kGroups) {
-      const uint32_t votes = __ballot_sync(kFullMask, warp_scan(sh.fine[warp][lane]) >= sh.wanted[warp]);
-      const uint32_t bound = 32 * sh.coarse[warp] + 32 - __ffs(votes);
-      if (SIZE == 1) {
-        if (lane == 0) sh.bounds[0][0] = bound;
-      } else if (lane < SIZE) {
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bounds[warp][rank], lane)), "r"(bound) : "memory");
+      for (uint32_t part = 0; part < kParts; ++part)
+        if (mine / 32 == sh.coarse[part]) atomicAdd(&sh.fine[part][31 - mine % 32], 1u);
+      __syncthreads();
+      if (warp < kParts && sh.coarse[warp] < kGroups) {
+        const uint32_t votes = __ballot_sync(kFullMask, warp_scan(sh.fine[warp][lane]) >= sh.wanted[warp]);
+        const uint32_t bound = 32 * sh.coarse[warp] + 32 - __ffs(votes);
+        if (SIZE == 1) {
+          if (lane == 0) sh.bounds[0][0] = bound;
+        } else if (lane < SIZE) {
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bounds[warp][rank], lane)), "r"(bound) : "memory");
+        }
       }
+      sh.counts[hi] = sh.counts[hi - 1] = 0;
+    } else if (SIZE > 1 && threadIdx.x < SIZE && threadIdx.x != rank) {
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(&sh.bounds[0][rank], threadIdx.x)), "r"(sh.bounds[0][rank]) : "memory");
     }
-    sh.counts[hi] = sh.counts[hi - 1] = 0;
     row_sync<SIZE>();
     uint32_t bound = Keys<T>::kMinusInf + 1, least = ~0u;
 #pragma unroll
@@ -419,7 +433,7 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
       bound = max(bound, sh.bounds[0][q]);
       least = min(least, sh.bounds[1][q]);
     }
-    if (SIZE > 1) bound = max(bound, least);
+    if (SIZE > 1 && most > 1) bound = max(bound, least);
     const auto list = [&](const uint4 &v, uint32_t p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -923,6 +937,137 @@ k_sample(const uint16_t *logits, uint64_t stride, const float *temperatures, con
   if (SIZE > 1) cluster_sync();  // no block leaves while another may read its counters
 }
 
+// Rows of up to kShort logits: all are sorted, four a thread, as key << 16 | ~id (0: none), so that a block needs little shared memory
+// and an SM holds several. Without limits, us here and through the histogram: 250 logits, 1 row 3.9 and 10.7, 1024 rows 9.4 and 74;
+// 2000 logits 8.0 and 10.3, 42 and 70; 4096 logits 14.6 and 10.3, 102 and 71.
+constexpr uint32_t kShort = 2048;
+
+template <typename T>
+__global__ void __launch_bounds__(kShort / 4)
+k_sample_short(const uint16_t *logits, uint64_t stride, const float *temperatures, const int32_t *top_ks, const float *top_ps,
+               const float *min_ps, const float *us, int32_t *tokens, float *logprobs, uint32_t vocabulary) {
+  extern __shared__ __align__(16) uint4 exchange[];  // two of blockDim.x
+  __shared__ double warp_mass[kWarps], total;
+  __shared__ uint32_t warp_most[kWarps], warp_kept[kWarps], warp_below[kWarps];
+  const uint32_t i = threadIdx.x, lane = i & 31, warp = i >> 5, row = blockIdx.x;
+  if (i < kWarps) {
+    warp_mass[i] = 0.0;
+    warp_most[i] = warp_kept[i] = warp_below[i] = 0;
+  }
+  grid_dep_launch();
+  grid_dep_wait();
+  const volatile float *const vt = temperatures, *const vp = top_ps, *const vm = min_ps, *const vu = us;
+  const volatile int32_t *const vk = top_ks;
+  const volatile uint16_t *const vl = logits + row * stride;
+  uint32_t e[4];
+  bool bad = false;
+#pragma unroll
+  for (uint32_t q = 0; q < 4; ++q) {
+    const uint32_t id = q * blockDim.x + i, bits = id < vocabulary ? vl[id] : Keys<T>::kMask & 0xffffu, key = key_of(bits);
+    constexpr uint32_t inf = Keys<T>::kPlusInf & 0x7fffu;
+    bad |= bits == inf || (bits & 0x7fffu) > inf;
+    e[q] = key > Keys<T>::kMinusInf ? key << 16 | (id ^ 0xffffu) : 0;
+  }
+  const float temperature = temperatures ? vt[row] : 1.f, top_p = top_ps ? vp[row] : 1.f, min_p = min_ps ? vm[row] : 0.f;
+  const int32_t top_k = top_ks ? vk[row] : 0;
+  const float u = vu[row];
+  const bool asked = temperature >= 0.f && top_p == top_p && min_p == min_p && u >= 0.f && u < 1.f && top_k >= 0;
+  const bool greedy = temperature == 0.f;
+  const uint32_t most = greedy ? 1 : (top_k == 0 ? UINT32_MAX : static_cast<uint32_t>(top_k));
+  const double slope = greedy ? 1.0 : 1.0 / static_cast<double>(temperature);
+  uint32_t first = __reduce_max_sync(kFullMask, max(max(e[0], e[1]), max(e[2], e[3])));
+  if (__syncthreads_or(bad)) first = 0;  // here the sums of absent warps are 0, too
+  if (lane == 0) warp_most[warp] = first;
+  __syncthreads();
+  first = __reduce_max_sync(kFullMask, warp_most[lane]);
+  if (!asked || first == 0 || most == 1) {
+    if (i == 0) {
+      const bool none = !asked || first == 0;
+      tokens[row] = none ? -1 : static_cast<int32_t>((first & 0xffffu) ^ 0xffffu);
+      if (logprobs) logprobs[row] = none ? -INFINITY : 0.f;
+    }
+    return;
+  }
+
+  // Bitonic, the largest first: thread i has places 4 i to 4 i + 3.
+  const auto pick = [](uint32_t &mine, uint32_t other, bool larger) { mine = larger ? max(mine, other) : min(mine, other); };
+  const auto both = [](uint32_t &a, uint32_t &b, bool larger_first) {
+    const uint32_t hi = max(a, b), lo = min(a, b);
+    a = larger_first ? hi : lo;
+    b = larger_first ? lo : hi;
+  };
+  both(e[0], e[1], true);
+  both(e[2], e[3], false);
+  uint32_t turn = 0;
+  for (uint32_t run = 1; run <= blockDim.x; run *= 2) {  // of threads
+    const bool falling = (i & run) == 0;
+    for (uint32_t far = run / 2; far > 0; far /= 2) {
+      const bool larger = falling == ((i & far) == 0);
+      if (far >= 32) {
+        uint4 *const at = exchange + (turn ^= 1) * blockDim.x;  // the other half may still be read
+        at[i] = make_uint4(e[0], e[1], e[2], e[3]);
+        __syncthreads();
+        const uint4 other = at[i ^ far];
+        pick(e[0], other.x, larger), pick(e[1], other.y, larger), pick(e[2], other.z, larger), pick(e[3], other.w, larger);
+      } else {
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q) pick(e[q], __shfl_xor_sync(kFullMask, e[q], far), larger);
+      }
+    }
+    both(e[0], e[2], falling), both(e[1], e[3], falling);
+    both(e[0], e[1], falling), both(e[2], e[3], falling);
+  }
+
+  const double largest = value_of<T>(first >> 16);
+  double z[4], weight[4], sum[4], thread_sum = 0.0;
+#pragma unroll
+  for (uint32_t q = 0; q < 4; ++q) {
+    z[q] = weight[q] = 0.0;
+    if (e[q] && 4 * i + q < most) {
+      z[q] = (value_of<T>(e[q] >> 16) - largest) * slope;
+      weight[q] = exp(z[q]);
+    }
+    sum[q] = thread_sum += weight[q];
+  }
+  const double inc = warp_scan(thread_sum), up = __shfl_up_sync(kFullMask, inc, 1);
+  if (lane == 31) warp_mass[warp] = inc;
+  __syncthreads();
+  const double masses = warp_scan(warp_mass[lane]), all = __shfl_sync(kFullMask, masses, 31);
+  const double lower = warp ? __shfl_sync(kFullMask, masses, warp - 1) : 0.0, before = lower + (lane ? up : 0.0);
+  uint32_t kept = 0;
+  bool keep[4];
+#pragma unroll
+  for (uint32_t q = 0; q < 4; ++q) {
+    sum[q] = fmin(before + sum[q], lower + inc);  // never above the next thread's
+    const bool counts = e[q] && 4 * i + q < most;
+    keep[q] = counts && (4 * i + q == 0 || ((top_p >= 1.f || (q ? sum[q ? q - 1 : 0] : before) < static_cast<double>(top_p) * all) &&
+                                            weight[q] >= static_cast<double>(min_p) && weight[q] > 0.0));
+    kept += keep[q];
+  }
+  kept = __reduce_add_sync(kFullMask, kept);
+  if (lane == 0) warp_kept[warp] = kept;
+  __syncthreads();
+  kept = __reduce_add_sync(kFullMask, warp_kept[lane]);
+#pragma unroll
+  for (uint32_t q = 0; q < 4; ++q)
+    if (4 * i + q + 1 == kept) total = sum[q];
+  __syncthreads();
+  uint32_t below = 0;
+#pragma unroll
+  for (uint32_t q = 0; q < 4; ++q) below += keep[q] && sum[q] <= static_cast<double>(u) * total;
+  below = __reduce_add_sync(kFullMask, below);
+  if (lane == 0) warp_below[warp] = below;
+  __syncthreads();
+  const uint32_t at = min(__reduce_add_sync(kFullMask, warp_below[lane]), kept - 1);
+#pragma unroll
+  for (uint32_t q = 0; q < 4; ++q) {
+    if (4 * i + q == at) {
+      tokens[row] = static_cast<int32_t>((e[q] & 0xffffu) ^ 0xffffu);
+      if (logprobs) logprobs[row] = static_cast<float>(z[q] - log(total));
+    }
+  }
+}
+
 template <typename T, int SIZE>
 cudaError_t launch(const SampleArgs &a, cudaStream_t s, bool *fits) {
   const auto kernel = k_sample<T, SIZE>;
@@ -963,6 +1108,12 @@ template <typename T>
 cudaError_t best_launch(const SampleArgs &a, cudaStream_t s) {
   bool done = false;
   cudaError_t e = cudaSuccess;
+  if (a.vocabulary <= kShort) {
+    uint32_t threads = 32;
+    while (4 * threads < a.vocabulary) threads *= 2;
+    return launch_after(k_sample_short<T>, a.rows, threads, 2 * threads * sizeof(uint4), s, a.logits, a.stride, a.temperature, a.top_k,
+                        a.top_p, a.min_p, a.u, a.tokens, a.logprobs, a.vocabulary);
+  }
   // up to 8 blocks x kHeld x 1024 pieces, one piece more where the row's address is odd
   const uint32_t pieces = (a.vocabulary + 14) / 8;
   if (a.vocabulary >= 8 * 4096 && (pieces + 7) / 8 <= kHeld * kThreads) e = launch<T, 8>(a, s, &done);
