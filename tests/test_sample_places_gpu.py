@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from tests.test_sample_gpu import BF16, FP16, INF, NAN, check, randn, settings
+from xpu_playground_b200 import kernels as K
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +66,22 @@ def test_short_rows(vocabulary, dtype):
     apart = torch.empty(rows, vocabulary + 3, dtype=dtype, device="cuda")[:, 1:vocabulary + 1]  # rows at odd places
     apart.copy_(x)
     check(apart, u, **settings(vocabulary + 1, rows))
+
+
+@pytest.mark.parametrize("vocabulary", [1000, 5000])
+def test_captured_with_other_numbers(vocabulary):
+    x, u = randn(3, 64, vocabulary, BF16).cuda(), torch.rand(64, device="cuda")
+    tokens, logprobs = torch.empty(64, dtype=torch.int32, device="cuda"), torch.empty(64, device="cuda")
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.sample(x, u, tokens=tokens, logprobs=logprobs)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        K.sample(x, u, tokens=tokens, logprobs=logprobs)
+    for seed in range(3):
+        u.copy_(torch.rand(64, generator=torch.Generator().manual_seed(seed)))
+        x.copy_(randn(seed, 64, vocabulary, BF16))
+        graph.replay()
+        want = check(x, u.cpu())
+        assert torch.equal(tokens, want[0]) and torch.equal(logprobs, want[1])
