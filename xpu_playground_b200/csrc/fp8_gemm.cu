@@ -77,10 +77,11 @@ __device__ __forceinline__ void tmem_landed(uint32_t (&r)[16]) {
                : "memory");
 }
 
-// Arrives on a barrier of the even block. Not with a release at cluster scope: that one waits for every access of the warp,
-// 1000 cycles a group here, where what is passed on is TMEM that has been read, or shared memory of the same block.
+// Arrives on a barrier of the even block to say that this warp has read a TMEM buffer. Nothing that it wrote is passed on: the loads
+// have been waited for, and the next products overwrite what they read. So relaxed: a release at cluster scope waits for
+// every access of the warp, 1000 cycles a group here. What one warp writes for another passes through a barrier of their own block.
 __device__ __forceinline__ void pair_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 template <typename T>
@@ -359,9 +360,9 @@ constexpr uint32_t kPair = 256;                     // rows and columns of a pai
 constexpr uint32_t kWideStages = 4, kWideStage = 2 * kTileBytes;
 constexpr uint32_t kSumWarps = 8, kWideThreads = 128 + 32 * kSumWarps;
 constexpr uint32_t kOutBox = 32 * 128;              // bytes of 32 rows x 64 outputs, swizzled; two a warp
-constexpr uint32_t kScaleSlots = 8;                 // groups whose scales are held, 256 each
+constexpr uint32_t kScaleGroups = 4;                // groups whose scales are handed over at once, twice
 constexpr uint32_t kScalesAt = kWideStages * kWideStage + kSumWarps * 2 * kOutBox;
-constexpr uint32_t kWideSmem = 1024 + kScalesAt + kScaleSlots * kPair * 4;
+constexpr uint32_t kWideSmem = 1024 + kScalesAt + 2 * kScaleGroups * kPair * 4;
 constexpr uint32_t kGroupRows = 8;                  // tile rows whose tiles follow one another, for the L2; 16 is no faster, 4 3% slower
 
 // Into this block's shared memory, completing on the even block's barrier.
@@ -403,33 +404,35 @@ __device__ __forceinline__ WideTile wide_tile(uint32_t t, uint32_t tiles_m, uint
 //
 // The sums of a group can only be taken out of TMEM when they are complete, and TMEM holds two groups: a group's time is half of
 // its products (512 cycles) and of the way round: their completion seen (200), 128 columns read and added up (450), the buffer
-// known to be free (150), the next products issued. So the loop of the adding warps has nothing in it that can stand elsewhere:
-// another pair of warps multiplies the scales of row and block and says through the barrier of the operands that they are
-// there. The issuing warp stays converged and an elected lane issues, so that operands are in uniform registers: from one
-// lane's branch a group took 1.3 times as long.
+// known to be free (150), the next products issued. So the loop of the adding warps has little in it that can stand elsewhere:
+// another pair of warps multiplies the scales of row and block ahead of their use and hands over four groups at a time, through
+// barriers of this block alone; from there on the adding warps hold them in registers. The issuing warp stays converged and an
+// elected lane issues, so that operands are in uniform registers: from one lane's branch a group took 1.3 times as long.
 template <typename T, bool TMA_OUT>
 __global__ void __launch_bounds__(kWideThreads, 1)
 k_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
        const float *a_scales, const float *w_scales, T *c, uint32_t m, uint32_t n, uint32_t groups) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ uint64_t full[kWideStages], empty[kWideStages], sum_full[2], sum_empty[2], drain;
+  __shared__ uint64_t full[kWideStages], empty[kWideStages], sum_full[2], sum_empty[2], scale_full[2], scale_empty[2], drain;
   __shared__ uint32_t tmem_base;
   __shared__ int failed;
   const uint32_t a0 = smem_addr(smem_raw);
   uint8_t *const ring = smem_raw + ((a0 + 1023u) / 1024u * 1024u - a0);
-  float *const scales = reinterpret_cast<float *>(ring + kScalesAt);  // [slot][column half][row]
+  float *const scales = reinterpret_cast<float *>(ring + kScalesAt);  // [half of the places][group of four][column half][row]
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t tiles_m = (m + kPair - 1) / kPair, tiles_n = (n + kPair - 1) / kPair, tiles = tiles_m * tiles_n;
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kWideStages; ++i) {
-      mbar_init(&full[i], 1 + 2 * 2);  // both blocks' operands, and their scale warps
+      mbar_init(&full[i], 1);  // the even block's, for both blocks' operands
       mbar_init(&empty[i], 1);
     }
     for (uint32_t i = 0; i < 2; ++i) {
       mbar_init(&sum_full[i], 1);
       mbar_init(&sum_empty[i], 2 * kSumWarps);
+      mbar_init(&scale_full[i], 2);
+      mbar_init(&scale_empty[i], kSumWarps);
     }
     mbar_init(&drain, 1);
     fence_mbar_init();
@@ -495,40 +498,34 @@ k_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         warp_wait(&failed, &drain, 0);
       }
     } else {
-      // A stage's scales are written when its operands' place is free: then the group four before it has been multiplied, hence
-      // the one six before it added up, and its slot is free too.
-      static_assert(kScaleSlots >= kWideStages + 2, "scales are held until they are used");
       const uint32_t half = warp - 2;
-      uint32_t i = 0;
+      uint32_t chunk = 0;  // of four groups, of all tiles
       bool ok = true;
       for (uint32_t t = pair; ok && t < tiles; t += pairs) {
         const WideTile tile = wide_tile(t, tiles_m, tiles_n);
         const uint32_t row0 = tile.m * kPair + rank * 128 + lane, block = tile.n * 2 + half;
         const bool real = block * kGroup < n;
         const float *const sw = w_scales + static_cast<uint64_t>(block) * groups;
-        float row_scale[4][4], block_scale[4];  // of four groups on their way
-        const auto bring = [&](uint32_t g, int at) {
+        float row_scale[kScaleGroups][4], block_scale[kScaleGroups];  // on their way; 0 behind the last group
+        const auto bring = [&](uint32_t g, uint32_t at) {
           block_scale[at] = real && g < groups ? ld_f32(sw + g) : 0.f;
 #pragma unroll
           for (uint32_t q = 0; q < 4; ++q)
             row_scale[at][q] = real && g < groups && row0 + 32 * q < m ? ld_f32(a_scales + static_cast<uint64_t>(g) * m + row0 + 32 * q) : 0.f;
         };
 #pragma unroll
-        for (int at = 0; at < 4; ++at) bring(at, at);
-        for (uint32_t g0 = 0; ok && g0 < groups; g0 += 4) {
+        for (uint32_t at = 0; at < kScaleGroups; ++at) bring(at, at);
+        for (uint32_t g0 = 0; g0 < groups; g0 += kScaleGroups, ++chunk) {
+          if (!(ok = chunk < 2 || warp_wait(&failed, &scale_empty[chunk & 1], ((chunk >> 1) - 1) & 1))) break;
+          float *const place = scales + (chunk & 1) * kScaleGroups * kPair + half * 128 + lane;
 #pragma unroll
-          for (int at = 0; at < 4; ++at) {
-            if (g0 + at >= groups) break;
-            const uint32_t s = i % kWideStages, use = i / kWideStages;
-            if (!(ok = use == 0 || warp_wait(&failed, &empty[s], (use - 1) & 1))) break;
+          for (uint32_t at = 0; at < kScaleGroups; ++at) {
 #pragma unroll
-            for (uint32_t q = 0; q < 4; ++q)
-              scales[i % kScaleSlots * kPair + half * 128 + 32 * q + lane] = row_scale[at][q] * block_scale[at];
-            __syncwarp();
-            if (lane == 0) pair_arrive(full_bars + 8 * s);
-            bring(g0 + at + 4, at);
-            ++i;
+            for (uint32_t q = 0; q < 4; ++q) place[at * kPair + 32 * q] = row_scale[at][q] * block_scale[at];
+            bring(g0 + kScaleGroups + at, at);
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_full[chunk & 1]);
         }
       }
     }
@@ -539,7 +536,7 @@ k_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     const uint32_t scale_at = smem_addr(scales + half * 128 + quarter * 32 + lane);
     uint8_t *const stage = ring + kWideStages * kWideStage + (warp - 4) * 2 * kOutBox;
     bool ok = true;  // a warp that gives up goes on without waiting, to the end of its tile
-    uint32_t i = 0;
+    uint32_t i = 0, chunk = 0;
     for (uint32_t t = pair; t < tiles; t += pairs) {
       if (__any_sync(kFullMask, has_failed(&failed))) break;
       const WideTile tile = wide_tile(t, tiles_m, tiles_n);
@@ -547,13 +544,27 @@ k_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
       uint64_t sums[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) sums[j] = 0;
+      uint32_t held[kScaleGroups];  // this row's scales of the next groups
       for (uint32_t g = 0; g < groups; ++g, ++i) {
         const uint32_t b = i & 1;
+        if (g % kScaleGroups == 0) {
+          if (ok && !mbar_wait(&scale_full[chunk & 1], chunk >> 1 & 1)) failed = 1, ok = false;
+#pragma unroll
+          for (uint32_t at = 0; at < kScaleGroups; ++at)
+            asm volatile("ld.shared.b32 %0, [%1];"
+                         : "=r"(held[at])
+                         : "r"(scale_at + ((chunk & 1) * kScaleGroups + at) * (kPair * 4))
+                         : "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_empty[chunk & 1]);
+          ++chunk;
+        }
+        const uint32_t scale = held[0];
+#pragma unroll
+        for (uint32_t at = 0; at + 1 < kScaleGroups; ++at) held[at] = held[at + 1];
         if (ok && !mbar_wait(&sum_full[b], i >> 1 & 1)) failed = 1, ok = false;
         __syncwarp();
         tc_fence_after();
-        uint32_t scale;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(scale) : "r"(scale_at + i % kScaleSlots * (kPair * 4)) : "memory");
         uint32_t d[2][16];
         tmem_ld16_nowait(taddr + b * kPair, d[0]);
         const uint64_t both = static_cast<uint64_t>(scale) << 32 | scale;
