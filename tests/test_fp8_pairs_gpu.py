@@ -39,3 +39,21 @@ def test_scales_that_jump_from_group_to_group(m, n, k, dtype):
         K.fp8_gemm(a, a_scales, w, w_scales, out=again)
         assert torch.equal(again, first)
     assert K.device_status() == 0
+
+
+def test_calls_of_one_group_one_after_the_other():
+    """A pair ends as soon as its only group is done, and another block takes its place: both blocks stay until every arrival of
+    the products on their barriers is in."""
+    calls = [operands(m, n, k, i, 1.0) for i, (m, n, k) in enumerate([(257, 9999, 16), (777, 4096, 128), (300, 7000, 112), (20, 640, 128)])]
+    assert [by_pairs(*x) for x in calls] == [True, True, True, False]
+    want = [K.fp8_gemm(*x) for x in calls]
+    for x, c in zip(calls, want):
+        check_product(c, *product(*x), x[0].shape[1])
+    outs = [[torch.empty_like(c) for c in want] for _ in range(8)]
+    for _ in range(25):
+        for out in outs:
+            for x, c in zip(calls, out):
+                K.fp8_gemm(*x, out=c)
+    torch.cuda.synchronize()
+    assert all(torch.equal(c, w) for out in outs for c, w in zip(out, want))
+    assert K.device_status() == 0

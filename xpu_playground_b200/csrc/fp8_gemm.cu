@@ -471,6 +471,10 @@ k_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         if (has_failed(&failed) && rank == 0)  // no copy may land once this shared memory is another block's
           for (uint32_t back = 0; back < kWideStages && back < i; ++back)
             mbar_wait(&full[(i - 1 - back) % kWideStages], (i - 1 - back) / kWideStages & 1);
+        // The products' last arrivals in this block, before it leaves with its barriers.
+        for (uint32_t back = min(i, kWideStages); back > 0 && !has_failed(&failed); --back)
+          if (!mbar_wait(&empty[(i - back) % kWideStages], (i - back) / kWideStages & 1)) failed = 1;
+        if (!mbar_wait(&drain, 0)) failed = 1;
       }
     } else if (warp == 1) {
       if (rank == 0) {
