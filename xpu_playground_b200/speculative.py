@@ -13,7 +13,8 @@ token. With ``width`` 0 a tree is one node and the loop is plain greedy decoding
 drafts change how many steps it takes, not the tokens (up to logits that differ
 by no more than their rounding). With a ``Sampling`` every token is drawn
 (``kernels.sample``) instead, from a random number of its own sequence and position, so
-that drafts do not change it either: a drafted token stands where it is the one drawn.
+that drafts do not change it either: a drafted token stands where it is the one drawn. The
+seed and the requests before decide the numbers: the same prompt again is drawn anew.
 
 With ``eight_bits`` the projections are held and multiplied in 8 bits: the residual's
 addition and the norm (``kernels.fp8_rms_norm``), the attention's output
@@ -197,9 +198,19 @@ class Server:
         s = model.shape
         self.model, self.steps, self.emitted, self.sampling = model, 0, 0, sampling
         if sampling is not None:  # one random number for what follows each position of each sequence
-            g = torch.Generator(device="cuda").manual_seed(sampling.seed)
-            self.u = torch.rand(sequences, max_positions, device="cuda", generator=g)
+            self.random = torch.Generator(device="cuda").manual_seed(sampling.seed)
+            self.u = torch.rand(sequences, max_positions, device="cuda", generator=self.random)
+            self.begun: set[int] = set()  # places whose numbers a sequence has had
         self.cache = KvCache(s.layers, pages, page_size, s.kv_heads, HEAD_DIM, sequences, max_positions)
+
+    def _begin(self, sequences: list[int]) -> None:
+        """Sequences begin in these places: where there was one before, with random numbers of their own."""
+        if self.sampling is None:
+            return
+        again = [i for i in sequences if i in self.begun]
+        if again:
+            self.u[torch.tensor(again, device="cuda")] = torch.rand(len(again), self.u.shape[1], device="cuda", generator=self.random)
+        self.begun.update(sequences)
 
     def choose(self, logits: torch.Tensor, sequences: list[int], positions: list[int]) -> list[int]:
         """The token after each row's position: the likeliest, or one drawn."""
@@ -218,6 +229,7 @@ class Server:
     def prefill(self, prompts: list[list[int]], sequences: list[int]) -> torch.Tensor:
         """Packed prompts into empty sequences; the logits after each."""
         s, cache = self.model.shape, self.cache
+        self._begin(sequences)
         lens = [len(p) for p in prompts]
         plan = kernels.PromptPlan(lens, s.q_heads, s.kv_heads, HEAD_DIM)
         ids, starts = _ints(sequences), _starts(lens)
@@ -277,6 +289,7 @@ class Server:
         if samples > 1:
             children = [many + i for i in range(many * (samples - 1))]
             cache.fork(_ints(p for p in range(many) for _ in range(samples - 1)), _ints(children))
+            self._begin(children)
         slots = [p if i == 0 else many + p * (samples - 1) + i - 1 for p in range(many) for i in range(samples)]
         if self.sampling is None:
             first = logits.topk(samples, -1).indices.flatten().tolist()
