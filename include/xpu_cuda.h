@@ -67,8 +67,8 @@ int xpu_gemm(int dtype, const void *a, const void *b, void *c, uint32_t m, uint3
 int xpu_gemm_bt(int dtype, const void *a, const void *w, void *c, uint32_t m, uint32_t n, uint32_t k, void *stream);
 
 /* Sticky device-side error word of this library's asynchronous kernels,
- * read and cleared (synchronises the device). Bit 0: a GEMM pipeline wait
- * timed out and its tile is incomplete; bit 1: a calibrator wait timed out;
+ * read and cleared (synchronises the device). Bit 0: a pipeline wait of
+ * xpu_gemm, xpu_gemm_bt or xpu_fp8_gemm timed out and its tile is incomplete; bit 1: a calibrator wait timed out;
  * bit 2: a serving attention wait timed out and its outputs are incomplete. No reference counterpart (the
  * reference's kernels have no bounded waits). */
 int xpu_device_status(uint32_t *flags);

@@ -19,8 +19,8 @@
 // memory and 128 x 256 sums in its TMEM, twice. Eight warps a block hold the tile's
 // FP32 sums in registers: a thread has one row and the 128 columns of one scale block, so
 // that a group's scale is one number a thread. The finished tile leaves through shared
-// memory while the next one's products run. 8192 x 24576 x 4096: 725 us on a cool card, 820 on a hot one (2.27 and 2.0 PFLOP/s:
-// power), 565 with the adding up left out; 777 x 4096 x 12288: 49 (1.6 PFLOP/s; 64 tiles for 74 pairs).
+// memory while the next one's products run. 8192 x 24576 x 4096: 878 us in a long run (1.88 PFLOP/s: power), 726 on a cool card
+// (2.27), 565 there with the adding up left out; 777 x 4096 x 12288: 57.6 and 48 (1.36 and 1.63 PFLOP/s; 64 tiles for 74 pairs).
 #include <cuda.h>
 
 #include <algorithm>
